@@ -462,6 +462,81 @@ int ramnet_segment_plan(int64_t B, int64_t H, int64_t A, int64_t C, int64_t w_to
 int ramnet_segment_call_form(int64_t B, int64_t H, int64_t T, int64_t A, int64_t C, int64_t w_top_k, int64_t r_top_k,
                              int dtype, int mass_aware, int *slot_ranges, int *crowded_form);
 
+/*
+ * Gated delta rule over whole sequences or the tokens of a decode step. No
+ * counterpart in the reference. One fp32 matrix S (Dk x Dv) per sequence and
+ * value head; per token, in order:
+ *     S <- e^g S;  u = beta (v - S^T k);  S <- S + k u^T;  o = scale S^T q
+ *   q, k            (B, T, Hk, Dk) `dtype`; value head h reads key head h / (Hv / Hk)
+ *   v, o            (B, T, Hv, Dv) `dtype`
+ *   g, beta         (B, T, Hv) `g_dtype`, `beta_dtype`; g is the logarithm of the
+ *                   decay (-inf clears the state)
+ *   init_state      (N, Hv, Dk, Dv) fp32, or NULL: zeros
+ *   state           (N, Hv, Dk, Dv) fp32 after the last token; may be init_state
+ *   cu_seqlens      (N + 1) int32 bounds of sequences packed in a batch of one, or
+ *                   NULL: N == B, one sequence a row. Bounds out of range or order
+ *                   are held to [0, T]: wrong values, no access out of range.
+ *                   Tokens of no sequence have output 0.
+ *   lengths         (B) int32 tokens of each row that count, or NULL: T; the others
+ *                   leave the state and have output 0. Not with cu_seqlens.
+ *   strides         15: of batch row, token and head in elements, of q, k, v, g, beta
+ *                   (last dimensions, o and the states are dense)
+ *   kept            what ramnet_delta_rule_backward takes of this call
+ *                   (ramnet_delta_rule_kept_bytes), or NULL
+ *   workspace       ramnet_delta_rule_workspace_bytes, kind 0, or 1 with `kept`
+ * Sums, states and norms are fp32, decays' sums within a chunk fp64.
+ * Requires Dk <= 256, Hv a multiple of Hk.
+ */
+int ramnet_delta_rule_forward(const void *q, const void *k, const void *v, int dtype, const void *g, int g_dtype,
+                              const void *beta, int beta_dtype, const float *init_state, float *state, void *o,
+                              const int32_t *cu_seqlens, const int32_t *lengths, int64_t B, int64_t T, int64_t N,
+                              int64_t Hk, int64_t Hv, int64_t Dk, int64_t Dv, float scale, const int64_t *strides,
+                              void *kept, int64_t kept_bytes, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * Its gradients, from d_o (B, T, Hv, Dv) `dtype` and d_state (N, Hv, Dk, Dv)
+ * fp32 (or NULL: zeros): dq, dk, dv, dg, dbeta in their inputs' shapes and
+ * types, dense, and dinit (N, Hv, Dk, Dv) fp32 (or NULL). `strides` are the
+ * forward's 15 and three of d_o; `workspace` of kind 2. Value heads that share
+ * a key head add to its gradient in one order: results do not change from
+ * call to call.
+ */
+int ramnet_delta_rule_backward(const void *q, const void *k, const void *v, int dtype, const void *g, int g_dtype,
+                               const void *beta, int beta_dtype, const int32_t *cu_seqlens, const int32_t *lengths,
+                               const void *d_o, const float *d_state, void *dq, void *dk, void *dv, void *dg,
+                               void *dbeta, float *dinit, int64_t B, int64_t T, int64_t N, int64_t Hk, int64_t Hv,
+                               int64_t Dk, int64_t Dv, float scale, const int64_t *strides, const void *kept,
+                               int64_t kept_bytes, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Bytes of their device workspace (kind 0: forward, 1: forward that keeps, 2:
+ * backward) and of what a forward keeps; -1 for sizes they do not take. */
+int64_t ramnet_delta_rule_workspace_bytes(int64_t B, int64_t T, int64_t N, int64_t Hk, int64_t Hv, int64_t Dk, int64_t Dv,
+                                          int packed, int kind);
+int64_t ramnet_delta_rule_kept_bytes(int64_t B, int64_t T, int64_t N, int64_t Hk, int64_t Hv, int64_t Dk, int64_t Dv,
+                                     int packed);
+
+/*
+ * Verification of drafted tokens (speculative decoding) from given random
+ * numbers. No counterpart in the reference. Draft s of a row stays if all
+ * before it did and accept[s] * q(x_s) < p(x_s); then one more token is drawn
+ * with `sample`: at the first refused place from max(p - q, 0) (from p where
+ * that is 0 everywhere), after the last draft from p. The drawn token is the
+ * lowest index with a weight above 0 whose running sum passes sample * total.
+ *   tokens          (B, S) int64; one outside [0, V) is refused
+ *   target          (B, S + 1, V) `dtype` probabilities p after each draft
+ *   draft           (B, S, V) `dtype` probabilities q the drafts were drawn from,
+ *                   or NULL: q = 1 at the drafted token, 0 elsewhere
+ *   accept, sample  (B, S), (B) fp32 uniform in [0, 1)
+ *   draft_lens      (B) int32 drafts of each row, or NULL: S
+ *   strides         4: of row and place in elements, of target and draft
+ *   out             (B, S + 1) int64: the drafts that stay, the drawn token, then -1
+ *   taken           (B) int32: how many drafts stay
+ * Sums are in 64 bits.
+ */
+int ramnet_verify_drafts(const int64_t *tokens, const void *target, const void *draft, int dtype, const float *accept,
+                         const float *sample, const int32_t *draft_lens, int64_t B, int64_t S, int64_t V,
+                         const int64_t *strides, int64_t *out, int32_t *taken, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -29,7 +29,8 @@ PROBE_SOURCE = "lds_probe.hip"
 
 SOURCES = ("topk_addr.hip", "segment_forward.hip", "segment_scan_f32.hip", "segment_scan_f16.hip",
            "segment_scan_bf16.hip", "segment_level_f32.hip", "segment_level_f16.hip", "segment_level_bf16.hip",
-           "segment_backward.hip", "autoregressive.hip", "readout.hip", "capi.hip")
+           "segment_backward.hip", "autoregressive.hip", "readout.hip", "delta_recurrent.hip", "delta_chunk.hip",
+           "delta_backward.hip", "verify_drafts.hip", "capi.hip")
 ARCH = "gfx950"
 
 

@@ -1135,6 +1135,136 @@ int ramnet_readout_stepwise(const void *y, const void *gate, const void *weight,
     return readout(y, gate, weight, dtype, rows, C, eps, true, out, stream);
 }
 
+// The gated delta rule's sizes.
+static int check_delta(ramnet::DeltaJob &job, int64_t B, int64_t T, int64_t N, int64_t Hk, int64_t Hv, int64_t Dk, int64_t Dv,
+                       bool packed) {
+    RAMNET_REQUIRE(B >= 0 && T >= 0 && N >= 0 && Hk > 0 && Hv > 0 && Dk > 0 && Dv > 0,
+                   "delta rule shape must have B, T, N >= 0 and Hk, Hv, Dk, Dv > 0");
+    RAMNET_REQUIRE(Hv % Hk == 0, "delta rule: Hv must be a multiple of Hk");
+    RAMNET_REQUIRE(Dk <= ramnet::kDeltaMaxDk, "delta rule: Dk must be at most 256");
+    RAMNET_REQUIRE(packed ? B == 1 : N == B, "delta rule: packed sequences lie in a batch of one, others one to a row");
+    // launches and chunk counts are in 32 bits, tensor offsets in 64
+    RAMNET_REQUIRE(Hv <= 65535 && Dv < (1 << 24) && fits_int({B, T, N, B * (T + 64) + N * 64}),
+                   "delta rule: index overflow");
+    job.B = static_cast<int>(B), job.T = static_cast<int>(T), job.N = static_cast<int>(N);
+    job.Hk = static_cast<int>(Hk), job.Hv = static_cast<int>(Hv), job.Dk = static_cast<int>(Dk);
+    job.Dv = static_cast<int>(Dv);
+    return RAMNET_OK;
+}
+
+int64_t ramnet_delta_rule_workspace_bytes(int64_t B, int64_t T, int64_t N, int64_t Hk, int64_t Hv, int64_t Dk, int64_t Dv,
+                                          int packed, int kind) {
+    ramnet::DeltaJob job{};
+    ramnet::DeltaWork work{};
+    if (kind < 0 || kind > 2 || check_delta(job, B, T, N, Hk, Hv, Dk, Dv, packed != 0) != RAMNET_OK)
+        return -1;
+    if (kind == 0 && ramnet::delta_is_recurrent(job))
+        return 0;
+    return ramnet::delta_layout(job, packed != 0, kind == 2, nullptr, &work);
+}
+
+int64_t ramnet_delta_rule_kept_bytes(int64_t B, int64_t T, int64_t N, int64_t Hk, int64_t Hv, int64_t Dk, int64_t Dv,
+                                     int packed) {
+    ramnet::DeltaJob job{};
+    ramnet::DeltaWork work{};
+    if (check_delta(job, B, T, N, Hk, Hv, Dk, Dv, packed != 0) != RAMNET_OK)
+        return -1;
+    return ramnet::delta_kept(job, packed != 0, nullptr, &work);
+}
+
+static void delta_strides(ramnet::DeltaJob &job, const int64_t *strides) {
+    int64_t *to[5] = {job.q_at, job.k_at, job.v_at, job.g_at, job.beta_at};
+    for (int i = 0; i < 15; ++i)
+        to[i / 3][i % 3] = strides[i];
+}
+
+int ramnet_delta_rule_forward(const void *q, const void *k, const void *v, int dtype, const void *g, int g_dtype,
+                              const void *beta, int beta_dtype, const float *init_state, float *state, void *o,
+                              const int32_t *cu_seqlens, const int32_t *lengths, int64_t B, int64_t T, int64_t N,
+                              int64_t Hk, int64_t Hv, int64_t Dk, int64_t Dv, float scale, const int64_t *strides,
+                              void *kept, int64_t kept_bytes, void *workspace, int64_t workspace_bytes, void *stream) {
+    ramnet::DeltaJob job{};
+    if (int rc = check_delta(job, B, T, N, Hk, Hv, Dk, Dv, cu_seqlens != nullptr))
+        return rc;
+    RAMNET_REQUIRE(valid_dtype(dtype) && valid_dtype(g_dtype) && valid_dtype(beta_dtype),
+                   "delta rule dtype must be float32, float16 or bfloat16");
+    RAMNET_REQUIRE(!(cu_seqlens && lengths), "delta rule: packed sequences have no lengths beside their bounds");
+    if (N == 0)
+        return RAMNET_OK;
+    RAMNET_REQUIRE(strides && state && (T == 0 || (q && k && v && g && beta && o)), "null tensor pointer");
+    job.q = q, job.k = k, job.v = v, job.g = g, job.beta = beta, job.init = init_state, job.state = state, job.o = o;
+    job.cu = cu_seqlens, job.lengths = lengths, job.dtype = dtype, job.g_dtype = g_dtype, job.beta_dtype = beta_dtype;
+    job.scale = scale;
+    delta_strides(job, strides);
+    const char *why = nullptr;
+    const hipStream_t on = static_cast<hipStream_t>(stream);
+    if (T == 0 || (!kept && ramnet::delta_is_recurrent(job)))
+        return finish(ramnet::launch_delta_recurrent(job, on, &why), why, "delta rule launch");
+    ramnet::DeltaWork work{};
+    RAMNET_REQUIRE(!kept || kept_bytes >= ramnet::delta_kept(job, cu_seqlens != nullptr, static_cast<char *>(kept), &work),
+                   "delta rule: kept region too small");
+    RAMNET_REQUIRE(workspace && workspace_bytes >= ramnet::delta_layout(job, cu_seqlens != nullptr, false,
+                                                                        static_cast<char *>(workspace), &work),
+                   "delta rule: workspace too small");
+    hipError_t err = ramnet::launch_delta_prepare(job, work, false, on, &why);
+    if (err == hipSuccess)
+        err = ramnet::launch_delta_chain(job, work, on, &why);
+    return finish(err, why, "delta rule launch");
+}
+
+int ramnet_delta_rule_backward(const void *q, const void *k, const void *v, int dtype, const void *g, int g_dtype,
+                               const void *beta, int beta_dtype, const int32_t *cu_seqlens, const int32_t *lengths,
+                               const void *d_o, const float *d_state, void *dq, void *dk, void *dv, void *dg,
+                               void *dbeta, float *dinit, int64_t B, int64_t T, int64_t N, int64_t Hk, int64_t Hv,
+                               int64_t Dk, int64_t Dv, float scale, const int64_t *strides, const void *kept,
+                               int64_t kept_bytes, void *workspace, int64_t workspace_bytes, void *stream) {
+    ramnet::DeltaJob job{};
+    if (int rc = check_delta(job, B, T, N, Hk, Hv, Dk, Dv, cu_seqlens != nullptr))
+        return rc;
+    RAMNET_REQUIRE(valid_dtype(dtype) && valid_dtype(g_dtype) && valid_dtype(beta_dtype),
+                   "delta rule dtype must be float32, float16 or bfloat16");
+    RAMNET_REQUIRE(!(cu_seqlens && lengths), "delta rule: packed sequences have no lengths beside their bounds");
+    RAMNET_REQUIRE(T > 0, "delta rule: a backward call needs tokens");
+    if (N == 0)
+        return RAMNET_OK;
+    RAMNET_REQUIRE(strides && q && k && v && g && beta && d_o && dq && dk && dv && dg && dbeta && kept,
+                   "null tensor pointer");
+    job.q = q, job.k = k, job.v = v, job.g = g, job.beta = beta, job.cu = cu_seqlens, job.lengths = lengths;
+    job.dtype = dtype, job.g_dtype = g_dtype, job.beta_dtype = beta_dtype, job.scale = scale;
+    delta_strides(job, strides);
+    ramnet::DeltaWork work{};
+    RAMNET_REQUIRE(kept_bytes >= ramnet::delta_kept(job, cu_seqlens != nullptr,
+                                                    const_cast<char *>(static_cast<const char *>(kept)), &work),
+                   "delta rule: kept region too small");
+    RAMNET_REQUIRE(workspace && workspace_bytes >= ramnet::delta_layout(job, cu_seqlens != nullptr, true,
+                                                                        static_cast<char *>(workspace), &work),
+                   "delta rule: workspace too small");
+    ramnet::DeltaGrads grads{d_o, d_state, dq, dk, dv, dg, dbeta, dinit, {strides[15], strides[16], strides[17]}};
+    const char *why = nullptr;
+    const hipStream_t on = static_cast<hipStream_t>(stream);
+    hipError_t err = ramnet::launch_delta_prepare(job, work, true, on, &why);
+    if (err == hipSuccess)
+        err = ramnet::launch_delta_backward(job, work, grads, on, &why);
+    return finish(err, why, "delta rule backward launch");
+}
+
+int ramnet_verify_drafts(const int64_t *tokens, const void *target, const void *draft, int dtype, const float *accept,
+                         const float *sample, const int32_t *draft_lens, int64_t B, int64_t S, int64_t V,
+                         const int64_t *strides, int64_t *out, int32_t *taken, void *stream) {
+    RAMNET_REQUIRE(B >= 0 && S >= 0 && V > 0, "verify_drafts shape must have B, S >= 0 and V > 0");
+    RAMNET_REQUIRE(B < kIntMax && S < kIntMax && V < (1LL << 30), "verify_drafts: index overflow");
+    RAMNET_REQUIRE(valid_dtype(dtype), "verify_drafts dtype must be float32, float16 or bfloat16");
+    if (B == 0)
+        return RAMNET_OK;
+    RAMNET_REQUIRE(target && sample && out && taken && strides && (S == 0 || (tokens && accept)), "null tensor pointer");
+    const ramnet::VerifyJob job{tokens, target, S ? draft : nullptr, accept, sample, draft_lens, out, taken, dtype,
+                                static_cast<int>(B), static_cast<int>(S), static_cast<int>(V),
+                                {strides[0], strides[1]}, {strides[2], strides[3]}};
+    const char *why = nullptr;
+    const hipError_t err = ramnet::launch_verify_drafts(job, static_cast<hipStream_t>(stream), &why);
+    return finish(err, why, "verify_drafts launch");
+}
+
 // The query has no token count: it answers for a call of kPlanQueryTokens
 // tokens (the form can differ for much shorter calls, where the mass-wave
 // form's saving of the pre-pass launches decides).

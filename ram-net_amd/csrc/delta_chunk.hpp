@@ -1,0 +1,86 @@
+// Chunked form of the gated delta rule: helpers of its kernels.
+//
+// Within a chunk of 64 tokens, gamma_i the sum of the decays up to token i and
+// L_ij = e^(gamma_i - gamma_j) for i >= j:
+//     Bl = strictlower(K K^T . L),  N = I + Bl diag(beta),  Y = N^-1
+//     E = Y (V - e^gamma . K S)           (E_i = v_i - S_i^T k_i, decayed S_i)
+//     O = scale e^gamma . (Q S) + P diag(beta) E,   P = scale lower(Q K^T . L)
+//     S <- e^gamma_C S + K^T diag(e^(gamma_C - gamma) beta) E
+#pragma once
+
+#include "delta_rule.hpp"
+
+namespace ramnet {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// One 16x16 tile += A (16 x 4 steps) B: lane l gives A[l % 16][4 (l / 16) + r]
+// and B[4 (l / 16) + r][l % 16] for the four steps r, and holds rows
+// 4 (l / 16) + r of column l % 16: a result tile is a B operand as it lies.
+__device__ __forceinline__ f32x4 mfma4(f32x4 a, f32x4 b, f32x4 c) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+        c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], b[r], c, 0, 0, 0);
+    return c;
+}
+
+__device__ __forceinline__ f32x4 load4(const float *p) { return *reinterpret_cast<const f32x4 *>(p); }
+// Four rows of a column.
+__device__ __forceinline__ f32x4 load4(const float *p, int64_t step) {
+    return f32x4{p[0], p[step], p[2 * step], p[3 * step]};
+}
+
+// A chunk: record-level place, its tokens t0 .. t0 + len of row b (len 0: none).
+struct DeltaPlace {
+    int n, b, t0, len;
+};
+
+__device__ __forceinline__ DeltaPlace delta_place(const DeltaJob &job, const DeltaWork &work, int chunk) {
+    int n, first;
+    if (work.offsets) {
+        if (chunk >= work.offsets[job.N])
+            return {-1, 0, 0, 0};
+        int lo = 0, hi = job.N;  // offsets[lo] <= chunk < offsets[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (work.offsets[mid] <= chunk)
+                lo = mid;
+            else
+                hi = mid;
+        }
+        n = lo;
+        first = work.offsets[n];
+    } else {
+        n = chunk / work.per_row;
+        first = n * work.per_row;
+    }
+    const DeltaSpan span = delta_span(job, n);
+    const int from = (chunk - first) * kDeltaChunk;
+    return {n, span.b, span.t0 + from, max(0, min(kDeltaChunk, span.len - from))};
+}
+
+// First chunk and number of chunks of a sequence.
+__device__ __forceinline__ void delta_chunks(const DeltaJob &job, const DeltaWork &work, int n, const DeltaSpan &span,
+                                             int &first, int &count) {
+    count = (span.len + kDeltaChunk - 1) / kDeltaChunk;
+    if (work.offsets) {
+        first = work.offsets[n];
+        count = min(count, work.offsets[n + 1] - first);  // (fewer only where the bounds are out of order)
+    } else {
+        first = n * work.per_row;
+    }
+}
+
+// 64 rows of D values into fp32 rows of `pitch`, zeros after `len` rows and up
+// to `wide` columns; `step` between rows of the source.
+template<typename Scalar>
+__device__ __forceinline__ void stage_rows(const Scalar *src, int64_t step, int len, int D, int wide, float *dst,
+                                           int pitch) {
+    const int total = kDeltaChunk * wide;
+    for (int i = threadIdx.x; i < total; i += blockDim.x) {
+        const int t = i / wide, d = i - t * wide;
+        dst[t * pitch + d] = t < len && d < D ? load_f32(src + t * step + d) : 0.f;
+    }
+}
+
+}  // namespace ramnet

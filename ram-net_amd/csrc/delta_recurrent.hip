@@ -1,0 +1,218 @@
+// Gated delta rule, token by token: decode steps and short prompts.
+//
+// A block holds 32 columns of one head's state in registers (columns of S do
+// not meet: each has its own u and o). Rows lie over row groups of threads,
+// four columns to a thread where Dv and the addresses allow 16-byte accesses.
+// A token costs one reduction over rows: with S the state before it,
+//     S_new^T q = e^g S^T q + (k.q) u,
+// so S^T k, S^T q and k.q are summed together, within a wave by shuffles and
+// over the four waves through LDS, in a fixed order. The next token's inputs
+// are on their way meanwhile.
+//
+// A decode step is bound by reading and writing the state once.
+#include "delta_rule.hpp"
+#include "ramnet_kernels.hpp"
+
+namespace ramnet {
+
+namespace {
+
+constexpr int kSlice = 32;    // columns of a block
+constexpr int kThreads = 256;
+
+template<typename Scalar, int R>
+struct Token {
+    uint32_t k[R], q[R];
+    uint32_t v[4];
+    float g, beta;
+};
+
+template<typename Scalar, int VEC, int R>
+__global__ __launch_bounds__(kThreads) void recurrent_kernel(const DeltaJob job, int slices) {
+    constexpr int CL = kSlice / VEC, RG = kThreads / CL;  // column lanes, row groups
+    __shared__ float part[2][kThreads / kWave][kSlice][2];
+    __shared__ float part_kq[2][kThreads / kWave];
+    const int tid = static_cast<int>(threadIdx.x), wave = tid / kWave;
+    const int cl = tid % CL, rg = tid / CL;
+    const int slice = static_cast<int>(blockIdx.x) % slices;
+    const int head = static_cast<int>(blockIdx.x) / slices % job.Hv;
+    const int n = static_cast<int>(blockIdx.x) / slices / job.Hv;
+    const int c = slice * kSlice + cl * VEC;
+    const bool on = c < job.Dv;
+    const DeltaSpan span = delta_span(job, n);
+    const int kh = head / (job.Hv / job.Hk);
+
+    const Scalar *q = static_cast<const Scalar *>(job.q) + span.b * job.q_at[0] + kh * job.q_at[2];
+    const Scalar *k = static_cast<const Scalar *>(job.k) + span.b * job.k_at[0] + kh * job.k_at[2];
+    const Scalar *v = static_cast<const Scalar *>(job.v) + span.b * job.v_at[0] + head * job.v_at[2] + (on ? c : 0);
+    const int64_t g0 = span.b * job.g_at[0] + head * job.g_at[2];
+    const int64_t b0 = span.b * job.beta_at[0] + head * job.beta_at[2];
+    Scalar *o = static_cast<Scalar *>(job.o) + (static_cast<int64_t>(span.b) * job.T * job.Hv + head) * job.Dv + c;
+    const int64_t o_step = static_cast<int64_t>(job.Hv) * job.Dv;
+    const int64_t matrix = (static_cast<int64_t>(n) * job.Hv + head) * job.Dk * job.Dv;
+
+    float s[R][VEC];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int r = rg + RG * i;
+        const bool have = on && r < job.Dk && job.init;
+        if constexpr (VEC == 4) {
+            float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (have)
+                w = *reinterpret_cast<const float4 *>(job.init + matrix + static_cast<int64_t>(r) * job.Dv + c);
+            s[i][0] = w.x, s[i][1] = w.y, s[i][2] = w.z, s[i][3] = w.w;
+        } else {
+            s[i][0] = have ? job.init[matrix + static_cast<int64_t>(r) * job.Dv + c] : 0.f;
+        }
+    }
+
+    auto fetch = [&](int t, Token<Scalar, R> &x) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int r = rg + RG * i;
+            x.k[i] = r < job.Dk ? load_bits(k + t * job.k_at[1] + r) : 0u;
+            x.q[i] = r < job.Dk ? load_bits(q + t * job.q_at[1] + r) : 0u;
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+            x.v[e] = load_bits(v + t * job.v_at[1] + (on ? e : 0));
+        x.g = load_code(job.g, job.g_dtype, g0 + t * job.g_at[1]);
+        x.beta = load_code(job.beta, job.beta_dtype, b0 + t * job.beta_at[1]);
+    };
+
+    Token<Scalar, R> now, next;
+    if (span.len > 0)
+        fetch(span.t0, now);
+    for (int i = 0; i < span.len; ++i) {
+        const int t = span.t0 + i, buf = i & 1;
+        if (i + 1 < span.len)
+            fetch(t + 1, next);
+        float sk[VEC] = {}, sq[VEC] = {}, kq = 0.f, kr[R];
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            const float qr = bits_f32<Scalar>(now.q[j]);
+            kr[j] = bits_f32<Scalar>(now.k[j]);
+            kq = fmaf(kr[j], qr, kq);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                sk[e] = fmaf(kr[j], s[j][e], sk[e]);
+                sq[e] = fmaf(qr, s[j][e], sq[e]);
+            }
+        }
+#pragma unroll
+        for (int m = CL; m < kWave; m <<= 1) {
+            kq += __shfl_xor(kq, m);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                sk[e] += __shfl_xor(sk[e], m);
+                sq[e] += __shfl_xor(sq[e], m);
+            }
+        }
+        if (tid % kWave < CL) {
+            if (cl == 0)
+                part_kq[buf][wave] = kq;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                part[buf][wave][cl * VEC + e][0] = sk[e];
+                part[buf][wave][cl * VEC + e][1] = sq[e];
+            }
+        }
+        __syncthreads();  // (the other buffer is written next: one barrier a token)
+        kq = 0.f;
+#pragma unroll
+        for (int w = 0; w < kThreads / kWave; ++w)
+            kq += part_kq[buf][w];
+        const float alpha = expf(now.g);
+        float out[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            float a = 0.f, b = 0.f;
+#pragma unroll
+            for (int w = 0; w < kThreads / kWave; ++w) {
+                a += part[buf][w][cl * VEC + e][0];
+                b += part[buf][w][cl * VEC + e][1];
+            }
+            const float u = now.beta * (bits_f32<Scalar>(now.v[e]) - alpha * a);
+            out[e] = job.scale * (alpha * b + kq * u);
+#pragma unroll
+            for (int j = 0; j < R; ++j)
+                s[j][e] = fmaf(kr[j], u, alpha * s[j][e]);
+        }
+        if (rg == 0 && on) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                store_f32(o + t * o_step + e, out[e]);
+        }
+        now = next;
+    }
+
+    if (on) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int r = rg + RG * i;
+            if (r >= job.Dk)
+                continue;
+            float *dst = job.state + matrix + static_cast<int64_t>(r) * job.Dv + c;
+            if constexpr (VEC == 4)
+                *reinterpret_cast<float4 *>(dst) = make_float4(s[i][0], s[i][1], s[i][2], s[i][3]);
+            else
+                *dst = s[i][0];
+        }
+        // tokens that do not count
+        auto clear = [&](int from, int to) {
+            for (int t = from + rg; t < to; t += RG)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e)
+                    store_f32(o + t * o_step + e, 0.f);
+        };
+        if (!job.cu)
+            clear(span.len, job.T);
+        else {
+            if (n == 0)
+                clear(0, span.t0);
+            if (n == job.N - 1)
+                clear(span.t0 + span.len, job.T);
+        }
+    }
+}
+
+template<typename Scalar>
+hipError_t launch_typed(const DeltaJob &job, hipStream_t stream, const char **why) {
+    auto aligned = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+    const bool wide = job.Dv % 4 == 0 && (!job.init || aligned(job.init)) && aligned(job.state);
+    const int slices = (job.Dv + kSlice - 1) / kSlice;
+    const int64_t blocks = static_cast<int64_t>(job.N) * job.Hv * slices;
+    if (blocks > 0x7fffffff) {
+        *why = "delta rule: too many state columns for one launch";
+        return hipErrorInvalidValue;
+    }
+    const dim3 grid(static_cast<unsigned>(blocks));
+    const int per = (job.Dk + (wide ? 31 : 7)) / (wide ? 32 : 8);  // rows of a thread
+#define RAMNET_DELTA(VEC, R)                                                                                     \
+    if (wide == (VEC == 4) && per <= R) {                                                                        \
+        hipLaunchKernelGGL((recurrent_kernel<Scalar, VEC, R>), grid, dim3(kThreads), 0, stream, job, slices);    \
+        return hipGetLastError();                                                                                \
+    }
+    RAMNET_DELTA(4, 2)
+    RAMNET_DELTA(4, 4)
+    RAMNET_DELTA(4, 8)
+    RAMNET_DELTA(1, 8)
+    RAMNET_DELTA(1, 16)
+    RAMNET_DELTA(1, 32)
+#undef RAMNET_DELTA
+    *why = "delta rule: Dk must be at most 256";
+    return hipErrorInvalidValue;
+}
+
+}  // namespace
+
+hipError_t launch_delta_recurrent(const DeltaJob &job, hipStream_t stream, const char **why) {
+    switch (job.dtype) {
+        case kF32: return launch_typed<float>(job, stream, why);
+        case kF16: return launch_typed<_Float16>(job, stream, why);
+        case kBF16: return launch_typed<bf16_t>(job, stream, why);
+        default: *why = "delta rule: unsupported dtype"; return hipErrorInvalidValue;
+    }
+}
+
+}  // namespace ramnet

@@ -1,0 +1,80 @@
+// The gated delta rule: jobs of its launches and device helpers they share.
+//
+// One matrix S (Dk x Dv, fp32) per sequence and value head, per token:
+//     S <- e^g S;   u = beta (v - S^T k);   S <- S + k u^T;   o = scale S^T q
+#pragma once
+
+#include "ramnet_device.hpp"
+
+namespace ramnet {
+
+enum : int { kDeltaMaxDk = 256, kDeltaChunk = 64 };
+
+// Tensors of one call; strides in elements, of batch row, token and head (the
+// last dimension is dense). Value head h reads key head h / (Hv / Hk).
+struct DeltaJob {
+    const void *q, *k, *v;      // (B, T, Hk, Dk) twice, (B, T, Hv, Dv)
+    const void *g, *beta;       // (B, T, Hv)
+    const float *init;          // (N, Hv, Dk, Dv), or null: zeros
+    float *state;               // (N, Hv, Dk, Dv); may be init
+    void *o;                    // (B, T, Hv, Dv), dense
+    const int32_t *cu;          // (N + 1) bounds of packed sequences (B == 1), or null: N == B
+    const int32_t *lengths;     // (B) tokens that count, or null: all
+    int dtype, g_dtype, beta_dtype;
+    int B, T, N, Hk, Hv, Dk, Dv;
+    float scale;
+    int64_t q_at[3], k_at[3], v_at[3], g_at[3], beta_at[3];
+};
+
+// Workspace of a call in chunks of 64 tokens (one record per chunk and value
+// head, record = chunk * Hv + head), and what a training forward keeps.
+struct DeltaWork {
+    int32_t *offsets;  // (N + 1) first chunk of each packed sequence; null where sequences are rows
+    double *gamma;     // [record][64] running sums of the decays within the chunk
+    float *y;          // [record][64][64] N^-1
+    float *p;          // [record][64][64] scale lower(Q K^T . L)
+    float *bl;         // [record][64][64] strictlower(K K^T . L)   (backward)
+    float *x;          // [record][64][Dv] gradient of the values    (backward)
+    float *dstate;     // [record][Dk][Dv] gradient after the chunk  (backward)
+    float *e;          // [record][64][Dv] v - S^T k of each token   (kept)
+    float *states;     // [record][Dk][Dv] state before the chunk    (kept)
+    int per_row;       // chunks of a row where sequences are rows
+    int chunks;        // records / Hv
+};
+
+// Gradients; those of the inputs have their types, strides dense.
+struct DeltaGrads {
+    const void *d_o;       // (B, T, Hv, Dv), strides d_o_at
+    const float *d_state;  // (N, Hv, Dk, Dv), or null: zeros
+    void *dq, *dk, *dv, *dg, *dbeta;
+    float *dinit;          // or null
+    int64_t d_o_at[3];
+};
+
+__device__ __forceinline__ float load_code(const void *p, int code, int64_t at) {
+    if (code == 0)
+        return static_cast<const float *>(p)[at];
+    if (code == 1)
+        return static_cast<float>(static_cast<const _Float16 *>(p)[at]);
+    return load_f32(static_cast<const bf16_t *>(p) + at);
+}
+
+// Tokens of one sequence: `len` from token t0 of batch row b. Bounds that are
+// out of order or out of range give fewer tokens, never ones outside [0, T).
+struct DeltaSpan {
+    int b, t0, len;
+};
+
+__device__ __forceinline__ DeltaSpan delta_span(const DeltaJob &job, int n) {
+    if (job.cu) {
+        const int lo = min(max(job.cu[n], 0), job.T), hi = min(max(job.cu[n + 1], lo), job.T);
+        return {0, lo, hi - lo};
+    }
+    return {n, 0, job.lengths ? min(max(job.lengths[n], 0), job.T) : job.T};
+}
+
+// A decay of one step. e^-200 is 0 in fp32 as e^-inf is; held there, sums of
+// decays stay finite and differences of them free of inf - inf. (A NaN stays.)
+__device__ __forceinline__ float delta_decay(float g) { return g < -200.f ? -200.f : g; }
+
+}  // namespace ramnet

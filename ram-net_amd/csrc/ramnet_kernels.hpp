@@ -3,6 +3,7 @@
 // scalars. Shapes are validated by the C-ABI layer before any launch.
 #pragma once
 
+#include "delta_rule.hpp"
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -315,5 +316,38 @@ bool segment_forward_can_save(int B, int H, int T, int A, int C, int Kw, int Kr,
 // (MassAux): the record-keeping pre-pass holds the slot space in one piece.
 bool segment_saved_aux(int A);
 hipError_t launch_segment_backward(const SegmentBwdJob &job, hipStream_t stream, const char **why);
+
+// Gated delta rule. launch_delta_recurrent walks the tokens of each sequence;
+// the chunked form is prepare (what a chunk's own tokens give) and then chain
+// (the states from chunk to chunk); launch_delta_backward follows a prepare
+// with `backward`. delta_layout places the buffers of a call in chunks in
+// `base`, or sizes them (null base); kept: what a training forward leaves for
+// its backward (a second region, delta_kept).
+hipError_t launch_delta_recurrent(const DeltaJob &job, hipStream_t stream, const char **why);
+int64_t delta_layout(const DeltaJob &job, bool packed, bool backward, char *base, DeltaWork *work);
+int64_t delta_kept(const DeltaJob &job, bool packed, char *base, DeltaWork *work);
+// Whether a call without gradients walks its tokens.
+bool delta_is_recurrent(const DeltaJob &job);
+hipError_t launch_delta_prepare(const DeltaJob &job, const DeltaWork &work, bool backward, hipStream_t stream,
+                                const char **why);
+hipError_t launch_delta_chain(const DeltaJob &job, const DeltaWork &work, hipStream_t stream, const char **why);
+hipError_t launch_delta_backward(const DeltaJob &job, const DeltaWork &work, const DeltaGrads &grads, hipStream_t stream,
+                                 const char **why);
+
+// Verification of drafted tokens; strides in elements, of row and place.
+struct VerifyJob {
+    const int64_t *tokens;  // (B, S)
+    const void *target;     // (B, S + 1, V)
+    const void *draft;      // (B, S, V), or null
+    const float *accept;    // (B, S)
+    const float *sample;    // (B)
+    const int32_t *lens;    // (B), or null: S
+    int64_t *out;           // (B, S + 1)
+    int32_t *taken;         // (B)
+    int dtype;
+    int B, S, V;
+    int64_t target_at[2], draft_at[2];
+};
+hipError_t launch_verify_drafts(const VerifyJob &job, hipStream_t stream, const char **why);
 
 }  // namespace ramnet

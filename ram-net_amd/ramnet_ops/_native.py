@@ -128,6 +128,19 @@ SIGNATURES: dict[str, tuple[type, list]] = {
         _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
         _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64,
         _c_int, _c_float, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr]),
+    "ramnet_delta_rule_forward": (_c_int, [
+        _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
+        _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_float, _c_i64s, _c_ptr, _c_i64, _c_ptr, _c_i64,
+        _c_ptr]),
+    "ramnet_delta_rule_backward": (_c_int, [
+        _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
+        _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_float,
+        _c_i64s, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr]),
+    "ramnet_delta_rule_workspace_bytes": (_c_i64, [_c_i64] * 7 + [_c_int, _c_int]),
+    "ramnet_delta_rule_kept_bytes": (_c_i64, [_c_i64] * 7 + [_c_int]),
+    "ramnet_verify_drafts": (_c_int, [
+        _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64s, _c_ptr, _c_ptr,
+        _c_ptr]),
     "ramnet_segment_plan": (_c_int, [
         _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_int, ctypes.POINTER(_c_int), ctypes.POINTER(_c_int),
         ctypes.POINTER(_c_int)]),

@@ -1,0 +1,115 @@
+"""Public API of the gated delta rule and of draft verification.
+
+The reference has neither; both follow this package's rules: argument errors
+before any launch (``TypeError`` for wrong kinds, ``ValueError`` for wrong
+choices, ``RuntimeError`` for tensors the kernels do not take), work on the
+current stream of the inputs' device, no fallback.
+"""
+from __future__ import annotations
+
+import torch
+
+from .ram_attn import _unavailable
+
+try:
+    from .impl import _delta
+    _delta_error: Exception | None = None
+except ImportError as exc:  # library not built: fail at call time
+    _delta = None
+    _delta_error = exc
+
+
+def _require_tensors(optional: tuple[str, ...] = (), **named) -> None:
+    for name, t in named.items():
+        if not isinstance(t, torch.Tensor) and not (t is None and name in optional):
+            raise TypeError(f"Expected {name} to be a Tensor{' or None' if name in optional else ''}, "
+                            f"got {type(t).__name__}.")
+
+
+def gated_delta_rule(
+        q: torch.Tensor,
+        k: torch.Tensor,
+        v: torch.Tensor,
+        g: torch.Tensor,
+        beta: torch.Tensor,
+        scale: float | None = None,
+        init_state: torch.Tensor | None = None,
+        cu_seqlens: torch.Tensor | None = None,
+        lengths: torch.Tensor | None = None,
+        inplace: bool = False,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Gated delta rule: one (Dk, Dv) state per sequence and value head.
+
+    Per token: ``S = exp(g) S``, ``S = S + k (beta (v - S^T k))^T``, ``o = scale S^T q``.
+    Differentiable in q, k, v, g, beta and init_state. Whole prompts run in
+    chunks of 64 tokens, decode steps and short prompts token by token.
+
+    :param q: Queries (B, T, Hk, Dk), Dk up to 256; their last dimension dense, any other strides.
+    :param k: Keys (B, T, Hk, Dk), as a rule of norm 1.
+    :param v: Values (B, T, Hv, Dv); value head h reads key head ``h // (Hv // Hk)``.
+    :param g: Logarithm of the decay (B, T, Hv), any float type; -inf clears the state.
+    :param beta: Write strength (B, T, Hv).
+    :param scale: Factor of o; default ``Dk ** -0.5``.
+    :param init_state: State before the first token (N, Hv, Dk, Dv); default zeros.
+    :param cu_seqlens: (N + 1) bounds of N sequences packed one after the other in a batch of one.
+    :param lengths: (B) tokens of each row that count; the others leave the state and have o = 0.
+    :param inplace: Update init_state in place (contiguous float32, no gradients).
+    :return: ``(o, state)``: (B, T, Hv, Dv) in v's type and (N, Hv, Dk, Dv) float32. N is B without cu_seqlens.
+    """
+    _require_tensors(("init_state", "cu_seqlens", "lengths"), q=q, k=k, v=v, g=g, beta=beta, init_state=init_state,
+                     cu_seqlens=cu_seqlens, lengths=lengths)
+    if scale is None:
+        scale = q.shape[-1] ** -0.5 if q.dim() and q.shape[-1] else 1.0
+    elif not isinstance(scale, (int, float)):
+        raise TypeError(f"Expected scale to be a number or None, got {type(scale).__name__}.")
+    if inplace and init_state is None:
+        raise ValueError("`inplace` needs an init_state to update.")
+    if _delta is None:
+        raise _unavailable("gated_delta_rule")
+    scale = float(scale)
+    grad = _delta.wants_grad(q, k, v, g, beta, init_state)
+    if inplace:
+        if grad:
+            raise ValueError("`inplace` has no gradients.")
+        if _delta.is_eager(q, k, v, g, beta, init_state, cu_seqlens, lengths):
+            _delta._require_state("gated_delta_rule", init_state)
+            return _delta._forward("gated_delta_rule", q, k, v, g, beta, init_state, cu_seqlens, lengths, scale,
+                                   init_state)[:2]
+        return _delta.gated_delta_rule_(q, k, v, g, beta, init_state, cu_seqlens, lengths, scale), init_state
+    if grad:
+        return _delta.gated_delta_rule_kept(q, k, v, g, beta, init_state, cu_seqlens, lengths, scale)[:2]
+    if _delta.is_eager(q, k, v, g, beta, init_state, cu_seqlens, lengths):
+        return _delta._forward("gated_delta_rule", q, k, v, g, beta, init_state, cu_seqlens, lengths, scale)[:2]
+    return _delta.gated_delta_rule(q, k, v, g, beta, init_state, cu_seqlens, lengths, scale)
+
+
+def verify_drafts(
+        tokens: torch.Tensor,
+        target: torch.Tensor,
+        draft: torch.Tensor | None,
+        accept: torch.Tensor,
+        sample: torch.Tensor,
+        draft_lens: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Which drafted tokens stay, and the token after them, from given random numbers.
+
+    Draft s stays if all before it did and ``accept[s] * draft[s, x] < target[s, x]`` for its token x. Then one
+    token is drawn with ``sample``: at the first refused place from ``max(target - draft, 0)`` (from target where
+    that is 0 everywhere), after the last draft from target. Tokens so taken are distributed as the target's own.
+
+    :param tokens: Drafted tokens (B, S).
+    :param target: The target's probabilities after each of 0 .. S drafts (B, S + 1, V).
+    :param draft: Probabilities the drafts were drawn from (B, S, V), in target's type; None for drafts without
+        (looked up, or greedy): 1 at the drafted token.
+    :param accept: Uniform numbers in [0, 1) (B, S).
+    :param sample: Uniform numbers in [0, 1) (B).
+    :param draft_lens: Drafts of each row (B); default S.
+    :return: ``(tokens, taken)``: (B, S + 1) int64 -- the drafts that stay, the drawn token, then -1 -- and (B) int32.
+    """
+    _require_tensors(("draft", "draft_lens"), tokens=tokens, target=target, draft=draft, accept=accept, sample=sample,
+                     draft_lens=draft_lens)
+    if _delta is None:
+        raise _unavailable("verify_drafts")
+    if _delta.is_eager(tokens, target, draft, accept, sample, draft_lens):
+        return _delta._verify(tokens, target, draft, accept, sample, draft_lens)
+    return _delta.verify_drafts(tokens, target, draft, accept, sample, draft_lens)
