@@ -511,7 +511,7 @@ int ramnet_delta_rule_backward(const void *q, const void *k, const void *v, int 
 /* Bytes of their device workspace (kind 0: forward, 1: forward that keeps, 2:
  * backward) and of what a forward keeps; -1 for sizes they do not take. */
 int64_t ramnet_delta_rule_workspace_bytes(int64_t B, int64_t T, int64_t N, int64_t Hk, int64_t Hv, int64_t Dk, int64_t Dv,
-                                          int packed, int kind);
+                                          int dtype, int packed, int kind);
 int64_t ramnet_delta_rule_kept_bytes(int64_t B, int64_t T, int64_t N, int64_t Hk, int64_t Hv, int64_t Dk, int64_t Dv,
                                      int packed);
 

@@ -1153,11 +1153,12 @@ static int check_delta(ramnet::DeltaJob &job, int64_t B, int64_t T, int64_t N, i
 }
 
 int64_t ramnet_delta_rule_workspace_bytes(int64_t B, int64_t T, int64_t N, int64_t Hk, int64_t Hv, int64_t Dk, int64_t Dv,
-                                          int packed, int kind) {
+                                          int dtype, int packed, int kind) {
     ramnet::DeltaJob job{};
     ramnet::DeltaWork work{};
-    if (kind < 0 || kind > 2 || check_delta(job, B, T, N, Hk, Hv, Dk, Dv, packed != 0) != RAMNET_OK)
+    if (kind < 0 || kind > 2 || !valid_dtype(dtype) || check_delta(job, B, T, N, Hk, Hv, Dk, Dv, packed != 0) != RAMNET_OK)
         return -1;
+    job.dtype = dtype;
     if (kind == 0 && ramnet::delta_is_recurrent(job))
         return 0;
     return ramnet::delta_layout(job, packed != 0, kind == 2, nullptr, &work);

@@ -11,146 +11,240 @@
 //     dbeta_j = sum_i (P . R1 + Bl . R2)_ij + e^(gamma_C - gamma_j) K_j . (E D^T)_j
 //     dgamma_i: the row sums less the column sums of (P . R1 + Bl . R2) beta_j, and what
 //               e^gamma_i, e^(gamma_C - gamma_i) and e^gamma_C multiply;  dg: its sums from the end
-#include "delta_chunk.hpp"
+#include "delta_split.hpp"
 #include "ramnet_kernels.hpp"
 
 namespace ramnet {
 
 namespace {
 
-template<typename Scalar, int DT>
-__global__ __launch_bounds__(256) void chain_back_kernel(const DeltaJob job, const DeltaWork work, const DeltaGrads grads,
-                                                         int groups) {
-    extern __shared__ __align__(16) float lds[];
-    constexpr int C = kDeltaChunk, wide = 16 * DT, pitch = wide + 4;
-    float *ks = lds, *qs = ks + C * pitch;
-    __shared__ float grow[C], left[C], beta_s[C];
+// The states' gradient from the last chunk to the first; waves as in the
+// forward's chain. The state's gradient and dv are fp32 results of fp32 values:
+// every product takes both parts of both sides (dO's own 16 bits are one part).
+template<typename Scalar, int DT, int PIECES, int BUFS>
+__global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, const DeltaWork work,
+                                                            const DeltaGrads grads, int groups) {
+    extern __shared__ __align__(16) float lds_base[];
+    using Lds = ChunkLds<DT, PIECES, true>;
+    constexpr int C = kDeltaChunk, BT = DT / 2;
     const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave, wave = tid / kWave;
     const int row = lane & 15, grp = lane >> 4;
     const int group = static_cast<int>(blockIdx.x) % groups;
     const int head = static_cast<int>(blockIdx.x) / groups % job.Hv;
     const int n = static_cast<int>(blockIdx.x) / groups / job.Hv;
     const int kh = head / (job.Hv / job.Hk);
-    const int c = (group * 4 + wave) * 16 + row;
-    const bool on = c < job.Dv;
-    const int cc = on ? c : 0;
     const DeltaSpan span = delta_span(job, n);
     int first, count;
     delta_chunks(job, work, n, span, first, count);
+    auto buffer = [&](int i) {
+        return Lds{reinterpret_cast<uint16_t *>(reinterpret_cast<char *>(lds_base) + (BUFS == 2 ? (i & 1) * Lds::kBytes : 0))};
+    };
 
+    if (wave >= 4) {
+        const int at = tid - 256;
+        const bool whole = rows_whole<Scalar>(job);
+        const Scalar *k = static_cast<const Scalar *>(job.k) + span.b * job.k_at[0] + kh * job.k_at[2];
+        const Scalar *q = static_cast<const Scalar *>(job.q) + span.b * job.q_at[0] + kh * job.q_at[2];
+        Stager<Scalar, DT, PIECES, true> stager;
+        auto load = [&](int i) {
+            const int64_t t0 = span.t0 + i * C;
+            stager.load(k + t0 * job.k_at[1], job.k_at[1], q + t0 * job.q_at[1], job.q_at[1], min(C, span.len - i * C),
+                        job.Dk, whole, work.vec + (static_cast<int64_t>(first + i) * job.Hv + head) * kVecs * C, at);
+        };
+        if (count > 0) {
+            load(count - 1);
+            stager.store(buffer(count - 1), at);
+        }
+        __syncthreads();
+        for (int i = count - 1; i >= 0; --i) {
+            if (i > 0)
+                load(i - 1);
+            if constexpr (BUFS == 1)
+                __syncthreads();  // chunk i is done with
+            if (i > 0)
+                stager.store(buffer(i - 1), at);
+            __syncthreads();
+        }
+        return;
+    }
+
+    const int c = (group * 4 + wave) * 16 + row;
+    const bool on = c < job.Dv;
+    const int cc = on ? c : 0;
     const int64_t matrix = (static_cast<int64_t>(n) * job.Hv + head) * job.Dk * job.Dv;
+    const Columns<const float> before(grads.d_state + matrix, job.Dv, grp, cc);
     f32x4 s[DT];
 #pragma unroll
     for (int t = 0; t < DT; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int d = 16 * t + 4 * grp + r;
-            s[t][r] = grads.d_state && on && d < job.Dk
-                          ? grads.d_state[matrix + static_cast<int64_t>(d) * job.Dv + c] : 0.f;
-        }
-    const Scalar *k = static_cast<const Scalar *>(job.k) + span.b * job.k_at[0] + kh * job.k_at[2];
-    const Scalar *q = static_cast<const Scalar *>(job.q) + span.b * job.q_at[0] + kh * job.q_at[2];
-    const Scalar *d_o = static_cast<const Scalar *>(grads.d_o) + span.b * grads.d_o_at[0] + head * grads.d_o_at[2] + cc;
-    Scalar *dv = static_cast<Scalar *>(grads.dv) + (static_cast<int64_t>(span.b) * job.T * job.Hv + head) * job.Dv + cc;
-    const int64_t dv_step = static_cast<int64_t>(job.Hv) * job.Dv;
+        for (int r = 0; r < 4; ++r)
+            s[t][r] = grads.d_state && on && 16 * t + 4 * grp + r < job.Dk ? *before.at(0, t, r) : 0.f;
+    const Columns<const Scalar> d_o(static_cast<const Scalar *>(grads.d_o) + span.b * grads.d_o_at[0] +
+                                    head * grads.d_o_at[2], grads.d_o_at[1], grp, cc);
+    const Columns<Scalar> dv(static_cast<Scalar *>(grads.dv) + (static_cast<int64_t>(span.b) * job.T * job.Hv + head) * job.Dv,
+                             static_cast<int64_t>(job.Hv) * job.Dv, grp, cc);
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+    uint32_t o_bits[16];
+    auto load_o = [&](int i) {
+        const int64_t t0 = span.t0 + i * C;
+        const int len = on ? min(C, span.len - i * C) : 0;
+#pragma unroll
+        for (int m = 0; m < 16; ++m) {
+            o_bits[m] = 16 * (m / 4) + 4 * grp + m % 4 < len ? load_bits(d_o.at(t0, m / 4, m % 4)) : 0u;
+        }
+    };
+    if (count > 0)
+        load_o(count - 1);
+    __syncthreads();
 
     for (int i = count - 1; i >= 0; --i) {
         const int64_t t0 = span.t0 + i * C;
         const int len = min(C, span.len - i * C);
         const int64_t record = static_cast<int64_t>(first + i) * job.Hv + head;
-        __syncthreads();
-        stage_rows(k + t0 * job.k_at[1], job.k_at[1], len, job.Dk, wide, ks, pitch);
-        stage_rows(q + t0 * job.q_at[1], job.q_at[1], len, job.Dk, wide, qs, pitch);
-        if (wave == 0) {
-            const double gam = work.gamma[record * C + lane], end = work.gamma[record * C + C - 1];
-            grow[lane] = expf(static_cast<float>(gam));
-            left[lane] = expf(static_cast<float>(end - gam));
-            beta_s[lane] = lane < len ? load_code(job.beta, job.beta_dtype, span.b * job.beta_at[0] +
-                                                  (t0 + lane) * job.beta_at[1] + head * job.beta_at[2]) : 0.f;
+        const Lds lds = buffer(i);
+        const float *vec = lds.vec();
+        const u32x4 *yf = reinterpret_cast<const u32x4 *>(work.y + record * 2 * kFragWords) + lane;
+        const u32x4 *pf = reinterpret_cast<const u32x4 *>(work.p_frags + record * 2 * kFragWords) + lane;
+        u32x4 p_hi[kFrags], p_lo[kFrags];
+#pragma unroll
+        for (int f = 0; f < kFrags; ++f)
+            p_hi[f] = pf[f * kWave], p_lo[f] = pf[(kFrags + f) * kWave];
+        const float total = expf(static_cast<float>(work.gamma[record * C + C - 1]));
+        if (on) {
+            const Columns<float> keep(work.dstate + record * job.Dk * job.Dv, job.Dv, grp, cc);
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (16 * t + 4 * grp + r < job.Dk)
+                        *keep.at(0, t, r) = s[t][r];
         }
         f32x4 out[4], du[4], x[4];
 #pragma unroll
         for (int m = 0; m < 4; ++m)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int t = 16 * m + 4 * grp + r;
-                out[m][r] = t < len && on ? load_f32(d_o + (t0 + t) * grads.d_o_at[1]) : 0.f;
-            }
-        if (on) {
-            float *keep = work.dstate + record * job.Dk * job.Dv + c;
+            for (int r = 0; r < 4; ++r)
+                out[m][r] = bits_f32<Scalar>(o_bits[4 * m + r]);
+        if (i > 0)
+            load_o(i - 1);
+        {
+            Operand<4, true> oo;
+            oo.set(out);
 #pragma unroll
-            for (int t = 0; t < DT; ++t)
+            for (int m = 0; m < 4; ++m) {
+                x[m] = zero;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int d = 16 * t + 4 * grp + r;
-                    if (d < job.Dk)
-                        keep[static_cast<int64_t>(d) * job.Dv] = s[t][r];
+                for (int b = m / 2; b < 2; ++b) {
+                    const int f = m < 2 ? m * 2 + b : m + 2;
+                    x[m] = mfma16(p_hi[f], oo.hi[b], x[m]);
+                    x[m] = mfma16(p_lo[f], oo.hi[b], x[m]);
+                    if constexpr (!__is_same(Scalar, bf16_t))
+                        x[m] = mfma16(p_hi[f], oo.lo[b], x[m]);  // (0 for bf16 but far below a column's largest)
                 }
+                x[m] = x[m] * (load4(vec + kVecInvP * C + 16 * m + 4 * grp) * oo.inverse);
+            }
         }
-        __syncthreads();
-        const float *y = work.y + record * C * C, *p = work.p + record * C * C;
+        u32x4 y_hi[kFrags], y_lo[kFrags];
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            du[m] = zero;
+        for (int f = 0; f < kFrags; ++f)
+            y_hi[f] = yf[f * kWave], y_lo[f] = yf[(kFrags + f) * kWave];
+        {
+            Operand<DT, true> so;
+            so.set(s);
 #pragma unroll
-            for (int t = 0; t < DT; ++t)
-                du[m] = mfma4(load4(ks + (16 * m + row) * pitch + 16 * t + 4 * grp), s[t], du[m]);
-            du[m] = du[m] * load4(left + 16 * m + 4 * grp);
+            for (int m = 0; m < 4; ++m)
+                du[m] = zero;
 #pragma unroll
-            for (int j = m; j < 4; ++j)
-                du[m] = mfma4(load4(p + (16 * j + 4 * grp) * C + 16 * m + row, C), out[j], du[m]);
-            du[m] = du[m] * load4(beta_s + 16 * m + 4 * grp);
+            for (int b = 0; b < BT; ++b) {
+                __builtin_amdgcn_sched_barrier(0);  // (operands of one block at a time: registers)
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {
+                    const u32x4 kf = lds.row_frag(lds.k(0), m, b, lane);
+                    du[m] = mfma16(kf, so.hi[b], du[m]);
+                    du[m] = mfma16(kf, so.lo[b], du[m]);
+                    if constexpr (PIECES == 2)
+                        du[m] = mfma16(lds.row_frag(lds.k(1), m, b, lane), so.hi[b], du[m]);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+                du[m] = (x[m] + du[m] * (load4(vec + kVecLeftK * C + 16 * m + 4 * grp) * so.inverse)) *
+                        load4(vec + kVecBeta * C + 16 * m + 4 * grp);
         }
+        {
+            Operand<4, true> uo;
+            uo.set(du);
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            x[m] = zero;
+            for (int m = 0; m < 4; ++m) {
+                x[m] = zero;
 #pragma unroll
-            for (int j = m; j < 4; ++j)
-                x[m] = mfma4(load4(y + (16 * j + 4 * grp) * C + 16 * m + row, C), du[j], x[m]);
+                for (int b = m / 2; b < 2; ++b) {
+                    const int f = m < 2 ? m * 2 + b : m + 2;
+                    x[m] = mfma16(y_hi[f], uo.hi[b], x[m]);
+                    x[m] = mfma16(y_hi[f], uo.lo[b], x[m]);
+                    x[m] = mfma16(y_lo[f], uo.hi[b], x[m]);
+                }
+                x[m] = x[m] * (load4(vec + kVecInvY * C + 16 * m + 4 * grp) * uo.inverse);
+            }
         }
         if (on) {
-            float *keep = work.x + record * C * job.Dv + c;
+            const Columns<float> keep(work.x + record * C * job.Dv, job.Dv, grp, cc);
 #pragma unroll
             for (int m = 0; m < 4; ++m)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int t = 16 * m + 4 * grp + r;
-                    keep[static_cast<int64_t>(t) * job.Dv] = x[m][r];
-                    if (t < len)
-                        store_f32(dv + (t0 + t) * dv_step, x[m][r]);
+                    *keep.at(0, m, r) = x[m][r];
+                    if (16 * m + 4 * grp + r < len)
+                        store_f32(dv.at(t0, m, r), x[m][r]);
                 }
         }
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-            const f32x4 gr = load4(grow + 16 * m + 4 * grp);
-            x[m] = -gr * x[m];
-            out[m] = job.scale * gr * out[m];
+            x[m] = -(load4(vec + kVecGrowK * C + 16 * m + 4 * grp) * x[m]);
+            out[m] = out[m] * load4(vec + kVecGrowQ * C + 16 * m + 4 * grp);
         }
-        const float total = grow[C - 1];
+        Operand<4, true> xo, oo;
+        xo.set(x);
+        oo.set(out);
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
-            s[t] = s[t] * total;
+            if (t % 2 == 0)
+                __builtin_amdgcn_sched_barrier(0);
+            f32x4 a = zero, z = zero;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                s[t] = mfma4(load4(ks + (16 * j + 4 * grp) * pitch + 16 * t + row, pitch), x[j], s[t]);
-                s[t] = mfma4(load4(qs + (16 * j + 4 * grp) * pitch + 16 * t + row, pitch), out[j], s[t]);
+            for (int b = 0; b < 2; ++b) {
+                const u32x4 kf = lds.col_frag(lds.kt(0), t, b, lane), qf = lds.col_frag(lds.qt(0), t, b, lane);
+                a = mfma16(kf, xo.hi[b], a);
+                z = mfma16(qf, oo.hi[b], z);
+                a = mfma16(kf, xo.lo[b], a);
+                z = mfma16(qf, oo.lo[b], z);
+                if constexpr (PIECES == 2) {
+                    a = mfma16(lds.col_frag(lds.kt(1), t, b, lane), xo.hi[b], a);
+                    z = mfma16(lds.col_frag(lds.qt(1), t, b, lane), oo.hi[b], z);
+                }
             }
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                s[t][r] = fmaf(a[r], xo.inverse, fmaf(z[r], oo.inverse, total * s[t][r]));
         }
+        __syncthreads();
+        if constexpr (BUFS == 1)
+            __syncthreads();  // chunk i - 1 is there
     }
     if (on) {
-        if (grads.dinit)
+        if (grads.dinit) {
+            const Columns<float> after(grads.dinit + matrix, job.Dv, grp, cc);
 #pragma unroll
             for (int t = 0; t < DT; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int d = 16 * t + 4 * grp + r;
-                    if (d < job.Dk)
-                        grads.dinit[matrix + static_cast<int64_t>(d) * job.Dv + c] = s[t][r];
-                }
+                for (int r = 0; r < 4; ++r)
+                    if (16 * t + 4 * grp + r < job.Dk)
+                        *after.at(0, t, r) = s[t][r];
+        }
         if (!job.cu)  // tokens that do not count
-            for (int t = span.len + grp; t < job.T; t += 4)
-                store_f32(dv + t * dv_step, 0.f);
+            for (int64_t t = span.len + grp; t < job.T; t += 4)
+                store_f32(dv.base + t * dv.step + cc, 0.f);
     }
 }
 
@@ -430,19 +524,18 @@ hipError_t backward_typed(const DeltaJob &job, const DeltaWork &work, const Delt
         *why = "delta rule: too many state columns for one launch";
         return hipErrorInvalidValue;
     }
-    const size_t bytes = 2 * C * (wide + 4) * sizeof(float);
-    if (bytes + 2 * C * (C + 4) * sizeof(float) > 160 * 1024 - 4096) {
-        *why = "delta rule: gradients take Dk up to 160";
-        return hipErrorInvalidValue;
-    }
+    constexpr int PIECES = sizeof(Scalar) == 4 ? 2 : 1;
+    const size_t bytes = (2 * C * (wide + 4) + 2 * C * (C + 4)) * sizeof(float);
 #define RAMNET_BACK(DT)                                                                                              \
     if (wide == 16 * DT) {                                                                                           \
-        hipLaunchKernelGGL((chain_back_kernel<Scalar, DT>), dim3(static_cast<unsigned>(blocks)), dim3(256), bytes,   \
-                           stream, job, work, grads, groups);                                                        \
+        constexpr int each = ChunkLds<DT, PIECES, true>::kBytes, bufs = 2 * each <= kLdsBytes ? 2 : 1;               \
+        static_assert(each <= kLdsBytes);                                                                            \
+        hipLaunchKernelGGL((chain_back_kernel<Scalar, DT, PIECES, bufs>), dim3(static_cast<unsigned>(blocks)),       \
+                           dim3(512), bufs * each, stream, job, work, grads, groups);                                \
         if (const hipError_t err = hipGetLastError())                                                                \
             return err;                                                                                              \
-        hipLaunchKernelGGL((inputs_back_kernel<Scalar, DT>), dim3(work.chunks, job.Hk), dim3(256),                   \
-                           bytes + 2 * C * (C + 4) * sizeof(float), stream, job, work, grads);                       \
+        hipLaunchKernelGGL((inputs_back_kernel<Scalar, DT>), dim3(work.chunks, job.Hk), dim3(256), bytes, stream,    \
+                           job, work, grads);                                                                        \
     }
     RAMNET_BACK(2)
     RAMNET_BACK(4)

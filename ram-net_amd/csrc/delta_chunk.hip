@@ -1,7 +1,9 @@
 // Gated delta rule in chunks of 64 tokens: what the chunks' own tokens give
 // (prepare), then the states from chunk to chunk (chain).
-#include "delta_chunk.hpp"
+#include "delta_split.hpp"
 #include "ramnet_kernels.hpp"
+
+#include <algorithm>
 
 namespace ramnet {
 
@@ -41,16 +43,74 @@ __global__ __launch_bounds__(1024) void offsets_kernel(const DeltaJob job, const
     }
 }
 
-// Y, P and gamma of one chunk and value head. Four waves.
+// K (or Q) of a chunk in LDS, 64 rows of `pitch` elements as they are, zeros
+// past the last token and Dk.
+template<typename Scalar>
+__device__ __forceinline__ void stage_raw(const Scalar *src, int64_t step, int len, int D, int wide, bool whole,
+                                          Scalar *dst, int pitch) {
+    constexpr int V = 16 / static_cast<int>(sizeof(Scalar));
+    const int pieces = wide / V;
+    for (int i = threadIdx.x; i < kDeltaChunk * pieces; i += 256) {
+        const int t = i / pieces, d = (i - t * pieces) * V;
+        u32x4 x = {0u, 0u, 0u, 0u};
+        if (t < len && d < D) {
+            const Scalar *p = src + t * step + d;
+            if (whole) {
+                x = *reinterpret_cast<const u32x4 *>(p);
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    if (d + e < D)
+                        x[e * sizeof(Scalar) / 4] |= load_bits(p + e) << (e * sizeof(Scalar) % 4 * 8);
+            }
+        }
+        *reinterpret_cast<u32x4 *>(dst + t * pitch + d) = x;
+    }
+}
+
+// 16 x 16 of A B^T, rows of `wide` elements in LDS.
+template<typename Scalar>
+__device__ __forceinline__ f32x4 rows_product(const Scalar *a, const Scalar *b, int wide, int grp) {
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    if constexpr (sizeof(Scalar) == 4) {
+        for (int d = 4 * grp; d < wide; d += 16)
+            acc = mfma4(load4(a + d), load4(b + d), acc);
+    } else {
+        for (int d = 8 * grp; d < wide; d += 32) {
+            const u32x4 x = *reinterpret_cast<const u32x4 *>(a + d), y = *reinterpret_cast<const u32x4 *>(b + d);
+            if constexpr (__is_same(Scalar, bf16_t)) {
+                typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y),
+                                                              acc, 0, 0, 0);
+            } else {
+                acc = mfma16(x, y, acc);
+            }
+        }
+    }
+    return acc;
+}
+
+// The largest of each row of 64 (or of Dk), four threads a row.
+template<typename F>
+__device__ __forceinline__ float quad_max(int tid, int n, F value) {
+    float m = 0.f;
+    for (int i = tid % 4; i < n; i += 4)
+        m = fmaxf(m, fabsf(value(tid / 4, i)));
+    m = fmaxf(m, __shfl_xor(m, 1));
+    return fmaxf(m, __shfl_xor(m, 2));
+}
+
+// Y, P, gamma and the scales of one chunk and value head. Four waves.
 template<typename Scalar>
 __global__ __launch_bounds__(256) void prepare_kernel(const DeltaJob job, const DeltaWork work, int wide, bool backward) {
     extern __shared__ __align__(16) float lds[];
     constexpr int C = kDeltaChunk, NP = C + 4;
-    const int pitch = wide + 4;
-    float *ks = lds, *qs = ks + C * pitch, *nm = qs + C * pitch;
-    float *ys = lds;  // (once the keys are done with)
+    const int pitch = wide + 16 / static_cast<int>(sizeof(Scalar));
+    float *nm = lds, *pm = nm + C * NP;
+    Scalar *ks = reinterpret_cast<Scalar *>(pm + C * NP), *qs = ks + C * pitch;
+    float *ys = pm + C * NP;  // (once the keys are done with)
     __shared__ double gam[C];
-    __shared__ float beta_s[C];
+    __shared__ float beta_s[C], sk_s[C], sq_s[C], scale_y[C], scale_p[C];
     const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave, wave = tid / kWave;
     const int chunk = blockIdx.x, head = blockIdx.y, kh = head / (job.Hv / job.Hk);
     const DeltaPlace at = delta_place(job, work, chunk);
@@ -62,7 +122,7 @@ __global__ __launch_bounds__(256) void prepare_kernel(const DeltaJob job, const 
             Scalar *o = static_cast<Scalar *>(job.o) + static_cast<int64_t>(head) * job.Dv;
             auto clear = [&](int from, int to) {
                 for (int64_t t = from; t < to; ++t)
-                    for (int c = tid; c < job.Dv; c += blockDim.x)
+                    for (int c = tid; c < job.Dv; c += 256)
                         store_f32(o + t * job.Hv * job.Dv + c, 0.f);
             };
             clear(0, first);
@@ -70,14 +130,17 @@ __global__ __launch_bounds__(256) void prepare_kernel(const DeltaJob job, const 
         }
         return;
     }
-    stage_rows(static_cast<const Scalar *>(job.k) + at.b * job.k_at[0] + at.t0 * job.k_at[1] + kh * job.k_at[2],
-               job.k_at[1], at.len, job.Dk, wide, ks, pitch);
-    stage_rows(static_cast<const Scalar *>(job.q) + at.b * job.q_at[0] + at.t0 * job.q_at[1] + kh * job.q_at[2],
-               job.q_at[1], at.len, job.Dk, wide, qs, pitch);
+    const bool whole = rows_whole<Scalar>(job);
+    stage_raw(static_cast<const Scalar *>(job.k) + at.b * job.k_at[0] + at.t0 * job.k_at[1] + kh * job.k_at[2],
+              job.k_at[1], at.len, job.Dk, wide, whole, ks, pitch);
+    stage_raw(static_cast<const Scalar *>(job.q) + at.b * job.q_at[0] + at.t0 * job.q_at[1] + kh * job.q_at[2],
+              job.q_at[1], at.len, job.Dk, wide, whole, qs, pitch);
+    const int64_t record = static_cast<int64_t>(chunk) * job.Hv + head;
     if (wave == 0) {
         const int64_t t = at.t0 + lane;
         const bool have = lane < at.len;
-        double x = have ? delta_decay(load_code(job.g, job.g_dtype, at.b * job.g_at[0] + t * job.g_at[1] + head * job.g_at[2])) : 0.f;
+        double x = have ? delta_decay(load_code(job.g, job.g_dtype, at.b * job.g_at[0] + t * job.g_at[1] +
+                                                head * job.g_at[2])) : 0.f;
 #pragma unroll
         for (int m = 1; m < kWave; m <<= 1) {
             const double y = __shfl_up(x, m);
@@ -86,31 +149,40 @@ __global__ __launch_bounds__(256) void prepare_kernel(const DeltaJob job, const 
         gam[lane] = x;
         beta_s[lane] = have ? load_code(job.beta, job.beta_dtype,
                                         at.b * job.beta_at[0] + t * job.beta_at[1] + head * job.beta_at[2]) : 0.f;
-        work.gamma[(static_cast<int64_t>(chunk) * job.Hv + head) * C + lane] = x;
+        work.gamma[record * C + lane] = x;
     }
     __syncthreads();
 
+    // the tokens' scales: fp16 inputs are multiplied as they are
+    if constexpr (__is_same(Scalar, _Float16)) {
+        if (tid < C)
+            sk_s[tid] = sq_s[tid] = 1.f;
+    } else {
+        float inverse;
+        const float k_max = quad_max(tid, wide, [&](int t, int d) { return load_f32(ks + t * pitch + d); });
+        const float q_max = quad_max(tid, wide, [&](int t, int d) { return load_f32(qs + t * pitch + d); });
+        if (tid % 4 == 0)
+            sk_s[tid / 4] = scale_of(k_max, inverse), sq_s[tid / 4] = scale_of(q_max, inverse);
+    }
+
     // K K^T and Q K^T, lower tiles; tile pairs go round the waves
     const int row = lane & 15, grp = lane >> 4;
-    const int64_t record = static_cast<int64_t>(chunk) * job.Hv + head;
-    float *y_out = work.y + record * C * C, *p_out = work.p + record * C * C;
-    float *bl_out = backward ? work.bl + record * C * C : nullptr;
+    float *p_out = backward ? work.p + record * C * C : nullptr, *bl_out = backward ? work.bl + record * C * C : nullptr;
     for (int tile = wave; tile < 32; tile += 4) {
         const bool is_p = tile >= 16;
         const int ti = (tile & 15) >> 2, tj = tile & 3;
         f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-        if (tj <= ti) {
-            const float *a = (is_p ? qs : ks) + (16 * ti + row) * pitch + 4 * grp;
-            const float *b = ks + (16 * tj + row) * pitch + 4 * grp;
-            for (int d = 0; d < wide; d += 16)
-                acc = mfma4(load4(a + d), load4(b + d), acc);
-        }
+        if (tj <= ti)
+            acc = rows_product((is_p ? qs : ks) + (16 * ti + row) * pitch, ks + (16 * tj + row) * pitch, wide, grp);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int i = 16 * ti + 4 * grp + r, j = 16 * tj + row;
             const float decay = i >= j ? expf(static_cast<float>(gam[i] - gam[j])) : 0.f;
             if (is_p) {
-                p_out[i * C + j] = i >= j ? job.scale * acc[r] * decay : 0.f;
+                const float x = i >= j ? job.scale * acc[r] * decay : 0.f;
+                pm[i * NP + j] = backward ? x : x * beta_s[j];
+                if (p_out)
+                    p_out[i * C + j] = x;
             } else {
                 const float x = i > j ? acc[r] * decay : 0.f;
                 nm[i * NP + j] = x * beta_s[j];
@@ -153,7 +225,6 @@ __global__ __launch_bounds__(256) void prepare_kernel(const DeltaJob job, const 
             ys[(b + 4 * grp + r) * NP + a + row] = -t[r];
     }
     __syncthreads();
-    f32x4 low[2];
     if (wave < 2) {
         const int c = 16 * wave;
         f32x4 t[2];
@@ -167,163 +238,304 @@ __global__ __launch_bounds__(256) void prepare_kernel(const DeltaJob job, const 
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            low[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+            f32x4 low = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int m = 0; m < 2; ++m)
-                low[i] = mfma4(load4(ys + (32 + 16 * i + row) * NP + 32 + 16 * m + 4 * grp), t[m], low[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
+                low = mfma4(load4(ys + (32 + 16 * i + row) * NP + 32 + 16 * m + 4 * grp), t[m], low);
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                ys[(32 + 16 * i + 4 * grp + r) * NP + c + row] = -low[i][r];
+                ys[(32 + 16 * i + 4 * grp + r) * NP + c + row] = -low[r];
+        }
     }
     __syncthreads();
-    for (int i = tid; i < C * C; i += 256)
-        y_out[i] = ys[i / C * NP + i % C];
+
+    // scales of the rows (backward: the columns) of Y and P, and the vectors
+    {
+        float inverse;
+        const float y_max = quad_max(tid, C, [&](int i, int j) { return backward ? ys[j * NP + i] : ys[i * NP + j]; });
+        const float p_max = quad_max(tid, C, [&](int i, int j) { return backward ? pm[j * NP + i] : pm[i * NP + j]; });
+        float *vec = work.vec + record * kVecs * C;
+        if (tid % 4 == 0) {
+            const int i = tid / 4;
+            const float sk = sk_s[i], sq = sq_s[i];
+            scale_y[i] = scale_of(y_max, inverse);
+            vec[kVecInvY * C + i] = inverse;
+            scale_p[i] = scale_of(p_max, inverse);
+            vec[kVecInvP * C + i] = inverse;
+            const float grow = expf(static_cast<float>(gam[i])), left = expf(static_cast<float>(gam[C - 1] - gam[i]));
+            vec[kVecSk * C + i] = sk;
+            vec[kVecSq * C + i] = sq;
+            vec[kVecGrowK * C + i] = grow / sk;
+            vec[kVecGrowQ * C + i] = job.scale * grow / sq;
+            vec[kVecLeftK * C + i] = left / sk;
+            vec[kVecBeta * C + i] = beta_s[i];
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < 2 * kFrags * kWave; i += 256) {
+        const bool is_p = i >= kFrags * kWave;
+        const int f = (is_p ? i - kFrags * kWave : i) / kWave;
+        int tile, block;
+        frag_place(f, backward, tile, block);
+        const float *m = is_p ? pm : ys;
+        const int a = 16 * tile + row, b = 32 * block + 4 * grp;  // (256 is a multiple of a wave: row and grp are i's too)
+        f32x4 x, y;
+        if (backward)
+            x = load4(m + b * NP + a, NP), y = load4(m + (b + 16) * NP + a, NP);
+        else
+            x = load4(m + a * NP + b), y = load4(m + a * NP + b + 16);
+        const float s = is_p ? scale_p[a] : scale_y[a];
+        u32x4 hi, lo;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const f32x4 z = w < 2 ? x : y;
+            uint32_t h, l;
+            split2(z[w % 2 * 2], z[w % 2 * 2 + 1], s, h, l);
+            hi[w] = h, lo[w] = l;
+        }
+        uint32_t *out = (is_p ? work.p_frags : work.y) + record * 2 * kFragWords + (f * kWave + lane) * 4;
+        *reinterpret_cast<u32x4 *>(out) = hi;
+        *reinterpret_cast<u32x4 *>(out + kFragWords) = lo;
+    }
 }
 
-// The states, 16 columns a wave: they do not meet, so a wave keeps its part of
-// S in registers and needs no other wave's results. DT: Dk in tiles of 16.
-template<typename Scalar, int DT>
-__global__ __launch_bounds__(256) void chain_kernel(const DeltaJob job, const DeltaWork work, int groups) {
-    extern __shared__ __align__(16) float lds[];
-    constexpr int C = kDeltaChunk, wide = 16 * DT, pitch = wide + 4;
-    float *ks = lds, *qs = ks + C * pitch;
-    __shared__ float grow[C], left[C], beta_s[C];
+// The states from chunk to chunk. Columns of S do not meet: each of the first
+// four waves keeps 16 of them in registers and needs no other wave's results.
+// The other four bring the next chunk's K and Q to LDS as matrix operands.
+// DT: Dk in tiles of 16; PIECES: fp16 parts of q and k; LO: whether products
+// that go to o alone take the second parts too (bf16 outputs do not show them:
+// their rounding is 2^-9, what is left out 2^-12).
+template<typename Scalar, int DT, int PIECES, bool LO, int BUFS>
+__global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const DeltaWork work, int groups) {
+    extern __shared__ __align__(16) float lds_base[];
+    using Lds = ChunkLds<DT, PIECES, false>;
+    constexpr int C = kDeltaChunk, BT = DT / 2;
     const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave, wave = tid / kWave;
     const int row = lane & 15, grp = lane >> 4;
     const int group = static_cast<int>(blockIdx.x) % groups;
     const int head = static_cast<int>(blockIdx.x) / groups % job.Hv;
     const int n = static_cast<int>(blockIdx.x) / groups / job.Hv;
     const int kh = head / (job.Hv / job.Hk);
-    const int c = (group * 4 + wave) * 16 + row;
-    const bool on = c < job.Dv;
-    const int cc = on ? c : 0;
     const DeltaSpan span = delta_span(job, n);
     int first, count;
     delta_chunks(job, work, n, span, first, count);
+    auto buffer = [&](int i) {
+        return Lds{reinterpret_cast<uint16_t *>(reinterpret_cast<char *>(lds_base) + (BUFS == 2 ? (i & 1) * Lds::kBytes : 0))};
+    };
 
+    if (wave >= 4) {
+        const int at = tid - 256;
+        const bool whole = rows_whole<Scalar>(job);
+        const Scalar *k = static_cast<const Scalar *>(job.k) + span.b * job.k_at[0] + kh * job.k_at[2];
+        const Scalar *q = static_cast<const Scalar *>(job.q) + span.b * job.q_at[0] + kh * job.q_at[2];
+        Stager<Scalar, DT, PIECES, false> stager;
+        auto load = [&](int i) {
+            const int64_t t0 = span.t0 + i * C;
+            stager.load(k + t0 * job.k_at[1], job.k_at[1], q + t0 * job.q_at[1], job.q_at[1], min(C, span.len - i * C),
+                        job.Dk, whole, work.vec + (static_cast<int64_t>(first + i) * job.Hv + head) * kVecs * C, at);
+        };
+        if (count > 0) {
+            load(0);
+            stager.store(buffer(0), at);
+        }
+        __syncthreads();
+        for (int i = 0; i < count; ++i) {
+            if (i + 1 < count)
+                load(i + 1);
+            if constexpr (BUFS == 1)
+                __syncthreads();  // chunk i is done with
+            if (i + 1 < count)
+                stager.store(buffer(i + 1), at);
+            __syncthreads();
+        }
+        return;
+    }
+
+    const int c = (group * 4 + wave) * 16 + row;
+    const bool on = c < job.Dv;
+    const int cc = on ? c : 0;
     const int64_t matrix = (static_cast<int64_t>(n) * job.Hv + head) * job.Dk * job.Dv;
+    const Columns<const float> before(job.init + matrix, job.Dv, grp, cc);
     f32x4 s[DT];
 #pragma unroll
     for (int t = 0; t < DT; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int d = 16 * t + 4 * grp + r;
-            s[t][r] = job.init && on && d < job.Dk ? job.init[matrix + static_cast<int64_t>(d) * job.Dv + c] : 0.f;
+            s[t][r] = job.init && on && 16 * t + 4 * grp + r < job.Dk ? *before.at(0, t, r) : 0.f;
         }
-    const Scalar *k = static_cast<const Scalar *>(job.k) + span.b * job.k_at[0] + kh * job.k_at[2];
-    const Scalar *q = static_cast<const Scalar *>(job.q) + span.b * job.q_at[0] + kh * job.q_at[2];
-    const Scalar *v = static_cast<const Scalar *>(job.v) + span.b * job.v_at[0] + head * job.v_at[2] + cc;
-    Scalar *o = static_cast<Scalar *>(job.o) + (static_cast<int64_t>(span.b) * job.T * job.Hv + head) * job.Dv + cc;
-    const int64_t o_step = static_cast<int64_t>(job.Hv) * job.Dv;
+    const Columns<const Scalar> v(static_cast<const Scalar *>(job.v) + span.b * job.v_at[0] + head * job.v_at[2],
+                                  job.v_at[1], grp, cc);
+    const Columns<Scalar> o(static_cast<Scalar *>(job.o) + (static_cast<int64_t>(span.b) * job.T * job.Hv + head) * job.Dv,
+                            static_cast<int64_t>(job.Hv) * job.Dv, grp, cc);
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+    uint32_t v_bits[16];
+    auto load_v = [&](int i) {
+        const int64_t t0 = span.t0 + i * C;
+        const int len = on ? min(C, span.len - i * C) : 0;
+#pragma unroll
+        for (int m = 0; m < 16; ++m) {
+            v_bits[m] = 16 * (m / 4) + 4 * grp + m % 4 < len ? load_bits(v.at(t0, m / 4, m % 4)) : 0u;
+        }
+    };
+    if (count > 0)
+        load_v(0);
+    __syncthreads();
 
     for (int i = 0; i < count; ++i) {
         const int64_t t0 = span.t0 + i * C;
         const int len = min(C, span.len - i * C);
         const int64_t record = static_cast<int64_t>(first + i) * job.Hv + head;
-        __syncthreads();
-        stage_rows(k + t0 * job.k_at[1], job.k_at[1], len, job.Dk, wide, ks, pitch);
-        stage_rows(q + t0 * job.q_at[1], job.q_at[1], len, job.Dk, wide, qs, pitch);
-        if (wave == 0) {
-            const double gam = work.gamma[record * C + lane], end = work.gamma[record * C + C - 1];
-            grow[lane] = expf(static_cast<float>(gam));
-            left[lane] = expf(static_cast<float>(end - gam));
-            beta_s[lane] = lane < len ? load_code(job.beta, job.beta_dtype, span.b * job.beta_at[0] +
-                                                  (t0 + lane) * job.beta_at[1] + head * job.beta_at[2]) : 0.f;
-        }
-        f32x4 e[4], g[4], qo[4];
+        const Lds lds = buffer(i);
+        const float *vec = lds.vec();
+        const u32x4 *yf = reinterpret_cast<const u32x4 *>(work.y + record * 2 * kFragWords) + lane;
+        const u32x4 *pf = reinterpret_cast<const u32x4 *>(work.p_frags + record * 2 * kFragWords) + lane;
+        u32x4 y_hi[kFrags], y_lo[kFrags];
 #pragma unroll
-        for (int m = 0; m < 4; ++m)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int t = 16 * m + 4 * grp + r;
-                e[m][r] = t < len && on ? load_f32(v + (t0 + t) * job.v_at[1]) : 0.f;
-            }
+        for (int f = 0; f < kFrags; ++f)
+            y_hi[f] = yf[f * kWave], y_lo[f] = yf[(kFrags + f) * kWave];
+        const float total = expf(static_cast<float>(work.gamma[record * C + C - 1]));
         if (work.states && on) {
-            float *keep = work.states + record * job.Dk * job.Dv + c;
+            const Columns<float> keep(work.states + record * job.Dk * job.Dv, job.Dv, grp, cc);
 #pragma unroll
             for (int t = 0; t < DT; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int d = 16 * t + 4 * grp + r;
-                    if (d < job.Dk)
-                        keep[static_cast<int64_t>(d) * job.Dv] = s[t][r];
-                }
+                for (int r = 0; r < 4; ++r)
+                    if (16 * t + 4 * grp + r < job.Dk)
+                        *keep.at(0, t, r) = s[t][r];
         }
-        __syncthreads();
+
+        f32x4 g[4], qo[4];
+        float s_inverse;
+        {
+            Operand<DT, true> so;
+            so.set(s);
+            s_inverse = so.inverse;
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+                g[m] = qo[m] = zero;
+#pragma unroll
+            for (int b = 0; b < BT; ++b) {
+                __builtin_amdgcn_sched_barrier(0);  // (operands of one block at a time: registers)
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {
+                    const u32x4 kf = lds.row_frag(lds.k(0), m, b, lane), qf = lds.row_frag(lds.q(0), m, b, lane);
+                    g[m] = mfma16(kf, so.hi[b], g[m]);
+                    qo[m] = mfma16(qf, so.hi[b], qo[m]);
+                    g[m] = mfma16(kf, so.lo[b], g[m]);
+                    if constexpr (LO)
+                        qo[m] = mfma16(qf, so.lo[b], qo[m]);
+                    if constexpr (PIECES == 2) {
+                        g[m] = mfma16(lds.row_frag(lds.k(1), m, b, lane), so.hi[b], g[m]);
+                        qo[m] = mfma16(lds.row_frag(lds.q(1), m, b, lane), so.hi[b], qo[m]);
+                    }
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        // what the state gives o, and v - S^T k but for the chunk's own tokens
+        f32x4 e[4];
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-            g[m] = qo[m] = zero;
+            const f32x4 gr = load4(vec + kVecGrowK * C + 16 * m + 4 * grp) * s_inverse;
+            qo[m] = qo[m] * (load4(vec + kVecGrowQ * C + 16 * m + 4 * grp) * s_inverse);
 #pragma unroll
-            for (int t = 0; t < DT; ++t) {
-                g[m] = mfma4(load4(ks + (16 * m + row) * pitch + 16 * t + 4 * grp), s[t], g[m]);
-                qo[m] = mfma4(load4(qs + (16 * m + row) * pitch + 16 * t + 4 * grp), s[t], qo[m]);
+            for (int r = 0; r < 4; ++r)
+                g[m][r] = fmaf(-gr[r], g[m][r], bits_f32<Scalar>(v_bits[4 * m + r]));
+        }
+        u32x4 p_hi[kFrags], p_lo[LO ? kFrags : 1];
+        {
+            Operand<4, true> ro;
+            ro.set(g);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int f = 0; f < kFrags; ++f) {
+                p_hi[f] = pf[f * kWave];
+                if constexpr (LO)
+                    p_lo[f] = pf[(kFrags + f) * kWave];
+            }
+            if (i + 1 < count)
+                load_v(i + 1);
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                e[m] = zero;
+#pragma unroll
+                for (int b = 0; b <= m / 2; ++b) {
+                    const int f = m < 2 ? m : 2 + (m - 2) * 2 + b;
+                    e[m] = mfma16(y_hi[f], ro.hi[b], e[m]);
+                    e[m] = mfma16(y_hi[f], ro.lo[b], e[m]);
+                    e[m] = mfma16(y_lo[f], ro.hi[b], e[m]);
+                }
+                e[m] = e[m] * (load4(vec + kVecInvY * C + 16 * m + 4 * grp) * ro.inverse);
             }
         }
-        const float *y = work.y + record * C * C, *p = work.p + record * C * C;
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            const f32x4 gr = load4(grow + 16 * m + 4 * grp);
-            g[m] = e[m] - gr * g[m];
-            qo[m] = job.scale * gr * qo[m];
-        }
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            e[m] = zero;
-#pragma unroll
-            for (int j = 0; j <= m; ++j)
-                e[m] = mfma4(load4(y + (16 * m + row) * C + 16 * j + 4 * grp), g[j], e[m]);
-        }
         if (work.e && on) {
-            float *keep = work.e + record * C * job.Dv + c;
+            const Columns<float> keep(work.e + record * C * job.Dv, job.Dv, grp, cc);
 #pragma unroll
             for (int m = 0; m < 4; ++m)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    keep[static_cast<int64_t>(16 * m + 4 * grp + r) * job.Dv] = e[m][r];
+                    *keep.at(0, m, r) = e[m][r];
         }
+        {
+            Operand<4, LO> eo;
+            eo.set(e);
 #pragma unroll
-        for (int m = 0; m < 4; ++m)
-            e[m] = e[m] * load4(beta_s + 16 * m + 4 * grp);  // now u
+            for (int m = 0; m < 4; ++m) {
+                f32x4 x = zero;
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
+                for (int b = 0; b <= m / 2; ++b) {
+                    const int f = m < 2 ? m : 2 + (m - 2) * 2 + b;
+                    x = mfma16(p_hi[f], eo.hi[b], x);
+                    if constexpr (LO) {
+                        x = mfma16(p_hi[f], eo.lo[b], x);
+                        x = mfma16(p_lo[f], eo.hi[b], x);
+                    }
+                }
+                qo[m] = qo[m] + x * (load4(vec + kVecInvP * C + 16 * m + 4 * grp) * eo.inverse);
 #pragma unroll
-            for (int j = 0; j <= m; ++j)
-                qo[m] = mfma4(load4(p + (16 * m + row) * C + 16 * j + 4 * grp), e[j], qo[m]);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int t = 16 * m + 4 * grp + r;
-                if (t < len && on)
-                    store_f32(o + (t0 + t) * o_step, qo[m][r]);
+                for (int r = 0; r < 4; ++r) {
+                    if (16 * m + 4 * grp + r < len && on)
+                        store_f32(o.at(t0, m, r), qo[m][r]);
+                }
             }
         }
-        const float total = grow[C - 1];
 #pragma unroll
         for (int m = 0; m < 4; ++m)
-            e[m] = e[m] * load4(left + 16 * m + 4 * grp);
+            e[m] = e[m] * (load4(vec + kVecLeftK * C + 16 * m + 4 * grp) * load4(vec + kVecBeta * C + 16 * m + 4 * grp));
+        Operand<4, true> wo;
+        wo.set(e);
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
-            s[t] = s[t] * total;
+            if (t % 2 == 0)
+                __builtin_amdgcn_sched_barrier(0);
+            f32x4 x = zero;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                s[t] = mfma4(load4(ks + (16 * j + 4 * grp) * pitch + 16 * t + row, pitch), e[j], s[t]);
+            for (int b = 0; b < 2; ++b) {
+                const u32x4 kf = lds.col_frag(lds.kt(0), t, b, lane);
+                x = mfma16(kf, wo.hi[b], x);
+                x = mfma16(kf, wo.lo[b], x);
+                if constexpr (PIECES == 2)
+                    x = mfma16(lds.col_frag(lds.kt(1), t, b, lane), wo.hi[b], x);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                s[t][r] = fmaf(x[r], wo.inverse, total * s[t][r]);
         }
+        __syncthreads();
+        if constexpr (BUFS == 1)
+            __syncthreads();  // chunk i + 1 is there
     }
     if (on) {
+        const Columns<float> after(job.state + matrix, job.Dv, grp, cc);
 #pragma unroll
         for (int t = 0; t < DT; ++t)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int d = 16 * t + 4 * grp + r;
-                if (d < job.Dk)
-                    job.state[matrix + static_cast<int64_t>(d) * job.Dv + c] = s[t][r];
-            }
+            for (int r = 0; r < 4; ++r)
+                if (16 * t + 4 * grp + r < job.Dk)
+                    *after.at(0, t, r) = s[t][r];
         if (!job.cu)  // tokens that do not count
-            for (int t = span.len + grp; t < job.T; t += 4)
-                store_f32(o + t * o_step, 0.f);
+            for (int64_t t = span.len + grp; t < job.T; t += 4)
+                store_f32(o.base + t * o.step + cc, 0.f);
     }
 }
 
@@ -332,10 +544,23 @@ int padded(int Dk) { return Dk <= 32 ? 32 : Dk <= 64 ? 64 : Dk <= 96 ? 96 : Dk <
 template<typename Scalar>
 hipError_t prepare_typed(const DeltaJob &job, const DeltaWork &work, bool backward, hipStream_t stream) {
     const int wide = padded(job.Dk);
-    const size_t bytes = (2 * kDeltaChunk * (wide + 4) + kDeltaChunk * (kDeltaChunk + 4)) * sizeof(float);
-    hipLaunchKernelGGL(prepare_kernel<Scalar>, dim3(work.chunks, job.Hv), dim3(256), bytes, stream, job, work, wide,
-                       backward);
+    const size_t rows = 2 * kDeltaChunk * (wide * sizeof(Scalar) + 16), square = kDeltaChunk * (kDeltaChunk + 4) * sizeof(float);
+    hipLaunchKernelGGL(prepare_kernel<Scalar>, dim3(work.chunks, job.Hv), dim3(256), 2 * square + std::max(rows, square),
+                       stream, job, work, wide, backward);
     return hipGetLastError();
+}
+
+template<typename Scalar, int DT>
+constexpr bool kChainFits = ChunkLds<DT, sizeof(Scalar) == 4 ? 2 : 1, false>::kBytes <= kLdsBytes;
+
+template<typename Scalar, int DT>
+void chain_launch(const DeltaJob &job, const DeltaWork &work, unsigned blocks, int groups, hipStream_t stream) {
+    constexpr int PIECES = sizeof(Scalar) == 4 ? 2 : 1;
+    constexpr bool LO = !__is_same(Scalar, bf16_t);
+    constexpr int bytes = ChunkLds<DT, PIECES, false>::kBytes;
+    constexpr int BUFS = 2 * bytes <= kLdsBytes ? 2 : 1;
+    hipLaunchKernelGGL((chain_kernel<Scalar, DT, PIECES, LO, BUFS>), dim3(blocks), dim3(512), BUFS * bytes, stream, job,
+                       work, groups);
 }
 
 template<typename Scalar>
@@ -346,11 +571,10 @@ hipError_t chain_typed(const DeltaJob &job, const DeltaWork &work, hipStream_t s
         *why = "delta rule: too many state columns for one launch";
         return hipErrorInvalidValue;
     }
-    const size_t bytes = 2 * kDeltaChunk * (wide + 4) * sizeof(float);
-#define RAMNET_CHAIN(DT)                                                                                        \
-    if (wide == 16 * DT)                                                                                        \
-        hipLaunchKernelGGL((chain_kernel<Scalar, DT>), dim3(static_cast<unsigned>(blocks)), dim3(256), bytes,   \
-                           stream, job, work, groups)
+#define RAMNET_CHAIN(DT)                           \
+    if constexpr (kChainFits<Scalar, DT>)          \
+        if (wide == 16 * DT)                       \
+    chain_launch<Scalar, DT>(job, work, static_cast<unsigned>(blocks), groups, stream)
     RAMNET_CHAIN(2);
     RAMNET_CHAIN(4);
     RAMNET_CHAIN(6);
@@ -363,7 +587,11 @@ hipError_t chain_typed(const DeltaJob &job, const DeltaWork &work, hipStream_t s
 
 }  // namespace
 
-bool delta_is_recurrent(const DeltaJob &job) { return job.T <= 32; }
+// Short calls, and those whose chunks (two fp16 parts of each fp32 key and
+// query) do not fit the LDS.
+bool delta_is_recurrent(const DeltaJob &job) {
+    return job.T <= 32 || (job.dtype == kF32 && padded(job.Dk) > 160);
+}
 
 namespace {
 
@@ -393,9 +621,11 @@ int64_t delta_layout(const DeltaJob &job, bool packed, bool backward, char *base
     const int64_t records = static_cast<int64_t>(work->chunks) * job.Hv, square = kDeltaChunk * kDeltaChunk;
     work->offsets = packed ? carve.take<int32_t>(job.N + 1) : nullptr;
     work->gamma = carve.take<double>(records * kDeltaChunk);
-    work->y = carve.take<float>(records * square);
-    work->p = carve.take<float>(records * square);
+    work->vec = carve.take<float>(records * kVecs * kDeltaChunk);
+    work->y = carve.take<uint32_t>(records * 2 * kFragWords);
+    work->p_frags = carve.take<uint32_t>(records * 2 * kFragWords);
     if (backward) {
+        work->p = carve.take<float>(records * square);
         work->bl = carve.take<float>(records * square);
         work->x = carve.take<float>(records * kDeltaChunk * job.Dv);
         work->dstate = carve.take<float>(records * job.Dk * job.Dv);

@@ -71,6 +71,17 @@ __device__ __forceinline__ void delta_chunks(const DeltaJob &job, const DeltaWor
     }
 }
 
+constexpr int kLdsBytes = 160 * 1024;
+
+// Whether rows of q and k are whole pieces of 16 bytes at 16-byte addresses.
+template<typename Scalar>
+__device__ __forceinline__ bool rows_whole(const DeltaJob &job) {
+    constexpr int V = 16 / static_cast<int>(sizeof(Scalar));
+    const int64_t steps = job.q_at[0] | job.q_at[1] | job.q_at[2] | job.k_at[0] | job.k_at[1] | job.k_at[2];
+    const uintptr_t starts = reinterpret_cast<uintptr_t>(job.q) | reinterpret_cast<uintptr_t>(job.k);
+    return job.Dk % 8 == 0 && steps % V == 0 && starts % 16 == 0;
+}
+
 // 64 rows of D values into fp32 rows of `pitch`, zeros after `len` rows and up
 // to `wide` columns; `step` between rows of the source.
 template<typename Scalar>

@@ -31,8 +31,10 @@ struct DeltaJob {
 struct DeltaWork {
     int32_t *offsets;  // (N + 1) first chunk of each packed sequence; null where sequences are rows
     double *gamma;     // [record][64] running sums of the decays within the chunk
-    float *y;          // [record][64][64] N^-1
-    float *p;          // [record][64][64] scale lower(Q K^T . L)
+    float *vec;        // [record][8][64] scales and decays of the tokens (delta_split.hpp)
+    uint32_t *y;       // [record][2][6][64][4] N^-1 as matrix operands of fp16 parts (backward: transposed)
+    uint32_t *p_frags; // the same of scale lower(Q K^T . L) diag(beta) (backward: transposed, without beta)
+    float *p;          // [record][64][64] scale lower(Q K^T . L)    (backward)
     float *bl;         // [record][64][64] strictlower(K K^T . L)   (backward)
     float *x;          // [record][64][Dv] gradient of the values    (backward)
     float *dstate;     // [record][Dk][Dv] gradient after the chunk  (backward)

@@ -117,7 +117,7 @@ def _forward(op: str, q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, 
     if keep:
         kept_bytes = _bytes(op, lib.ramnet_delta_rule_kept_bytes(*sizes, packed), sizes)
         kept = torch.empty(kept_bytes, dtype=torch.uint8, device=q.device)
-    n = _bytes(op, lib.ramnet_delta_rule_workspace_bytes(*sizes, packed, int(keep)), sizes)
+    n = _bytes(op, lib.ramnet_delta_rule_workspace_bytes(*sizes, _code(q), packed, int(keep)), sizes)
     ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
     if N == 0:
         return o.zero_(), state, kept
@@ -197,7 +197,7 @@ def gated_delta_rule_backward(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: 
         d_state = d_state.to(torch.float32).contiguous()
     grads = [torch.empty(t.shape, dtype=t.dtype, device=q.device) for t in (q, k, v, g, beta)]
     dinit = torch.empty((N, Hv, Dk, Dv), dtype=torch.float32, device=q.device)
-    n = _bytes(op, nat.lib().ramnet_delta_rule_workspace_bytes(*sizes, packed, 2), sizes)
+    n = _bytes(op, nat.lib().ramnet_delta_rule_workspace_bytes(*sizes, _code(q), packed, 2), sizes)
     if N == 0 or T == 0 or B == 0:
         for t in grads:
             t.zero_()
