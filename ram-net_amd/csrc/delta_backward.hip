@@ -93,8 +93,20 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
             o_bits[m] = 16 * (m / 4) + 4 * grp + m % 4 < len ? load_bits(d_o.at(t0, m / 4, m % 4)) : 0u;
         }
     };
-    if (count > 0)
+    // the next chunk's operands are asked for as soon as this one's have been used
+    u32x4 y_hi[kFrags], y_lo[kFrags], p_hi[kFrags], p_lo[kFrags];
+    auto load_frags = [&](const uint32_t *from, int i, u32x4 (&hi)[kFrags], u32x4 (&lo)[kFrags]) {
+        const int64_t record = static_cast<int64_t>(first + i) * job.Hv + head;
+        const u32x4 *at = reinterpret_cast<const u32x4 *>(from + record * 2 * kFragWords);
+#pragma unroll
+        for (int f = 0; f < kFrags; ++f)
+            hi[f] = at[f * kWave + lane], lo[f] = at[(kFrags + f) * kWave + lane];
+    };
+    if (count > 0) {
         load_o(count - 1);
+        load_frags(work.p_frags, count - 1, p_hi, p_lo);
+        load_frags(work.y, count - 1, y_hi, y_lo);
+    }
     __syncthreads();
 
     for (int i = count - 1; i >= 0; --i) {
@@ -103,13 +115,7 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
         const int64_t record = static_cast<int64_t>(first + i) * job.Hv + head;
         const Lds lds = buffer(i);
         const float *vec = lds.vec();
-        const u32x4 *yf = reinterpret_cast<const u32x4 *>(work.y + record * 2 * kFragWords) + lane;
-        const u32x4 *pf = reinterpret_cast<const u32x4 *>(work.p_frags + record * 2 * kFragWords) + lane;
-        u32x4 p_hi[kFrags], p_lo[kFrags];
-#pragma unroll
-        for (int f = 0; f < kFrags; ++f)
-            p_hi[f] = pf[f * kWave], p_lo[f] = pf[(kFrags + f) * kWave];
-        const float total = expf(static_cast<float>(work.gamma[record * C + C - 1]));
+        const float total = vec[kVecGrowK * C + C - 1] * vec[kVecSk * C + C - 1];  // (a power of two: e^gamma_C)
         if (on) {
             const Columns<float> keep(work.dstate + record * job.Dk * job.Dv, job.Dv, grp, cc);
 #pragma unroll
@@ -143,11 +149,9 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
                 }
                 x[m] = x[m] * (load4(vec + kVecInvP * C + 16 * m + 4 * grp) * oo.inverse);
             }
+            if (i > 0)
+                load_frags(work.p_frags, i - 1, p_hi, p_lo);
         }
-        u32x4 y_hi[kFrags], y_lo[kFrags];
-#pragma unroll
-        for (int f = 0; f < kFrags; ++f)
-            y_hi[f] = yf[f * kWave], y_lo[f] = yf[(kFrags + f) * kWave];
         {
             Operand<DT, true> so;
             so.set(s);
@@ -156,7 +160,6 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
                 du[m] = zero;
 #pragma unroll
             for (int b = 0; b < BT; ++b) {
-                __builtin_amdgcn_sched_barrier(0);  // (operands of one block at a time: registers)
 #pragma unroll
                 for (int m = 0; m < 4; ++m) {
                     const u32x4 kf = lds.row_frag(lds.k(0), m, b, lane);
@@ -166,7 +169,6 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
                         du[m] = mfma16(lds.row_frag(lds.k(1), m, b, lane), so.hi[b], du[m]);
                 }
             }
-            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int m = 0; m < 4; ++m)
                 du[m] = (x[m] + du[m] * (load4(vec + kVecLeftK * C + 16 * m + 4 * grp) * so.inverse)) *
@@ -187,6 +189,8 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
                 }
                 x[m] = x[m] * (load4(vec + kVecInvY * C + 16 * m + 4 * grp) * uo.inverse);
             }
+            if (i > 0)
+                load_frags(work.y, i - 1, y_hi, y_lo);
         }
         if (on) {
             const Columns<float> keep(work.x + record * C * job.Dv, job.Dv, grp, cc);
@@ -209,8 +213,6 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
         oo.set(out);
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
-            if (t % 2 == 0)
-                __builtin_amdgcn_sched_barrier(0);
             f32x4 a = zero, z = zero;
 #pragma unroll
             for (int b = 0; b < 2; ++b) {

@@ -43,75 +43,87 @@ __global__ __launch_bounds__(1024) void offsets_kernel(const DeltaJob job, const
     }
 }
 
-// K (or Q) of a chunk in LDS, 64 rows of `pitch` elements as they are, zeros
-// past the last token and Dk.
-template<typename Scalar>
-__device__ __forceinline__ void stage_raw(const Scalar *src, int64_t step, int len, int D, int wide, bool whole,
-                                          Scalar *dst, int pitch) {
-    constexpr int V = 16 / static_cast<int>(sizeof(Scalar));
-    const int pieces = wide / V;
-    for (int i = threadIdx.x; i < kDeltaChunk * pieces; i += 256) {
-        const int t = i / pieces, d = (i - t * pieces) * V;
-        u32x4 x = {0u, 0u, 0u, 0u};
-        if (t < len && d < D) {
-            const Scalar *p = src + t * step + d;
+// The rows of one wave's tile of K (or Q) as matrix operands, 16 bytes of a
+// row a lane and block; zeros past the last token and Dk.
+template<typename Scalar, int DT>
+struct TileRows {
+    static constexpr int kPer = 16 / static_cast<int>(sizeof(Scalar)), kN = 16 * DT / (4 * kPer);
+    u32x4 x[kN];
+
+    __device__ __forceinline__ void load(const Scalar *src, int64_t step, int row, int grp, int len, int D, bool whole) {
+#pragma unroll
+        for (int b = 0; b < kN; ++b) {
+            const int d = (4 * b + grp) * kPer;
+            const Scalar *p = src + row * step + d;
+            x[b] = u32x4{0u, 0u, 0u, 0u};
+            if (row >= len || d >= D)
+                continue;
             if (whole) {
-                x = *reinterpret_cast<const u32x4 *>(p);
+                x[b] = *reinterpret_cast<const u32x4 *>(p);
             } else {
 #pragma unroll
-                for (int e = 0; e < V; ++e)
+                for (int e = 0; e < kPer; ++e)
                     if (d + e < D)
-                        x[e * sizeof(Scalar) / 4] |= load_bits(p + e) << (e * sizeof(Scalar) % 4 * 8);
+                        x[b][e * sizeof(Scalar) / 4] |= load_bits(p + e) << (e * sizeof(Scalar) % 4 * 8);
             }
         }
-        *reinterpret_cast<u32x4 *>(dst + t * pitch + d) = x;
     }
-}
-
-// 16 x 16 of A B^T, rows of `wide` elements in LDS.
-template<typename Scalar>
-__device__ __forceinline__ f32x4 rows_product(const Scalar *a, const Scalar *b, int wide, int grp) {
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    if constexpr (sizeof(Scalar) == 4) {
-        for (int d = 4 * grp; d < wide; d += 16)
-            acc = mfma4(load4(a + d), load4(b + d), acc);
-    } else {
-        for (int d = 8 * grp; d < wide; d += 32) {
-            const u32x4 x = *reinterpret_cast<const u32x4 *>(a + d), y = *reinterpret_cast<const u32x4 *>(b + d);
-            if constexpr (__is_same(Scalar, bf16_t)) {
+    // the largest of each row, in all lanes of it
+    __device__ __forceinline__ float row_max() const {
+        float m = 0.f;
+#pragma unroll
+        for (int b = 0; b < kN; ++b)
+#pragma unroll
+            for (int e = 0; e < kPer; ++e)
+                m = fmaxf(m, fabsf(bits_f32<Scalar>(sizeof(Scalar) == 4 ? x[b][e] : (x[b][e / 2] >> (e % 2 * 16)) & 0xFFFFu)));
+        return column_max(m);
+    }
+    // += this tile times the transpose of the rows at `other` (this lane's row)
+    __device__ __forceinline__ f32x4 times(const Scalar *other, int grp, f32x4 acc) const {
+#pragma unroll
+        for (int b = 0; b < kN; ++b) {
+            const u32x4 y = *reinterpret_cast<const u32x4 *>(other + (4 * b + grp) * kPer);
+            if constexpr (sizeof(Scalar) == 4) {
+                acc = mfma4(__builtin_bit_cast(f32x4, x[b]), __builtin_bit_cast(f32x4, y), acc);
+            } else if constexpr (__is_same(Scalar, bf16_t)) {
                 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y),
-                                                              acc, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x[b]),
+                                                              __builtin_bit_cast(bf16x8, y), acc, 0, 0, 0);
             } else {
-                acc = mfma16(x, y, acc);
+                acc = mfma16(x[b], y, acc);
             }
         }
+        return acc;
     }
-    return acc;
+};
+
+// The largest of 64 values of a row (or column), four threads a row.
+__device__ __forceinline__ float line_max(const float *m, int line, int part, bool column, int pitch) {
+    float x = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+        const int at = 4 * part + 4 * i;  // (pieces of the four threads side by side)
+        const f32x4 v = column ? load4(m + at * pitch + line, pitch) : load4(m + line * pitch + at);
+        x = fmaxf(fmaxf(fmaxf(x, fabsf(v[0])), fmaxf(fabsf(v[1]), fabsf(v[2]))), fabsf(v[3]));
+    }
+    x = fmaxf(x, __shfl_xor(x, 1));
+    return fmaxf(x, __shfl_xor(x, 2));
 }
 
-// The largest of each row of 64 (or of Dk), four threads a row.
-template<typename F>
-__device__ __forceinline__ float quad_max(int tid, int n, F value) {
-    float m = 0.f;
-    for (int i = tid % 4; i < n; i += 4)
-        m = fmaxf(m, fabsf(value(tid / 4, i)));
-    m = fmaxf(m, __shfl_xor(m, 1));
-    return fmaxf(m, __shfl_xor(m, 2));
-}
-
-// Y, P, gamma and the scales of one chunk and value head. Four waves.
-template<typename Scalar>
-__global__ __launch_bounds__(256) void prepare_kernel(const DeltaJob job, const DeltaWork work, int wide, bool backward) {
+// Y, P, gamma and the scales of one chunk and value head: wave w has the
+// tokens of tile w.
+template<typename Scalar, int DT>
+__global__ __launch_bounds__(256) void prepare_kernel(const DeltaJob job, const DeltaWork work, bool backward) {
+    constexpr int C = kDeltaChunk, NP = C + 4, wide = 16 * DT, pitch = wide + 16 / static_cast<int>(sizeof(Scalar));
+    constexpr int kSquare = C * NP, kRows = C * pitch * static_cast<int>(sizeof(Scalar)) / 4;
     extern __shared__ __align__(16) float lds[];
-    constexpr int C = kDeltaChunk, NP = C + 4;
-    const int pitch = wide + 16 / static_cast<int>(sizeof(Scalar));
-    float *nm = lds, *pm = nm + C * NP;
-    Scalar *ks = reinterpret_cast<Scalar *>(pm + C * NP), *qs = ks + C * pitch;
-    float *ys = pm + C * NP;  // (once the keys are done with)
+    float *nm = lds, *pm = nm + kSquare;
+    float *ys = pm + kSquare;  // over the keys, once they are done with
+    Scalar *ks = reinterpret_cast<Scalar *>(ys);
     __shared__ double gam[C];
     __shared__ float beta_s[C], sk_s[C], sq_s[C], scale_y[C], scale_p[C];
     const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave, wave = tid / kWave;
+    const int row = lane & 15, grp = lane >> 4;
     const int chunk = blockIdx.x, head = blockIdx.y, kh = head / (job.Hv / job.Hk);
     const DeltaPlace at = delta_place(job, work, chunk);
     if (at.len == 0) {
@@ -131,88 +143,90 @@ __global__ __launch_bounds__(256) void prepare_kernel(const DeltaJob job, const 
         return;
     }
     const bool whole = rows_whole<Scalar>(job);
-    stage_raw(static_cast<const Scalar *>(job.k) + at.b * job.k_at[0] + at.t0 * job.k_at[1] + kh * job.k_at[2],
-              job.k_at[1], at.len, job.Dk, wide, whole, ks, pitch);
-    stage_raw(static_cast<const Scalar *>(job.q) + at.b * job.q_at[0] + at.t0 * job.q_at[1] + kh * job.q_at[2],
-              job.q_at[1], at.len, job.Dk, wide, whole, qs, pitch);
+    TileRows<Scalar, DT> kt, qt;
+    kt.load(static_cast<const Scalar *>(job.k) + at.b * job.k_at[0] + at.t0 * job.k_at[1] + kh * job.k_at[2], job.k_at[1],
+            16 * wave + row, grp, at.len, job.Dk, whole);
+    qt.load(static_cast<const Scalar *>(job.q) + at.b * job.q_at[0] + at.t0 * job.q_at[1] + kh * job.q_at[2], job.q_at[1],
+            16 * wave + row, grp, at.len, job.Dk, whole);
     const int64_t record = static_cast<int64_t>(chunk) * job.Hv + head;
     if (wave == 0) {
         const int64_t t = at.t0 + lane;
         const bool have = lane < at.len;
         double x = have ? delta_decay(load_code(job.g, job.g_dtype, at.b * job.g_at[0] + t * job.g_at[1] +
                                                 head * job.g_at[2])) : 0.f;
+        beta_s[lane] = have ? load_code(job.beta, job.beta_dtype,
+                                        at.b * job.beta_at[0] + t * job.beta_at[1] + head * job.beta_at[2]) : 0.f;
 #pragma unroll
         for (int m = 1; m < kWave; m <<= 1) {
             const double y = __shfl_up(x, m);
             x += lane >= m ? y : 0.0;
         }
         gam[lane] = x;
-        beta_s[lane] = have ? load_code(job.beta, job.beta_dtype,
-                                        at.b * job.beta_at[0] + t * job.beta_at[1] + head * job.beta_at[2]) : 0.f;
         work.gamma[record * C + lane] = x;
+    }
+#pragma unroll
+    for (int b = 0; b < kt.kN; ++b)
+        *reinterpret_cast<u32x4 *>(ks + (16 * wave + row) * pitch + (4 * b + grp) * kt.kPer) = kt.x[b];
+    // the tokens' scales: fp16 inputs are multiplied as they are
+    {
+        float sk = 1.f, sq = 1.f, inverse;
+        if constexpr (!__is_same(Scalar, _Float16))
+            sk = scale_of(kt.row_max(), inverse), sq = scale_of(qt.row_max(), inverse);
+        if (grp == 0)
+            sk_s[16 * wave + row] = sk, sq_s[16 * wave + row] = sq;
     }
     __syncthreads();
 
-    // the tokens' scales: fp16 inputs are multiplied as they are
-    if constexpr (__is_same(Scalar, _Float16)) {
-        if (tid < C)
-            sk_s[tid] = sq_s[tid] = 1.f;
-    } else {
-        float inverse;
-        const float k_max = quad_max(tid, wide, [&](int t, int d) { return load_f32(ks + t * pitch + d); });
-        const float q_max = quad_max(tid, wide, [&](int t, int d) { return load_f32(qs + t * pitch + d); });
-        if (tid % 4 == 0)
-            sk_s[tid / 4] = scale_of(k_max, inverse), sq_s[tid / 4] = scale_of(q_max, inverse);
-    }
-
-    // K K^T and Q K^T, lower tiles; tile pairs go round the waves
-    const int row = lane & 15, grp = lane >> 4;
+    // K K^T and Q K^T, lower tiles
     float *p_out = backward ? work.p + record * C * C : nullptr, *bl_out = backward ? work.bl + record * C * C : nullptr;
-    for (int tile = wave; tile < 32; tile += 4) {
-        const bool is_p = tile >= 16;
-        const int ti = (tile & 15) >> 2, tj = tile & 3;
-        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-        if (tj <= ti)
-            acc = rows_product((is_p ? qs : ks) + (16 * ti + row) * pitch, ks + (16 * tj + row) * pitch, wide, grp);
+    for (int tj = 0; tj < 4; ++tj) {
+        f32x4 a = {0.f, 0.f, 0.f, 0.f}, p = a;
+        const int j = 16 * tj + row;
+        if (tj <= wave) {
+            a = kt.times(ks + j * pitch, grp, a);
+            p = qt.times(ks + j * pitch, grp, p);
+        }
+        const double gj = gam[j];
+        const float bj = beta_s[j];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int i = 16 * ti + 4 * grp + r, j = 16 * tj + row;
-            const float decay = i >= j ? expf(static_cast<float>(gam[i] - gam[j])) : 0.f;
-            if (is_p) {
-                const float x = i >= j ? job.scale * acc[r] * decay : 0.f;
-                pm[i * NP + j] = backward ? x : x * beta_s[j];
-                if (p_out)
-                    p_out[i * C + j] = x;
-            } else {
-                const float x = i > j ? acc[r] * decay : 0.f;
-                nm[i * NP + j] = x * beta_s[j];
-                if (bl_out)
-                    bl_out[i * C + j] = x;
-            }
+            const int i = 16 * wave + 4 * grp + r;
+            const float decay = i >= j ? expf(static_cast<float>(gam[i] - gj)) : 0.f;
+            const float pij = i >= j ? job.scale * p[r] * decay : 0.f, aij = i > j ? a[r] * decay : 0.f;
+            pm[i * NP + j] = backward ? pij : pij * bj;
+            nm[i * NP + j] = aij * bj;
+            if (backward)
+                p_out[i * C + j] = pij, bl_out[i * C + j] = aij;
         }
     }
     __syncthreads();
-    for (int i = tid; i < C * NP; i += 256)
-        ys[i] = 0.f;
-    __syncthreads();
+    for (int i = tid; i < kSquare / 4; i += 256)
+        reinterpret_cast<f32x4 *>(ys)[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 
     // inverse of the unit lower triangular N: 16-blocks by substitution (lane = column),
     // then pairs of blocks: low part -Yb Nba Ya
     {
+        const float *block = nm + 16 * wave * NP + 16 * wave;
+        f32x4 rows[16][4];
+#pragma unroll
+        for (int i = 1; i < 16; ++i)
+#pragma unroll
+            for (int j = 0; j < i; j += 4)
+                rows[i][j / 4] = load4(block + i * NP + j);
         float x[16];
-        const int o = 16 * wave;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             float sum = i == row ? 1.f : 0.f;
 #pragma unroll
             for (int j = 0; j < i; ++j)
-                sum = fmaf(-nm[(o + i) * NP + o + j], x[j], sum);
+                sum = fmaf(-rows[i][j / 4][j % 4], x[j], sum);
             x[i] = sum;
         }
+        __syncthreads();
         if (grp == 0)
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-                ys[(o + i) * NP + o + row] = x[i];
+                ys[(16 * wave + i) * NP + 16 * wave + row] = x[i];
     }
     __syncthreads();
     if (wave < 2) {
@@ -225,35 +239,32 @@ __global__ __launch_bounds__(256) void prepare_kernel(const DeltaJob job, const 
             ys[(b + 4 * grp + r) * NP + a + row] = -t[r];
     }
     __syncthreads();
-    if (wave < 2) {
-        const int c = 16 * wave;
-        f32x4 t[2];
+    {
+        // wave: row tile wave / 2, column tile wave % 2 of the low 32 x 32
+        const int c = 16 * (wave & 1), i = 32 + 16 * (wave >> 1);
+        f32x4 t[2], low = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            t[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
-                t[i] = mfma4(load4(nm + (32 + 16 * i + row) * NP + 16 * m + 4 * grp),
-                             load4(ys + (16 * m + 4 * grp) * NP + c + row, NP), t[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            f32x4 low = {0.f, 0.f, 0.f, 0.f};
+        for (int h = 0; h < 2; ++h) {
+            t[h] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int m = 0; m < 2; ++m)
-                low = mfma4(load4(ys + (32 + 16 * i + row) * NP + 32 + 16 * m + 4 * grp), t[m], low);
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                ys[(32 + 16 * i + 4 * grp + r) * NP + c + row] = -low[r];
+                t[h] = mfma4(load4(nm + (32 + 16 * h + row) * NP + 16 * m + 4 * grp),
+                             load4(ys + (16 * m + 4 * grp) * NP + c + row, NP), t[h]);
         }
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+            low = mfma4(load4(ys + (i + row) * NP + 32 + 16 * m + 4 * grp), t[m], low);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            ys[(i + 4 * grp + r) * NP + c + row] = -low[r];
     }
     __syncthreads();
 
     // scales of the rows (backward: the columns) of Y and P, and the vectors
     {
         float inverse;
-        const float y_max = quad_max(tid, C, [&](int i, int j) { return backward ? ys[j * NP + i] : ys[i * NP + j]; });
-        const float p_max = quad_max(tid, C, [&](int i, int j) { return backward ? pm[j * NP + i] : pm[i * NP + j]; });
+        const float y_max = line_max(ys, tid / 4, tid % 4, backward, NP);
+        const float p_max = line_max(pm, tid / 4, tid % 4, backward, NP);
         float *vec = work.vec + record * kVecs * C;
         if (tid % 4 == 0) {
             const int i = tid / 4;
@@ -295,7 +306,8 @@ __global__ __launch_bounds__(256) void prepare_kernel(const DeltaJob job, const 
         }
         uint32_t *out = (is_p ? work.p_frags : work.y) + record * 2 * kFragWords + (f * kWave + lane) * 4;
         *reinterpret_cast<u32x4 *>(out) = hi;
-        *reinterpret_cast<u32x4 *>(out + kFragWords) = lo;
+        if (!__is_same(Scalar, bf16_t) || backward || !is_p)  // (what the chains read)
+            *reinterpret_cast<u32x4 *>(out + kFragWords) = lo;
     }
 }
 
@@ -377,8 +389,30 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
             v_bits[m] = 16 * (m / 4) + 4 * grp + m % 4 < len ? load_bits(v.at(t0, m / 4, m % 4)) : 0u;
         }
     };
-    if (count > 0)
+    // the next chunk's operands are asked for as soon as this one's have been used
+    u32x4 y_hi[kFrags], y_lo[kFrags], p_hi[kFrags], p_lo[LO ? kFrags : 1];
+    auto load_y = [&](int i) {
+        const int64_t record = static_cast<int64_t>(first + i) * job.Hv + head;
+        const u32x4 *yf = reinterpret_cast<const u32x4 *>(work.y + record * 2 * kFragWords);
+#pragma unroll
+        for (int f = 0; f < kFrags; ++f)
+            y_hi[f] = yf[f * kWave + lane], y_lo[f] = yf[(kFrags + f) * kWave + lane];
+    };
+    auto load_p = [&](int i) {
+        const int64_t record = static_cast<int64_t>(first + i) * job.Hv + head;
+        const u32x4 *pf = reinterpret_cast<const u32x4 *>(work.p_frags + record * 2 * kFragWords);
+#pragma unroll
+        for (int f = 0; f < kFrags; ++f) {
+            p_hi[f] = pf[f * kWave + lane];
+            if constexpr (LO)
+                p_lo[f] = pf[(kFrags + f) * kWave + lane];
+        }
+    };
+    if (count > 0) {
         load_v(0);
+        load_y(0);
+        load_p(0);
+    }
     __syncthreads();
 
     for (int i = 0; i < count; ++i) {
@@ -387,13 +421,7 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
         const int64_t record = static_cast<int64_t>(first + i) * job.Hv + head;
         const Lds lds = buffer(i);
         const float *vec = lds.vec();
-        const u32x4 *yf = reinterpret_cast<const u32x4 *>(work.y + record * 2 * kFragWords) + lane;
-        const u32x4 *pf = reinterpret_cast<const u32x4 *>(work.p_frags + record * 2 * kFragWords) + lane;
-        u32x4 y_hi[kFrags], y_lo[kFrags];
-#pragma unroll
-        for (int f = 0; f < kFrags; ++f)
-            y_hi[f] = yf[f * kWave], y_lo[f] = yf[(kFrags + f) * kWave];
-        const float total = expf(static_cast<float>(work.gamma[record * C + C - 1]));
+        const float total = vec[kVecGrowK * C + C - 1] * vec[kVecSk * C + C - 1];  // (a power of two: e^gamma_C)
         if (work.states && on) {
             const Columns<float> keep(work.states + record * job.Dk * job.Dv, job.Dv, grp, cc);
 #pragma unroll
@@ -415,7 +443,6 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
                 g[m] = qo[m] = zero;
 #pragma unroll
             for (int b = 0; b < BT; ++b) {
-                __builtin_amdgcn_sched_barrier(0);  // (operands of one block at a time: registers)
 #pragma unroll
                 for (int m = 0; m < 4; ++m) {
                     const u32x4 kf = lds.row_frag(lds.k(0), m, b, lane), qf = lds.row_frag(lds.q(0), m, b, lane);
@@ -430,7 +457,6 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
                     }
                 }
             }
-            __builtin_amdgcn_sched_barrier(0);
         }
         // what the state gives o, and v - S^T k but for the chunk's own tokens
         f32x4 e[4];
@@ -442,19 +468,11 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
             for (int r = 0; r < 4; ++r)
                 g[m][r] = fmaf(-gr[r], g[m][r], bits_f32<Scalar>(v_bits[4 * m + r]));
         }
-        u32x4 p_hi[kFrags], p_lo[LO ? kFrags : 1];
+        if (i + 1 < count)
+            load_v(i + 1);
         {
             Operand<4, true> ro;
             ro.set(g);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int f = 0; f < kFrags; ++f) {
-                p_hi[f] = pf[f * kWave];
-                if constexpr (LO)
-                    p_lo[f] = pf[(kFrags + f) * kWave];
-            }
-            if (i + 1 < count)
-                load_v(i + 1);
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
                 e[m] = zero;
@@ -467,6 +485,8 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
                 }
                 e[m] = e[m] * (load4(vec + kVecInvY * C + 16 * m + 4 * grp) * ro.inverse);
             }
+            if (i + 1 < count)
+                load_y(i + 1);
         }
         if (work.e && on) {
             const Columns<float> keep(work.e + record * C * job.Dv, job.Dv, grp, cc);
@@ -492,12 +512,16 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
                     }
                 }
                 qo[m] = qo[m] + x * (load4(vec + kVecInvP * C + 16 * m + 4 * grp) * eo.inverse);
+            }
+            if (i + 1 < count)
+                load_p(i + 1);  // (before the stores: what waits for it does not wait for them)
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     if (16 * m + 4 * grp + r < len && on)
                         store_f32(o.at(t0, m, r), qo[m][r]);
                 }
-            }
         }
 #pragma unroll
         for (int m = 0; m < 4; ++m)
@@ -506,8 +530,6 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
         wo.set(e);
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
-            if (t % 2 == 0)
-                __builtin_amdgcn_sched_barrier(0);
             f32x4 x = zero;
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
@@ -544,9 +566,18 @@ int padded(int Dk) { return Dk <= 32 ? 32 : Dk <= 64 ? 64 : Dk <= 96 ? 96 : Dk <
 template<typename Scalar>
 hipError_t prepare_typed(const DeltaJob &job, const DeltaWork &work, bool backward, hipStream_t stream) {
     const int wide = padded(job.Dk);
-    const size_t rows = 2 * kDeltaChunk * (wide * sizeof(Scalar) + 16), square = kDeltaChunk * (kDeltaChunk + 4) * sizeof(float);
-    hipLaunchKernelGGL(prepare_kernel<Scalar>, dim3(work.chunks, job.Hv), dim3(256), 2 * square + std::max(rows, square),
-                       stream, job, work, wide, backward);
+    const size_t rows = kDeltaChunk * (wide * sizeof(Scalar) + 16), square = kDeltaChunk * (kDeltaChunk + 4) * sizeof(float);
+#define RAMNET_PREPARE(DT)                                                                                    \
+    if (wide == 16 * DT)                                                                                      \
+        hipLaunchKernelGGL((prepare_kernel<Scalar, DT>), dim3(work.chunks, job.Hv), dim3(256),                \
+                           2 * square + std::max(rows, square), stream, job, work, backward)
+    RAMNET_PREPARE(2);
+    RAMNET_PREPARE(4);
+    RAMNET_PREPARE(6);
+    RAMNET_PREPARE(8);
+    RAMNET_PREPARE(10);
+    RAMNET_PREPARE(16);
+#undef RAMNET_PREPARE
     return hipGetLastError();
 }
 
