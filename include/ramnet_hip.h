@@ -480,7 +480,8 @@ int ramnet_segment_call_form(int64_t B, int64_t H, int64_t T, int64_t A, int64_t
  *   lengths         (B) int32 tokens of each row that count, or NULL: T; the others
  *                   leave the state and have output 0. Not with cu_seqlens.
  *   strides         15: of batch row, token and head in elements, of q, k, v, g, beta
- *                   (last dimensions, o and the states are dense)
+ *                   (last dimensions, o and the states are dense; the tokens of
+ *                   q, k and v lie at least a row and less than 2**22 elements apart)
  *   kept            what ramnet_delta_rule_backward takes of this call
  *                   (ramnet_delta_rule_kept_bytes), or NULL
  *   workspace       ramnet_delta_rule_workspace_bytes, kind 0, or 1 with `kept`

@@ -1135,6 +1135,17 @@ int ramnet_readout_stepwise(const void *y, const void *gate, const void *weight,
     return readout(y, gate, weight, dtype, rows, C, eps, true, out, stream);
 }
 
+// The gated delta rule's chunks lie within int32 bytes of their first token,
+// and the rows of a chunk's matrices apart from each other: a window over its
+// tokens is then a range of addresses.
+constexpr int64_t kDeltaRow = 1LL << 22;
+
+static int check_delta_rows(const char *name, int64_t T, int64_t step, int64_t width) {
+    RAMNET_REQUIRE(T <= 1 || (step >= width && step < kDeltaRow),
+                   std::string("delta rule: tokens of ") + name + " must lie one row to 2**22 elements apart");
+    return RAMNET_OK;
+}
+
 // The gated delta rule's sizes.
 static int check_delta(ramnet::DeltaJob &job, int64_t B, int64_t T, int64_t N, int64_t Hk, int64_t Hv, int64_t Dk, int64_t Dv,
                        bool packed) {
@@ -1144,7 +1155,7 @@ static int check_delta(ramnet::DeltaJob &job, int64_t B, int64_t T, int64_t N, i
     RAMNET_REQUIRE(Dk <= ramnet::kDeltaMaxDk, "delta rule: Dk must be at most 256");
     RAMNET_REQUIRE(packed ? B == 1 : N == B, "delta rule: packed sequences lie in a batch of one, others one to a row");
     // launches and chunk counts are in 32 bits, tensor offsets in 64
-    RAMNET_REQUIRE(Hv <= 65535 && Dv < (1 << 24) && fits_int({B, T, N, B * (T + 64) + N * 64}),
+    RAMNET_REQUIRE(Hv <= 65535 && Dv < kDeltaRow && Hv * Dv < kDeltaRow && fits_int({B, T, N, B * (T + 64) + N * 64}),
                    "delta rule: index overflow");
     job.B = static_cast<int>(B), job.T = static_cast<int>(T), job.N = static_cast<int>(N);
     job.Hk = static_cast<int>(Hk), job.Hv = static_cast<int>(Hv), job.Dk = static_cast<int>(Dk);
@@ -1173,10 +1184,17 @@ int64_t ramnet_delta_rule_kept_bytes(int64_t B, int64_t T, int64_t N, int64_t Hk
     return ramnet::delta_kept(job, packed != 0, nullptr, &work);
 }
 
-static void delta_strides(ramnet::DeltaJob &job, const int64_t *strides) {
+static int delta_strides(ramnet::DeltaJob &job, const int64_t *strides) {
     int64_t *to[5] = {job.q_at, job.k_at, job.v_at, job.g_at, job.beta_at};
     for (int i = 0; i < 15; ++i)
         to[i / 3][i % 3] = strides[i];
+    if (job.T == 1)  // (any, there is no second token)
+        job.q_at[1] = job.k_at[1] = job.Dk, job.v_at[1] = job.Dv;
+    if (int rc = check_delta_rows("q", job.T, job.q_at[1], job.Dk))
+        return rc;
+    if (int rc = check_delta_rows("k", job.T, job.k_at[1], job.Dk))
+        return rc;
+    return check_delta_rows("v", job.T, job.v_at[1], job.Dv);
 }
 
 int ramnet_delta_rule_forward(const void *q, const void *k, const void *v, int dtype, const void *g, int g_dtype,
@@ -1196,7 +1214,8 @@ int ramnet_delta_rule_forward(const void *q, const void *k, const void *v, int d
     job.q = q, job.k = k, job.v = v, job.g = g, job.beta = beta, job.init = init_state, job.state = state, job.o = o;
     job.cu = cu_seqlens, job.lengths = lengths, job.dtype = dtype, job.g_dtype = g_dtype, job.beta_dtype = beta_dtype;
     job.scale = scale;
-    delta_strides(job, strides);
+    if (int rc = delta_strides(job, strides))
+        return rc;
     const char *why = nullptr;
     const hipStream_t on = static_cast<hipStream_t>(stream);
     if (T == 0 || (!kept && ramnet::delta_is_recurrent(job)))
@@ -1232,7 +1251,8 @@ int ramnet_delta_rule_backward(const void *q, const void *k, const void *v, int 
                    "null tensor pointer");
     job.q = q, job.k = k, job.v = v, job.g = g, job.beta = beta, job.cu = cu_seqlens, job.lengths = lengths;
     job.dtype = dtype, job.g_dtype = g_dtype, job.beta_dtype = beta_dtype, job.scale = scale;
-    delta_strides(job, strides);
+    if (int rc = delta_strides(job, strides))
+        return rc;
     ramnet::DeltaWork work{};
     RAMNET_REQUIRE(kept_bytes >= ramnet::delta_kept(job, cu_seqlens != nullptr,
                                                     const_cast<char *>(static_cast<const char *>(kept)), &work),
@@ -1240,7 +1260,10 @@ int ramnet_delta_rule_backward(const void *q, const void *k, const void *v, int 
     RAMNET_REQUIRE(workspace && workspace_bytes >= ramnet::delta_layout(job, cu_seqlens != nullptr, true,
                                                                         static_cast<char *>(workspace), &work),
                    "delta rule: workspace too small");
-    ramnet::DeltaGrads grads{d_o, d_state, dq, dk, dv, dg, dbeta, dinit, {strides[15], strides[16], strides[17]}};
+    ramnet::DeltaGrads grads{d_o, d_state, dq, dk, dv, dg, dbeta, dinit,
+                             {strides[15], T == 1 ? Dv : strides[16], strides[17]}};
+    if (int rc = check_delta_rows("d_o", T, grads.d_o_at[1], Dv))
+        return rc;
     const char *why = nullptr;
     const hipStream_t on = static_cast<hipStream_t>(stream);
     hipError_t err = ramnet::launch_delta_prepare(job, work, true, on, &why);

@@ -69,29 +69,24 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
     }
 
     const int c = (group * 4 + wave) * 16 + row;
-    const bool on = c < job.Dv;
-    const int cc = on ? c : 0;
     const int64_t matrix = (static_cast<int64_t>(n) * job.Hv + head) * job.Dk * job.Dv;
-    const Columns<const float> before(grads.d_state + matrix, job.Dv, grp, cc);
+    const Columns<float> state(job.Dv, job.Dv, grp, c);
     f32x4 s[DT];
-#pragma unroll
-    for (int t = 0; t < DT; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-            s[t][r] = grads.d_state && on && 16 * t + 4 * grp + r < job.Dk ? *before.at(0, t, r) : 0.f;
-    const Columns<const Scalar> d_o(static_cast<const Scalar *>(grads.d_o) + span.b * grads.d_o_at[0] +
-                                    head * grads.d_o_at[2], grads.d_o_at[1], grp, cc);
-    const Columns<Scalar> dv(static_cast<Scalar *>(grads.dv) + (static_cast<int64_t>(span.b) * job.T * job.Hv + head) * job.Dv,
-                             static_cast<int64_t>(job.Hv) * job.Dv, grp, cc);
+    {
+        const auto from = state.rows(grads.d_state + matrix, grads.d_state ? job.Dk : 0);
+        state.each<DT>([&](int t, int r, int at) { s[t][r] = __uint_as_float(buffer_bits<float>(from, at)); });
+    }
+    const Scalar *d_o = static_cast<const Scalar *>(grads.d_o) + span.b * grads.d_o_at[0] + head * grads.d_o_at[2] +
+                        span.t0 * grads.d_o_at[1];
+    const int64_t dv_step = static_cast<int64_t>(job.Hv) * job.Dv;
+    Scalar *dv = static_cast<Scalar *>(grads.dv) + (static_cast<int64_t>(span.b) * job.T + span.t0) * dv_step +
+                 static_cast<int64_t>(head) * job.Dv;
+    const Columns<Scalar> o_cols(grads.d_o_at[1], job.Dv, grp, c), v_cols(dv_step, job.Dv, grp, c);
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
     uint32_t o_bits[16];
     auto load_o = [&](int i) {
-        const int64_t t0 = span.t0 + i * C;
-        const int len = on ? min(C, span.len - i * C) : 0;
-#pragma unroll
-        for (int m = 0; m < 16; ++m) {
-            o_bits[m] = 16 * (m / 4) + 4 * grp + m % 4 < len ? load_bits(d_o.at(t0, m / 4, m % 4)) : 0u;
-        }
+        const auto from = o_cols.rows(d_o + static_cast<int64_t>(i) * C * grads.d_o_at[1], min(C, span.len - i * C));
+        o_cols.template each<4>([&](int m, int r, int at) { o_bits[4 * m + r] = buffer_bits<Scalar>(from, at); });
     };
     // the next chunk's operands are asked for as soon as this one's have been used
     u32x4 y_hi[kFrags], y_lo[kFrags], p_hi[kFrags], p_lo[kFrags];
@@ -110,20 +105,13 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
     __syncthreads();
 
     for (int i = count - 1; i >= 0; --i) {
-        const int64_t t0 = span.t0 + i * C;
-        const int len = min(C, span.len - i * C);
         const int64_t record = static_cast<int64_t>(first + i) * job.Hv + head;
         const Lds lds = buffer(i);
         const float *vec = lds.vec();
         const float total = vec[kVecGrowK * C + C - 1] * vec[kVecSk * C + C - 1];  // (a power of two: e^gamma_C)
-        if (on) {
-            const Columns<float> keep(work.dstate + record * job.Dk * job.Dv, job.Dv, grp, cc);
-#pragma unroll
-            for (int t = 0; t < DT; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (16 * t + 4 * grp + r < job.Dk)
-                        *keep.at(0, t, r) = s[t][r];
+        {
+            const auto to = state.rows(work.dstate + record * job.Dk * job.Dv, job.Dk);
+            state.each<DT>([&](int t, int r, int at) { buffer_store<float>(s[t][r], to, at); });
         }
         f32x4 out[4], du[4], x[4];
 #pragma unroll
@@ -192,16 +180,11 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
             if (i > 0)
                 load_frags(work.y, i - 1, y_hi, y_lo);
         }
-        if (on) {
-            const Columns<float> keep(work.x + record * C * job.Dv, job.Dv, grp, cc);
-#pragma unroll
-            for (int m = 0; m < 4; ++m)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    *keep.at(0, m, r) = x[m][r];
-                    if (16 * m + 4 * grp + r < len)
-                        store_f32(dv.at(t0, m, r), x[m][r]);
-                }
+        {
+            const auto to = state.rows(work.x + record * C * job.Dv, C);
+            state.each<4>([&](int m, int r, int at) { buffer_store<float>(x[m][r], to, at); });
+            const auto out_to = v_cols.rows(dv + static_cast<int64_t>(i) * C * dv_step, min(C, span.len - i * C));
+            v_cols.template each<4>([&](int m, int r, int at) { buffer_store<Scalar>(x[m][r], out_to, at); });
         }
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
@@ -234,20 +217,13 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
         if constexpr (BUFS == 1)
             __syncthreads();  // chunk i - 1 is there
     }
-    if (on) {
-        if (grads.dinit) {
-            const Columns<float> after(grads.dinit + matrix, job.Dv, grp, cc);
-#pragma unroll
-            for (int t = 0; t < DT; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (16 * t + 4 * grp + r < job.Dk)
-                        *after.at(0, t, r) = s[t][r];
-        }
-        if (!job.cu)  // tokens that do not count
-            for (int64_t t = span.len + grp; t < job.T; t += 4)
-                store_f32(dv.base + t * dv.step + cc, 0.f);
+    if (grads.dinit) {
+        const auto to = state.rows(grads.dinit + matrix, job.Dk);
+        state.each<DT>([&](int t, int r, int at) { buffer_store<float>(s[t][r], to, at); });
     }
+    if (!job.cu && c < job.Dv)  // tokens that do not count
+        for (int64_t t = span.len + grp; t < job.T; t += 4)
+            store_f32(dv + t * dv_step + c, 0.f);
 }
 
 // Sum over the 16 lanes of a row group.

@@ -364,30 +364,24 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
     }
 
     const int c = (group * 4 + wave) * 16 + row;
-    const bool on = c < job.Dv;
-    const int cc = on ? c : 0;
     const int64_t matrix = (static_cast<int64_t>(n) * job.Hv + head) * job.Dk * job.Dv;
-    const Columns<const float> before(job.init + matrix, job.Dv, grp, cc);
+    const Columns<float> state(job.Dv, job.Dv, grp, c);
     f32x4 s[DT];
-#pragma unroll
-    for (int t = 0; t < DT; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            s[t][r] = job.init && on && 16 * t + 4 * grp + r < job.Dk ? *before.at(0, t, r) : 0.f;
-        }
-    const Columns<const Scalar> v(static_cast<const Scalar *>(job.v) + span.b * job.v_at[0] + head * job.v_at[2],
-                                  job.v_at[1], grp, cc);
-    const Columns<Scalar> o(static_cast<Scalar *>(job.o) + (static_cast<int64_t>(span.b) * job.T * job.Hv + head) * job.Dv,
-                            static_cast<int64_t>(job.Hv) * job.Dv, grp, cc);
+    {
+        const auto from = state.rows(job.init + matrix, job.init ? job.Dk : 0);
+        state.each<DT>([&](int t, int r, int at) { s[t][r] = __uint_as_float(buffer_bits<float>(from, at)); });
+    }
+    const Scalar *v = static_cast<const Scalar *>(job.v) + span.b * job.v_at[0] + head * job.v_at[2] +
+                      span.t0 * job.v_at[1];
+    const int64_t o_step = static_cast<int64_t>(job.Hv) * job.Dv;
+    Scalar *o = static_cast<Scalar *>(job.o) + (static_cast<int64_t>(span.b) * job.T + span.t0) * o_step +
+                static_cast<int64_t>(head) * job.Dv;
+    const Columns<Scalar> v_cols(job.v_at[1], job.Dv, grp, c), o_cols(o_step, job.Dv, grp, c);
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
     uint32_t v_bits[16];
     auto load_v = [&](int i) {
-        const int64_t t0 = span.t0 + i * C;
-        const int len = on ? min(C, span.len - i * C) : 0;
-#pragma unroll
-        for (int m = 0; m < 16; ++m) {
-            v_bits[m] = 16 * (m / 4) + 4 * grp + m % 4 < len ? load_bits(v.at(t0, m / 4, m % 4)) : 0u;
-        }
+        const auto from = v_cols.rows(v + static_cast<int64_t>(i) * C * job.v_at[1], min(C, span.len - i * C));
+        v_cols.template each<4>([&](int m, int r, int at) { v_bits[4 * m + r] = buffer_bits<Scalar>(from, at); });
     };
     // the next chunk's operands are asked for as soon as this one's have been used
     u32x4 y_hi[kFrags], y_lo[kFrags], p_hi[kFrags], p_lo[LO ? kFrags : 1];
@@ -416,20 +410,13 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
     __syncthreads();
 
     for (int i = 0; i < count; ++i) {
-        const int64_t t0 = span.t0 + i * C;
-        const int len = min(C, span.len - i * C);
         const int64_t record = static_cast<int64_t>(first + i) * job.Hv + head;
         const Lds lds = buffer(i);
         const float *vec = lds.vec();
         const float total = vec[kVecGrowK * C + C - 1] * vec[kVecSk * C + C - 1];  // (a power of two: e^gamma_C)
-        if (work.states && on) {
-            const Columns<float> keep(work.states + record * job.Dk * job.Dv, job.Dv, grp, cc);
-#pragma unroll
-            for (int t = 0; t < DT; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (16 * t + 4 * grp + r < job.Dk)
-                        *keep.at(0, t, r) = s[t][r];
+        if (work.states) {
+            const auto to = state.rows(work.states + record * job.Dk * job.Dv, job.Dk);
+            state.each<DT>([&](int t, int r, int at) { buffer_store<float>(s[t][r], to, at); });
         }
 
         f32x4 g[4], qo[4];
@@ -488,13 +475,9 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
             if (i + 1 < count)
                 load_y(i + 1);
         }
-        if (work.e && on) {
-            const Columns<float> keep(work.e + record * C * job.Dv, job.Dv, grp, cc);
-#pragma unroll
-            for (int m = 0; m < 4; ++m)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    *keep.at(0, m, r) = e[m][r];
+        if (work.e) {
+            const auto to = state.rows(work.e + record * C * job.Dv, C);
+            state.each<4>([&](int m, int r, int at) { buffer_store<float>(e[m][r], to, at); });
         }
         {
             Operand<4, LO> eo;
@@ -515,13 +498,8 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
             }
             if (i + 1 < count)
                 load_p(i + 1);  // (before the stores: what waits for it does not wait for them)
-#pragma unroll
-            for (int m = 0; m < 4; ++m)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    if (16 * m + 4 * grp + r < len && on)
-                        store_f32(o.at(t0, m, r), qo[m][r]);
-                }
+            const auto to = o_cols.rows(o + static_cast<int64_t>(i) * C * o_step, min(C, span.len - i * C));
+            o_cols.template each<4>([&](int m, int r, int at) { buffer_store<Scalar>(qo[m][r], to, at); });
         }
 #pragma unroll
         for (int m = 0; m < 4; ++m)
@@ -547,18 +525,11 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
         if constexpr (BUFS == 1)
             __syncthreads();  // chunk i + 1 is there
     }
-    if (on) {
-        const Columns<float> after(job.state + matrix, job.Dv, grp, cc);
-#pragma unroll
-        for (int t = 0; t < DT; ++t)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (16 * t + 4 * grp + r < job.Dk)
-                    *after.at(0, t, r) = s[t][r];
-        if (!job.cu)  // tokens that do not count
-            for (int64_t t = span.len + grp; t < job.T; t += 4)
-                store_f32(o.base + t * o.step + cc, 0.f);
-    }
+    const auto to = state.rows(job.state + matrix, job.Dk);
+    state.each<DT>([&](int t, int r, int at) { buffer_store<float>(s[t][r], to, at); });
+    if (!job.cu && c < job.Dv)  // tokens that do not count
+        for (int64_t t = span.len + grp; t < job.T; t += 4)
+            store_f32(o + t * o_step + c, 0.f);
 }
 
 int padded(int Dk) { return Dk <= 32 ? 32 : Dk <= 64 ? 64 : Dk <= 96 ? 96 : Dk <= 128 ? 128 : Dk <= 160 ? 160 : 256; }

@@ -92,20 +92,56 @@ __device__ __forceinline__ int operand_at(int k) {
     return (k & ~31) | ((quad < 4 ? 2 * quad : 2 * quad - 7) << 2) | (k & 3);
 }
 
-// A wave's 16 columns of a matrix in memory whose rows are `step` apart: a
-// uniform address for each row of the first lane group, and the lane's offset
-// from it in 32 bits.
+// A window of rows in memory: loads past it give 0, stores past it are dropped.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t window(const void *base, int64_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, static_cast<int>(bytes), kBufWord3);
+}
+
+constexpr int kNowhere = 1 << 30;  // past every window, with any row's offset on top
+
+// A wave's 16 columns of a matrix whose rows are `step` elements apart (at
+// least its width): rows 16 m + 4 (lane / 16) + r, in order of m and r.
 template<typename T>
 struct Columns {
-    T *base;         // of row 0, uniform
-    int64_t step;    // uniform
-    uint32_t lane;   // elements: 4 (lane / 16) rows and the column
+    int lane, step;  // bytes: this lane's first element, and of a row
+    int width;
 
-    __device__ __forceinline__ Columns(T *from, int64_t row_step, int grp, int column)
-        : base(from), step(row_step), lane(static_cast<uint32_t>(4 * grp * row_step) + static_cast<uint32_t>(column)) {}
-    // row 16 m + 4 (lane / 16) + r
-    __device__ __forceinline__ T *at(int64_t row0, int m, int r) const { return base + (row0 + 16 * m + r) * step + lane; }
+    __device__ __forceinline__ Columns(int64_t row_step, int wide, int grp, int column)
+        : step(static_cast<int>(row_step * static_cast<int64_t>(sizeof(T)))), width(wide * static_cast<int>(sizeof(T))) {
+        lane = column < wide ? 4 * grp * step + column * static_cast<int>(sizeof(T)) : kNowhere;
+    }
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows(const T *base, int count) const {
+        return window(base, count > 0 ? static_cast<int64_t>(count - 1) * step + width : 0);
+    }
+    template<int TILES, typename F>
+    __device__ __forceinline__ void each(F f) const {
+        int at = lane;
+        asm volatile("" : "+v"(at));  // (the rows' offsets are made here: kept over a loop they would fill the registers)
+#pragma unroll
+        for (int m = 0; m < TILES; ++m, at += 12 * step)
+#pragma unroll
+            for (int r = 0; r < 4; ++r, at += step)
+                f(m, r, at);
+    }
 };
+
+template<typename T>
+__device__ __forceinline__ uint32_t buffer_bits(__amdgpu_buffer_rsrc_t from, int at) {
+    if constexpr (sizeof(T) == 4)
+        return __builtin_amdgcn_raw_buffer_load_b32(from, at, 0, 0);
+    else
+        return __builtin_amdgcn_raw_buffer_load_b16(from, at, 0, 0);
+}
+
+template<typename T>
+__device__ __forceinline__ void buffer_store(float v, __amdgpu_buffer_rsrc_t to, int at) {
+    if constexpr (sizeof(T) == 4)
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), to, at, 0, 0);
+    else if constexpr (__is_same(T, bf16_t))
+        __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, static_cast<__bf16>(v)), to, at, 0, 0);
+    else
+        __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, static_cast<_Float16>(v)), to, at, 0, 0);
+}
 
 // What prepare leaves per record, 64 values each, for the chain kernels: K and
 // Q are scaled by sk and sq a token, the rows of Y and P (backward: their
@@ -168,33 +204,32 @@ struct Stager {
 
     __device__ __forceinline__ void load_one(const Scalar *src, int64_t step, int len, int Dk, bool whole, int tid,
                                              uint32_t (&to)[kItems][4][kWords]) {
+        constexpr int size = static_cast<int>(sizeof(Scalar));
+        const int pitch = static_cast<int>(step) * size;
+        const auto rows = window(src, len > 0 ? static_cast<int64_t>(len - 1) * pitch + Dk * size : 0);
 #pragma unroll
         for (int n = 0; n < kItems; ++n) {
             const int item = tid + 256 * n, quad = item % 16, d = item / 16 * 8;
+            const int first = d < Dk ? 4 * quad * pitch + d * size : kNowhere;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int t = 4 * quad + e;
-                const bool have = t < len && d < Dk;
-                const Scalar *p = src + t * step + d;
+                const int at = first + e * pitch;
                 if (whole) {  // 16-byte accesses
 #pragma unroll
                     for (int w = 0; w < kWords; w += 4) {
-                        u32x4 x = {0u, 0u, 0u, 0u};
-                        if (have)
-                            x = *reinterpret_cast<const u32x4 *>(reinterpret_cast<const uint32_t *>(p) + w);
+                        const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(rows, at + 4 * w, 0, 0);
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
                             to[n][e][w + i] = x[i];
                     }
-                } else if constexpr (sizeof(Scalar) == 4) {
+                } else {
+                    uint32_t x[8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        to[n][e][i] = have && d + i < Dk ? load_bits(p + i) : 0u;
-                } else {
+                        x[i] = buffer_bits<Scalar>(rows, d + i < Dk ? at + i * size : kNowhere);
 #pragma unroll
-                    for (int i = 0; i < 8; i += 2)
-                        to[n][e][i / 2] = (have && d + i < Dk ? load_bits(p + i) : 0u) |
-                                          (have && d + i + 1 < Dk ? load_bits(p + i + 1) << 16 : 0u);
+                    for (int i = 0; i < kWords; ++i)
+                        to[n][e][i] = size == 4 ? x[i] : x[(2 * i) % 8] | x[(2 * i + 1) % 8] << 16;
                 }
             }
         }

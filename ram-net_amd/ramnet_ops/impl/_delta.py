@@ -73,6 +73,12 @@ def _dense(t: Tensor) -> Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def _rows(t: Tensor) -> Tensor:
+    """t (B, T, H, D) whose heads are dense and whose tokens lie apart, within the kernels' reach."""
+    D, (_, step, _, last) = t.shape[3], t.stride()
+    return t if (last == 1 or D == 1) and (D <= step < 2 ** 22 or t.shape[1] == 1) else t.contiguous()
+
+
 def _whole(t: Tensor | None) -> Tensor | None:
     if t is None or (t.dtype == torch.int32 and t.is_contiguous()):
         return t
@@ -81,7 +87,7 @@ def _whole(t: Tensor | None) -> Tensor | None:
 
 def _args(q, k, v, g, beta, cu_seqlens, lengths):
     """The inputs as the native calls read them."""
-    return _dense(q), _dense(k), _dense(v), g, beta, _whole(cu_seqlens), _whole(lengths)
+    return _rows(q), _rows(k), _rows(v), g, beta, _whole(cu_seqlens), _whole(lengths)
 
 
 def _at(q, k, v, g, beta, *more):
@@ -192,7 +198,7 @@ def gated_delta_rule_backward(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: 
     packed = cu_seqlens is not None
     _check_shapes(op, d_o=(d_o, (B, T, Hv, Dv)), d_state=(d_state, (N, Hv, Dk, Dv)))
     q, k, v, g, beta, cu_seqlens, lengths = _args(q, k, v, g, beta, cu_seqlens, lengths)
-    d_o = _dense(d_o.to(q.dtype))
+    d_o = _rows(d_o.to(q.dtype))
     if d_state is not None:
         d_state = d_state.to(torch.float32).contiguous()
     grads = [torch.empty(t.shape, dtype=t.dtype, device=q.device) for t in (q, k, v, g, beta)]

@@ -80,7 +80,7 @@ def _einval(name, args, match):
 def test_native_delta_rule():
     nat = _native()
     ok = dict(q=FAKE, k=FAKE, v=FAKE, dtype=2, g=FAKE, g_dtype=0, beta=FAKE, beta_dtype=2, init=None, state=FAKE, o=FAKE,
-              cu=None, lengths=None, B=2, T=100, N=2, Hk=2, Hv=4, Dk=64, Dv=64, scale=1.0, strides=nat.strides(*[1] * 18),
+              cu=None, lengths=None, B=2, T=100, N=2, Hk=2, Hv=4, Dk=64, Dv=64, scale=1.0, strides=nat.strides(*[64] * 18),
               kept=None, kept_bytes=0, ws=FAKE, ws_bytes=1 << 30, stream=None)
 
     def call(match, **kw):
@@ -97,12 +97,14 @@ def test_native_delta_rule():
     call("no lengths", B=1, cu=FAKE, lengths=FAKE)
     call("null tensor", q=None)
     call("null tensor", state=None)
+    call("one row to", strides=nat.strides(*[63] * 18))
+    call("one row to", strides=nat.strides(*[1 << 22] * 18))
     call("workspace too small", ws_bytes=16)
     call("workspace too small", ws=None)
     call("kept region too small", kept=FAKE, kept_bytes=16)
     back = dict(q=FAKE, k=FAKE, v=FAKE, dtype=2, g=FAKE, g_dtype=0, beta=FAKE, beta_dtype=2, cu=None, lengths=None,
                 d_o=FAKE, d_state=None, dq=FAKE, dk=FAKE, dv=FAKE, dg=FAKE, dbeta=FAKE, dinit=None, B=2, T=100, N=2,
-                Hk=2, Hv=4, Dk=64, Dv=64, scale=1.0, strides=nat.strides(*[1] * 18), kept=FAKE, kept_bytes=1 << 30,
+                Hk=2, Hv=4, Dk=64, Dv=64, scale=1.0, strides=nat.strides(*[64] * 18), kept=FAKE, kept_bytes=1 << 30,
                 ws=FAKE, ws_bytes=1 << 30, stream=None)
 
     def call_back(match, **kw):
