@@ -1176,10 +1176,11 @@ int64_t ramnet_delta_rule_workspace_bytes(int64_t B, int64_t T, int64_t N, int64
 }
 
 int64_t ramnet_delta_rule_kept_bytes(int64_t B, int64_t T, int64_t N, int64_t Hk, int64_t Hv, int64_t Dk, int64_t Dv,
-                                     int packed) {
+                                     int dtype, int packed) {
     ramnet::DeltaJob job{};
     ramnet::DeltaWork work{};
-    if (check_delta(job, B, T, N, Hk, Hv, Dk, Dv, packed != 0) != RAMNET_OK)
+    job.dtype = dtype;
+    if (!valid_dtype(dtype) || check_delta(job, B, T, N, Hk, Hv, Dk, Dv, packed != 0) != RAMNET_OK)
         return -1;
     return ramnet::delta_kept(job, packed != 0, nullptr, &work);
 }
@@ -1221,8 +1222,11 @@ int ramnet_delta_rule_forward(const void *q, const void *k, const void *v, int d
     if (T == 0 || (!kept && ramnet::delta_is_recurrent(job)))
         return finish(ramnet::launch_delta_recurrent(job, on, &why), why, "delta rule launch");
     ramnet::DeltaWork work{};
-    RAMNET_REQUIRE(!kept || kept_bytes >= ramnet::delta_kept(job, cu_seqlens != nullptr, static_cast<char *>(kept), &work),
-                   "delta rule: kept region too small");
+    if (kept) {
+        const int64_t need = ramnet::delta_kept(job, cu_seqlens != nullptr, static_cast<char *>(kept), &work);
+        RAMNET_REQUIRE(need >= 0, "delta rule: gradients of float32 take Dk up to 160");
+        RAMNET_REQUIRE(kept_bytes >= need, "delta rule: kept region too small");
+    }
     RAMNET_REQUIRE(workspace && workspace_bytes >= ramnet::delta_layout(job, cu_seqlens != nullptr, false,
                                                                         static_cast<char *>(workspace), &work),
                    "delta rule: workspace too small");
@@ -1254,9 +1258,10 @@ int ramnet_delta_rule_backward(const void *q, const void *k, const void *v, int 
     if (int rc = delta_strides(job, strides))
         return rc;
     ramnet::DeltaWork work{};
-    RAMNET_REQUIRE(kept_bytes >= ramnet::delta_kept(job, cu_seqlens != nullptr,
-                                                    const_cast<char *>(static_cast<const char *>(kept)), &work),
-                   "delta rule: kept region too small");
+    const int64_t need = ramnet::delta_kept(job, cu_seqlens != nullptr,
+                                            const_cast<char *>(static_cast<const char *>(kept)), &work);
+    RAMNET_REQUIRE(need >= 0, "delta rule: gradients of float32 take Dk up to 160");
+    RAMNET_REQUIRE(kept_bytes >= need, "delta rule: kept region too small");
     RAMNET_REQUIRE(workspace && workspace_bytes >= ramnet::delta_layout(job, cu_seqlens != nullptr, true,
                                                                         static_cast<char *>(workspace), &work),
                    "delta rule: workspace too small");

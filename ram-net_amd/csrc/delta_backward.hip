@@ -226,12 +226,16 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
             store_f32(dv + t * dv_step + c, 0.f);
 }
 
-// Sum over the 16 lanes of a row group.
+// Sum over the 16 lanes of a row group (rotations within it).
+template<int ROR>
+__device__ __forceinline__ float rotated(float x) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x120 + ROR, 0xF, 0xF, true));
+}
 __device__ __forceinline__ float row_sum(float x) {
-#pragma unroll
-    for (int m = 1; m < 16; m <<= 1)
-        x += __shfl_xor(x, m);
-    return x;
+    x += rotated<8>(x);
+    x += rotated<4>(x);
+    x += rotated<2>(x);
+    return x + rotated<1>(x);
 }
 
 __device__ __forceinline__ void store_code(void *p, int code, int64_t at, float v) {
@@ -243,17 +247,74 @@ __device__ __forceinline__ void store_code(void *p, int code, int64_t at, float 
         store_f32(static_cast<bf16_t *>(p) + at, v);
 }
 
+// Eight values of a row from column v on, zeros from `wide` on; `even`: rows
+// begin at multiples of 16 bytes.
+template<typename Scalar>
+__device__ __forceinline__ void load8(const Scalar *row, int v, int wide, bool have, bool even, float (&x)[8]) {
+    if (even && v + 8 <= wide) {
+        constexpr int kWords = 2 * static_cast<int>(sizeof(Scalar));
+        uint32_t w[kWords] = {};
+        if (have)
+#pragma unroll
+            for (int i = 0; i < kWords; i += 4)
+                *reinterpret_cast<u32x4 *>(w + i) = *reinterpret_cast<const u32x4 *>(
+                    reinterpret_cast<const uint32_t *>(row + v) + i);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            x[e] = bits_f32<Scalar>(sizeof(Scalar) == 4 ? w[e % kWords] : (w[e / 2 % kWords] >> (e % 2 * 16)) & 0xFFFFu);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            x[e] = have && v + e < wide ? load_f32(row + v + e) : 0.f;
+    }
+}
+
+// The fp16 parts of eight values.
+__device__ __forceinline__ void split8(const float (&x)[8], float scale, u32x4 &hi, u32x4 &lo) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        uint32_t h, l;
+        split2(x[2 * w], x[2 * w + 1], scale, h, l);
+        hi[w] = h, lo[w] = l;
+    }
+}
+
+__device__ __forceinline__ float max8(const float (&x)[8], float m) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        m = fmaxf(m, fabsf(x[e]));
+    return m;
+}
+
+// LDS of inputs_back_kernel, in halves: K and Q by element, then 64 columns of
+// dO, X and E by token; where the products of these are done with, the token by
+// token matrices of the second stage take their place.
+template<int DT, int PIECES, bool LO>
+struct BackLds {
+    static constexpr int kSlab = 64, kPitch = kSlab + 8, kPart = kDeltaChunk * kPitch;
+    static constexpr int kCols = 16 * DT * (kDeltaChunk + 8);  // of K or Q, a part
+    static constexpr int kKeys = 2 * PIECES * kCols;
+    static constexpr int kParts = PIECES + 4, kSquares = 3 * (LO ? 2 : 1);
+    static constexpr int kBytes = 2 * (kKeys + kPart * (kParts > kSquares ? kParts : kSquares));
+};
+
 // The other gradients of one chunk and key head; its value heads one after the
-// other, so that a shared head's sums have one order. Wave w has the tokens of
-// tile w.
-template<typename Scalar, int DT>
+// other, so that a shared head's sums have one order. Products over Dv with S
+// and D: a wave has every fourth tile of Dk and all tokens, S and D come from
+// memory straight into its registers, dO, X and E through LDS.
+template<typename Scalar, int DT, int PIECES, bool LO>
 __global__ __launch_bounds__(256) void inputs_back_kernel(const DeltaJob job, const DeltaWork work,
                                                           const DeltaGrads grads) {
-    extern __shared__ __align__(16) float lds[];
-    constexpr int C = kDeltaChunk, wide = 16 * DT, pitch = wide + 4, NP = C + 4;
-    float *ks = lds, *qs = ks + C * pitch, *da = qs + C * pitch, *db = da + C * NP;
+    extern __shared__ __align__(16) float lds_base[];
+    using Lds = BackLds<DT, PIECES, LO>;
+    constexpr int C = kDeltaChunk, TW = (DT + 3) / 4, kPitchT = C + 8;
+    uint16_t *const halves = reinterpret_cast<uint16_t *>(lds_base);
+    uint16_t *const kt = halves, *const qt = halves + PIECES * Lds::kCols, *const parts = halves + Lds::kKeys;
     __shared__ double gam[C];
-    __shared__ float beta_s[C], grow[C], left[C], rows[C], cols[4][C], diag[C], dots[C], state_dot[4];
+    __shared__ float beta_s[C], grow[C], left[C], inv_k[C], inv_q[C];
+    __shared__ float inv_o[C], inv_x[C], inv_e[C];              // of a slab's rows
+    __shared__ float dots[3][4][C];                             // [q, x, e][wave]
+    __shared__ float rows[4][C], cols[4][C], diag[C], state_dot[4], largest[3][4];
     const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave, wave = tid / kWave;
     const int row = lane & 15, grp = lane >> 4;
     const int chunk = blockIdx.x, kh = blockIdx.y, shared = job.Hv / job.Hk;
@@ -295,84 +356,169 @@ __global__ __launch_bounds__(256) void inputs_back_kernel(const DeltaJob job, co
     if (at.len == 0)
         return;
 
-    stage_rows(static_cast<const Scalar *>(job.k) + at.b * job.k_at[0] + at.t0 * job.k_at[1] + kh * job.k_at[2],
-               job.k_at[1], at.len, Dk, wide, ks, pitch);
-    stage_rows(static_cast<const Scalar *>(job.q) + at.b * job.q_at[0] + at.t0 * job.q_at[1] + kh * job.q_at[2],
-               job.q_at[1], at.len, Dk, wide, qs, pitch);
+    {
+        using Keys = Stager<Scalar, DT, PIECES, true>;
+        Keys keys;
+        keys.load(static_cast<const Scalar *>(job.k) + at.b * job.k_at[0] + at.t0 * job.k_at[1] + kh * job.k_at[2],
+                  job.k_at[1],
+                  static_cast<const Scalar *>(job.q) + at.b * job.q_at[0] + at.t0 * job.q_at[1] + kh * job.q_at[2],
+                  job.q_at[1], at.len, Dk, rows_whole<Scalar>(job),
+                  work.vec + (static_cast<int64_t>(chunk) * job.Hv + kh * shared) * kVecs * C, tid);
+        Keys::store_one(keys.raw[0], keys.scales[0], tid, nullptr, kt);
+        Keys::store_one(keys.raw[1], keys.scales[1], tid, nullptr, qt);
+    }
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-    f32x4 sum_q[DT], sum_k[DT];
+    f32x4 sum_q[TW][4], sum_k[TW][4];
 #pragma unroll
-    for (int t = 0; t < DT; ++t)
-        sum_q[t] = sum_k[t] = zero;
+    for (int t = 0; t < TW; ++t)
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+            sum_q[t][m] = sum_k[t][m] = zero;
     const int64_t token0 = static_cast<int64_t>(at.b) * job.T + at.t0;
+    const bool even = Dv % 4 == 0;
+    const bool even_o = Dv % 8 == 0 && reinterpret_cast<uintptr_t>(grads.d_o) % 16 == 0 &&
+                        (grads.d_o_at[0] | grads.d_o_at[1] | grads.d_o_at[2]) % (16 / static_cast<int>(sizeof(Scalar))) == 0;
 
     for (int h = 0; h < shared; ++h) {
         const int head = kh * shared + h;
         const int64_t record = static_cast<int64_t>(chunk) * job.Hv + head;
+        const float *vec = work.vec + record * kVecs * C;
         __syncthreads();
         if (wave == 0) {
             const double own = work.gamma[record * C + lane], end = work.gamma[record * C + C - 1];
             gam[lane] = own;
             grow[lane] = expf(static_cast<float>(own));
             left[lane] = expf(static_cast<float>(end - own));
-            beta_s[lane] = lane < at.len ? load_code(job.beta, job.beta_dtype, at.b * job.beta_at[0] +
-                                                     static_cast<int64_t>(at.t0 + lane) * job.beta_at[1] +
-                                                     head * job.beta_at[2]) : 0.f;
+            beta_s[lane] = vec[kVecBeta * C + lane];
+            inv_k[lane] = 1.f / vec[kVecSk * C + lane];
+            inv_q[lane] = 1.f / vec[kVecSq * C + lane];
         }
-        __syncthreads();
         const float *e = work.e + record * C * Dv, *x = work.x + record * C * Dv;
         const float *s = work.states + record * Dk * Dv, *d = work.dstate + record * Dk * Dv;
         const Scalar *d_o = static_cast<const Scalar *>(grads.d_o) + at.b * grads.d_o_at[0] +
                             at.t0 * grads.d_o_at[1] + head * grads.d_o_at[2];
 
-        // dO S^T, X S^T, E D^T (rows: this wave's tokens) and R1, R2, over Dv
-        const int tok = 16 * wave + row;
-        auto of_row = [&](const float *src, int at_row, int rows_there, int v) {
-            f32x4 f = zero;
-            if (at_row < rows_there) {
-                const float *from = src + static_cast<int64_t>(at_row) * Dv + v;
-                if (v + 4 <= Dv && Dv % 4 == 0)
-                    f = load4(from);
-                else
+        // dO S^T, X S^T, E D^T (this wave's tiles of Dk) and R1, R2 (every fourth lower tile)
+        f32x4 os[TW][4], xs[TW][4], ed[TW][4], r1[3], r2[3];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        f[r] = v + r < Dv ? from[r] : 0.f;
-            }
-            return f;
-        };
-        f32x4 os[DT], xs[DT], ed[DT], r1[4], r2[4];
-#pragma unroll
-        for (int t = 0; t < DT; ++t)
-            os[t] = xs[t] = ed[t] = zero;
-#pragma unroll
-        for (int m = 0; m < 4; ++m)
-            r1[m] = r2[m] = zero;
-        float both = 0.f;
-        for (int v = 4 * grp; v < (Dv + 15) / 16 * 16; v += 16) {
-            f32x4 ao = zero;
-            if (tok < at.len)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    ao[r] = v + r < Dv ? load_f32(d_o + tok * grads.d_o_at[1] + v + r) : 0.f;
-            const f32x4 ax = of_row(x, tok, C, v), ae = of_row(e, tok, C, v);
-#pragma unroll
-            for (int t = 0; t < DT; ++t) {
-                const f32x4 bs = of_row(s, 16 * t + row, Dk, v), bd = of_row(d, 16 * t + row, Dk, v);
-                os[t] = mfma4(ao, bs, os[t]);
-                xs[t] = mfma4(ax, bs, xs[t]);
-                ed[t] = mfma4(ae, bd, ed[t]);
-                if (t % 4 == wave)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        both = fmaf(bs[r], bd[r], both);
-            }
+        for (int t = 0; t < TW; ++t)
 #pragma unroll
             for (int m = 0; m < 4; ++m)
-                if (m <= wave) {
-                    const f32x4 be = of_row(e, 16 * m + row, C, v);
-                    r1[m] = mfma4(ao, be, r1[m]);
-                    r2[m] = mfma4(ax, be, r2[m]);
+                os[t][m] = xs[t][m] = ed[t][m] = zero;
+#pragma unroll
+        for (int n = 0; n < 3; ++n)
+            r1[n] = r2[n] = zero;
+        float both = 0.f;
+        for (int v0 = 0; v0 < Dv; v0 += Lds::kSlab) {
+            if (v0 > 0)
+                __syncthreads();
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const int item = tid + 256 * n, t = item / 8, c = item % 8 * 8;
+                float xo[8], xx[8], xe[8];
+                load8<Scalar>(d_o + t * grads.d_o_at[1], v0 + c, Dv, t < at.len, even_o, xo);
+                load8<float>(x + static_cast<int64_t>(t) * Dv, v0 + c, Dv, true, even, xx);
+                load8<float>(e + static_cast<int64_t>(t) * Dv, v0 + c, Dv, true, even, xe);
+                float mo = max8(xo, 0.f), mx = max8(xx, 0.f), me = max8(xe, 0.f);
+#pragma unroll
+                for (int k = 1; k < 8; k <<= 1) {
+                    mo = fmaxf(mo, __shfl_xor(mo, k));
+                    mx = fmaxf(mx, __shfl_xor(mx, k));
+                    me = fmaxf(me, __shfl_xor(me, k));
                 }
+                float io, ix, ie;
+                const float so = scale_of(mo, io), sx = scale_of(mx, ix), se = scale_of(me, ie);
+                if (item % 8 == 0)
+                    inv_o[t] = io, inv_x[t] = ix, inv_e[t] = ie;
+                u32x4 hi, lo;
+                auto put = [&](int part, u32x4 w) {
+                    *reinterpret_cast<u32x4 *>(parts + part * Lds::kPart + t * Lds::kPitch + c) = w;
+                };
+                split8(xx, sx, hi, lo);
+                put(0, hi), put(1, lo);
+                split8(xe, se, hi, lo);
+                put(2, hi), put(3, lo);
+                split8(xo, so, hi, lo);
+                put(4, hi);
+                if constexpr (PIECES == 2)
+                    put(5, lo);
+            }
+            __syncthreads();
+            auto frag = [&](int part, int tile, int b) {
+                return *reinterpret_cast<const u32x4 *>(parts + part * Lds::kPart + (16 * tile + row) * Lds::kPitch + 32 * b +
+                                                        8 * grp);
+            };
+#pragma unroll
+            for (int tw = 0; tw < TW; ++tw) {
+                const int t = wave + 4 * tw;
+                if (t >= DT)
+                    continue;
+                float sv[2][8], dv[2][8], s_max = 0.f, d_max = 0.f;
+                const int at_row = 16 * t + row;
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const int v = v0 + 32 * b + 8 * grp;
+                    load8<float>(s + static_cast<int64_t>(at_row) * Dv, v, Dv, at_row < Dk, even, sv[b]);
+                    load8<float>(d + static_cast<int64_t>(at_row) * Dv, v, Dv, at_row < Dk, even, dv[b]);
+                    s_max = max8(sv[b], s_max), d_max = max8(dv[b], d_max);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        both = fmaf(sv[b][k], dv[b][k], both);
+                }
+                float s_inv, d_inv;
+                const float s_scale = scale_of(column_max(s_max), s_inv), d_scale = scale_of(column_max(d_max), d_inv);
+                u32x4 s_hi[2], s_lo[2], d_hi[2], d_lo[2];
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    split8(sv[b], s_scale, s_hi[b], s_lo[b]);
+                    split8(dv[b], d_scale, d_hi[b], d_lo[b]);
+                }
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {
+                    f32x4 a = zero, z = zero, w = zero;
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        const u32x4 fo = frag(4, m, b), fx = frag(0, m, b), fxl = frag(1, m, b), fe = frag(2, m, b),
+                                    fel = frag(3, m, b);
+                        a = mfma16(fo, s_hi[b], a);
+                        z = mfma16(fx, s_hi[b], z);
+                        w = mfma16(fe, d_hi[b], w);
+                        a = mfma16(fo, s_lo[b], a);
+                        z = mfma16(fx, s_lo[b], z);
+                        w = mfma16(fe, d_lo[b], w);
+                        if constexpr (PIECES == 2)
+                            a = mfma16(frag(5, m, b), s_hi[b], a);
+                        z = mfma16(fxl, s_hi[b], z);
+                        w = mfma16(fel, d_hi[b], w);
+                    }
+                    const int i = 16 * m + 4 * grp;
+                    os[tw][m] += a * (load4(inv_o + i) * s_inv);
+                    xs[tw][m] += z * (load4(inv_x + i) * s_inv);
+                    ed[tw][m] += w * (load4(inv_e + i) * d_inv);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < 3; ++n) {
+                const int tile = wave + 4 * n;  // (0,0) (1,0) (1,1) (2,0) ...
+                if (tile >= 10)
+                    continue;
+                const int ti = tile >= 6 ? 3 : tile >= 3 ? 2 : tile >= 1 ? 1 : 0, tj = tile - ti * (ti + 1) / 2;
+                f32x4 a = zero, z = zero;
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const u32x4 fo = frag(4, ti, b), fx = frag(0, ti, b), fe = frag(2, tj, b), fel = frag(3, tj, b);
+                    a = mfma16(fo, fe, a);
+                    z = mfma16(fx, fe, z);
+                    a = mfma16(fo, fel, a);
+                    z = mfma16(fx, fel, z);
+                    if constexpr (PIECES == 2)
+                        a = mfma16(frag(5, ti, b), fe, a);
+                    z = mfma16(frag(1, ti, b), fe, z);
+                }
+                const float ie = inv_e[16 * tj + row];
+                r1[n] += a * (load4(inv_o + 16 * ti + 4 * grp) * ie);
+                r2[n] += z * (load4(inv_x + 16 * ti + 4 * grp) * ie);
+            }
         }
         both = row_sum(both);
         both += __shfl_xor(both, 16);
@@ -381,73 +527,105 @@ __global__ __launch_bounds__(256) void inputs_back_kernel(const DeltaJob job, co
             state_dot[wave] = both;
 
         // with the rows of Q and K: what e^gamma and e^(gamma_C - gamma) multiply
-        const f32x4 gr = load4(grow + 16 * wave + 4 * grp), le = load4(left + 16 * wave + 4 * grp);
-        const f32x4 be = load4(beta_s + 16 * wave + 4 * grp);
-        f32x4 q_dot = zero, x_dot = zero, e_dot = zero;
 #pragma unroll
-        for (int t = 0; t < DT; ++t)
+        for (int m = 0; m < 4; ++m) {
+            const int i = 16 * m + 4 * grp;
+            const f32x4 gr = load4(grow + i), le = load4(left + i) * load4(beta_s + i);
+            const f32x4 ik = load4(inv_k + i), iq = load4(inv_q + i);
+            f32x4 q_dot = zero, x_dot = zero, e_dot = zero;
+#pragma unroll
+            for (int tw = 0; tw < TW; ++tw) {
+                const int t = wave + 4 * tw;
+                if (t >= DT)
+                    continue;
+                const int place = (16 * t + row) * kPitchT + operand_at(i);
+                f32x4 qv = zero, kv = zero;
+#pragma unroll
+                for (int p = 0; p < PIECES; ++p)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        kv[r] += static_cast<float>(__builtin_bit_cast(_Float16, kt[p * Lds::kCols + place + r]));
+                        qv[r] += static_cast<float>(__builtin_bit_cast(_Float16, qt[p * Lds::kCols + place + r]));
+                    }
+                q_dot += qv * os[tw][m];
+                x_dot += kv * xs[tw][m];
+                e_dot += kv * ed[tw][m];
+                sum_q[tw][m] += (job.scale * gr) * os[tw][m];
+                sum_k[tw][m] += le * ed[tw][m] - gr * xs[tw][m];
+            }
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float kv = ks[(16 * wave + 4 * grp + r) * pitch + 16 * t + row];
-                const float qv = qs[(16 * wave + 4 * grp + r) * pitch + 16 * t + row];
-                q_dot[r] = fmaf(qv, os[t][r], q_dot[r]);
-                x_dot[r] = fmaf(kv, xs[t][r], x_dot[r]);
-                e_dot[r] = fmaf(kv, ed[t][r], e_dot[r]);
-                sum_q[t][r] = fmaf(job.scale * gr[r], os[t][r], sum_q[t][r]);
-                sum_k[t][r] += le[r] * be[r] * ed[t][r] - gr[r] * xs[t][r];
+                const float a = row_sum(q_dot[r] * iq[r]), b = row_sum(x_dot[r] * ik[r]), w = row_sum(e_dot[r] * ik[r]);
+                if (row == 0)
+                    dots[0][wave][i + r] = a, dots[1][wave][i + r] = b, dots[2][wave][i + r] = w;
             }
-        f32x4 own = zero, last = zero;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            own[r] = gr[r] * (job.scale * row_sum(q_dot[r]) - row_sum(x_dot[r]));
-            last[r] = le[r] * row_sum(e_dot[r]);
         }
 
         // R1 and R2 with L: dA, dB, and their sums
         const float *p = work.p + record * C * C, *bl = work.bl + record * C * C;
-        f32x4 of_rows = zero;
+        float a_max = 0.f, t_max = 0.f, b_max = 0.f;
+        // from here on r1 is dA and r2 dB, without the scales of K and Q
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
+        for (int n = 0; n < 3; ++n) {
+            const int tile = wave + 4 * n;
+            if (tile >= 10)
+                continue;
+            const int ti = tile >= 6 ? 3 : tile >= 3 ? 2 : tile >= 1 ? 1 : 0, tj = tile - ti * (ti + 1) / 2;
+            const int j = 16 * tj + row;
             float of_cols = 0.f;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int i = 16 * wave + 4 * grp + r, j = 16 * m + row;
+                const int i = 16 * ti + 4 * grp + r;
                 float a = 0.f, b = 0.f, both_ij = 0.f;
                 if (i >= j) {
                     const float decay = expf(static_cast<float>(gam[i] - gam[j])) * beta_s[j];
-                    a = job.scale * decay * r1[m][r];
-                    b = i > j ? -decay * r2[m][r] : 0.f;
-                    both_ij = p[i * C + j] * r1[m][r] - bl[i * C + j] * r2[m][r];
+                    a = job.scale * decay * r1[n][r];
+                    b = i > j ? -decay * r2[n][r] : 0.f;
+                    both_ij = p[i * C + j] * r1[n][r] - bl[i * C + j] * r2[n][r];
                     if (i == j)
-                        diag[i] = both_ij;
-                    else
-                        of_cols += both_ij;
+                        diag[i] = both_ij, both_ij = 0.f;
                 }
-                da[i * NP + j] = a;
-                db[i * NP + j] = b;
-                of_rows[r] += i > j ? both_ij * beta_s[j] : 0.f;
+                of_cols += both_ij;
+                const float of_rows = row_sum(both_ij * beta_s[j]);
+                if (row == 0)
+                    rows[tj][i] = of_rows;
+                r1[n][r] = a, r2[n][r] = b;
+                a_max = fmaxf(a_max, fabsf(a * inv_k[j]));
+                t_max = fmaxf(t_max, fabsf(a * inv_q[i]));
+                b_max = fmaxf(b_max, fmaxf(fabsf(b * inv_k[j]), fabsf(b * inv_k[i])));
             }
             of_cols += __shfl_xor(of_cols, 16);
             of_cols += __shfl_xor(of_cols, 32);
             if (grp == 0)
-                cols[wave][16 * m + row] = of_cols;
+                cols[ti][j] = of_cols;
         }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const float sum = row_sum(of_rows[r]);
-            if (row == 0) {
-                rows[16 * wave + 4 * grp + r] = own[r] + sum;
-                dots[16 * wave + 4 * grp + r] = last[r];
-            }
+        for (int k = 1; k < 16; k <<= 1) {
+            a_max = fmaxf(a_max, __shfl_xor(a_max, k));
+            t_max = fmaxf(t_max, __shfl_xor(t_max, k));
+            b_max = fmaxf(b_max, __shfl_xor(b_max, k));
         }
+        a_max = column_max(a_max), t_max = column_max(t_max), b_max = column_max(b_max);
+        if (lane == 0)
+            largest[0][wave] = a_max, largest[1][wave] = t_max, largest[2][wave] = b_max;
         __syncthreads();
         if (wave == 0) {
-            const float strict = cols[0][lane] + cols[1][lane] + cols[2][lane] + cols[3][lane];
-            const float beta = beta_s[lane];
-            const float h = beta * dots[lane];
+            float strict = 0.f, of_rows = 0.f;
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                strict += m >= lane / 16 ? cols[m][lane] : 0.f;
+                of_rows += m <= lane / 16 ? rows[m][lane] : 0.f;
+            }
+            float q_dot = 0.f, x_dot = 0.f, e_dot = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+                q_dot += dots[0][w][lane], x_dot += dots[1][w][lane], e_dot += dots[2][w][lane];
+            const float beta = beta_s[lane], last = left[lane] * e_dot, held = beta * last;
+            const float own = grow[lane] * (job.scale * q_dot - x_dot);
             // decays' sums from the end: 64 bits, their terms cancel
-            double part = static_cast<double>(rows[lane]) - static_cast<double>(beta * strict) - static_cast<double>(h);
-            double all = h;
+            double part = static_cast<double>(own) + static_cast<double>(of_rows) - static_cast<double>(beta * strict) -
+                          static_cast<double>(held);
+            double all = held;
 #pragma unroll
             for (int m = 1; m < kWave; m <<= 1) {
                 const double y = __shfl_down(part, m);
@@ -459,43 +637,114 @@ __global__ __launch_bounds__(256) void inputs_back_kernel(const DeltaJob job, co
             if (lane < at.len) {
                 const int64_t out = (token0 + lane) * job.Hv + head;
                 store_code(grads.dg, job.g_dtype, out, static_cast<float>(part + all));
-                store_code(grads.dbeta, job.beta_dtype, out, strict + diag[lane] + dots[lane]);
+                store_code(grads.dbeta, job.beta_dtype, out, strict + diag[lane] + last);
             }
         }
-        // dA K, dA^T Q, (dB + dB^T) K
+        // dA, dA^T and dB + dB^T as operands, K's and Q's scales taken out of their columns
+        float a_inv, t_inv, b_inv;
+        auto all_max = [&](int k) { return fmaxf(fmaxf(largest[k][0], largest[k][1]), fmaxf(largest[k][2], largest[k][3])); };
+        const float a_scale = scale_of(all_max(0), a_inv), t_scale = scale_of(all_max(1), t_inv),
+                    b_scale = scale_of(all_max(2), b_inv);
+        auto put = [&](int matrix, int i, int j, float v, float scale) {
+            const _Float16 hi = static_cast<_Float16>(v * scale);
+            uint16_t *to = parts + matrix * Lds::kPart + i * Lds::kPitch + operand_at(j);
+            *to = __builtin_bit_cast(uint16_t, hi);
+            if constexpr (LO)
+                to[3 * Lds::kPart] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(fmaf(v, scale, -static_cast<float>(hi))));
+        };
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const f32x4 qa = load4(da + (16 * wave + row) * NP + 16 * j + 4 * grp);
-            const f32x4 ka = load4(db + (16 * wave + row) * NP + 16 * j + 4 * grp);
-            const f32x4 qt = load4(da + (16 * j + 4 * grp) * NP + 16 * wave + row, NP);
-            const f32x4 kt = ka + load4(db + (16 * j + 4 * grp) * NP + 16 * wave + row, NP);
+        for (int n = 0; n < 3; ++n) {
+            const int tile = wave + 4 * n;
+            if (tile >= 10)
+                continue;
+            const int ti = tile >= 6 ? 3 : tile >= 3 ? 2 : tile >= 1 ? 1 : 0, tj = tile - ti * (ti + 1) / 2;
+            const int j = 16 * tj + row;
 #pragma unroll
-            for (int t = 0; t < DT; ++t) {
-                const f32x4 kb = load4(ks + (16 * j + 4 * grp) * pitch + 16 * t + row, pitch);
-                sum_q[t] = mfma4(qa, kb, sum_q[t]);
-                sum_k[t] = mfma4(kt, kb, sum_k[t]);
-                sum_k[t] = mfma4(qt, load4(qs + (16 * j + 4 * grp) * pitch + 16 * t + row, pitch), sum_k[t]);
+            for (int r = 0; r < 4; ++r) {
+                const int i = 16 * ti + 4 * grp + r;
+                const float a = r1[n][r], b = r2[n][r];
+                put(0, i, j, a * inv_k[j], a_scale);
+                put(1, j, i, a * inv_q[i], t_scale);
+                if (ti != tj) {
+                    put(2, i, j, b * inv_k[j], b_scale);
+                    put(2, j, i, b * inv_k[i], b_scale);
+                    put(0, j, i, 0.f, 0.f);
+                    put(1, i, j, 0.f, 0.f);
+                } else if (i >= j) {
+                    put(2, i, j, b * inv_k[j], b_scale);
+                    if (i > j)
+                        put(2, j, i, b * inv_k[i], b_scale);
+                }
+            }
+        }
+        __syncthreads();
+        auto square = [&](int matrix, int tile, int b) {
+            return *reinterpret_cast<const u32x4 *>(parts + matrix * Lds::kPart + (16 * tile + row) * Lds::kPitch + 32 * b +
+                                                    8 * grp);
+        };
+#pragma unroll
+        for (int tw = 0; tw < TW; ++tw) {
+            const int t = wave + 4 * tw;
+            if (t >= DT)
+                continue;
+            u32x4 kf[PIECES][2], qf[PIECES][2];
+#pragma unroll
+            for (int n = 0; n < PIECES; ++n)
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const int place = n * Lds::kCols + (16 * t + row) * kPitchT + 32 * b + 8 * grp;
+                    kf[n][b] = *reinterpret_cast<const u32x4 *>(kt + place);
+                    qf[n][b] = *reinterpret_cast<const u32x4 *>(qt + place);
+                }
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                f32x4 a = zero, z = zero, w = zero;
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    auto product = [&](int matrix, const u32x4 (&f)[PIECES][2], f32x4 acc) {
+                        const u32x4 hi = square(matrix, m, b);
+                        acc = mfma16(hi, f[0][b], acc);
+                        if constexpr (LO)
+                            acc = mfma16(square(matrix + 3, m, b), f[0][b], acc);
+                        if constexpr (PIECES == 2)
+                            acc = mfma16(hi, f[PIECES - 1][b], acc);
+                        return acc;
+                    };
+                    if (b <= m / 2)
+                        a = product(0, kf, a);
+                    if (b >= m / 2)
+                        z = product(1, qf, z);
+                    w = product(2, kf, w);
+                }
+                sum_q[tw][m] += a * a_inv;
+                sum_k[tw][m] += z * t_inv + w * b_inv;
             }
         }
     }
 #pragma unroll
-    for (int t = 0; t < DT; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int i = 16 * wave + 4 * grp + r, d = 16 * t + row;
-            if (i < at.len && d < Dk) {
-                store_f32(dq + (token0 + i) * dk_step + d, sum_q[t][r]);
-                store_f32(dk + (token0 + i) * dk_step + d, sum_k[t][r]);
-            }
-        }
+    for (int tw = 0; tw < TW; ++tw) {
+        const int t = wave + 4 * tw;
+        if (t >= DT)
+            continue;
+        const Columns<Scalar> to(dk_step, Dk, grp, 16 * t + row);
+        const auto q_rows = to.rows(dq + token0 * dk_step, at.len), k_rows = to.rows(dk + token0 * dk_step, at.len);
+        to.template each<4>([&](int m, int r, int place) {
+            buffer_store<Scalar>(sum_q[tw][m][r], q_rows, place);
+            buffer_store<Scalar>(sum_k[tw][m][r], k_rows, place);
+        });
+    }
 }
+
+// Whether a chunk's operands and the gradients' products fit the LDS.
+template<int DT, int PIECES>
+constexpr bool delta_trains = ChunkLds<DT, PIECES, true>::kBytes <= kLdsBytes &&
+                              BackLds<DT, PIECES, true>::kBytes + 8192 <= kLdsBytes;
+static_assert(delta_trains<16, 1> && delta_trains<10, 2> && !delta_trains<16, 2>);  // as delta_kept has it
 
 template<typename Scalar>
 hipError_t backward_typed(const DeltaJob &job, const DeltaWork &work, const DeltaGrads &grads, hipStream_t stream,
                           const char **why) {
-    constexpr int C = kDeltaChunk;
-    const int wide = job.Dk <= 32 ? 32 : job.Dk <= 64 ? 64 : job.Dk <= 96 ? 96 : job.Dk <= 128 ? 128
-                     : job.Dk <= 160 ? 160 : 256;
+    const int wide = delta_padded(job.Dk);
     const int groups = (job.Dv + 63) / 64;
     const int64_t blocks = static_cast<int64_t>(job.N) * job.Hv * groups;
     if (blocks > 0x7fffffff) {
@@ -503,23 +752,26 @@ hipError_t backward_typed(const DeltaJob &job, const DeltaWork &work, const Delt
         return hipErrorInvalidValue;
     }
     constexpr int PIECES = sizeof(Scalar) == 4 ? 2 : 1;
-    const size_t bytes = (2 * C * (wide + 4) + 2 * C * (C + 4)) * sizeof(float);
-#define RAMNET_BACK(DT)                                                                                              \
-    if (wide == 16 * DT) {                                                                                           \
-        constexpr int each = ChunkLds<DT, PIECES, true>::kBytes, bufs = 2 * each <= kLdsBytes ? 2 : 1;               \
-        static_assert(each <= kLdsBytes);                                                                            \
-        hipLaunchKernelGGL((chain_back_kernel<Scalar, DT, PIECES, bufs>), dim3(static_cast<unsigned>(blocks)),       \
-                           dim3(512), bufs * each, stream, job, work, grads, groups);                                \
-        if (const hipError_t err = hipGetLastError())                                                                \
-            return err;                                                                                              \
-        hipLaunchKernelGGL((inputs_back_kernel<Scalar, DT>), dim3(work.chunks, job.Hk), dim3(256), bytes, stream,    \
-                           job, work, grads);                                                                        \
+    constexpr bool LO = !__is_same(Scalar, bf16_t);
+#define RAMNET_BACK(DT)                                                                                            \
+    if constexpr (delta_trains<DT, PIECES>) {                                                                      \
+        if (wide == 16 * DT) {                                                                                     \
+            constexpr int each = ChunkLds<DT, PIECES, true>::kBytes, bufs = 2 * each <= kLdsBytes ? 2 : 1;         \
+            constexpr int back = BackLds<DT, PIECES, LO>::kBytes;                                                  \
+            hipLaunchKernelGGL((chain_back_kernel<Scalar, DT, PIECES, bufs>), dim3(static_cast<unsigned>(blocks)), \
+                               dim3(512), bufs * each, stream, job, work, grads, groups);                          \
+            if (const hipError_t err = hipGetLastError())                                                          \
+                return err;                                                                                        \
+            hipLaunchKernelGGL((inputs_back_kernel<Scalar, DT, PIECES, LO>), dim3(work.chunks, job.Hk), dim3(256), \
+                               back, stream, job, work, grads);                                                    \
+        }                                                                                                          \
     }
     RAMNET_BACK(2)
     RAMNET_BACK(4)
     RAMNET_BACK(6)
     RAMNET_BACK(8)
     RAMNET_BACK(10)
+    RAMNET_BACK(16)
 #undef RAMNET_BACK
     return hipGetLastError();
 }

@@ -532,11 +532,10 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
             store_f32(o + t * o_step + c, 0.f);
 }
 
-int padded(int Dk) { return Dk <= 32 ? 32 : Dk <= 64 ? 64 : Dk <= 96 ? 96 : Dk <= 128 ? 128 : Dk <= 160 ? 160 : 256; }
 
 template<typename Scalar>
 hipError_t prepare_typed(const DeltaJob &job, const DeltaWork &work, bool backward, hipStream_t stream) {
-    const int wide = padded(job.Dk);
+    const int wide = delta_padded(job.Dk);
     const size_t rows = kDeltaChunk * (wide * sizeof(Scalar) + 16), square = kDeltaChunk * (kDeltaChunk + 4) * sizeof(float);
 #define RAMNET_PREPARE(DT)                                                                                    \
     if (wide == 16 * DT)                                                                                      \
@@ -567,7 +566,7 @@ void chain_launch(const DeltaJob &job, const DeltaWork &work, unsigned blocks, i
 
 template<typename Scalar>
 hipError_t chain_typed(const DeltaJob &job, const DeltaWork &work, hipStream_t stream, const char **why) {
-    const int wide = padded(job.Dk), groups = (job.Dv + 63) / 64;
+    const int wide = delta_padded(job.Dk), groups = (job.Dv + 63) / 64;
     const int64_t blocks = static_cast<int64_t>(job.N) * job.Hv * groups;
     if (blocks > 0x7fffffff) {
         *why = "delta rule: too many state columns for one launch";
@@ -592,7 +591,7 @@ hipError_t chain_typed(const DeltaJob &job, const DeltaWork &work, hipStream_t s
 // Short calls, and those whose chunks (two fp16 parts of each fp32 key and
 // query) do not fit the LDS.
 bool delta_is_recurrent(const DeltaJob &job) {
-    return job.T <= 32 || (job.dtype == kF32 && padded(job.Dk) > 160);
+    return job.T <= 32 || (job.dtype == kF32 && delta_padded(job.Dk) > 160);
 }
 
 namespace {
@@ -636,6 +635,8 @@ int64_t delta_layout(const DeltaJob &job, bool packed, bool backward, char *base
 }
 
 int64_t delta_kept(const DeltaJob &job, bool packed, char *base, DeltaWork *work) {
+    if (job.dtype == kF32 && delta_padded(job.Dk) > 160)
+        return -1;
     count_chunks(job, packed, work);
     Carver carve{base};
     const int64_t records = static_cast<int64_t>(work->chunks) * job.Hv;

@@ -75,6 +75,11 @@ __device__ __forceinline__ DeltaSpan delta_span(const DeltaJob &job, int n) {
     return {n, 0, job.lengths ? min(max(job.lengths[n], 0), job.T) : job.T};
 }
 
+// Dk as the chunked kernels are built for it.
+inline int delta_padded(int Dk) {
+    return Dk <= 32 ? 32 : Dk <= 64 ? 64 : Dk <= 96 ? 96 : Dk <= 128 ? 128 : Dk <= 160 ? 160 : 256;
+}
+
 // A decay of one step. e^-200 is 0 in fp32 as e^-inf is; held there, sums of
 // decays stay finite and differences of them free of inf - inf. (A NaN stays.)
 __device__ __forceinline__ float delta_decay(float g) { return g < -200.f ? -200.f : g; }

@@ -137,7 +137,7 @@ SIGNATURES: dict[str, tuple[type, list]] = {
         _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_float,
         _c_i64s, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr]),
     "ramnet_delta_rule_workspace_bytes": (_c_i64, [_c_i64] * 7 + [_c_int] * 3),
-    "ramnet_delta_rule_kept_bytes": (_c_i64, [_c_i64] * 7 + [_c_int]),
+    "ramnet_delta_rule_kept_bytes": (_c_i64, [_c_i64] * 7 + [_c_int] * 2),
     "ramnet_verify_drafts": (_c_int, [
         _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64s, _c_ptr, _c_ptr,
         _c_ptr]),

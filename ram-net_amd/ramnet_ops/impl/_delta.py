@@ -100,7 +100,7 @@ def _at(q, k, v, g, beta, *more):
 def _bytes(op: str, count: int, sizes) -> int:
     if count < 0:
         raise RuntimeError(f"{op}: sizes (B, T, N, Hk, Hv, Dk, Dv) = {tuple(sizes)} are not supported "
-                           "(Dk up to 256, tokens within int32)")
+                           "(Dk up to 256, up to 160 for gradients of float32; tokens within int32)")
     return count
 
 
@@ -121,7 +121,7 @@ def _forward(op: str, q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, 
     kept = None
     kept_bytes = 0
     if keep:
-        kept_bytes = _bytes(op, lib.ramnet_delta_rule_kept_bytes(*sizes, packed), sizes)
+        kept_bytes = _bytes(op, lib.ramnet_delta_rule_kept_bytes(*sizes, _code(q), packed), sizes)
         kept = torch.empty(kept_bytes, dtype=torch.uint8, device=q.device)
     n = _bytes(op, lib.ramnet_delta_rule_workspace_bytes(*sizes, _code(q), packed, int(keep)), sizes)
     ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
@@ -183,7 +183,7 @@ def gated_delta_rule_kept(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tens
 def _(q, k, v, g, beta, init_state, cu_seqlens, lengths, scale):
     B, T, Hk, Dk = q.shape
     N = B if cu_seqlens is None else cu_seqlens.shape[0] - 1
-    n = nat.lib().ramnet_delta_rule_kept_bytes(B, T, N, Hk, v.shape[2], Dk, v.shape[3], cu_seqlens is not None)
+    n = nat.lib().ramnet_delta_rule_kept_bytes(B, T, N, Hk, v.shape[2], Dk, v.shape[3], _code(q), cu_seqlens is not None)
     return *_out_shapes(q, k, v, cu_seqlens), q.new_empty((n,), dtype=torch.uint8)
 
 

@@ -112,11 +112,14 @@ def test_native_delta_rule():
     call_back("needs tokens", T=0)
     call_back("null tensor", dg=None)
     call_back("kept region too small", kept_bytes=16)
+    call_back("Dk up to 160", dtype=0, Dk=200, strides=nat.strides(*[256] * 18))
     call_back("workspace too small", ws_bytes=16)
     lib = nat.lib()
     assert lib.ramnet_delta_rule_workspace_bytes(2, 100, 2, 2, 4, 300, 64, 2, 0, 0) == -1
     assert lib.ramnet_delta_rule_workspace_bytes(2, 1, 2, 2, 4, 64, 64, 2, 0, 0) == 0  # a step needs none
-    assert lib.ramnet_delta_rule_kept_bytes(2, 100, 3, 2, 4, 64, 64, 0) == -1
+    assert lib.ramnet_delta_rule_kept_bytes(2, 100, 3, 2, 4, 64, 64, 2, 0) == -1
+    assert lib.ramnet_delta_rule_kept_bytes(2, 100, 2, 2, 4, 161, 64, 0, 0) == -1
+    assert lib.ramnet_delta_rule_kept_bytes(2, 100, 2, 2, 4, 161, 64, 2, 0) > 0
 
 
 def test_native_verify_drafts():

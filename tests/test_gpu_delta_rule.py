@@ -366,6 +366,15 @@ def test_gradients_head_sizes(Dk, Dv):
     _check_grads(_case(T=70, Hk=1, Hv=2, Dk=Dk, Dv=Dv, seed=Dk))
 
 
+@pytest.mark.parametrize("Dk,Dv", [(200, 40), (256, 130)])
+def test_gradients_widest_heads(Dk, Dv):
+    _check_grads(_case(T=70, Hk=1, Hv=2, Dk=Dk, Dv=Dv, dtype="fp16", seed=Dk))
+    from ramnet_ops import gated_delta_rule
+    case = [t.to(DEV).requires_grad_() for t in _case(T=70, Dk=Dk, Dv=Dv)]
+    with pytest.raises(RuntimeError, match="up to 160 for gradients of float32"):
+        gated_delta_rule(*case[:5], init_state=case[5])
+
+
 @pytest.mark.parametrize("Hk,Hv", [(1, 3), (2, 4)])
 def test_gradients_shared_key_heads(Hk, Hv):
     _check_grads(_case(T=70, Hk=Hk, Hv=Hv, Dk=32, Dv=48, state=False, seed=Hv))
