@@ -27,7 +27,7 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
     extern __shared__ __align__(16) float lds_base[];
     using Lds = ChunkLds<DT, PIECES, true>;
     constexpr int C = kDeltaChunk, BT = DT / 2;
-    const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave, wave = tid / kWave;
+    const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave, wave = uniform(tid / kWave);
     const int row = lane & 15, grp = lane >> 4;
     const int group = static_cast<int>(blockIdx.x) % groups;
     const int head = static_cast<int>(blockIdx.x) / groups % job.Hv;
@@ -70,7 +70,7 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
 
     const int c = (group * 4 + wave) * 16 + row;
     const int64_t matrix = (static_cast<int64_t>(n) * job.Hv + head) * job.Dk * job.Dv;
-    const Columns<float> state(job.Dv, job.Dv, grp, c);
+    const Columns<float> state(job.Dv, job.Dv, grp, c), kept(delta_row(job.Dv), delta_row(job.Dv), grp, c);
     f32x4 s[DT];
     {
         const auto from = state.rows(grads.d_state + matrix, grads.d_state ? job.Dk : 0);
@@ -110,8 +110,8 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
         const float *vec = lds.vec();
         const float total = vec[kVecGrowK * C + C - 1] * vec[kVecSk * C + C - 1];  // (a power of two: e^gamma_C)
         {
-            const auto to = state.rows(work.dstate + record * job.Dk * job.Dv, job.Dk);
-            state.each<DT>([&](int t, int r, int at) { buffer_store<float>(s[t][r], to, at); });
+            const auto to = kept.rows(work.dstate + record * job.Dk * delta_row(job.Dv), job.Dk);
+            kept.each<DT>([&](int t, int r, int at) { buffer_store<float>(s[t][r], to, at); });
         }
         f32x4 out[4], du[4], x[4];
 #pragma unroll
@@ -181,8 +181,8 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
                 load_frags(work.y, i - 1, y_hi, y_lo);
         }
         {
-            const auto to = state.rows(work.x + record * C * job.Dv, C);
-            state.each<4>([&](int m, int r, int at) { buffer_store<float>(x[m][r], to, at); });
+            const auto to = kept.rows(work.x + record * C * delta_row(job.Dv), C);
+            kept.each<4>([&](int m, int r, int at) { buffer_store<float>(x[m][r], to, at); });
             const auto out_to = v_cols.rows(dv + static_cast<int64_t>(i) * C * dv_step, min(C, span.len - i * C));
             v_cols.template each<4>([&](int m, int r, int at) { buffer_store<Scalar>(x[m][r], out_to, at); });
         }
@@ -247,43 +247,57 @@ __device__ __forceinline__ void store_code(void *p, int code, int64_t at, float 
         store_f32(static_cast<bf16_t *>(p) + at, v);
 }
 
-// Eight values of a row from column v on, zeros from `wide` on; `even`: rows
-// begin at multiples of 16 bytes.
+// Eight values of a row as they are in memory.
 template<typename Scalar>
-__device__ __forceinline__ void load8(const Scalar *row, int v, int wide, bool have, bool even, float (&x)[8]) {
-    if (even && v + 8 <= wide) {
-        constexpr int kWords = 2 * static_cast<int>(sizeof(Scalar));
-        uint32_t w[kWords] = {};
-        if (have)
+struct Eight {
+    static constexpr int kWords = 2 * static_cast<int>(sizeof(Scalar));
+    uint32_t w[kWords];
+
+    // from column v of the row that begins at byte `at` of the window on, zeros from
+    // `wide` on; EVEN: rows begin at multiples of 16 bytes and are whole pieces of them
+    template<bool EVEN>
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t from, int at, int v, int wide) {
+        constexpr int size = static_cast<int>(sizeof(Scalar)), each = 16 / size;
+        at += v * size;
+        if constexpr (EVEN) {
 #pragma unroll
-            for (int i = 0; i < kWords; i += 4)
-                *reinterpret_cast<u32x4 *>(w + i) = *reinterpret_cast<const u32x4 *>(
-                    reinterpret_cast<const uint32_t *>(row + v) + i);
+            for (int i = 0; i < kWords; i += 4) {
+                const int e = i / 4 * each;
+                const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(from, v + e < wide ? at + 4 * i : kNowhere, 0, 0);
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            x[e] = bits_f32<Scalar>(sizeof(Scalar) == 4 ? w[e % kWords] : (w[e / 2 % kWords] >> (e % 2 * 16)) & 0xFFFFu);
-    } else {
+                for (int k = 0; k < 4; ++k)
+                    w[i + k] = x[k];
+            }
+        } else {
+            uint32_t x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            x[e] = have && v + e < wide ? load_f32(row + v + e) : 0.f;
+            for (int e = 0; e < 8; ++e)
+                x[e] = buffer_bits<Scalar>(from, v + e < wide ? at + e * size : kNowhere);
+#pragma unroll
+            for (int i = 0; i < kWords; ++i)
+                w[i] = size == 4 ? x[i] : x[(2 * i) % 8] | x[(2 * i + 1) % 8] << 16;
+        }
     }
-}
+    __device__ __forceinline__ float operator[](int e) const {
+        return bits_f32<Scalar>(sizeof(Scalar) == 4 ? w[e % kWords] : (w[e / 2 % kWords] >> (e % 2 * 16)) & 0xFFFFu);
+    }
+    __device__ __forceinline__ float largest(float m) const {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            m = fmaxf(m, fabsf((*this)[e]));
+        return m;
+    }
+};
 
 // The fp16 parts of eight values.
-__device__ __forceinline__ void split8(const float (&x)[8], float scale, u32x4 &hi, u32x4 &lo) {
+template<typename Scalar>
+__device__ __forceinline__ void split8(const Eight<Scalar> &x, float scale, u32x4 &hi, u32x4 &lo) {
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
         uint32_t h, l;
         split2(x[2 * w], x[2 * w + 1], scale, h, l);
         hi[w] = h, lo[w] = l;
     }
-}
-
-__device__ __forceinline__ float max8(const float (&x)[8], float m) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-        m = fmaxf(m, fabsf(x[e]));
-    return m;
 }
 
 // LDS of inputs_back_kernel, in halves: K and Q by element, then 64 columns of
@@ -300,42 +314,44 @@ struct BackLds {
 
 // The other gradients of one chunk and key head; its value heads one after the
 // other, so that a shared head's sums have one order. Products over Dv with S
-// and D: a wave has every fourth tile of Dk and all tokens, S and D come from
-// memory straight into its registers, dO, X and E through LDS.
-template<typename Scalar, int DT, int PIECES, bool LO>
-__global__ __launch_bounds__(256) void inputs_back_kernel(const DeltaJob job, const DeltaWork work,
+// and D: a wave has every eighth tile of Dk and all tokens, S and D come from
+// memory straight into its registers, dO, X and E through LDS; what comes from
+// memory is asked for one step ahead of its use.
+// WIDE: q, k and d_o are read in pieces of 16 bytes.
+template<typename Scalar, int DT, int PIECES, bool LO, bool WIDE>
+__global__ __launch_bounds__(512, 2) void inputs_back_kernel(const DeltaJob job, const DeltaWork work,
                                                           const DeltaGrads grads) {
     extern __shared__ __align__(16) float lds_base[];
     using Lds = BackLds<DT, PIECES, LO>;
-    constexpr int C = kDeltaChunk, TW = (DT + 3) / 4, kPitchT = C + 8;
+    constexpr int C = kDeltaChunk, TW = (DT + 7) / 8, kPitchT = C + 8;
     uint16_t *const halves = reinterpret_cast<uint16_t *>(lds_base);
     uint16_t *const kt = halves, *const qt = halves + PIECES * Lds::kCols, *const parts = halves + Lds::kKeys;
     __shared__ double gam[C];
     __shared__ float beta_s[C], grow[C], left[C], inv_k[C], inv_q[C];
     __shared__ float inv_o[C], inv_x[C], inv_e[C];              // of a slab's rows
-    __shared__ float dots[3][4][C];                             // [q, x, e][wave]
-    __shared__ float rows[4][C], cols[4][C], diag[C], state_dot[4], largest[3][4];
-    const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave, wave = tid / kWave;
-    const int row = lane & 15, grp = lane >> 4;
+    __shared__ float dots[3][8][C];                             // [q, x, e][wave]
+    __shared__ float rows[4][C], cols[4][C], diag[C], state_dot[8], largest[3][8];
+    const int tid = static_cast<int>(threadIdx.x), wave = uniform(tid / kWave);
+    int lane = tid % kWave, row = lane & 15, grp = lane >> 4;
     const int chunk = blockIdx.x, kh = blockIdx.y, shared = job.Hv / job.Hk;
     const DeltaPlace at = delta_place(job, work, chunk);
-    const int Dk = job.Dk, Dv = job.Dv;
+    const int Dk = job.Dk, Dv = job.Dv, row_v = delta_row(Dv);
     const int64_t dk_step = static_cast<int64_t>(job.Hk) * Dk;
     Scalar *dq = static_cast<Scalar *>(grads.dq) + static_cast<int64_t>(kh) * Dk;
     Scalar *dk = static_cast<Scalar *>(grads.dk) + static_cast<int64_t>(kh) * Dk;
     // tokens of no sequence or past a row's length
     auto clear = [&](int64_t from, int64_t to) {
         for (int64_t t = from; t < to; ++t) {
-            for (int d = tid; d < Dk; d += 256) {
+            for (int d = tid; d < Dk; d += 512) {
                 store_f32(dq + t * dk_step + d, 0.f);
                 store_f32(dk + t * dk_step + d, 0.f);
             }
-            for (int h = tid; h < shared; h += 256) {
+            for (int h = tid; h < shared; h += 512) {
                 store_code(grads.dg, job.g_dtype, t * job.Hv + kh * shared + h, 0.f);
                 store_code(grads.dbeta, job.beta_dtype, t * job.Hv + kh * shared + h, 0.f);
             }
             if (job.cu)
-                for (int i = tid; i < shared * Dv; i += 256)
+                for (int i = tid; i < shared * Dv; i += 512)
                     store_f32(static_cast<Scalar *>(grads.dv) + (t * job.Hv + kh * shared) * Dv + i, 0.f);
         }
     };
@@ -356,16 +372,17 @@ __global__ __launch_bounds__(256) void inputs_back_kernel(const DeltaJob job, co
     if (at.len == 0)
         return;
 
+    // K by the first four waves, Q by the others
     {
         using Keys = Stager<Scalar, DT, PIECES, true>;
         Keys keys;
-        keys.load(static_cast<const Scalar *>(job.k) + at.b * job.k_at[0] + at.t0 * job.k_at[1] + kh * job.k_at[2],
-                  job.k_at[1],
-                  static_cast<const Scalar *>(job.q) + at.b * job.q_at[0] + at.t0 * job.q_at[1] + kh * job.q_at[2],
-                  job.q_at[1], at.len, Dk, rows_whole<Scalar>(job),
-                  work.vec + (static_cast<int64_t>(chunk) * job.Hv + kh * shared) * kVecs * C, tid);
-        Keys::store_one(keys.raw[0], keys.scales[0], tid, nullptr, kt);
-        Keys::store_one(keys.raw[1], keys.scales[1], tid, nullptr, qt);
+        const bool is_q = wave >= 4;
+        const Scalar *src = is_q ? static_cast<const Scalar *>(job.q) + at.b * job.q_at[0] + at.t0 * job.q_at[1] + kh * job.q_at[2]
+                                 : static_cast<const Scalar *>(job.k) + at.b * job.k_at[0] + at.t0 * job.k_at[1] + kh * job.k_at[2];
+        const f32x4 scales = load4(work.vec + ((static_cast<int64_t>(chunk) * job.Hv + kh * shared) * kVecs +
+                                               (is_q ? kVecSq : kVecSk)) * C + tid % 16 * 4);
+        keys.load_one(src, is_q ? job.q_at[1] : job.k_at[1], at.len, Dk, WIDE, tid % 256, keys.raw[0]);
+        Keys::store_one(keys.raw[0], scales, tid % 256, nullptr, is_q ? qt : kt);
     }
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
     f32x4 sum_q[TW][4], sum_k[TW][4];
@@ -375,51 +392,83 @@ __global__ __launch_bounds__(256) void inputs_back_kernel(const DeltaJob job, co
         for (int m = 0; m < 4; ++m)
             sum_q[t][m] = sum_k[t][m] = zero;
     const int64_t token0 = static_cast<int64_t>(at.b) * job.T + at.t0;
-    const bool even = Dv % 4 == 0;
-    const bool even_o = Dv % 8 == 0 && reinterpret_cast<uintptr_t>(grads.d_o) % 16 == 0 &&
-                        (grads.d_o_at[0] | grads.d_o_at[1] | grads.d_o_at[2]) % (16 / static_cast<int>(sizeof(Scalar))) == 0;
 
     for (int h = 0; h < shared; ++h) {
         const int head = kh * shared + h;
+        // (addresses made here are not kept over the loop: they would fill the registers)
+        asm volatile("" : "+v"(lane));
+        row = lane & 15, grp = lane >> 4;
         const int64_t record = static_cast<int64_t>(chunk) * job.Hv + head;
         const float *vec = work.vec + record * kVecs * C;
+        const float *e = work.e + record * C * row_v, *x = work.x + record * C * row_v;
+        const float *s = work.states + record * Dk * row_v, *d = work.dstate + record * Dk * row_v;
+        const Scalar *d_o = static_cast<const Scalar *>(grads.d_o) + at.b * grads.d_o_at[0] +
+                            at.t0 * grads.d_o_at[1] + head * grads.d_o_at[2];
+        // a slab of dO, X and E: eight columns of a token a thread
+        Eight<Scalar> xo;
+        Eight<float> xx, xe, sv[2], dv[2];
+        const int slab_t = tid / 8, slab_c = tid % 8 * 8;
+        const auto o_rows = window(d_o, (at.len - 1) * grads.d_o_at[1] * static_cast<int64_t>(sizeof(Scalar)) + Dv * sizeof(Scalar));
+        const auto x_rows = window(x, static_cast<int64_t>(C) * row_v * 4), e_rows = window(e, static_cast<int64_t>(C) * row_v * 4);
+        const auto s_rows = window(s, static_cast<int64_t>(Dk) * row_v * 4), d_rows = window(d, static_cast<int64_t>(Dk) * row_v * 4);
+        auto load_slab = [&](int v0) {
+            xo.template load<WIDE>(o_rows, slab_t * static_cast<int>(grads.d_o_at[1] * sizeof(Scalar)), v0 + slab_c, Dv);
+            xx.template load<true>(x_rows, slab_t * row_v * 4, v0 + slab_c, row_v);
+            xe.template load<true>(e_rows, slab_t * row_v * 4, v0 + slab_c, row_v);
+        };
+        auto load_states = [&](int v0, int t) {
+            const int at_row = (16 * t + row) * row_v * 4;
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                sv[b].template load<true>(s_rows, at_row, v0 + 32 * b + 8 * grp, row_v);
+                dv[b].template load<true>(d_rows, at_row, v0 + 32 * b + 8 * grp, row_v);
+            }
+        };
+        load_slab(0);
+        if (wave < DT)
+            load_states(0, wave);
+        const float *p = work.p + record * C * C, *bl = work.bl + record * C * C;
+        float p_ij[2][4], bl_ij[2][4];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const int tile = min(wave + 8 * n, 9);
+            const int ti = tile >= 6 ? 3 : tile >= 3 ? 2 : tile >= 1 ? 1 : 0, tj = tile - ti * (ti + 1) / 2;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int place = (16 * ti + 4 * grp + r) * C + 16 * tj + row;
+                p_ij[n][r] = p[place], bl_ij[n][r] = bl[place];
+            }
+        }
         __syncthreads();
         if (wave == 0) {
             const double own = work.gamma[record * C + lane], end = work.gamma[record * C + C - 1];
             gam[lane] = own;
             grow[lane] = expf(static_cast<float>(own));
             left[lane] = expf(static_cast<float>(end - own));
+        } else if (wave == 1) {
             beta_s[lane] = vec[kVecBeta * C + lane];
             inv_k[lane] = 1.f / vec[kVecSk * C + lane];
             inv_q[lane] = 1.f / vec[kVecSq * C + lane];
         }
-        const float *e = work.e + record * C * Dv, *x = work.x + record * C * Dv;
-        const float *s = work.states + record * Dk * Dv, *d = work.dstate + record * Dk * Dv;
-        const Scalar *d_o = static_cast<const Scalar *>(grads.d_o) + at.b * grads.d_o_at[0] +
-                            at.t0 * grads.d_o_at[1] + head * grads.d_o_at[2];
 
         // dO S^T, X S^T, E D^T (this wave's tiles of Dk) and R1, R2 (every fourth lower tile)
-        f32x4 os[TW][4], xs[TW][4], ed[TW][4], r1[3], r2[3];
+        f32x4 os[TW][4], xs[TW][4], ed[TW][4], r1[2], r2[2];
 #pragma unroll
         for (int t = 0; t < TW; ++t)
 #pragma unroll
             for (int m = 0; m < 4; ++m)
                 os[t][m] = xs[t][m] = ed[t][m] = zero;
 #pragma unroll
-        for (int n = 0; n < 3; ++n)
+        for (int n = 0; n < 2; ++n)
             r1[n] = r2[n] = zero;
         float both = 0.f;
         for (int v0 = 0; v0 < Dv; v0 += Lds::kSlab) {
+            asm volatile("" : "+v"(lane));
+            row = lane & 15, grp = lane >> 4;
             if (v0 > 0)
                 __syncthreads();
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                const int item = tid + 256 * n, t = item / 8, c = item % 8 * 8;
-                float xo[8], xx[8], xe[8];
-                load8<Scalar>(d_o + t * grads.d_o_at[1], v0 + c, Dv, t < at.len, even_o, xo);
-                load8<float>(x + static_cast<int64_t>(t) * Dv, v0 + c, Dv, true, even, xx);
-                load8<float>(e + static_cast<int64_t>(t) * Dv, v0 + c, Dv, true, even, xe);
-                float mo = max8(xo, 0.f), mx = max8(xx, 0.f), me = max8(xe, 0.f);
+            {
+                float mo = xo.largest(0.f), mx = xx.largest(0.f), me = xe.largest(0.f);
 #pragma unroll
                 for (int k = 1; k < 8; k <<= 1) {
                     mo = fmaxf(mo, __shfl_xor(mo, k));
@@ -428,11 +477,11 @@ __global__ __launch_bounds__(256) void inputs_back_kernel(const DeltaJob job, co
                 }
                 float io, ix, ie;
                 const float so = scale_of(mo, io), sx = scale_of(mx, ix), se = scale_of(me, ie);
-                if (item % 8 == 0)
-                    inv_o[t] = io, inv_x[t] = ix, inv_e[t] = ie;
+                if (tid % 8 == 0)
+                    inv_o[slab_t] = io, inv_x[slab_t] = ix, inv_e[slab_t] = ie;
                 u32x4 hi, lo;
                 auto put = [&](int part, u32x4 w) {
-                    *reinterpret_cast<u32x4 *>(parts + part * Lds::kPart + t * Lds::kPitch + c) = w;
+                    *reinterpret_cast<u32x4 *>(parts + part * Lds::kPart + slab_t * Lds::kPitch + slab_c) = w;
                 };
                 split8(xx, sx, hi, lo);
                 put(0, hi), put(1, lo);
@@ -444,23 +493,22 @@ __global__ __launch_bounds__(256) void inputs_back_kernel(const DeltaJob job, co
                     put(5, lo);
             }
             __syncthreads();
+            const int v1 = v0 + Lds::kSlab;
+            if (v1 < Dv)
+                load_slab(v1);
             auto frag = [&](int part, int tile, int b) {
                 return *reinterpret_cast<const u32x4 *>(parts + part * Lds::kPart + (16 * tile + row) * Lds::kPitch + 32 * b +
                                                         8 * grp);
             };
 #pragma unroll
             for (int tw = 0; tw < TW; ++tw) {
-                const int t = wave + 4 * tw;
+                const int t = wave + 8 * tw;
                 if (t >= DT)
                     continue;
-                float sv[2][8], dv[2][8], s_max = 0.f, d_max = 0.f;
-                const int at_row = 16 * t + row;
+                float s_max = 0.f, d_max = 0.f;
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
-                    const int v = v0 + 32 * b + 8 * grp;
-                    load8<float>(s + static_cast<int64_t>(at_row) * Dv, v, Dv, at_row < Dk, even, sv[b]);
-                    load8<float>(d + static_cast<int64_t>(at_row) * Dv, v, Dv, at_row < Dk, even, dv[b]);
-                    s_max = max8(sv[b], s_max), d_max = max8(dv[b], d_max);
+                    s_max = sv[b].largest(s_max), d_max = dv[b].largest(d_max);
 #pragma unroll
                     for (int k = 0; k < 8; ++k)
                         both = fmaf(sv[b][k], dv[b][k], both);
@@ -473,8 +521,13 @@ __global__ __launch_bounds__(256) void inputs_back_kernel(const DeltaJob job, co
                     split8(sv[b], s_scale, s_hi[b], s_lo[b]);
                     split8(dv[b], d_scale, d_hi[b], d_lo[b]);
                 }
+                if (t + 8 < DT)
+                    load_states(v0, t + 8);
+                else if (v1 < Dv)
+                    load_states(v1, wave);
 #pragma unroll
                 for (int m = 0; m < 4; ++m) {
+                    __builtin_amdgcn_sched_barrier(0);  // (one tile's operands at a time: registers)
                     f32x4 a = zero, z = zero, w = zero;
 #pragma unroll
                     for (int b = 0; b < 2; ++b) {
@@ -498,8 +551,8 @@ __global__ __launch_bounds__(256) void inputs_back_kernel(const DeltaJob job, co
                 }
             }
 #pragma unroll
-            for (int n = 0; n < 3; ++n) {
-                const int tile = wave + 4 * n;  // (0,0) (1,0) (1,1) (2,0) ...
+            for (int n = 0; n < 2; ++n) {
+                const int tile = wave + 8 * n;  // (0,0) (1,0) (1,1) (2,0) ...
                 if (tile >= 10)
                     continue;
                 const int ti = tile >= 6 ? 3 : tile >= 3 ? 2 : tile >= 1 ? 1 : 0, tj = tile - ti * (ti + 1) / 2;
@@ -520,6 +573,8 @@ __global__ __launch_bounds__(256) void inputs_back_kernel(const DeltaJob job, co
                 r2[n] += z * (load4(inv_x + 16 * ti + 4 * grp) * ie);
             }
         }
+        asm volatile("" : "+v"(lane));
+        row = lane & 15, grp = lane >> 4;
         both = row_sum(both);
         both += __shfl_xor(both, 16);
         both += __shfl_xor(both, 32);
@@ -529,13 +584,14 @@ __global__ __launch_bounds__(256) void inputs_back_kernel(const DeltaJob job, co
         // with the rows of Q and K: what e^gamma and e^(gamma_C - gamma) multiply
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
+            __builtin_amdgcn_sched_barrier(0);
             const int i = 16 * m + 4 * grp;
             const f32x4 gr = load4(grow + i), le = load4(left + i) * load4(beta_s + i);
             const f32x4 ik = load4(inv_k + i), iq = load4(inv_q + i);
             f32x4 q_dot = zero, x_dot = zero, e_dot = zero;
 #pragma unroll
             for (int tw = 0; tw < TW; ++tw) {
-                const int t = wave + 4 * tw;
+                const int t = wave + 8 * tw;
                 if (t >= DT)
                     continue;
                 const int place = (16 * t + row) * kPitchT + operand_at(i);
@@ -562,12 +618,11 @@ __global__ __launch_bounds__(256) void inputs_back_kernel(const DeltaJob job, co
         }
 
         // R1 and R2 with L: dA, dB, and their sums
-        const float *p = work.p + record * C * C, *bl = work.bl + record * C * C;
         float a_max = 0.f, t_max = 0.f, b_max = 0.f;
         // from here on r1 is dA and r2 dB, without the scales of K and Q
 #pragma unroll
-        for (int n = 0; n < 3; ++n) {
-            const int tile = wave + 4 * n;
+        for (int n = 0; n < 2; ++n) {
+            const int tile = wave + 8 * n;
             if (tile >= 10)
                 continue;
             const int ti = tile >= 6 ? 3 : tile >= 3 ? 2 : tile >= 1 ? 1 : 0, tj = tile - ti * (ti + 1) / 2;
@@ -581,7 +636,7 @@ __global__ __launch_bounds__(256) void inputs_back_kernel(const DeltaJob job, co
                     const float decay = expf(static_cast<float>(gam[i] - gam[j])) * beta_s[j];
                     a = job.scale * decay * r1[n][r];
                     b = i > j ? -decay * r2[n][r] : 0.f;
-                    both_ij = p[i * C + j] * r1[n][r] - bl[i * C + j] * r2[n][r];
+                    both_ij = p_ij[n][r] * r1[n][r] - bl_ij[n][r] * r2[n][r];
                     if (i == j)
                         diag[i] = both_ij, both_ij = 0.f;
                 }
@@ -618,7 +673,7 @@ __global__ __launch_bounds__(256) void inputs_back_kernel(const DeltaJob job, co
             }
             float q_dot = 0.f, x_dot = 0.f, e_dot = 0.f;
 #pragma unroll
-            for (int w = 0; w < 4; ++w)
+            for (int w = 0; w < 8; ++w)
                 q_dot += dots[0][w][lane], x_dot += dots[1][w][lane], e_dot += dots[2][w][lane];
             const float beta = beta_s[lane], last = left[lane] * e_dot, held = beta * last;
             const float own = grow[lane] * (job.scale * q_dot - x_dot);
@@ -632,8 +687,11 @@ __global__ __launch_bounds__(256) void inputs_back_kernel(const DeltaJob job, co
                 part += lane + m < kWave ? y : 0.0;
                 all += __shfl_xor(all, m);
             }
-            all += static_cast<double>(grow[C - 1]) *
-                   (static_cast<double>(state_dot[0]) + state_dot[1] + state_dot[2] + state_dot[3]);
+            double both_all = 0.0;
+#pragma unroll
+            for (int w = 0; w < 8; ++w)
+                both_all += static_cast<double>(state_dot[w]);
+            all += static_cast<double>(grow[C - 1]) * both_all;
             if (lane < at.len) {
                 const int64_t out = (token0 + lane) * job.Hv + head;
                 store_code(grads.dg, job.g_dtype, out, static_cast<float>(part + all));
@@ -642,7 +700,13 @@ __global__ __launch_bounds__(256) void inputs_back_kernel(const DeltaJob job, co
         }
         // dA, dA^T and dB + dB^T as operands, K's and Q's scales taken out of their columns
         float a_inv, t_inv, b_inv;
-        auto all_max = [&](int k) { return fmaxf(fmaxf(largest[k][0], largest[k][1]), fmaxf(largest[k][2], largest[k][3])); };
+        auto all_max = [&](int k) {
+            float m = largest[k][0];
+#pragma unroll
+            for (int w = 1; w < 8; ++w)
+                m = fmaxf(m, largest[k][w]);
+            return m;
+        };
         const float a_scale = scale_of(all_max(0), a_inv), t_scale = scale_of(all_max(1), t_inv),
                     b_scale = scale_of(all_max(2), b_inv);
         auto put = [&](int matrix, int i, int j, float v, float scale) {
@@ -653,8 +717,8 @@ __global__ __launch_bounds__(256) void inputs_back_kernel(const DeltaJob job, co
                 to[3 * Lds::kPart] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(fmaf(v, scale, -static_cast<float>(hi))));
         };
 #pragma unroll
-        for (int n = 0; n < 3; ++n) {
-            const int tile = wave + 4 * n;
+        for (int n = 0; n < 2; ++n) {
+            const int tile = wave + 8 * n;
             if (tile >= 10)
                 continue;
             const int ti = tile >= 6 ? 3 : tile >= 3 ? 2 : tile >= 1 ? 1 : 0, tj = tile - ti * (ti + 1) / 2;
@@ -684,7 +748,7 @@ __global__ __launch_bounds__(256) void inputs_back_kernel(const DeltaJob job, co
         };
 #pragma unroll
         for (int tw = 0; tw < TW; ++tw) {
-            const int t = wave + 4 * tw;
+            const int t = wave + 8 * tw;
             if (t >= DT)
                 continue;
             u32x4 kf[PIECES][2], qf[PIECES][2];
@@ -698,6 +762,7 @@ __global__ __launch_bounds__(256) void inputs_back_kernel(const DeltaJob job, co
                 }
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
+                __builtin_amdgcn_sched_barrier(0);
                 f32x4 a = zero, z = zero, w = zero;
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
@@ -723,7 +788,7 @@ __global__ __launch_bounds__(256) void inputs_back_kernel(const DeltaJob job, co
     }
 #pragma unroll
     for (int tw = 0; tw < TW; ++tw) {
-        const int t = wave + 4 * tw;
+        const int t = wave + 8 * tw;
         if (t >= DT)
             continue;
         const Columns<Scalar> to(dk_step, Dk, grp, 16 * t + row);
@@ -738,7 +803,7 @@ __global__ __launch_bounds__(256) void inputs_back_kernel(const DeltaJob job, co
 // Whether a chunk's operands and the gradients' products fit the LDS.
 template<int DT, int PIECES>
 constexpr bool delta_trains = ChunkLds<DT, PIECES, true>::kBytes <= kLdsBytes &&
-                              BackLds<DT, PIECES, true>::kBytes + 8192 <= kLdsBytes;
+                              BackLds<DT, PIECES, true>::kBytes + 12288 <= kLdsBytes;
 static_assert(delta_trains<16, 1> && delta_trains<10, 2> && !delta_trains<16, 2>);  // as delta_kept has it
 
 template<typename Scalar>
@@ -753,6 +818,9 @@ hipError_t backward_typed(const DeltaJob &job, const DeltaWork &work, const Delt
     }
     constexpr int PIECES = sizeof(Scalar) == 4 ? 2 : 1;
     constexpr bool LO = !__is_same(Scalar, bf16_t);
+    constexpr int V = 16 / static_cast<int>(sizeof(Scalar));
+    const bool pieces = rows_whole<Scalar>(job) && job.Dv % V == 0 && reinterpret_cast<uintptr_t>(grads.d_o) % 16 == 0 &&
+                        (grads.d_o_at[0] | grads.d_o_at[1] | grads.d_o_at[2]) % V == 0;
 #define RAMNET_BACK(DT)                                                                                            \
     if constexpr (delta_trains<DT, PIECES>) {                                                                      \
         if (wide == 16 * DT) {                                                                                     \
@@ -762,8 +830,12 @@ hipError_t backward_typed(const DeltaJob &job, const DeltaWork &work, const Delt
                                dim3(512), bufs * each, stream, job, work, grads, groups);                          \
             if (const hipError_t err = hipGetLastError())                                                          \
                 return err;                                                                                        \
-            hipLaunchKernelGGL((inputs_back_kernel<Scalar, DT, PIECES, LO>), dim3(work.chunks, job.Hk), dim3(256), \
-                               back, stream, job, work, grads);                                                    \
+            if (pieces)                                                                                            \
+                hipLaunchKernelGGL((inputs_back_kernel<Scalar, DT, PIECES, LO, true>), dim3(work.chunks, job.Hk),  \
+                                   dim3(512), back, stream, job, work, grads);                                     \
+            else                                                                                                   \
+                hipLaunchKernelGGL((inputs_back_kernel<Scalar, DT, PIECES, LO, false>), dim3(work.chunks, job.Hk), \
+                                   dim3(512), back, stream, job, work, grads);                                     \
         }                                                                                                          \
     }
     RAMNET_BACK(2)

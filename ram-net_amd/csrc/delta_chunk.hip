@@ -15,7 +15,7 @@ namespace {
 __global__ __launch_bounds__(1024) void offsets_kernel(const DeltaJob job, const DeltaWork work) {
     __shared__ int wave_sum[16];
     __shared__ int carry;
-    const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave, wave = tid / kWave;
+    const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave, wave = uniform(tid / kWave);
     if (tid == 0)
         carry = 0, work.offsets[0] = 0;
     __syncthreads();
@@ -122,7 +122,7 @@ __global__ __launch_bounds__(256) void prepare_kernel(const DeltaJob job, const 
     Scalar *ks = reinterpret_cast<Scalar *>(ys);
     __shared__ double gam[C];
     __shared__ float beta_s[C], sk_s[C], sq_s[C], scale_y[C], scale_p[C];
-    const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave, wave = tid / kWave;
+    const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave, wave = uniform(tid / kWave);
     const int row = lane & 15, grp = lane >> 4;
     const int chunk = blockIdx.x, head = blockIdx.y, kh = head / (job.Hv / job.Hk);
     const DeltaPlace at = delta_place(job, work, chunk);
@@ -322,7 +322,7 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
     extern __shared__ __align__(16) float lds_base[];
     using Lds = ChunkLds<DT, PIECES, false>;
     constexpr int C = kDeltaChunk, BT = DT / 2;
-    const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave, wave = tid / kWave;
+    const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave, wave = uniform(tid / kWave);
     const int row = lane & 15, grp = lane >> 4;
     const int group = static_cast<int>(blockIdx.x) % groups;
     const int head = static_cast<int>(blockIdx.x) / groups % job.Hv;
@@ -365,7 +365,7 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
 
     const int c = (group * 4 + wave) * 16 + row;
     const int64_t matrix = (static_cast<int64_t>(n) * job.Hv + head) * job.Dk * job.Dv;
-    const Columns<float> state(job.Dv, job.Dv, grp, c);
+    const Columns<float> state(job.Dv, job.Dv, grp, c), kept(delta_row(job.Dv), delta_row(job.Dv), grp, c);
     f32x4 s[DT];
     {
         const auto from = state.rows(job.init + matrix, job.init ? job.Dk : 0);
@@ -415,8 +415,8 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
         const float *vec = lds.vec();
         const float total = vec[kVecGrowK * C + C - 1] * vec[kVecSk * C + C - 1];  // (a power of two: e^gamma_C)
         if (work.states) {
-            const auto to = state.rows(work.states + record * job.Dk * job.Dv, job.Dk);
-            state.each<DT>([&](int t, int r, int at) { buffer_store<float>(s[t][r], to, at); });
+            const auto to = kept.rows(work.states + record * job.Dk * delta_row(job.Dv), job.Dk);
+            kept.each<DT>([&](int t, int r, int at) { buffer_store<float>(s[t][r], to, at); });
         }
 
         f32x4 g[4], qo[4];
@@ -476,8 +476,8 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
                 load_y(i + 1);
         }
         if (work.e) {
-            const auto to = state.rows(work.e + record * C * job.Dv, C);
-            state.each<4>([&](int m, int r, int at) { buffer_store<float>(e[m][r], to, at); });
+            const auto to = kept.rows(work.e + record * C * delta_row(job.Dv), C);
+            kept.each<4>([&](int m, int r, int at) { buffer_store<float>(e[m][r], to, at); });
         }
         {
             Operand<4, LO> eo;
@@ -628,8 +628,8 @@ int64_t delta_layout(const DeltaJob &job, bool packed, bool backward, char *base
     if (backward) {
         work->p = carve.take<float>(records * square);
         work->bl = carve.take<float>(records * square);
-        work->x = carve.take<float>(records * kDeltaChunk * job.Dv);
-        work->dstate = carve.take<float>(records * job.Dk * job.Dv);
+        work->x = carve.take<float>(records * kDeltaChunk * delta_row(job.Dv));
+        work->dstate = carve.take<float>(records * job.Dk * delta_row(job.Dv));
     }
     return carve.size;
 }
@@ -640,8 +640,8 @@ int64_t delta_kept(const DeltaJob &job, bool packed, char *base, DeltaWork *work
     count_chunks(job, packed, work);
     Carver carve{base};
     const int64_t records = static_cast<int64_t>(work->chunks) * job.Hv;
-    work->e = carve.take<float>(records * kDeltaChunk * job.Dv);
-    work->states = carve.take<float>(records * job.Dk * job.Dv);
+    work->e = carve.take<float>(records * kDeltaChunk * delta_row(job.Dv));
+    work->states = carve.take<float>(records * job.Dk * delta_row(job.Dv));
     return carve.size;
 }
 

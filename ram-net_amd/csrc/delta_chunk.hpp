@@ -75,7 +75,7 @@ constexpr int kLdsBytes = 160 * 1024;
 
 // Whether rows of q and k are whole pieces of 16 bytes at 16-byte addresses.
 template<typename Scalar>
-__device__ __forceinline__ bool rows_whole(const DeltaJob &job) {
+__host__ __device__ inline bool rows_whole(const DeltaJob &job) {
     constexpr int V = 16 / static_cast<int>(sizeof(Scalar));
     const int64_t steps = job.q_at[0] | job.q_at[1] | job.q_at[2] | job.k_at[0] | job.k_at[1] | job.k_at[2];
     const uintptr_t starts = reinterpret_cast<uintptr_t>(job.q) | reinterpret_cast<uintptr_t>(job.k);

@@ -36,10 +36,11 @@ struct DeltaWork {
     uint32_t *p_frags; // the same of scale lower(Q K^T . L) diag(beta) (backward: transposed, without beta)
     float *p;          // [record][64][64] scale lower(Q K^T . L)    (backward)
     float *bl;         // [record][64][64] strictlower(K K^T . L)   (backward)
-    float *x;          // [record][64][Dv] gradient of the values    (backward)
-    float *dstate;     // [record][Dk][Dv] gradient after the chunk  (backward)
-    float *e;          // [record][64][Dv] v - S^T k of each token   (kept)
-    float *states;     // [record][Dk][Dv] state before the chunk    (kept)
+    // rows of Dv values, zeros up to a multiple of 8 (delta_row):
+    float *x;          // [record][64][..] gradient of the values    (backward)
+    float *dstate;     // [record][Dk][..] gradient after the chunk  (backward)
+    float *e;          // [record][64][..] v - S^T k of each token   (kept)
+    float *states;     // [record][Dk][..] state before the chunk    (kept)
     int per_row;       // chunks of a row where sequences are rows
     int chunks;        // records / Hv
 };
@@ -61,6 +62,9 @@ __device__ __forceinline__ float load_code(const void *p, int code, int64_t at) 
     return load_f32(static_cast<const bf16_t *>(p) + at);
 }
 
+// A value that all lanes share, in a scalar register.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 // Tokens of one sequence: `len` from token t0 of batch row b. Bounds that are
 // out of order or out of range give fewer tokens, never ones outside [0, T).
 struct DeltaSpan {
@@ -79,6 +83,9 @@ __device__ __forceinline__ DeltaSpan delta_span(const DeltaJob &job, int n) {
 inline int delta_padded(int Dk) {
     return Dk <= 32 ? 32 : Dk <= 64 ? 64 : Dk <= 96 ? 96 : Dk <= 128 ? 128 : Dk <= 160 ? 160 : 256;
 }
+
+// Length of a row of Dv values in the workspace.
+__host__ __device__ inline int delta_row(int Dv) { return (Dv + 7) / 8 * 8; }
 
 // A decay of one step. e^-200 is 0 in fp32 as e^-inf is; held there, sums of
 // decays stay finite and differences of them free of inf - inf. (A NaN stays.)
