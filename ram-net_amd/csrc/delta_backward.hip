@@ -314,23 +314,25 @@ struct BackLds {
 
 // The other gradients of one chunk and key head; its value heads one after the
 // other, so that a shared head's sums have one order. Products over Dv with S
-// and D: a wave has every eighth tile of Dk and all tokens, S and D come from
+// and D: a wave has every eighth (or fourth) tile of Dk and all tokens, S and D come from
 // memory straight into its registers, dO, X and E through LDS; what comes from
 // memory is asked for one step ahead of its use.
-// WIDE: q, k and d_o are read in pieces of 16 bytes.
-template<typename Scalar, int DT, int PIECES, bool LO, bool WIDE>
-__global__ __launch_bounds__(512, 2) void inputs_back_kernel(const DeltaJob job, const DeltaWork work,
+// WIDE: q, k and d_o are read in pieces of 16 bytes. WAVES: 8, so that one's
+// loads hide behind another's products, or 4 of twice the registers.
+template<typename Scalar, int DT, int PIECES, bool LO, bool WIDE, int WAVES>
+__global__ __launch_bounds__(kWave *WAVES, WAVES / 4) void inputs_back_kernel(const DeltaJob job, const DeltaWork work,
                                                           const DeltaGrads grads) {
     extern __shared__ __align__(16) float lds_base[];
     using Lds = BackLds<DT, PIECES, LO>;
-    constexpr int C = kDeltaChunk, TW = (DT + 7) / 8, kPitchT = C + 8;
+    constexpr int C = kDeltaChunk, kPitchT = C + 8, kThreads = kWave * WAVES;
+    constexpr int TW = (DT + WAVES - 1) / WAVES, NR = (10 + WAVES - 1) / WAVES, NI = 512 / kThreads;
     uint16_t *const halves = reinterpret_cast<uint16_t *>(lds_base);
     uint16_t *const kt = halves, *const qt = halves + PIECES * Lds::kCols, *const parts = halves + Lds::kKeys;
     __shared__ double gam[C];
     __shared__ float beta_s[C], grow[C], left[C], inv_k[C], inv_q[C];
     __shared__ float inv_o[C], inv_x[C], inv_e[C];              // of a slab's rows
-    __shared__ float dots[3][8][C];                             // [q, x, e][wave]
-    __shared__ float rows[4][C], cols[4][C], diag[C], state_dot[8], largest[3][8];
+    __shared__ float dots[3][WAVES][C];                             // [q, x, e][wave]
+    __shared__ float rows[4][C], cols[4][C], diag[C], state_dot[WAVES], largest[3][WAVES];
     const int tid = static_cast<int>(threadIdx.x), wave = uniform(tid / kWave);
     int lane = tid % kWave, row = lane & 15, grp = lane >> 4;
     const int chunk = blockIdx.x, kh = blockIdx.y, shared = job.Hv / job.Hk;
@@ -342,16 +344,16 @@ __global__ __launch_bounds__(512, 2) void inputs_back_kernel(const DeltaJob job,
     // tokens of no sequence or past a row's length
     auto clear = [&](int64_t from, int64_t to) {
         for (int64_t t = from; t < to; ++t) {
-            for (int d = tid; d < Dk; d += 512) {
+            for (int d = tid; d < Dk; d += kThreads) {
                 store_f32(dq + t * dk_step + d, 0.f);
                 store_f32(dk + t * dk_step + d, 0.f);
             }
-            for (int h = tid; h < shared; h += 512) {
+            for (int h = tid; h < shared; h += kThreads) {
                 store_code(grads.dg, job.g_dtype, t * job.Hv + kh * shared + h, 0.f);
                 store_code(grads.dbeta, job.beta_dtype, t * job.Hv + kh * shared + h, 0.f);
             }
             if (job.cu)
-                for (int i = tid; i < shared * Dv; i += 512)
+                for (int i = tid; i < shared * Dv; i += kThreads)
                     store_f32(static_cast<Scalar *>(grads.dv) + (t * job.Hv + kh * shared) * Dv + i, 0.f);
         }
     };
@@ -372,17 +374,20 @@ __global__ __launch_bounds__(512, 2) void inputs_back_kernel(const DeltaJob job,
     if (at.len == 0)
         return;
 
-    // K by the first four waves, Q by the others
+    // K, and Q: by four waves each
     {
         using Keys = Stager<Scalar, DT, PIECES, true>;
         Keys keys;
+        const Scalar *k = static_cast<const Scalar *>(job.k) + at.b * job.k_at[0] + at.t0 * job.k_at[1] + kh * job.k_at[2];
+        const Scalar *q = static_cast<const Scalar *>(job.q) + at.b * job.q_at[0] + at.t0 * job.q_at[1] + kh * job.q_at[2];
+        const float *scales = work.vec + (static_cast<int64_t>(chunk) * job.Hv + kh * shared) * kVecs * C + tid % 16 * 4;
         const bool is_q = wave >= 4;
-        const Scalar *src = is_q ? static_cast<const Scalar *>(job.q) + at.b * job.q_at[0] + at.t0 * job.q_at[1] + kh * job.q_at[2]
-                                 : static_cast<const Scalar *>(job.k) + at.b * job.k_at[0] + at.t0 * job.k_at[1] + kh * job.k_at[2];
-        const f32x4 scales = load4(work.vec + ((static_cast<int64_t>(chunk) * job.Hv + kh * shared) * kVecs +
-                                               (is_q ? kVecSq : kVecSk)) * C + tid % 16 * 4);
-        keys.load_one(src, is_q ? job.q_at[1] : job.k_at[1], at.len, Dk, WIDE, tid % 256, keys.raw[0]);
-        Keys::store_one(keys.raw[0], scales, tid % 256, nullptr, is_q ? qt : kt);
+        keys.load_one(is_q ? q : k, is_q ? job.q_at[1] : job.k_at[1], at.len, Dk, WIDE, tid % 256, keys.raw[0]);
+        if constexpr (WAVES == 4)
+            keys.load_one(q, job.q_at[1], at.len, Dk, WIDE, tid, keys.raw[1]);
+        Keys::store_one(keys.raw[0], load4(scales + (is_q ? kVecSq : kVecSk) * C), tid % 256, nullptr, is_q ? qt : kt);
+        if constexpr (WAVES == 4)
+            Keys::store_one(keys.raw[1], load4(scales + kVecSq * C), tid, nullptr, qt);
     }
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
     f32x4 sum_q[TW][4], sum_k[TW][4];
@@ -405,16 +410,20 @@ __global__ __launch_bounds__(512, 2) void inputs_back_kernel(const DeltaJob job,
         const Scalar *d_o = static_cast<const Scalar *>(grads.d_o) + at.b * grads.d_o_at[0] +
                             at.t0 * grads.d_o_at[1] + head * grads.d_o_at[2];
         // a slab of dO, X and E: eight columns of a token a thread
-        Eight<Scalar> xo;
-        Eight<float> xx, xe, sv[2], dv[2];
+        Eight<Scalar> xo[NI];
+        Eight<float> xx[NI], xe[NI], sv[2], dv[2];
         const int slab_t = tid / 8, slab_c = tid % 8 * 8;
         const auto o_rows = window(d_o, (at.len - 1) * grads.d_o_at[1] * static_cast<int64_t>(sizeof(Scalar)) + Dv * sizeof(Scalar));
         const auto x_rows = window(x, static_cast<int64_t>(C) * row_v * 4), e_rows = window(e, static_cast<int64_t>(C) * row_v * 4);
         const auto s_rows = window(s, static_cast<int64_t>(Dk) * row_v * 4), d_rows = window(d, static_cast<int64_t>(Dk) * row_v * 4);
         auto load_slab = [&](int v0) {
-            xo.template load<WIDE>(o_rows, slab_t * static_cast<int>(grads.d_o_at[1] * sizeof(Scalar)), v0 + slab_c, Dv);
-            xx.template load<true>(x_rows, slab_t * row_v * 4, v0 + slab_c, row_v);
-            xe.template load<true>(e_rows, slab_t * row_v * 4, v0 + slab_c, row_v);
+#pragma unroll
+            for (int n = 0; n < NI; ++n) {
+                const int t = slab_t + n * (kThreads / 8);
+                xo[n].template load<WIDE>(o_rows, t * static_cast<int>(grads.d_o_at[1] * sizeof(Scalar)), v0 + slab_c, Dv);
+                xx[n].template load<true>(x_rows, t * row_v * 4, v0 + slab_c, row_v);
+                xe[n].template load<true>(e_rows, t * row_v * 4, v0 + slab_c, row_v);
+            }
         };
         auto load_states = [&](int v0, int t) {
             const int at_row = (16 * t + row) * row_v * 4;
@@ -427,18 +436,6 @@ __global__ __launch_bounds__(512, 2) void inputs_back_kernel(const DeltaJob job,
         load_slab(0);
         if (wave < DT)
             load_states(0, wave);
-        const float *p = work.p + record * C * C, *bl = work.bl + record * C * C;
-        float p_ij[2][4], bl_ij[2][4];
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            const int tile = min(wave + 8 * n, 9);
-            const int ti = tile >= 6 ? 3 : tile >= 3 ? 2 : tile >= 1 ? 1 : 0, tj = tile - ti * (ti + 1) / 2;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int place = (16 * ti + 4 * grp + r) * C + 16 * tj + row;
-                p_ij[n][r] = p[place], bl_ij[n][r] = bl[place];
-            }
-        }
         __syncthreads();
         if (wave == 0) {
             const double own = work.gamma[record * C + lane], end = work.gamma[record * C + C - 1];
@@ -452,14 +449,14 @@ __global__ __launch_bounds__(512, 2) void inputs_back_kernel(const DeltaJob job,
         }
 
         // dO S^T, X S^T, E D^T (this wave's tiles of Dk) and R1, R2 (every fourth lower tile)
-        f32x4 os[TW][4], xs[TW][4], ed[TW][4], r1[2], r2[2];
+        f32x4 os[TW][4], xs[TW][4], ed[TW][4], r1[NR], r2[NR];
 #pragma unroll
         for (int t = 0; t < TW; ++t)
 #pragma unroll
             for (int m = 0; m < 4; ++m)
                 os[t][m] = xs[t][m] = ed[t][m] = zero;
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < NR; ++n)
             r1[n] = r2[n] = zero;
         float both = 0.f;
         for (int v0 = 0; v0 < Dv; v0 += Lds::kSlab) {
@@ -467,8 +464,10 @@ __global__ __launch_bounds__(512, 2) void inputs_back_kernel(const DeltaJob job,
             row = lane & 15, grp = lane >> 4;
             if (v0 > 0)
                 __syncthreads();
-            {
-                float mo = xo.largest(0.f), mx = xx.largest(0.f), me = xe.largest(0.f);
+#pragma unroll
+            for (int n = 0; n < NI; ++n) {
+                const int t = slab_t + n * (kThreads / 8);
+                float mo = xo[n].largest(0.f), mx = xx[n].largest(0.f), me = xe[n].largest(0.f);
 #pragma unroll
                 for (int k = 1; k < 8; k <<= 1) {
                     mo = fmaxf(mo, __shfl_xor(mo, k));
@@ -478,16 +477,16 @@ __global__ __launch_bounds__(512, 2) void inputs_back_kernel(const DeltaJob job,
                 float io, ix, ie;
                 const float so = scale_of(mo, io), sx = scale_of(mx, ix), se = scale_of(me, ie);
                 if (tid % 8 == 0)
-                    inv_o[slab_t] = io, inv_x[slab_t] = ix, inv_e[slab_t] = ie;
+                    inv_o[t] = io, inv_x[t] = ix, inv_e[t] = ie;
                 u32x4 hi, lo;
                 auto put = [&](int part, u32x4 w) {
-                    *reinterpret_cast<u32x4 *>(parts + part * Lds::kPart + slab_t * Lds::kPitch + slab_c) = w;
+                    *reinterpret_cast<u32x4 *>(parts + part * Lds::kPart + t * Lds::kPitch + slab_c) = w;
                 };
-                split8(xx, sx, hi, lo);
+                split8(xx[n], sx, hi, lo);
                 put(0, hi), put(1, lo);
-                split8(xe, se, hi, lo);
+                split8(xe[n], se, hi, lo);
                 put(2, hi), put(3, lo);
-                split8(xo, so, hi, lo);
+                split8(xo[n], so, hi, lo);
                 put(4, hi);
                 if constexpr (PIECES == 2)
                     put(5, lo);
@@ -502,7 +501,7 @@ __global__ __launch_bounds__(512, 2) void inputs_back_kernel(const DeltaJob job,
             };
 #pragma unroll
             for (int tw = 0; tw < TW; ++tw) {
-                const int t = wave + 8 * tw;
+                const int t = wave + WAVES * tw;
                 if (t >= DT)
                     continue;
                 float s_max = 0.f, d_max = 0.f;
@@ -521,8 +520,8 @@ __global__ __launch_bounds__(512, 2) void inputs_back_kernel(const DeltaJob job,
                     split8(sv[b], s_scale, s_hi[b], s_lo[b]);
                     split8(dv[b], d_scale, d_hi[b], d_lo[b]);
                 }
-                if (t + 8 < DT)
-                    load_states(v0, t + 8);
+                if (t + WAVES < DT)
+                    load_states(v0, t + WAVES);
                 else if (v1 < Dv)
                     load_states(v1, wave);
 #pragma unroll
@@ -531,6 +530,8 @@ __global__ __launch_bounds__(512, 2) void inputs_back_kernel(const DeltaJob job,
                     f32x4 a = zero, z = zero, w = zero;
 #pragma unroll
                     for (int b = 0; b < 2; ++b) {
+                        if constexpr (PIECES == 2)
+                            __builtin_amdgcn_sched_barrier(0);
                         const u32x4 fo = frag(4, m, b), fx = frag(0, m, b), fxl = frag(1, m, b), fe = frag(2, m, b),
                                     fel = frag(3, m, b);
                         a = mfma16(fo, s_hi[b], a);
@@ -551,8 +552,8 @@ __global__ __launch_bounds__(512, 2) void inputs_back_kernel(const DeltaJob job,
                 }
             }
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                const int tile = wave + 8 * n;  // (0,0) (1,0) (1,1) (2,0) ...
+            for (int n = 0; n < NR; ++n) {
+                const int tile = wave + WAVES * n;  // (0,0) (1,0) (1,1) (2,0) ...
                 if (tile >= 10)
                     continue;
                 const int ti = tile >= 6 ? 3 : tile >= 3 ? 2 : tile >= 1 ? 1 : 0, tj = tile - ti * (ti + 1) / 2;
@@ -575,6 +576,18 @@ __global__ __launch_bounds__(512, 2) void inputs_back_kernel(const DeltaJob job,
         }
         asm volatile("" : "+v"(lane));
         row = lane & 15, grp = lane >> 4;
+        const float *p = work.p + record * C * C, *bl = work.bl + record * C * C;
+        float p_ij[NR][4], bl_ij[NR][4];
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            const int tile = min(wave + WAVES * n, 9);
+            const int ti = tile >= 6 ? 3 : tile >= 3 ? 2 : tile >= 1 ? 1 : 0, tj = tile - ti * (ti + 1) / 2;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int place = (16 * ti + 4 * grp + r) * C + 16 * tj + row;
+                p_ij[n][r] = p[place], bl_ij[n][r] = bl[place];
+            }
+        }
         both = row_sum(both);
         both += __shfl_xor(both, 16);
         both += __shfl_xor(both, 32);
@@ -591,7 +604,7 @@ __global__ __launch_bounds__(512, 2) void inputs_back_kernel(const DeltaJob job,
             f32x4 q_dot = zero, x_dot = zero, e_dot = zero;
 #pragma unroll
             for (int tw = 0; tw < TW; ++tw) {
-                const int t = wave + 8 * tw;
+                const int t = wave + WAVES * tw;
                 if (t >= DT)
                     continue;
                 const int place = (16 * t + row) * kPitchT + operand_at(i);
@@ -621,8 +634,8 @@ __global__ __launch_bounds__(512, 2) void inputs_back_kernel(const DeltaJob job,
         float a_max = 0.f, t_max = 0.f, b_max = 0.f;
         // from here on r1 is dA and r2 dB, without the scales of K and Q
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            const int tile = wave + 8 * n;
+        for (int n = 0; n < NR; ++n) {
+            const int tile = wave + WAVES * n;
             if (tile >= 10)
                 continue;
             const int ti = tile >= 6 ? 3 : tile >= 3 ? 2 : tile >= 1 ? 1 : 0, tj = tile - ti * (ti + 1) / 2;
@@ -673,7 +686,7 @@ __global__ __launch_bounds__(512, 2) void inputs_back_kernel(const DeltaJob job,
             }
             float q_dot = 0.f, x_dot = 0.f, e_dot = 0.f;
 #pragma unroll
-            for (int w = 0; w < 8; ++w)
+            for (int w = 0; w < WAVES; ++w)
                 q_dot += dots[0][w][lane], x_dot += dots[1][w][lane], e_dot += dots[2][w][lane];
             const float beta = beta_s[lane], last = left[lane] * e_dot, held = beta * last;
             const float own = grow[lane] * (job.scale * q_dot - x_dot);
@@ -689,7 +702,7 @@ __global__ __launch_bounds__(512, 2) void inputs_back_kernel(const DeltaJob job,
             }
             double both_all = 0.0;
 #pragma unroll
-            for (int w = 0; w < 8; ++w)
+            for (int w = 0; w < WAVES; ++w)
                 both_all += static_cast<double>(state_dot[w]);
             all += static_cast<double>(grow[C - 1]) * both_all;
             if (lane < at.len) {
@@ -703,7 +716,7 @@ __global__ __launch_bounds__(512, 2) void inputs_back_kernel(const DeltaJob job,
         auto all_max = [&](int k) {
             float m = largest[k][0];
 #pragma unroll
-            for (int w = 1; w < 8; ++w)
+            for (int w = 1; w < WAVES; ++w)
                 m = fmaxf(m, largest[k][w]);
             return m;
         };
@@ -711,35 +724,37 @@ __global__ __launch_bounds__(512, 2) void inputs_back_kernel(const DeltaJob job,
                     b_scale = scale_of(all_max(2), b_inv);
         auto put = [&](int matrix, int i, int j, float v, float scale) {
             const _Float16 hi = static_cast<_Float16>(v * scale);
-            uint16_t *to = parts + matrix * Lds::kPart + i * Lds::kPitch + operand_at(j);
+            uint16_t *to = parts + matrix * Lds::kPart + i * Lds::kPitch + j;
             *to = __builtin_bit_cast(uint16_t, hi);
             if constexpr (LO)
                 to[3 * Lds::kPart] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(fmaf(v, scale, -static_cast<float>(hi))));
         };
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            const int tile = wave + 8 * n;
+        for (int n = 0; n < NR; ++n) {
+            const int tile = wave + WAVES * n;
             if (tile >= 10)
                 continue;
             const int ti = tile >= 6 ? 3 : tile >= 3 ? 2 : tile >= 1 ? 1 : 0, tj = tile - ti * (ti + 1) / 2;
             const int j = 16 * tj + row;
+            // places of row i, and of column i in row j: positions of operands
+            const int at_j = operand_at(j), at_i = operand_at(16 * ti + 4 * grp);
+            const float kj = inv_k[j];
+            const f32x4 ki = load4(inv_k + 16 * ti + 4 * grp), qi = load4(inv_q + 16 * ti + 4 * grp);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int i = 16 * ti + 4 * grp + r;
                 const float a = r1[n][r], b = r2[n][r];
-                put(0, i, j, a * inv_k[j], a_scale);
-                put(1, j, i, a * inv_q[i], t_scale);
+                put(0, i, at_j, a * kj, a_scale);
+                put(1, j, at_i + r, a * qi[r], t_scale);
+                // (on the diagonal the upper half is the lower's mirror: what is not below goes to a row's padding)
+                put(2, i, ti != tj || i >= j ? at_j : C, b * kj, b_scale);
+                put(2, j, ti != tj || i > j ? at_i + r : C, b * ki[r], b_scale);
                 if (ti != tj) {
-                    put(2, i, j, b * inv_k[j], b_scale);
-                    put(2, j, i, b * inv_k[i], b_scale);
-                    put(0, j, i, 0.f, 0.f);
-                    put(1, i, j, 0.f, 0.f);
-                } else if (i >= j) {
-                    put(2, i, j, b * inv_k[j], b_scale);
-                    if (i > j)
-                        put(2, j, i, b * inv_k[i], b_scale);
+                    put(0, j, at_i + r, 0.f, 0.f);
+                    put(1, i, at_j, 0.f, 0.f);
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
         __syncthreads();
         auto square = [&](int matrix, int tile, int b) {
@@ -748,7 +763,7 @@ __global__ __launch_bounds__(512, 2) void inputs_back_kernel(const DeltaJob job,
         };
 #pragma unroll
         for (int tw = 0; tw < TW; ++tw) {
-            const int t = wave + 8 * tw;
+            const int t = wave + WAVES * tw;
             if (t >= DT)
                 continue;
             u32x4 kf[PIECES][2], qf[PIECES][2];
@@ -788,7 +803,7 @@ __global__ __launch_bounds__(512, 2) void inputs_back_kernel(const DeltaJob job,
     }
 #pragma unroll
     for (int tw = 0; tw < TW; ++tw) {
-        const int t = wave + 8 * tw;
+        const int t = wave + WAVES * tw;
         if (t >= DT)
             continue;
         const Columns<Scalar> to(dk_step, Dk, grp, 16 * t + row);
@@ -821,22 +836,23 @@ hipError_t backward_typed(const DeltaJob &job, const DeltaWork &work, const Delt
     constexpr int V = 16 / static_cast<int>(sizeof(Scalar));
     const bool pieces = rows_whole<Scalar>(job) && job.Dv % V == 0 && reinterpret_cast<uintptr_t>(grads.d_o) % 16 == 0 &&
                         (grads.d_o_at[0] | grads.d_o_at[1] | grads.d_o_at[2]) % V == 0;
-#define RAMNET_BACK(DT)                                                                                            \
-    if constexpr (delta_trains<DT, PIECES>) {                                                                      \
-        if (wide == 16 * DT) {                                                                                     \
-            constexpr int each = ChunkLds<DT, PIECES, true>::kBytes, bufs = 2 * each <= kLdsBytes ? 2 : 1;         \
-            constexpr int back = BackLds<DT, PIECES, LO>::kBytes;                                                  \
-            hipLaunchKernelGGL((chain_back_kernel<Scalar, DT, PIECES, bufs>), dim3(static_cast<unsigned>(blocks)), \
-                               dim3(512), bufs * each, stream, job, work, grads, groups);                          \
-            if (const hipError_t err = hipGetLastError())                                                          \
-                return err;                                                                                        \
-            if (pieces)                                                                                            \
-                hipLaunchKernelGGL((inputs_back_kernel<Scalar, DT, PIECES, LO, true>), dim3(work.chunks, job.Hk),  \
-                                   dim3(512), back, stream, job, work, grads);                                     \
-            else                                                                                                   \
-                hipLaunchKernelGGL((inputs_back_kernel<Scalar, DT, PIECES, LO, false>), dim3(work.chunks, job.Hk), \
-                                   dim3(512), back, stream, job, work, grads);                                     \
-        }                                                                                                          \
+#define RAMNET_BACK(DT)                                                                                                   \
+    if constexpr (delta_trains<DT, PIECES>) {                                                                             \
+        if (wide == 16 * DT) {                                                                                            \
+            constexpr int each = ChunkLds<DT, PIECES, true>::kBytes, bufs = 2 * each <= kLdsBytes ? 2 : 1;                \
+            constexpr int back = BackLds<DT, PIECES, LO>::kBytes;                                                         \
+            hipLaunchKernelGGL((chain_back_kernel<Scalar, DT, PIECES, bufs>), dim3(static_cast<unsigned>(blocks)),        \
+                               dim3(512), bufs * each, stream, job, work, grads, groups);                                 \
+            if (const hipError_t err = hipGetLastError())                                                                 \
+                return err;                                                                                               \
+            constexpr int waves = DT == 2 || (DT <= 8 && PIECES == 1) ? 8 : 4;                                            \
+            if (pieces)                                                                                                   \
+                hipLaunchKernelGGL((inputs_back_kernel<Scalar, DT, PIECES, LO, true, waves>), dim3(work.chunks, job.Hk),  \
+                                   dim3(kWave * waves), back, stream, job, work, grads);                                  \
+            else                                                                                                          \
+                hipLaunchKernelGGL((inputs_back_kernel<Scalar, DT, PIECES, LO, false, waves>), dim3(work.chunks, job.Hk), \
+                                   dim3(kWave * waves), back, stream, job, work, grads);                                  \
+        }                                                                                                                 \
     }
     RAMNET_BACK(2)
     RAMNET_BACK(4)
