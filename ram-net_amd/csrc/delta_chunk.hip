@@ -314,10 +314,18 @@ __global__ __launch_bounds__(256) void prepare_kernel(const DeltaJob job, const 
 // The states from chunk to chunk. Columns of S do not meet: each of the first
 // four waves keeps 16 of them in registers and needs no other wave's results.
 // The other four bring the next chunk's K and Q to LDS as matrix operands.
+//
+// A row's chunks can be cut into segments that run side by side: the states
+// are linear in the state before. A first launch (MAP) runs the segments but
+// the last from zeros and, with no values, from each unit vector: the second
+// gives the matrix that a segment multiplies the state before it with.
+// join_kernel puts the states at the segments' ends together, and the chain
+// proper starts each segment from there.
+//
 // DT: Dk in tiles of 16; PIECES: fp16 parts of q and k; LO: whether products
 // that go to o alone take the second parts too (bf16 outputs do not show them:
 // their rounding is 2^-9, what is left out 2^-12).
-template<typename Scalar, int DT, int PIECES, bool LO, int BUFS>
+template<typename Scalar, int DT, int PIECES, bool LO, int BUFS, bool MAP>
 __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const DeltaWork work, int groups) {
     extern __shared__ __align__(16) float lds_base[];
     using Lds = ChunkLds<DT, PIECES, false>;
@@ -325,12 +333,23 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
     const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave, wave = uniform(tid / kWave);
     const int row = lane & 15, grp = lane >> 4;
     const int group = static_cast<int>(blockIdx.x) % groups;
-    const int head = static_cast<int>(blockIdx.x) / groups % job.Hv;
-    const int n = static_cast<int>(blockIdx.x) / groups / job.Hv;
+    const int part = static_cast<int>(blockIdx.x) / groups % (MAP ? work.parts - 1 : work.parts);
+    const int line = static_cast<int>(blockIdx.x) / groups / (MAP ? work.parts - 1 : work.parts);
+    const int head = line % job.Hv, n = line / job.Hv;
     const int kh = head / (job.Hv / job.Hk);
-    const DeltaSpan span = delta_span(job, n);
+    const int tiles = (job.Dv + 15) / 16;
+    if (MAP && part == 0 && group * 4 >= tiles)
+        return;  // (the first segment starts from the row's own state)
+    DeltaSpan span = delta_span(job, n);
+    const int row_end = span.len;
     int first, count;
     delta_chunks(job, work, n, span, first, count);
+    if (work.parts > 1) {
+        const int from = min(part * work.part_chunks, count);
+        first += from;
+        count = min(count - from, work.part_chunks);
+        span.t0 += from * C, span.len -= from * C;
+    }
     auto buffer = [&](int i) {
         return Lds{reinterpret_cast<uint16_t *>(reinterpret_cast<char *>(lds_base) + (BUFS == 2 ? (i & 1) * Lds::kBytes : 0))};
     };
@@ -343,12 +362,12 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
         Stager<Scalar, DT, PIECES, false> stager;
         auto load = [&](int i) {
             const int64_t t0 = span.t0 + i * C;
-            stager.load(k + t0 * job.k_at[1], job.k_at[1], q + t0 * job.q_at[1], job.q_at[1], min(C, span.len - i * C),
+            stager.template load<!MAP>(k + t0 * job.k_at[1], job.k_at[1], q + t0 * job.q_at[1], job.q_at[1], min(C, span.len - i * C),
                         job.Dk, whole, work.vec + (static_cast<int64_t>(first + i) * job.Hv + head) * kVecs * C, at);
         };
         if (count > 0) {
             load(0);
-            stager.store(buffer(0), at);
+            stager.template store<!MAP>(buffer(0), at);
         }
         __syncthreads();
         for (int i = 0; i < count; ++i) {
@@ -357,18 +376,30 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
             if constexpr (BUFS == 1)
                 __syncthreads();  // chunk i is done with
             if (i + 1 < count)
-                stager.store(buffer(i + 1), at);
+                stager.template store<!MAP>(buffer(i + 1), at);
             __syncthreads();
         }
         return;
     }
 
-    const int c = (group * 4 + wave) * 16 + row;
-    const int64_t matrix = (static_cast<int64_t>(n) * job.Hv + head) * job.Dk * job.Dv;
+    const int tile = group * 4 + wave;
+    const bool is_map = MAP && tile >= tiles;
+    const int c = (is_map ? tile - tiles : tile) * 16 + row;
+    const int64_t matrix = static_cast<int64_t>(line) * job.Dk * job.Dv;
+    const int64_t piece = static_cast<int64_t>(line) * work.parts + part;  // of the segments' buffers
     const Columns<float> state(job.Dv, job.Dv, grp, c), kept(delta_row(job.Dv), delta_row(job.Dv), grp, c);
     f32x4 s[DT];
-    {
-        const auto from = state.rows(job.init + matrix, job.init ? job.Dk : 0);
+    if (is_map) {
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                s[t][r] = 16 * t + 4 * grp + r == c && c < job.Dk ? 1.f : 0.f;
+    } else {
+        const float *init = part == 0 ? job.init ? job.init + matrix : nullptr
+                            : MAP     ? nullptr
+                                      : work.ends + (piece - 1) * job.Dk * job.Dv;
+        const auto from = state.rows(init, init ? job.Dk : 0);
         state.each<DT>([&](int t, int r, int at) { s[t][r] = __uint_as_float(buffer_bits<float>(from, at)); });
     }
     const Scalar *v = static_cast<const Scalar *>(job.v) + span.b * job.v_at[0] + head * job.v_at[2] +
@@ -380,7 +411,7 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
     uint32_t v_bits[16];
     auto load_v = [&](int i) {
-        const auto from = v_cols.rows(v + static_cast<int64_t>(i) * C * job.v_at[1], min(C, span.len - i * C));
+        const auto from = v_cols.rows(v + static_cast<int64_t>(i) * C * job.v_at[1], is_map ? 0 : min(C, span.len - i * C));
         v_cols.template each<4>([&](int m, int r, int at) { v_bits[4 * m + r] = buffer_bits<Scalar>(from, at); });
     };
     // the next chunk's operands are asked for as soon as this one's have been used
@@ -405,7 +436,8 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
     if (count > 0) {
         load_v(0);
         load_y(0);
-        load_p(0);
+        if constexpr (!MAP)
+            load_p(0);
     }
     __syncthreads();
 
@@ -414,7 +446,7 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
         const Lds lds = buffer(i);
         const float *vec = lds.vec();
         const float total = vec[kVecGrowK * C + C - 1] * vec[kVecSk * C + C - 1];  // (a power of two: e^gamma_C)
-        if (work.states) {
+        if (!MAP && work.states) {
             const auto to = kept.rows(work.states + record * job.Dk * delta_row(job.Dv), job.Dk);
             kept.each<DT>([&](int t, int r, int at) { buffer_store<float>(s[t][r], to, at); });
         }
@@ -432,15 +464,18 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
             for (int b = 0; b < BT; ++b) {
 #pragma unroll
                 for (int m = 0; m < 4; ++m) {
-                    const u32x4 kf = lds.row_frag(lds.k(0), m, b, lane), qf = lds.row_frag(lds.q(0), m, b, lane);
+                    const u32x4 kf = lds.row_frag(lds.k(0), m, b, lane);
                     g[m] = mfma16(kf, so.hi[b], g[m]);
-                    qo[m] = mfma16(qf, so.hi[b], qo[m]);
                     g[m] = mfma16(kf, so.lo[b], g[m]);
-                    if constexpr (LO)
-                        qo[m] = mfma16(qf, so.lo[b], qo[m]);
-                    if constexpr (PIECES == 2) {
+                    if constexpr (PIECES == 2)
                         g[m] = mfma16(lds.row_frag(lds.k(1), m, b, lane), so.hi[b], g[m]);
-                        qo[m] = mfma16(lds.row_frag(lds.q(1), m, b, lane), so.hi[b], qo[m]);
+                    if constexpr (!MAP) {
+                        const u32x4 qf = lds.row_frag(lds.q(0), m, b, lane);
+                        qo[m] = mfma16(qf, so.hi[b], qo[m]);
+                        if constexpr (LO)
+                            qo[m] = mfma16(qf, so.lo[b], qo[m]);
+                        if constexpr (PIECES == 2)
+                            qo[m] = mfma16(lds.row_frag(lds.q(1), m, b, lane), so.hi[b], qo[m]);
                     }
                 }
             }
@@ -475,11 +510,11 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
             if (i + 1 < count)
                 load_y(i + 1);
         }
-        if (work.e) {
+        if (!MAP && work.e) {
             const auto to = kept.rows(work.e + record * C * delta_row(job.Dv), C);
             kept.each<4>([&](int m, int r, int at) { buffer_store<float>(e[m][r], to, at); });
         }
-        {
+        if constexpr (!MAP) {
             Operand<4, LO> eo;
             eo.set(e);
 #pragma unroll
@@ -525,13 +560,70 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
         if constexpr (BUFS == 1)
             __syncthreads();  // chunk i + 1 is there
     }
-    const auto to = state.rows(job.state + matrix, job.Dk);
+    if (is_map) {
+        if (tile < tiles + DT) {
+            constexpr int wide = 16 * DT;
+            const Columns<float> map(wide, wide, grp, c);
+            const auto to = map.rows(work.maps + piece * wide * wide, wide);
+            map.each<DT>([&](int t, int r, int at) { buffer_store<float>(s[t][r], to, at); });
+        }
+        return;
+    }
+    if (!MAP && part + 1 < work.parts)
+        return;
+    const auto to = state.rows(MAP ? work.ends + piece * job.Dk * job.Dv : job.state + matrix, job.Dk);
     state.each<DT>([&](int t, int r, int at) { buffer_store<float>(s[t][r], to, at); });
-    if (!job.cu && c < job.Dv)  // tokens that do not count
-        for (int64_t t = span.len + grp; t < job.T; t += 4)
-            store_f32(o + t * o_step + c, 0.f);
+    if (!MAP && !job.cu && c < job.Dv)  // tokens that do not count
+        for (int64_t t = row_end + grp; t < job.T; t += 4)
+            store_f32(o + (t - (row_end - span.len)) * o_step + c, 0.f);
 }
 
+// The states at the ends of a row's segments: what the segment adds, and its
+// map times the state before. One block per row, head and 16 columns, a wave a
+// tile of Dk: few small products one after the other, in fp32 instructions.
+template<int DT>
+__global__ __launch_bounds__(kWave *DT) void join_kernel(const DeltaJob job, const DeltaWork work, int groups) {
+    constexpr int wide = 16 * DT;
+    __shared__ __align__(16) float s[2][16][wide + 4];  // columns of the state before
+    const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave, wave = uniform(tid / kWave);
+    const int row = lane & 15, grp = lane >> 4;
+    const int group = static_cast<int>(blockIdx.x) % groups, line = static_cast<int>(blockIdx.x) / groups;
+    const int c = group * 16 + row, d = 16 * wave + 4 * grp;
+    const int64_t piece = static_cast<int64_t>(line) * work.parts, size = static_cast<int64_t>(job.Dk) * job.Dv;
+    const Columns<float> state(job.Dv, job.Dv, grp, c);
+    auto ends = [&](int i) { return work.ends + (piece + i) * size + static_cast<int64_t>(16 * wave) * job.Dv; };
+    const int rows = job.Dk - 16 * wave;  // (of this tile and those after it)
+    auto load = [&](int i) {
+        f32x4 x;
+        const auto from = state.rows(ends(i), rows);
+        state.each<1>([&](int, int r, int at) { x[r] = __uint_as_float(buffer_bits<float>(from, at)); });
+        return x;
+    };
+    *reinterpret_cast<f32x4 *>(&s[0][row][d]) = load(0);
+    f32x4 next = load(1), map[DT];
+    auto load_map = [&](int i) {
+        const float *from = work.maps + (piece + i) * wide * wide + (16 * wave + row) * wide + 4 * grp;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+            map[t] = load4(from + 16 * t);
+    };
+    load_map(1);
+    __syncthreads();
+    for (int i = 1; i + 1 < work.parts; ++i) {
+        f32x4 x = next;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+            x = mfma4(map[t], load4(&s[(i + 1) & 1][row][16 * t + 4 * grp]), x);
+        if (i + 2 < work.parts) {
+            next = load(i + 1);
+            load_map(i + 1);
+        }
+        const auto to = state.rows(ends(i), rows);
+        state.each<1>([&](int, int r, int at) { buffer_store<float>(x[r], to, at); });
+        *reinterpret_cast<f32x4 *>(&s[i & 1][row][d]) = x;
+        __syncthreads();
+    }
+}
 
 template<typename Scalar>
 hipError_t prepare_typed(const DeltaJob &job, const DeltaWork &work, bool backward, hipStream_t stream) {
@@ -555,27 +647,40 @@ template<typename Scalar, int DT>
 constexpr bool kChainFits = ChunkLds<DT, sizeof(Scalar) == 4 ? 2 : 1, false>::kBytes <= kLdsBytes;
 
 template<typename Scalar, int DT>
-void chain_launch(const DeltaJob &job, const DeltaWork &work, unsigned blocks, int groups, hipStream_t stream) {
+hipError_t chain_launch(const DeltaJob &job, const DeltaWork &work, hipStream_t stream, const char **why) {
     constexpr int PIECES = sizeof(Scalar) == 4 ? 2 : 1;
     constexpr bool LO = !__is_same(Scalar, bf16_t);
     constexpr int bytes = ChunkLds<DT, PIECES, false>::kBytes;
     constexpr int BUFS = 2 * bytes <= kLdsBytes ? 2 : 1;
-    hipLaunchKernelGGL((chain_kernel<Scalar, DT, PIECES, LO, BUFS>), dim3(blocks), dim3(512), BUFS * bytes, stream, job,
-                       work, groups);
+    const int tiles = (job.Dv + 15) / 16, groups = (tiles + 3) / 4, map_groups = (tiles + DT + 3) / 4;
+    const int64_t lines = static_cast<int64_t>(job.N) * job.Hv;
+    if (lines * work.parts * map_groups > 0x7fffffff || lines * tiles > 0x7fffffff) {
+        *why = "delta rule: too many state columns for one launch";
+        return hipErrorInvalidValue;
+    }
+    auto blocks = [&](int64_t n) { return dim3(static_cast<unsigned>(n)); };
+    if (work.parts > 1) {
+        hipLaunchKernelGGL((chain_kernel<Scalar, DT, PIECES, LO, BUFS, true>), blocks(lines * (work.parts - 1) * map_groups),
+                           dim3(512), BUFS * bytes, stream, job, work, map_groups);
+        if (const hipError_t err = hipGetLastError())
+            return err;
+        if (work.parts > 2)
+            hipLaunchKernelGGL(join_kernel<DT>, blocks(lines * tiles), dim3(kWave * DT), 0, stream, job, work, tiles);
+        if (const hipError_t err = hipGetLastError())
+            return err;
+    }
+    hipLaunchKernelGGL((chain_kernel<Scalar, DT, PIECES, LO, BUFS, false>), blocks(lines * work.parts * groups), dim3(512),
+                       BUFS * bytes, stream, job, work, groups);
+    return hipGetLastError();
 }
 
 template<typename Scalar>
 hipError_t chain_typed(const DeltaJob &job, const DeltaWork &work, hipStream_t stream, const char **why) {
-    const int wide = delta_padded(job.Dk), groups = (job.Dv + 63) / 64;
-    const int64_t blocks = static_cast<int64_t>(job.N) * job.Hv * groups;
-    if (blocks > 0x7fffffff) {
-        *why = "delta rule: too many state columns for one launch";
-        return hipErrorInvalidValue;
-    }
+    const int wide = delta_padded(job.Dk);
 #define RAMNET_CHAIN(DT)                           \
     if constexpr (kChainFits<Scalar, DT>)          \
         if (wide == 16 * DT)                       \
-    chain_launch<Scalar, DT>(job, work, static_cast<unsigned>(blocks), groups, stream)
+    return chain_launch<Scalar, DT>(job, work, stream, why)
     RAMNET_CHAIN(2);
     RAMNET_CHAIN(4);
     RAMNET_CHAIN(6);
@@ -583,7 +688,7 @@ hipError_t chain_typed(const DeltaJob &job, const DeltaWork &work, hipStream_t s
     RAMNET_CHAIN(10);
     RAMNET_CHAIN(16);
 #undef RAMNET_CHAIN
-    return hipGetLastError();
+    return hipErrorInvalidValue;
 }
 
 }  // namespace
@@ -616,8 +721,24 @@ void count_chunks(const DeltaJob &job, bool packed, DeltaWork *work) {
 
 }  // namespace
 
+// Segments of a row: as many as fill the GPU's 256 compute units with blocks of
+// 64 columns, each at least kPartChunks long. A segment's map costs its state
+// columns once more, so half full is left as it is: one row of 32768 tokens, 8
+// heads of 128 x 128 (16 blocks), takes 1.59 ms in one segment.
+void count_parts(const DeltaJob &job, bool packed, DeltaWork *work) {
+    constexpr int kUnits = 256, kPartChunks = 8;
+    const int64_t blocks = static_cast<int64_t>(job.N) * job.Hv * ((job.Dv + 63) / 64);
+    work->parts = 1, work->part_chunks = work->per_row;
+    if (packed || blocks > kUnits / 4 || work->per_row < 2 * kPartChunks)
+        return;
+    const int parts = std::min(static_cast<int>(kUnits / blocks), work->per_row / kPartChunks);
+    work->part_chunks = (work->per_row + parts - 1) / parts;
+    work->parts = (work->per_row + work->part_chunks - 1) / work->part_chunks;
+}
+
 int64_t delta_layout(const DeltaJob &job, bool packed, bool backward, char *base, DeltaWork *work) {
     count_chunks(job, packed, work);
+    count_parts(job, packed || backward, work);
     Carver carve{base};
     const int64_t records = static_cast<int64_t>(work->chunks) * job.Hv, square = kDeltaChunk * kDeltaChunk;
     work->offsets = packed ? carve.take<int32_t>(job.N + 1) : nullptr;
@@ -625,6 +746,11 @@ int64_t delta_layout(const DeltaJob &job, bool packed, bool backward, char *base
     work->vec = carve.take<float>(records * kVecs * kDeltaChunk);
     work->y = carve.take<uint32_t>(records * 2 * kFragWords);
     work->p_frags = carve.take<uint32_t>(records * 2 * kFragWords);
+    if (work->parts > 1) {
+        const int64_t pieces = static_cast<int64_t>(job.N) * job.Hv * work->parts, wide = delta_padded(job.Dk);
+        work->ends = carve.take<float>(pieces * job.Dk * job.Dv);
+        work->maps = carve.take<float>(pieces * wide * wide);
+    }
     if (backward) {
         work->p = carve.take<float>(records * square);
         work->bl = carve.take<float>(records * square);

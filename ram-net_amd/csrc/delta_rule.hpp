@@ -41,6 +41,11 @@ struct DeltaWork {
     float *dstate;     // [record][Dk][..] gradient after the chunk  (backward)
     float *e;          // [record][64][..] v - S^T k of each token   (kept)
     float *states;     // [record][Dk][..] state before the chunk    (kept)
+    // where the time axis of a row is cut into segments that run side by side (parts > 1),
+    // per row, value head and segment:
+    float *ends;       // [Dk][Dv] state after the segment: first from zeros (the first from init), then in full
+    float *maps;       // [wide][wide] what the segment makes of the state before it
+    int parts, part_chunks;
     int per_row;       // chunks of a row where sequences are rows
     int chunks;        // records / Hv
 };

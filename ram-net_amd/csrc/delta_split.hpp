@@ -235,13 +235,15 @@ struct Stager {
         }
     }
 
+    template<bool Q = true>
     __device__ __forceinline__ void load(const Scalar *k, int64_t k_step, const Scalar *q, int64_t q_step, int len, int Dk,
                                          bool whole, const float *vec, int tid) {
         vecs[0] = vec[tid], vecs[1] = vec[tid + 256];
         scales[0] = load4(vec + kVecSk * kDeltaChunk + tid % 16 * 4);
         scales[1] = load4(vec + kVecSq * kDeltaChunk + tid % 16 * 4);
         load_one(k, k_step, len, Dk, whole, tid, raw[0]);
-        load_one(q, q_step, len, Dk, whole, tid, raw[1]);
+        if constexpr (Q)
+            load_one(q, q_step, len, Dk, whole, tid, raw[1]);
     }
 
     static __device__ __forceinline__ float value(const uint32_t (&w)[kWords], int i) {
@@ -295,10 +297,12 @@ struct Stager {
         }
     }
 
+    template<bool Q = true>
     __device__ __forceinline__ void store(const Lds &lds, int tid) const {
         lds.vec()[tid] = vecs[0], lds.vec()[tid + 256] = vecs[1];
         store_one(raw[0], scales[0], tid, lds.k(0), lds.kt(0));
-        store_one(raw[1], scales[1], tid, QT ? nullptr : lds.q(0), QT ? lds.qt(0) : nullptr);
+        if constexpr (Q)
+            store_one(raw[1], scales[1], tid, QT ? nullptr : lds.q(0), QT ? lds.qt(0) : nullptr);
     }
 };
 

@@ -143,6 +143,29 @@ def test_counted_lengths(T):
     assert torch.equal(got[1][1].cpu(), case[5][1])  # no tokens: the state as it was
 
 
+@pytest.mark.parametrize("T,Dk,Dv,dtype", [(1024, 16, 16, "fp32"), (1100, 40, 24, "fp32"), (2049, 128, 100, "bf16"),
+                                           (1600, 200, 72, "fp16")])
+def test_long_rows(T, Dk, Dv, dtype):
+    """Rows long enough to be cut into segments that run side by side."""
+    _check(_case(T=T, Hk=1, Hv=2, Dk=Dk, Dv=Dv, dtype=dtype, seed=T), _call(_case(T=T, Hk=1, Hv=2, Dk=Dk, Dv=Dv,
+                                                                                 dtype=dtype, seed=T)))
+
+
+def test_long_rows_counted_lengths():
+    T, lens = 1500, [1500, 0, 1, 512, 700]
+    case = _case(B=5, T=T, Hk=1, Hv=1, Dk=24, Dv=40, seed=2)
+    got = _call(case, lengths=torch.tensor(lens, device=DEV))
+    _check(case, got, lens)
+    for b, n in enumerate(lens):
+        assert (got[0][b, n:] == 0).all()
+    case[5] = None
+    _check(case, _call(case, lengths=torch.tensor(lens, device=DEV)), lens)
+
+
+def test_long_rows_gradients():
+    _check_grads(_case(T=1100, Hk=1, Hv=2, Dk=24, Dv=40, seed=3))
+
+
 @pytest.mark.parametrize("T", [4, 129])
 def test_steps_continue_a_state(T):
     """A prompt in two calls, the second in place, is the prompt in one."""
