@@ -488,26 +488,34 @@ int ramnet_segment_call_form(int64_t B, int64_t H, int64_t T, int64_t A, int64_t
  * Sums, states and norms are fp32, decays' sums within a chunk fp64.
  * Requires Dk <= 256, Hv a multiple of Hk.
  */
-int ramnet_delta_rule_forward(const void *q, const void *k, const void *v, int dtype, const void *g, int g_dtype,
-                              const void *beta, int beta_dtype, const float *init_state, float *state, void *o,
-                              const int32_t *cu_seqlens, const int32_t *lengths, int64_t B, int64_t T, int64_t N,
-                              int64_t Hk, int64_t Hv, int64_t Dk, int64_t Dv, float scale, const int64_t *strides,
-                              void *kept, int64_t kept_bytes, void *workspace, int64_t workspace_bytes, void *stream);
+typedef struct ramnet_delta_rule_call {
+    const void *q, *k, *v, *g, *beta;
+    const float *init_state;
+    float *state;
+    void *o;
+    const int32_t *cu_seqlens, *lengths;
+    void *kept, *workspace;
+    int64_t kept_bytes, workspace_bytes;
+    int64_t B, T, N, Hk, Hv, Dk, Dv;
+    int64_t strides[15];
+    int64_t dtype, g_dtype, beta_dtype;
+    double scale;
+} ramnet_delta_rule_call;
+
+int ramnet_delta_rule_forward(const ramnet_delta_rule_call *call, void *stream);
 
 /*
- * Its gradients, from d_o (B, T, Hv, Dv) `dtype` and d_state (N, Hv, Dk, Dv)
- * fp32 (or NULL: zeros): dq, dk, dv, dg, dbeta in their inputs' shapes and
- * types, dense, and dinit (N, Hv, Dk, Dv) fp32 (or NULL). `strides` are the
- * forward's 15 and three of d_o; `workspace` of kind 2. Value heads that share
- * a key head add to its gradient in one order: results do not change from
- * call to call. float32 inputs take Dk up to 160 here.
+ * Its gradients, from d_o (B, T, Hv, Dv) `dtype`, of strides d_o_strides (batch
+ * row, token, head), and d_state (N, Hv, Dk, Dv) fp32 (or NULL: zeros): dq, dk,
+ * dv, dg, dbeta in their inputs' shapes and types, dense, and dinit (N, Hv, Dk,
+ * Dv) fp32 (or NULL). `call` is the forward's, with a workspace of kind 2; its
+ * init_state, state and o are not read. Value heads that share a key head add
+ * to its gradient in one order: results do not change from call to call.
+ * float32 inputs take Dk up to 160 here.
  */
-int ramnet_delta_rule_backward(const void *q, const void *k, const void *v, int dtype, const void *g, int g_dtype,
-                               const void *beta, int beta_dtype, const int32_t *cu_seqlens, const int32_t *lengths,
-                               const void *d_o, const float *d_state, void *dq, void *dk, void *dv, void *dg,
-                               void *dbeta, float *dinit, int64_t B, int64_t T, int64_t N, int64_t Hk, int64_t Hv,
-                               int64_t Dk, int64_t Dv, float scale, const int64_t *strides, const void *kept,
-                               int64_t kept_bytes, void *workspace, int64_t workspace_bytes, void *stream);
+int ramnet_delta_rule_backward(const ramnet_delta_rule_call *call, const void *d_o, const int64_t *d_o_strides,
+                               const float *d_state, void *dq, void *dk, void *dv, void *dg, void *dbeta, float *dinit,
+                               void *stream);
 
 /* Bytes of their device workspace (kind 0: forward, 1: forward that keeps, 2:
  * backward) and of what a forward keeps; -1 for sizes they do not take. */

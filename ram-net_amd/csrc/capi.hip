@@ -1185,10 +1185,26 @@ int64_t ramnet_delta_rule_kept_bytes(int64_t B, int64_t T, int64_t N, int64_t Hk
     return ramnet::delta_kept(job, packed != 0, nullptr, &work);
 }
 
-static int delta_strides(ramnet::DeltaJob &job, const int64_t *strides) {
+// What forward and backward check alike.
+static int delta_job(ramnet::DeltaJob &job, const ramnet_delta_rule_call &c) {
+    if (int rc = check_delta(job, c.B, c.T, c.N, c.Hk, c.Hv, c.Dk, c.Dv, c.cu_seqlens != nullptr))
+        return rc;
+    RAMNET_REQUIRE(valid_dtype(static_cast<int>(c.dtype)) && valid_dtype(static_cast<int>(c.g_dtype)) &&
+                       valid_dtype(static_cast<int>(c.beta_dtype)),
+                   "delta rule dtype must be float32, float16 or bfloat16");
+    RAMNET_REQUIRE(!(c.cu_seqlens && c.lengths), "delta rule: packed sequences have no lengths beside their bounds");
+    job.q = c.q, job.k = c.k, job.v = c.v, job.g = c.g, job.beta = c.beta;
+    job.init = c.init_state, job.state = c.state, job.o = c.o;
+    job.cu = c.cu_seqlens, job.lengths = c.lengths;
+    job.dtype = static_cast<int>(c.dtype), job.g_dtype = static_cast<int>(c.g_dtype);
+    job.beta_dtype = static_cast<int>(c.beta_dtype);
+    job.scale = static_cast<float>(c.scale);
+    if (job.N == 0)
+        return RAMNET_OK;
+    RAMNET_REQUIRE(job.T == 0 || (c.q && c.k && c.v && c.g && c.beta), "null tensor pointer");
     int64_t *to[5] = {job.q_at, job.k_at, job.v_at, job.g_at, job.beta_at};
     for (int i = 0; i < 15; ++i)
-        to[i / 3][i % 3] = strides[i];
+        to[i / 3][i % 3] = c.strides[i];
     if (job.T == 1)  // (any, there is no second token)
         job.q_at[1] = job.k_at[1] = job.Dk, job.v_at[1] = job.Dv;
     if (int rc = check_delta_rows("q", job.T, job.q_at[1], job.Dk))
@@ -1198,76 +1214,57 @@ static int delta_strides(ramnet::DeltaJob &job, const int64_t *strides) {
     return check_delta_rows("v", job.T, job.v_at[1], job.Dv);
 }
 
-int ramnet_delta_rule_forward(const void *q, const void *k, const void *v, int dtype, const void *g, int g_dtype,
-                              const void *beta, int beta_dtype, const float *init_state, float *state, void *o,
-                              const int32_t *cu_seqlens, const int32_t *lengths, int64_t B, int64_t T, int64_t N,
-                              int64_t Hk, int64_t Hv, int64_t Dk, int64_t Dv, float scale, const int64_t *strides,
-                              void *kept, int64_t kept_bytes, void *workspace, int64_t workspace_bytes, void *stream) {
+static int delta_regions(const ramnet::DeltaJob &job, const ramnet_delta_rule_call &c, bool backward, ramnet::DeltaWork &work) {
+    const bool packed = job.cu != nullptr;
+    if (c.kept) {
+        const int64_t need = ramnet::delta_kept(job, packed, static_cast<char *>(c.kept), &work);
+        RAMNET_REQUIRE(need >= 0, "delta rule: gradients of float32 take Dk up to 160");
+        RAMNET_REQUIRE(c.kept_bytes >= need, "delta rule: kept region too small");
+    }
+    RAMNET_REQUIRE(c.workspace && c.workspace_bytes >= ramnet::delta_layout(job, packed, backward,
+                                                                            static_cast<char *>(c.workspace), &work),
+                   "delta rule: workspace too small");
+    return RAMNET_OK;
+}
+
+int ramnet_delta_rule_forward(const ramnet_delta_rule_call *call, void *stream) {
+    RAMNET_REQUIRE(call, "null call");
     ramnet::DeltaJob job{};
-    if (int rc = check_delta(job, B, T, N, Hk, Hv, Dk, Dv, cu_seqlens != nullptr))
+    if (int rc = delta_job(job, *call))
         return rc;
-    RAMNET_REQUIRE(valid_dtype(dtype) && valid_dtype(g_dtype) && valid_dtype(beta_dtype),
-                   "delta rule dtype must be float32, float16 or bfloat16");
-    RAMNET_REQUIRE(!(cu_seqlens && lengths), "delta rule: packed sequences have no lengths beside their bounds");
-    if (N == 0)
+    if (job.N == 0)
         return RAMNET_OK;
-    RAMNET_REQUIRE(strides && state && (T == 0 || (q && k && v && g && beta && o)), "null tensor pointer");
-    job.q = q, job.k = k, job.v = v, job.g = g, job.beta = beta, job.init = init_state, job.state = state, job.o = o;
-    job.cu = cu_seqlens, job.lengths = lengths, job.dtype = dtype, job.g_dtype = g_dtype, job.beta_dtype = beta_dtype;
-    job.scale = scale;
-    if (int rc = delta_strides(job, strides))
-        return rc;
+    RAMNET_REQUIRE(job.state && (job.T == 0 || job.o), "null tensor pointer");
     const char *why = nullptr;
     const hipStream_t on = static_cast<hipStream_t>(stream);
-    if (T == 0 || (!kept && ramnet::delta_is_recurrent(job)))
+    if (job.T == 0 || (!call->kept && ramnet::delta_is_recurrent(job)))
         return finish(ramnet::launch_delta_recurrent(job, on, &why), why, "delta rule launch");
     ramnet::DeltaWork work{};
-    if (kept) {
-        const int64_t need = ramnet::delta_kept(job, cu_seqlens != nullptr, static_cast<char *>(kept), &work);
-        RAMNET_REQUIRE(need >= 0, "delta rule: gradients of float32 take Dk up to 160");
-        RAMNET_REQUIRE(kept_bytes >= need, "delta rule: kept region too small");
-    }
-    RAMNET_REQUIRE(workspace && workspace_bytes >= ramnet::delta_layout(job, cu_seqlens != nullptr, false,
-                                                                        static_cast<char *>(workspace), &work),
-                   "delta rule: workspace too small");
+    if (int rc = delta_regions(job, *call, false, work))
+        return rc;
     hipError_t err = ramnet::launch_delta_prepare(job, work, false, on, &why);
     if (err == hipSuccess)
         err = ramnet::launch_delta_chain(job, work, on, &why);
     return finish(err, why, "delta rule launch");
 }
 
-int ramnet_delta_rule_backward(const void *q, const void *k, const void *v, int dtype, const void *g, int g_dtype,
-                               const void *beta, int beta_dtype, const int32_t *cu_seqlens, const int32_t *lengths,
-                               const void *d_o, const float *d_state, void *dq, void *dk, void *dv, void *dg,
-                               void *dbeta, float *dinit, int64_t B, int64_t T, int64_t N, int64_t Hk, int64_t Hv,
-                               int64_t Dk, int64_t Dv, float scale, const int64_t *strides, const void *kept,
-                               int64_t kept_bytes, void *workspace, int64_t workspace_bytes, void *stream) {
+int ramnet_delta_rule_backward(const ramnet_delta_rule_call *call, const void *d_o, const int64_t *d_o_strides,
+                               const float *d_state, void *dq, void *dk, void *dv, void *dg, void *dbeta, float *dinit,
+                               void *stream) {
+    RAMNET_REQUIRE(call, "null call");
     ramnet::DeltaJob job{};
-    if (int rc = check_delta(job, B, T, N, Hk, Hv, Dk, Dv, cu_seqlens != nullptr))
+    if (int rc = delta_job(job, *call))
         return rc;
-    RAMNET_REQUIRE(valid_dtype(dtype) && valid_dtype(g_dtype) && valid_dtype(beta_dtype),
-                   "delta rule dtype must be float32, float16 or bfloat16");
-    RAMNET_REQUIRE(!(cu_seqlens && lengths), "delta rule: packed sequences have no lengths beside their bounds");
-    RAMNET_REQUIRE(T > 0, "delta rule: a backward call needs tokens");
-    if (N == 0)
+    RAMNET_REQUIRE(job.T > 0, "delta rule: a backward call needs tokens");
+    if (job.N == 0)
         return RAMNET_OK;
-    RAMNET_REQUIRE(strides && q && k && v && g && beta && d_o && dq && dk && dv && dg && dbeta && kept,
-                   "null tensor pointer");
-    job.q = q, job.k = k, job.v = v, job.g = g, job.beta = beta, job.cu = cu_seqlens, job.lengths = lengths;
-    job.dtype = dtype, job.g_dtype = g_dtype, job.beta_dtype = beta_dtype, job.scale = scale;
-    if (int rc = delta_strides(job, strides))
-        return rc;
+    RAMNET_REQUIRE(d_o && d_o_strides && dq && dk && dv && dg && dbeta && call->kept, "null tensor pointer");
     ramnet::DeltaWork work{};
-    const int64_t need = ramnet::delta_kept(job, cu_seqlens != nullptr,
-                                            const_cast<char *>(static_cast<const char *>(kept)), &work);
-    RAMNET_REQUIRE(need >= 0, "delta rule: gradients of float32 take Dk up to 160");
-    RAMNET_REQUIRE(kept_bytes >= need, "delta rule: kept region too small");
-    RAMNET_REQUIRE(workspace && workspace_bytes >= ramnet::delta_layout(job, cu_seqlens != nullptr, true,
-                                                                        static_cast<char *>(workspace), &work),
-                   "delta rule: workspace too small");
+    if (int rc = delta_regions(job, *call, true, work))
+        return rc;
     ramnet::DeltaGrads grads{d_o, d_state, dq, dk, dv, dg, dbeta, dinit,
-                             {strides[15], T == 1 ? Dv : strides[16], strides[17]}};
-    if (int rc = check_delta_rows("d_o", T, grads.d_o_at[1], Dv))
+                             {d_o_strides[0], job.T == 1 ? job.Dv : d_o_strides[1], d_o_strides[2]}};
+    if (int rc = check_delta_rows("d_o", job.T, grads.d_o_at[1], job.Dv))
         return rc;
     const char *why = nullptr;
     const hipStream_t on = static_cast<hipStream_t>(stream);

@@ -21,7 +21,10 @@ namespace {
 // The states' gradient from the last chunk to the first; waves as in the
 // forward's chain. The state's gradient and dv are fp32 results of fp32 values:
 // every product takes both parts of both sides (dO's own 16 bits are one part).
-template<typename Scalar, int DT, int PIECES, int BUFS>
+// Rows in segments as in the forward's chain, the last one first (PART: the
+// gradients at their starts from zeros at their ends; their maps are the
+// forward's, transposed).
+template<typename Scalar, int DT, int PIECES, int BUFS, bool PART>
 __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, const DeltaWork work,
                                                             const DeltaGrads grads, int groups) {
     extern __shared__ __align__(16) float lds_base[];
@@ -30,12 +33,22 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
     const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave, wave = uniform(tid / kWave);
     const int row = lane & 15, grp = lane >> 4;
     const int group = static_cast<int>(blockIdx.x) % groups;
-    const int head = static_cast<int>(blockIdx.x) / groups % job.Hv;
-    const int n = static_cast<int>(blockIdx.x) / groups / job.Hv;
+    const int part = static_cast<int>(blockIdx.x) / groups % (PART ? work.parts - 1 : work.parts);  // from the end
+    const int line = static_cast<int>(blockIdx.x) / groups / (PART ? work.parts - 1 : work.parts);
+    const int head = line % job.Hv, n = line / job.Hv;
     const int kh = head / (job.Hv / job.Hk);
-    const DeltaSpan span = delta_span(job, n);
+    DeltaSpan span = delta_span(job, n);
+    const int row_end = span.len;
     int first, count;
     delta_chunks(job, work, n, span, first, count);
+    int skipped = 0;
+    if (work.parts > 1) {
+        const int to = count;
+        skipped = min((work.parts - 1 - part) * work.part_chunks, to);
+        first += skipped;
+        count = min(to - skipped, work.part_chunks);
+        span.t0 += skipped * C, span.len = min(span.len - skipped * C, count * C);
+    }
     auto buffer = [&](int i) {
         return Lds{reinterpret_cast<uint16_t *>(reinterpret_cast<char *>(lds_base) + (BUFS == 2 ? (i & 1) * Lds::kBytes : 0))};
     };
@@ -69,11 +82,15 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
     }
 
     const int c = (group * 4 + wave) * 16 + row;
-    const int64_t matrix = (static_cast<int64_t>(n) * job.Hv + head) * job.Dk * job.Dv;
+    const int64_t matrix = static_cast<int64_t>(line) * job.Dk * job.Dv;
+    const int64_t piece = static_cast<int64_t>(line) * work.parts + part;  // of the segments' ends
     const Columns<float> state(job.Dv, job.Dv, grp, c), kept(delta_row(job.Dv), delta_row(job.Dv), grp, c);
     f32x4 s[DT];
     {
-        const auto from = state.rows(grads.d_state + matrix, grads.d_state ? job.Dk : 0);
+        const float *after = part == 0 ? grads.d_state ? grads.d_state + matrix : nullptr
+                             : PART    ? nullptr
+                                       : work.ends + (piece - 1) * job.Dk * job.Dv;
+        const auto from = state.rows(after, after ? job.Dk : 0);
         state.each<DT>([&](int t, int r, int at) { s[t][r] = __uint_as_float(buffer_bits<float>(from, at)); });
     }
     const Scalar *d_o = static_cast<const Scalar *>(grads.d_o) + span.b * grads.d_o_at[0] + head * grads.d_o_at[2] +
@@ -109,7 +126,7 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
         const Lds lds = buffer(i);
         const float *vec = lds.vec();
         const float total = vec[kVecGrowK * C + C - 1] * vec[kVecSk * C + C - 1];  // (a power of two: e^gamma_C)
-        {
+        if constexpr (!PART) {
             const auto to = kept.rows(work.dstate + record * job.Dk * delta_row(job.Dv), job.Dk);
             kept.each<DT>([&](int t, int r, int at) { buffer_store<float>(s[t][r], to, at); });
         }
@@ -180,7 +197,7 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
             if (i > 0)
                 load_frags(work.y, i - 1, y_hi, y_lo);
         }
-        {
+        if constexpr (!PART) {
             const auto to = kept.rows(work.x + record * C * delta_row(job.Dv), C);
             kept.each<4>([&](int m, int r, int at) { buffer_store<float>(x[m][r], to, at); });
             const auto out_to = v_cols.rows(dv + static_cast<int64_t>(i) * C * dv_step, min(C, span.len - i * C));
@@ -217,13 +234,16 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
         if constexpr (BUFS == 1)
             __syncthreads();  // chunk i - 1 is there
     }
-    if (grads.dinit) {
-        const auto to = state.rows(grads.dinit + matrix, job.Dk);
+    float *const before = PART ? work.ends + piece * job.Dk * job.Dv
+                          : part + 1 < work.parts || !grads.dinit ? nullptr
+                                                                   : grads.dinit + matrix;
+    if (before) {
+        const auto to = state.rows(before, job.Dk);
         state.each<DT>([&](int t, int r, int at) { buffer_store<float>(s[t][r], to, at); });
     }
-    if (!job.cu && c < job.Dv)  // tokens that do not count
-        for (int64_t t = span.len + grp; t < job.T; t += 4)
-            store_f32(dv + t * dv_step + c, 0.f);
+    if (!PART && part == 0 && !job.cu && c < job.Dv)  // tokens that do not count
+        for (int64_t t = row_end + grp; t < job.T; t += 4)
+            store_f32(dv + (t - skipped * C) * dv_step + c, 0.f);
 }
 
 // Sum over the 16 lanes of a row group (rotations within it).
@@ -825,34 +845,43 @@ template<typename Scalar>
 hipError_t backward_typed(const DeltaJob &job, const DeltaWork &work, const DeltaGrads &grads, hipStream_t stream,
                           const char **why) {
     const int wide = delta_padded(job.Dk);
-    const int groups = (job.Dv + 63) / 64;
-    const int64_t blocks = static_cast<int64_t>(job.N) * job.Hv * groups;
-    if (blocks > 0x7fffffff) {
+    const int tiles = (job.Dv + 15) / 16, groups = (tiles + 3) / 4;
+    const int64_t lines = static_cast<int64_t>(job.N) * job.Hv;
+    if (lines * work.parts * groups > 0x7fffffff || lines * tiles > 0x7fffffff) {
         *why = "delta rule: too many state columns for one launch";
         return hipErrorInvalidValue;
     }
+    const dim3 part_grid(static_cast<unsigned>(lines * (work.parts - 1) * groups));
+    const dim3 grid(static_cast<unsigned>(lines * work.parts * groups));
     constexpr int PIECES = sizeof(Scalar) == 4 ? 2 : 1;
     constexpr bool LO = !__is_same(Scalar, bf16_t);
     constexpr int V = 16 / static_cast<int>(sizeof(Scalar));
     const bool pieces = rows_whole<Scalar>(job) && job.Dv % V == 0 && reinterpret_cast<uintptr_t>(grads.d_o) % 16 == 0 &&
                         (grads.d_o_at[0] | grads.d_o_at[1] | grads.d_o_at[2]) % V == 0;
-#define RAMNET_BACK(DT)                                                                                                   \
-    if constexpr (delta_trains<DT, PIECES>) {                                                                             \
-        if (wide == 16 * DT) {                                                                                            \
-            constexpr int each = ChunkLds<DT, PIECES, true>::kBytes, bufs = 2 * each <= kLdsBytes ? 2 : 1;                \
-            constexpr int back = BackLds<DT, PIECES, LO>::kBytes;                                                         \
-            hipLaunchKernelGGL((chain_back_kernel<Scalar, DT, PIECES, bufs>), dim3(static_cast<unsigned>(blocks)),        \
-                               dim3(512), bufs * each, stream, job, work, grads, groups);                                 \
-            if (const hipError_t err = hipGetLastError())                                                                 \
-                return err;                                                                                               \
-            constexpr int waves = DT == 2 || (DT <= 8 && PIECES == 1) ? 8 : 4;                                            \
-            if (pieces)                                                                                                   \
-                hipLaunchKernelGGL((inputs_back_kernel<Scalar, DT, PIECES, LO, true, waves>), dim3(work.chunks, job.Hk),  \
-                                   dim3(kWave * waves), back, stream, job, work, grads);                                  \
-            else                                                                                                          \
-                hipLaunchKernelGGL((inputs_back_kernel<Scalar, DT, PIECES, LO, false, waves>), dim3(work.chunks, job.Hk), \
-                                   dim3(kWave * waves), back, stream, job, work, grads);                                  \
-        }                                                                                                                 \
+#define RAMNET_BACK(DT)                                                                                                         \
+    if constexpr (delta_trains<DT, PIECES>) {                                                                                   \
+        if (wide == 16 * DT) {                                                                                                  \
+            constexpr int each = ChunkLds<DT, PIECES, true>::kBytes, bufs = 2 * each <= kLdsBytes ? 2 : 1;                      \
+            constexpr int back = BackLds<DT, PIECES, LO>::kBytes;                                                               \
+            if (work.parts > 1) {                                                                                               \
+                hipLaunchKernelGGL((chain_back_kernel<Scalar, DT, PIECES, bufs, true>), part_grid, dim3(512), bufs * each,      \
+                                   stream, job, work, grads, groups);                                                           \
+                if (const hipError_t err = launch_delta_join(job, work, true, stream))                                          \
+                    return err;                                                                                                 \
+            }                                                                                                                   \
+            hipLaunchKernelGGL((chain_back_kernel<Scalar, DT, PIECES, bufs, false>), grid, dim3(512), bufs * each, stream,      \
+                               job, work, grads, groups);                                                                       \
+            if (const hipError_t err = hipGetLastError())                                                                       \
+                return err;                                                                                                     \
+            constexpr int waves = DT == 2 || (DT <= 8 && PIECES == 1) ? 8 : 4;                                                  \
+            const dim3 in_grid(work.chunks, job.Hk), in_block(kWave * waves);                                                   \
+            if (pieces)                                                                                                         \
+                hipLaunchKernelGGL((inputs_back_kernel<Scalar, DT, PIECES, LO, true, waves>), in_grid, in_block, back, stream,  \
+                                   job, work, grads);                                                                           \
+            else                                                                                                                \
+                hipLaunchKernelGGL((inputs_back_kernel<Scalar, DT, PIECES, LO, false, waves>), in_grid, in_block, back, stream, \
+                                   job, work, grads);                                                                           \
+        }                                                                                                                       \
     }
     RAMNET_BACK(2)
     RAMNET_BACK(4)

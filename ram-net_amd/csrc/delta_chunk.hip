@@ -581,7 +581,8 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
 // The states at the ends of a row's segments: what the segment adds, and its
 // map times the state before. One block per row, head and 16 columns, a wave a
 // tile of Dk: few small products one after the other, in fp32 instructions.
-template<int DT>
+// BACK: the ends lie from the last segment on, and the maps apply transposed.
+template<int DT, bool BACK>
 __global__ __launch_bounds__(kWave *DT) void join_kernel(const DeltaJob job, const DeltaWork work, int groups) {
     constexpr int wide = 16 * DT;
     __shared__ __align__(16) float s[2][16][wide + 4];  // columns of the state before
@@ -602,10 +603,11 @@ __global__ __launch_bounds__(kWave *DT) void join_kernel(const DeltaJob job, con
     *reinterpret_cast<f32x4 *>(&s[0][row][d]) = load(0);
     f32x4 next = load(1), map[DT];
     auto load_map = [&](int i) {
-        const float *from = work.maps + (piece + i) * wide * wide + (16 * wave + row) * wide + 4 * grp;
+        const float *from = work.maps + (piece + (BACK ? work.parts - 1 - i : i)) * wide * wide;
 #pragma unroll
         for (int t = 0; t < DT; ++t)
-            map[t] = load4(from + 16 * t);
+            map[t] = BACK ? load4(from + (16 * t + 4 * grp) * wide + 16 * wave + row, wide)
+                          : load4(from + (16 * wave + row) * wide + 4 * grp + 16 * t);
     };
     load_map(1);
     __syncthreads();
@@ -664,9 +666,7 @@ hipError_t chain_launch(const DeltaJob &job, const DeltaWork &work, hipStream_t 
                            dim3(512), BUFS * bytes, stream, job, work, map_groups);
         if (const hipError_t err = hipGetLastError())
             return err;
-        if (work.parts > 2)
-            hipLaunchKernelGGL(join_kernel<DT>, blocks(lines * tiles), dim3(kWave * DT), 0, stream, job, work, tiles);
-        if (const hipError_t err = hipGetLastError())
+        if (const hipError_t err = launch_delta_join(job, work, false, stream))
             return err;
     }
     hipLaunchKernelGGL((chain_kernel<Scalar, DT, PIECES, LO, BUFS, false>), blocks(lines * work.parts * groups), dim3(512),
@@ -719,8 +719,6 @@ void count_chunks(const DeltaJob &job, bool packed, DeltaWork *work) {
     work->chunks = packed ? work->per_row + job.N : job.N * work->per_row;
 }
 
-}  // namespace
-
 // Segments of a row: as many as fill the GPU's 256 compute units with blocks of
 // 64 columns, each at least kPartChunks long. A segment's map costs its state
 // columns once more, so half full is left as it is: one row of 32768 tokens, 8
@@ -736,9 +734,16 @@ void count_parts(const DeltaJob &job, bool packed, DeltaWork *work) {
     work->parts = (work->per_row + work->part_chunks - 1) / work->part_chunks;
 }
 
+int64_t map_floats(const DeltaJob &job, const DeltaWork &work) {
+    const int64_t wide = delta_padded(job.Dk);
+    return static_cast<int64_t>(job.N) * job.Hv * work.parts * wide * wide;
+}
+
+}  // namespace
+
 int64_t delta_layout(const DeltaJob &job, bool packed, bool backward, char *base, DeltaWork *work) {
     count_chunks(job, packed, work);
-    count_parts(job, packed || backward, work);
+    count_parts(job, packed, work);
     Carver carve{base};
     const int64_t records = static_cast<int64_t>(work->chunks) * job.Hv, square = kDeltaChunk * kDeltaChunk;
     work->offsets = packed ? carve.take<int32_t>(job.N + 1) : nullptr;
@@ -747,9 +752,10 @@ int64_t delta_layout(const DeltaJob &job, bool packed, bool backward, char *base
     work->y = carve.take<uint32_t>(records * 2 * kFragWords);
     work->p_frags = carve.take<uint32_t>(records * 2 * kFragWords);
     if (work->parts > 1) {
-        const int64_t pieces = static_cast<int64_t>(job.N) * job.Hv * work->parts, wide = delta_padded(job.Dk);
-        work->ends = carve.take<float>(pieces * job.Dk * job.Dv);
-        work->maps = carve.take<float>(pieces * wide * wide);
+        work->ends = carve.take<float>(static_cast<int64_t>(job.N) * job.Hv * work->parts * job.Dk * job.Dv);
+        float *maps = backward ? nullptr : carve.take<float>(map_floats(job, *work));
+        if (!work->maps)  // (else with what is kept)
+            work->maps = maps;
     }
     if (backward) {
         work->p = carve.take<float>(records * square);
@@ -768,6 +774,9 @@ int64_t delta_kept(const DeltaJob &job, bool packed, char *base, DeltaWork *work
     const int64_t records = static_cast<int64_t>(work->chunks) * job.Hv;
     work->e = carve.take<float>(records * kDeltaChunk * delta_row(job.Dv));
     work->states = carve.take<float>(records * job.Dk * delta_row(job.Dv));
+    count_parts(job, packed, work);
+    if (work->parts > 1)
+        work->maps = carve.take<float>(map_floats(job, *work));
     return carve.size;
 }
 
@@ -784,6 +793,28 @@ hipError_t launch_delta_prepare(const DeltaJob &job, const DeltaWork &work, bool
         case kBF16: return prepare_typed<bf16_t>(job, work, backward, stream);
         default: *why = "delta rule: unsupported dtype"; return hipErrorInvalidValue;
     }
+}
+
+hipError_t launch_delta_join(const DeltaJob &job, const DeltaWork &work, bool backward, hipStream_t stream) {
+    const int wide = delta_padded(job.Dk), tiles = (job.Dv + 15) / 16;
+    const dim3 grid(static_cast<unsigned>(job.N * job.Hv * tiles));
+    if (work.parts <= 2)  // (the first segment's end is whole)
+        return hipGetLastError();
+#define RAMNET_JOIN(DT)                                                                                                \
+    if (wide == 16 * DT) {                                                                                             \
+        if (backward)                                                                                                  \
+            hipLaunchKernelGGL((join_kernel<DT, true>), grid, dim3(kWave * DT), 0, stream, job, work, tiles);          \
+        else                                                                                                           \
+            hipLaunchKernelGGL((join_kernel<DT, false>), grid, dim3(kWave * DT), 0, stream, job, work, tiles);         \
+    }
+    RAMNET_JOIN(2)
+    RAMNET_JOIN(4)
+    RAMNET_JOIN(6)
+    RAMNET_JOIN(8)
+    RAMNET_JOIN(10)
+    RAMNET_JOIN(16)
+#undef RAMNET_JOIN
+    return hipGetLastError();
 }
 
 hipError_t launch_delta_chain(const DeltaJob &job, const DeltaWork &work, hipStream_t stream, const char **why) {

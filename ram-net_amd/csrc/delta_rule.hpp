@@ -44,7 +44,7 @@ struct DeltaWork {
     // where the time axis of a row is cut into segments that run side by side (parts > 1),
     // per row, value head and segment:
     float *ends;       // [Dk][Dv] state after the segment: first from zeros (the first from init), then in full
-    float *maps;       // [wide][wide] what the segment makes of the state before it
+    float *maps;       // [wide][wide] what the segment makes of the state before it (kept)
     int parts, part_chunks;
     int per_row;       // chunks of a row where sequences are rows
     int chunks;        // records / Hv

@@ -306,4 +306,8 @@ struct Stager {
     }
 };
 
+// The segments' ends put together (work.parts > 1); backward: from the last
+// segment on, with the maps transposed.
+hipError_t launch_delta_join(const DeltaJob &job, const DeltaWork &work, bool backward, hipStream_t stream);
+
 }  // namespace ramnet

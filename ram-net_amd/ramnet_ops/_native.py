@@ -128,14 +128,10 @@ SIGNATURES: dict[str, tuple[type, list]] = {
         _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
         _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64,
         _c_int, _c_float, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr]),
-    "ramnet_delta_rule_forward": (_c_int, [
-        _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
-        _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_float, _c_i64s, _c_ptr, _c_i64, _c_ptr, _c_i64,
-        _c_ptr]),
+    # (the struct of a call as bytes: a fifth of the time of as many arguments)
+    "ramnet_delta_rule_forward": (_c_int, [ctypes.c_char_p, _c_ptr]),
     "ramnet_delta_rule_backward": (_c_int, [
-        _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
-        _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_float,
-        _c_i64s, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr]),
+        ctypes.c_char_p, _c_ptr, _c_i64s, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr]),
     "ramnet_delta_rule_workspace_bytes": (_c_i64, [_c_i64] * 7 + [_c_int] * 3),
     "ramnet_delta_rule_kept_bytes": (_c_i64, [_c_i64] * 7 + [_c_int] * 2),
     "ramnet_verify_drafts": (_c_int, [

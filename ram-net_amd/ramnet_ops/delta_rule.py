@@ -19,10 +19,11 @@ except ImportError as exc:  # library not built: fail at call time
     _delta_error = exc
 
 
-def _require_tensors(optional: tuple[str, ...] = (), **named) -> None:
-    for name, t in named.items():
-        if not isinstance(t, torch.Tensor) and not (t is None and name in optional):
-            raise TypeError(f"Expected {name} to be a Tensor{' or None' if name in optional else ''}, "
+def _require_tensors(names: str, needed: int, *tensors) -> None:
+    """TypeError unless the first `needed` are tensors and the others are or are None."""
+    for i, (name, t) in enumerate(zip(names.split(), tensors)):
+        if not isinstance(t, torch.Tensor) and (t is not None or i < needed):
+            raise TypeError(f"Expected {name} to be a Tensor{' or None' if i >= needed else ''}, "
                             f"got {type(t).__name__}.")
 
 
@@ -56,29 +57,32 @@ def gated_delta_rule(
     :param inplace: Update init_state in place (contiguous float32, no gradients).
     :return: ``(o, state)``: (B, T, Hv, Dv) in v's type and (N, Hv, Dk, Dv) float32. N is B without cu_seqlens.
     """
-    _require_tensors(("init_state", "cu_seqlens", "lengths"), q=q, k=k, v=v, g=g, beta=beta, init_state=init_state,
-                     cu_seqlens=cu_seqlens, lengths=lengths)
+    if _delta is None:
+        raise _unavailable("gated_delta_rule")
+    eager = _delta.is_eager(q, k, v, g, beta, init_state, cu_seqlens, lengths)
+    if not eager or q is None or k is None or v is None or g is None or beta is None:
+        _require_tensors("q k v g beta init_state cu_seqlens lengths", 5, q, k, v, g, beta, init_state, cu_seqlens,
+                         lengths)
     if scale is None:
         scale = q.shape[-1] ** -0.5 if q.dim() and q.shape[-1] else 1.0
     elif not isinstance(scale, (int, float)):
         raise TypeError(f"Expected scale to be a number or None, got {type(scale).__name__}.")
+    else:
+        scale = float(scale)
     if inplace and init_state is None:
         raise ValueError("`inplace` needs an init_state to update.")
-    if _delta is None:
-        raise _unavailable("gated_delta_rule")
-    scale = float(scale)
     grad = _delta.wants_grad(q, k, v, g, beta, init_state)
     if inplace:
         if grad:
             raise ValueError("`inplace` has no gradients.")
-        if _delta.is_eager(q, k, v, g, beta, init_state, cu_seqlens, lengths):
+        if eager:
             _delta._require_state("gated_delta_rule", init_state)
             return _delta._forward("gated_delta_rule", q, k, v, g, beta, init_state, cu_seqlens, lengths, scale,
                                    init_state)[:2]
         return _delta.gated_delta_rule_(q, k, v, g, beta, init_state, cu_seqlens, lengths, scale), init_state
     if grad:
         return _delta.gated_delta_rule_kept(q, k, v, g, beta, init_state, cu_seqlens, lengths, scale)[:2]
-    if _delta.is_eager(q, k, v, g, beta, init_state, cu_seqlens, lengths):
+    if eager:
         return _delta._forward("gated_delta_rule", q, k, v, g, beta, init_state, cu_seqlens, lengths, scale)[:2]
     return _delta.gated_delta_rule(q, k, v, g, beta, init_state, cu_seqlens, lengths, scale)
 
@@ -106,10 +110,10 @@ def verify_drafts(
     :param draft_lens: Drafts of each row (B); default S.
     :return: ``(tokens, taken)``: (B, S + 1) int64 -- the drafts that stay, the drawn token, then -1 -- and (B) int32.
     """
-    _require_tensors(("draft", "draft_lens"), tokens=tokens, target=target, draft=draft, accept=accept, sample=sample,
-                     draft_lens=draft_lens)
     if _delta is None:
         raise _unavailable("verify_drafts")
-    if _delta.is_eager(tokens, target, draft, accept, sample, draft_lens):
+    if (_delta.is_eager(tokens, target, draft, accept, sample, draft_lens) and tokens is not None and target is not None
+            and accept is not None and sample is not None):
         return _delta._verify(tokens, target, draft, accept, sample, draft_lens)
+    _require_tensors("tokens target accept sample draft draft_lens", 4, tokens, target, accept, sample, draft, draft_lens)
     return _delta.verify_drafts(tokens, target, draft, accept, sample, draft_lens)

@@ -8,6 +8,9 @@ several times what a decode step costs the GPU.
 """
 from __future__ import annotations
 
+import struct
+from typing import NamedTuple
+
 import torch
 from torch import Tensor
 from torch.autograd import forward_ad
@@ -18,16 +21,31 @@ from ._ops import _check_shapes, _code, _dims, _NS, _require_gpu
 _FLOATS = tuple(nat.DTYPE_CODES)
 
 
+_peek, _modes = torch._C._functorch.peek_interpreter_stack, torch._C._len_torch_dispatch_stack
+_PLAIN = {Tensor, torch.nn.Parameter, type(None)}
+
+
 def is_eager(*tensors: Tensor | None) -> bool:
     """Whether a call on these tensors loses nothing beside the dispatcher: no
     tracing, mode, transform, forward-mode level or tensor subclass."""
-    return (not torch.compiler.is_compiling() and torch._C._functorch.peek_interpreter_stack() is None
-            and torch._C._len_torch_dispatch_stack() == 0 and forward_ad._current_level < 0
-            and all(t is None or type(t) in (Tensor, torch.nn.Parameter) for t in tensors))
+    return (not torch.compiler.is_compiling() and _peek() is None and _modes() == 0 and forward_ad._current_level < 0
+            and _PLAIN.issuperset(map(type, tensors)))
 
 
 def wants_grad(*tensors: Tensor | None) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if not torch.is_grad_enabled():
+        return False
+    return any(t is not None and t.requires_grad for t in tensors)
+
+
+class _Plans(dict):
+    """What calls of the same sizes, strides, types and devices share, by these."""
+
+    def keep(self, key, plan):
+        if len(self) >= 1024:
+            self.clear()
+        self[key] = plan
+        return plan
 
 
 # --------------------------------------------------------------------------
@@ -85,18 +103,6 @@ def _whole(t: Tensor | None) -> Tensor | None:
     return t.to(torch.int32).contiguous()
 
 
-def _args(q, k, v, g, beta, cu_seqlens, lengths):
-    """The inputs as the native calls read them."""
-    return _rows(q), _rows(k), _rows(v), g, beta, _whole(cu_seqlens), _whole(lengths)
-
-
-def _at(q, k, v, g, beta, *more):
-    s = q.stride()[:3] + k.stride()[:3] + v.stride()[:3] + g.stride() + beta.stride()
-    for t in more:
-        s += t.stride()[:3]
-    return nat.strides(*s)
-
-
 def _bytes(op: str, count: int, sizes) -> int:
     if count < 0:
         raise RuntimeError(f"{op}: sizes (B, T, N, Hk, Hv, Dk, Dv) = {tuple(sizes)} are not supported "
@@ -104,35 +110,75 @@ def _bytes(op: str, count: int, sizes) -> int:
     return count
 
 
+# ramnet_delta_rule_call: pointers and region sizes; sizes, strides and types; scale
+_HEAD, _TAIL, _SCALE = struct.Struct("=12Q2q"), struct.Struct("=22q3q"), struct.Struct("=d")
+
+
+class _Plan(NamedTuple):
+    sizes: tuple[int, ...]
+    tail: bytes
+    state_shape: tuple[int, ...]
+    workspace: tuple[int, int, int]  # bytes of kinds 0 to 2; -1: sizes not taken
+    kept: int
+
+
+_plans = _Plans()
+
+
+def _plan(op: str, q, k, v, g, beta, init_state, cu_seqlens, lengths):
+    """The call's plan, with q, k and v as the native calls read them."""
+    key = (q.shape, k.shape, v.shape, g.shape, beta.shape, q.stride(), k.stride(), v.stride(), g.stride(),
+           beta.stride(), q.dtype, k.dtype, v.dtype, g.dtype, beta.dtype, q.device, k.device, v.device, g.device,
+           beta.device, None if init_state is None else (init_state.shape, init_state.device),
+           None if cu_seqlens is None else (cu_seqlens.shape, cu_seqlens.dtype, cu_seqlens.device),
+           None if lengths is None else (lengths.shape, lengths.dtype, lengths.device))
+    plan = _plans.get(key)
+    if plan is not None:
+        return plan, q, k, v
+    sizes = _check(op, q, k, v, g, beta, init_state, cu_seqlens, lengths)
+    as_read = _rows(q), _rows(k), _rows(v)
+    if any(a is not b for a, b in zip(as_read, (q, k, v))):
+        return _plan(op, *as_read, g, beta, init_state, cu_seqlens, lengths)
+    B, T, N, Hk, Hv, Dk, Dv = sizes
+    packed = cu_seqlens is not None
+    lib, code = nat.lib(), _code(q)
+    tail = _TAIL.pack(*sizes, *(s for t in (q, k, v, g, beta) for s in t.stride()[:3]), code, _code(g), _code(beta))
+    return _plans.keep(key, _Plan(
+        sizes, tail, (N, Hv, Dk, Dv),
+        tuple(lib.ramnet_delta_rule_workspace_bytes(*sizes, code, packed, kind) for kind in range(3)),
+        lib.ramnet_delta_rule_kept_bytes(*sizes, code, packed))), q, k, v
+
+
 def _forward(op: str, q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, init_state: Tensor | None,
              cu_seqlens: Tensor | None, lengths: Tensor | None, scale: float, state: Tensor | None = None,
              keep: bool = False) -> tuple[Tensor, Tensor, Tensor | None]:
     """(o, state, kept). ``state``: where the state goes (init_state itself in place)."""
-    sizes = _check(op, q, k, v, g, beta, init_state, cu_seqlens, lengths)
-    B, T, N, Hk, Hv, Dk, Dv = sizes
-    packed = cu_seqlens is not None
-    q, k, v, g, beta, cu_seqlens, lengths = _args(q, k, v, g, beta, cu_seqlens, lengths)
-    if init_state is not None and init_state is not state:
+    plan, q, k, v = _plan(op, q, k, v, g, beta, init_state, cu_seqlens, lengths)
+    if init_state is not None and init_state is not state and not (init_state.dtype == torch.float32
+                                                                   and init_state.is_contiguous()):
         init_state = init_state.to(torch.float32).contiguous()
     if state is None:
-        state = torch.empty((N, Hv, Dk, Dv), dtype=torch.float32, device=q.device)
-    o = torch.empty((B, T, Hv, Dv), dtype=q.dtype, device=q.device)
-    lib = nat.lib()
-    kept = None
-    kept_bytes = 0
+        state = q.new_empty(plan.state_shape, dtype=torch.float32)
+    o = q.new_empty(v.shape)
+    n = _bytes(op, plan.workspace[keep], plan.sizes)
+    kept, kept_bytes = None, 0
     if keep:
-        kept_bytes = _bytes(op, lib.ramnet_delta_rule_kept_bytes(*sizes, _code(q), packed), sizes)
-        kept = torch.empty(kept_bytes, dtype=torch.uint8, device=q.device)
-    n = _bytes(op, lib.ramnet_delta_rule_workspace_bytes(*sizes, _code(q), packed, int(keep)), sizes)
-    ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-    if N == 0:
+        kept_bytes = _bytes(op, plan.kept, plan.sizes)
+        kept = q.new_empty((kept_bytes,), dtype=torch.uint8)
+    ws = q.new_empty((n,), dtype=torch.uint8) if n else None
+    if plan.sizes[2] == 0:
         return o.zero_(), state, kept
+    cu_seqlens, lengths = _whole(cu_seqlens), _whole(lengths)
     with nat.on_device(q):
-        nat.call("ramnet_delta_rule_forward", q.data_ptr(), k.data_ptr(), v.data_ptr(), _code(q), g.data_ptr(), _code(g),
-                 beta.data_ptr(), _code(beta), nat.ptr(init_state), state.data_ptr(), o.data_ptr(),
-                 nat.ptr(cu_seqlens), nat.ptr(lengths), *sizes, scale, _at(q, k, v, g, beta), nat.ptr(kept), kept_bytes,
-                 nat.ptr(ws), n, nat.stream_of(q))
+        nat.call("ramnet_delta_rule_forward", _HEAD.pack(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), _ptr(init_state), state.data_ptr(),
+            o.data_ptr(), _ptr(cu_seqlens), _ptr(lengths), _ptr(kept), _ptr(ws), kept_bytes, n) + plan.tail
+            + _SCALE.pack(scale), nat.stream_of(q))
     return o, state, kept
+
+
+def _ptr(t: Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _out_shapes(q, k, v, cu_seqlens):
@@ -193,28 +239,28 @@ def gated_delta_rule_backward(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: 
                               d_state: Tensor | None) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
     """Gradients (dq, dk, dv, dg, dbeta, dinit) of ``gated_delta_rule_kept``."""
     op = "gated_delta_rule_backward"
-    sizes = _check(op, q, k, v, g, beta, None, cu_seqlens, lengths)
-    B, T, N, Hk, Hv, Dk, Dv = sizes
-    packed = cu_seqlens is not None
-    _check_shapes(op, d_o=(d_o, (B, T, Hv, Dv)), d_state=(d_state, (N, Hv, Dk, Dv)))
-    q, k, v, g, beta, cu_seqlens, lengths = _args(q, k, v, g, beta, cu_seqlens, lengths)
+    plan, q, k, v = _plan(op, q, k, v, g, beta, None, cu_seqlens, lengths)
+    B, T, N, Hk, Hv, Dk, Dv = plan.sizes
+    _check_shapes(op, d_o=(d_o, (B, T, Hv, Dv)), d_state=(d_state, plan.state_shape))
     d_o = _rows(d_o.to(q.dtype))
     if d_state is not None:
         d_state = d_state.to(torch.float32).contiguous()
     grads = [torch.empty(t.shape, dtype=t.dtype, device=q.device) for t in (q, k, v, g, beta)]
-    dinit = torch.empty((N, Hv, Dk, Dv), dtype=torch.float32, device=q.device)
-    n = _bytes(op, nat.lib().ramnet_delta_rule_workspace_bytes(*sizes, _code(q), packed, 2), sizes)
+    dinit = q.new_empty(plan.state_shape, dtype=torch.float32)
+    n = _bytes(op, plan.workspace[2], plan.sizes)
     if N == 0 or T == 0 or B == 0:
         for t in grads:
             t.zero_()
         dinit.zero_() if d_state is None else dinit.copy_(d_state)
         return *grads, dinit
-    ws = torch.empty(n, dtype=torch.uint8, device=q.device)
+    ws = q.new_empty((n,), dtype=torch.uint8)
+    cu_seqlens, lengths = _whole(cu_seqlens), _whole(lengths)
     with nat.on_device(q):
-        nat.call("ramnet_delta_rule_backward", q.data_ptr(), k.data_ptr(), v.data_ptr(), _code(q), g.data_ptr(), _code(g),
-                 beta.data_ptr(), _code(beta), nat.ptr(cu_seqlens), nat.ptr(lengths), d_o.data_ptr(),
-                 nat.ptr(d_state), *(t.data_ptr() for t in grads), dinit.data_ptr(), *sizes, scale,
-                 _at(q, k, v, g, beta, d_o), kept.data_ptr(), kept.numel(), ws.data_ptr(), n, nat.stream_of(q))
+        nat.call("ramnet_delta_rule_backward", _HEAD.pack(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), 0, 0, 0, _ptr(cu_seqlens),
+            _ptr(lengths), kept.data_ptr(), ws.data_ptr(), kept.numel(), n) + plan.tail + _SCALE.pack(scale),
+            d_o.data_ptr(), nat.strides(*d_o.stride()[:3]), nat.ptr(d_state), *(t.data_ptr() for t in grads),
+            dinit.data_ptr(), nat.stream_of(q))
     return *grads, dinit
 
 
@@ -251,15 +297,16 @@ gated_delta_rule_kept.register_autograd(_backward, setup_context=_setup)
 # --------------------------------------------------------------------------
 # verification of drafted tokens
 
-def _verify(tokens: Tensor, target: Tensor, draft: Tensor | None, accept: Tensor, sample: Tensor,
-            draft_lens: Tensor | None) -> tuple[Tensor, Tensor]:
+_verify_plans = _Plans()
+
+
+def _verify_plan(key, tokens, target, draft, accept, sample, draft_lens):
+    """(B, S, V, dtype code, strides) of a call, its tensors checked."""
     op = "verify_drafts"
     B, S = _dims(op, "tokens", tokens, 2)
     V = _dims(op, "target", target, 3)[2]
-    if target.shape != (B, S + 1, V) or draft is not None and draft.shape != (B, S, V) or accept.shape != (B, S) \
-            or sample.shape != (B,) or draft_lens is not None and draft_lens.shape != (B,):
-        _check_shapes(op, target=(target, (B, S + 1, V)), draft=(draft, (B, S, V)), accept=(accept, (B, S)),
-                      sample=(sample, (B,)), draft_lens=(draft_lens, (B,)))
+    _check_shapes(op, target=(target, (B, S + 1, V)), draft=(draft, (B, S, V)), accept=(accept, (B, S)),
+                  sample=(sample, (B,)), draft_lens=(draft_lens, (B,)))
     if V == 0:
         raise RuntimeError(f"{op}: an empty vocabulary")
     device = target.device
@@ -269,20 +316,37 @@ def _verify(tokens: Tensor, target: Tensor, draft: Tensor | None, accept: Tensor
     if target.dtype not in _FLOATS or draft is not None and draft.dtype != target.dtype:
         raise RuntimeError(f"{op}: target and draft must share one of {_FLOATS}, got {target.dtype} and "
                            f"{None if draft is None else draft.dtype}")
-    if not target.is_cuda:
-        _require_gpu(op, target)
+    _require_gpu(op, target)
     for name, t in (("tokens", tokens), ("draft_lens", draft_lens)):
         if t is not None and t.dtype not in (torch.int32, torch.int64):
             raise RuntimeError(f"{op}: {name} must be int32 or int64, got {t.dtype}")
-    tokens = tokens.to(torch.int64).contiguous()
-    accept, sample = accept.to(torch.float32).contiguous(), sample.to(torch.float32).contiguous()
-    target, draft, draft_lens = _dense(target), None if draft is None else _dense(draft), _whole(draft_lens)
-    out = torch.empty((B, S + 1), dtype=torch.int64, device=device)
-    taken = torch.empty((B,), dtype=torch.int32, device=device)
     at = target.stride()[:2] + (draft.stride()[:2] if draft is not None else (0, 0))
+    return _verify_plans.keep(key, (B, S, V, _code(target), nat.strides(*at)))
+
+
+def _as(t: Tensor, dtype: torch.dtype) -> Tensor:
+    return t if t.dtype == dtype and t.is_contiguous() else t.to(dtype).contiguous()
+
+
+def _verify(tokens: Tensor, target: Tensor, draft: Tensor | None, accept: Tensor, sample: Tensor,
+            draft_lens: Tensor | None) -> tuple[Tensor, Tensor]:
+    if target.dim() == 3:
+        target = _dense(target)
+    if draft is not None and draft.dim() == 3:
+        draft = _dense(draft)
+    key = (tokens.shape, target.shape, accept.shape, sample.shape, target.stride(), target.dtype, tokens.dtype,
+           tokens.device, target.device, accept.device, sample.device,
+           None if draft is None else (draft.shape, draft.stride(), draft.dtype, draft.device),
+           None if draft_lens is None else (draft_lens.shape, draft_lens.dtype, draft_lens.device))
+    plan = _verify_plans.get(key) or _verify_plan(key, tokens, target, draft, accept, sample, draft_lens)
+    B, S, V, code, at = plan
+    tokens, draft_lens = _as(tokens, torch.int64), _whole(draft_lens)
+    accept, sample = _as(accept, torch.float32), _as(sample, torch.float32)
+    out = tokens.new_empty((B, S + 1))
+    taken = tokens.new_empty((B,), dtype=torch.int32)
     with nat.on_device(target):
-        nat.call("ramnet_verify_drafts", tokens.data_ptr(), target.data_ptr(), nat.ptr(draft), _code(target),
-                 accept.data_ptr(), sample.data_ptr(), nat.ptr(draft_lens), B, S, V, nat.strides(*at), out.data_ptr(),
+        nat.call("ramnet_verify_drafts", tokens.data_ptr(), target.data_ptr(), nat.ptr(draft), code,
+                 accept.data_ptr(), sample.data_ptr(), nat.ptr(draft_lens), B, S, V, at, out.data_ptr(),
                  taken.data_ptr(), nat.stream_of(target))
     return out, taken
 

@@ -1,6 +1,8 @@
 """Refusals of ``gated_delta_rule`` and ``verify_drafts``, before any launch (CPU)."""
 from __future__ import annotations
 
+import struct
+
 import pytest
 import torch
 
@@ -77,43 +79,56 @@ def _einval(name, args, match):
         nat.call(name, *args)
 
 
+FIELDS = ("q k v g beta init_state state o cu_seqlens lengths kept workspace kept_bytes workspace_bytes "
+          "B T N Hk Hv Dk Dv").split()
+
+
+def _packed(strides=64, **kw):
+    """A ramnet_delta_rule_call as bytes."""
+    x = dict(dict.fromkeys(FIELDS, 0), q=FAKE, k=FAKE, v=FAKE, g=FAKE, beta=FAKE, state=FAKE, o=FAKE, workspace=FAKE,
+             workspace_bytes=1 << 30, B=2, T=100, N=2, Hk=2, Hv=4, Dk=64, Dv=64, dtype=2, g_dtype=0, beta_dtype=2)
+    x.update(kw)
+    return struct.pack("=12Q2q22q3qd", *(x[n] for n in FIELDS), *[strides] * 15, x["dtype"], x["g_dtype"],
+                       x["beta_dtype"], 1.0)
+
+
 def test_native_delta_rule():
     nat = _native()
-    ok = dict(q=FAKE, k=FAKE, v=FAKE, dtype=2, g=FAKE, g_dtype=0, beta=FAKE, beta_dtype=2, init=None, state=FAKE, o=FAKE,
-              cu=None, lengths=None, B=2, T=100, N=2, Hk=2, Hv=4, Dk=64, Dv=64, scale=1.0, strides=nat.strides(*[64] * 18),
-              kept=None, kept_bytes=0, ws=FAKE, ws_bytes=1 << 30, stream=None)
 
     def call(match, **kw):
-        _einval("ramnet_delta_rule_forward", {**ok, **kw}.values(), match)
+        _einval("ramnet_delta_rule_forward", (_packed(**kw), None), match)
+    _einval("ramnet_delta_rule_forward", (None, None), "null call")
     call("shape must have", B=-1)
     call("shape must have", Dk=0)
     call("multiple of Hk", Hv=3)
     call("Dk must be at most", Dk=257)
-    call("batch of one", cu=FAKE)
+    call("batch of one", cu_seqlens=FAKE)
     call("batch of one", N=3)
     call("index overflow", T=1 << 30)
+    call("index overflow", Dv=1 << 21)
     call("dtype", dtype=3)
     call("dtype", g_dtype=-1)
-    call("no lengths", B=1, cu=FAKE, lengths=FAKE)
-    call("null tensor", q=None)
-    call("null tensor", state=None)
-    call("one row to", strides=nat.strides(*[63] * 18))
-    call("one row to", strides=nat.strides(*[1 << 22] * 18))
-    call("workspace too small", ws_bytes=16)
-    call("workspace too small", ws=None)
+    call("no lengths", B=1, cu_seqlens=FAKE, lengths=FAKE)
+    call("null tensor", q=0)
+    call("null tensor", state=0)
+    call("one row to", strides=63)
+    call("one row to", strides=1 << 22)
+    call("workspace too small", workspace_bytes=16)
+    call("workspace too small", workspace=0)
     call("kept region too small", kept=FAKE, kept_bytes=16)
-    back = dict(q=FAKE, k=FAKE, v=FAKE, dtype=2, g=FAKE, g_dtype=0, beta=FAKE, beta_dtype=2, cu=None, lengths=None,
-                d_o=FAKE, d_state=None, dq=FAKE, dk=FAKE, dv=FAKE, dg=FAKE, dbeta=FAKE, dinit=None, B=2, T=100, N=2,
-                Hk=2, Hv=4, Dk=64, Dv=64, scale=1.0, strides=nat.strides(*[64] * 18), kept=FAKE, kept_bytes=1 << 30,
-                ws=FAKE, ws_bytes=1 << 30, stream=None)
+    call("Dk up to 160", kept=FAKE, kept_bytes=1 << 40, dtype=0, Dk=200, strides=256)
 
-    def call_back(match, **kw):
-        _einval("ramnet_delta_rule_backward", {**back, **kw}.values(), match)
+    def call_back(match, strides=64, grads=(FAKE,) * 6, **kw):
+        kw = dict(dict(kept=FAKE, kept_bytes=1 << 30), **kw)
+        _einval("ramnet_delta_rule_backward",
+                (_packed(strides=kw.pop("rows", 64), **kw), FAKE, nat.strides(64, strides, 64), None, *grads, None), match)
     call_back("needs tokens", T=0)
-    call_back("null tensor", dg=None)
+    call_back("null tensor", grads=(FAKE, FAKE, FAKE, 0, FAKE, FAKE))
+    call_back("null tensor", kept=0)
     call_back("kept region too small", kept_bytes=16)
-    call_back("Dk up to 160", dtype=0, Dk=200, strides=nat.strides(*[256] * 18))
-    call_back("workspace too small", ws_bytes=16)
+    call_back("Dk up to 160", dtype=0, Dk=200, rows=256)
+    call_back("workspace too small", workspace_bytes=16)
+    call_back("tokens of d_o", strides=63)
     lib = nat.lib()
     assert lib.ramnet_delta_rule_workspace_bytes(2, 100, 2, 2, 4, 300, 64, 2, 0, 0) == -1
     assert lib.ramnet_delta_rule_workspace_bytes(2, 1, 2, 2, 4, 64, 64, 2, 0, 0) == 0  # a step needs none
