@@ -6,11 +6,14 @@
 // first index whose running sum passes sample * total, among those with a
 // weight above 0.
 //
-// Bound by reading one target row and one draft row of V. One block a row of
-// the batch: each of its 16 waves sums one stretch of the vocabulary, then the
-// block walks the one stretch in which the threshold falls (it comes from the
-// L2) with a running sum in order. All sums in 64 bits, in a fixed order: a
-// draw next to a border of the running sum would go by the rounding of 32.
+// Bound by reading one target row and one draft row of V; small batches by the
+// latency of what depends on what (tokens, their probabilities, the rows). One
+// block a row of the batch: each of its 16 waves sums one stretch of the
+// vocabulary, then the block walks the one stretch in which the threshold falls
+// (it comes from the L2) with a running sum in order. All sums in 64 bits, in a
+// fixed order: a draw next to a border of the running sum would go by the
+// rounding of 32. What waves find is put together by ballots: LDS atomics on one
+// word go lane by lane (20 us of a call).
 #include "ramnet_device.hpp"
 #include "ramnet_kernels.hpp"
 
@@ -51,37 +54,47 @@ __device__ __forceinline__ double wave_sum(double x) {
 
 template<typename Scalar>
 __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyJob job) {
-    __shared__ double sums[kWaves][2];
-    __shared__ double scan[kWaves];
-    __shared__ int taken_s, found_s, last_s;
-    const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave, wave = tid / kWave;
+    __shared__ double sums[kWaves], scan[kWaves];
+    __shared__ int refused_s[kWaves], found_s[kWaves], last_s[kWaves];
+    const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int64_t b = blockIdx.x;
     const int V = job.V, S = job.S;
     const int64_t *tokens = job.tokens + b * S;
     const Scalar *target = static_cast<const Scalar *>(job.target) + b * job.target_at[0];
     const Scalar *draft = job.draft ? static_cast<const Scalar *>(job.draft) + b * job.draft_at[0] : nullptr;
+    // the first place that is refused
     const int len = job.lens ? min(max(job.lens[b], 0), S) : S;
-
-    if (tid == 0)
-        taken_s = len, found_s = V, last_s = -1;
-    __syncthreads();
-    for (int s = tid; s < len; s += kThreads) {
-        const int64_t x = tokens[s];
-        bool stays = false;
-        if (x >= 0 && x < V) {
-            const double p = load_f32(target + s * job.target_at[1] + x);
-            const double q = draft ? static_cast<double>(load_f32(draft + s * job.draft_at[1] + x)) : 1.0;
-            stays = static_cast<double>(job.accept[b * S + s]) * q < p;
+    int first = S;
+    for (int s0 = wave * kWave; s0 < S; s0 += kThreads) {
+        const int s = s0 + lane;
+        bool stays = s >= S;
+        if (s < S) {
+            const int64_t x = tokens[s];
+            const double accept = job.accept[b * S + s];
+            if (s < len && x >= 0 && x < V) {
+                const double p = load_f32(target + s * job.target_at[1] + x);
+                const double q = draft ? static_cast<double>(load_f32(draft + s * job.draft_at[1] + x)) : 1.0;
+                stays = accept * q < p;
+            }
         }
-        if (!stays)
-            atomicMin(&taken_s, s);
+        const uint64_t out = __ballot(!stays);
+        if (out) {
+            first = s0 + __ffsll(static_cast<unsigned long long>(out)) - 1;
+            break;
+        }
     }
+    if (lane == 0)
+        refused_s[wave] = first;
     __syncthreads();
-    const int n = taken_s;
+    int n = S;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w)
+        n = min(n, refused_s[w]);
     const bool refused = n < len;
     const Scalar *p = target + n * job.target_at[1];
     const Scalar *q = refused && draft ? draft + n * job.draft_at[1] : nullptr;
-    const int64_t without = refused && !draft ? tokens[n] : -1;
+    const int64_t ruled = refused && !draft ? tokens[n] : -1;
+    const int without = ruled >= 0 && ruled < V ? static_cast<int>(ruled) : -1;
 
     // (comparisons keep a NaN, as a maximum of torch does; fmax would drop it)
     auto left = [&](float pv, float qv, int at) {
@@ -89,67 +102,66 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyJob job) {
         return at == without || d < 0.0 ? 0.0 : d;
     };
 
-    // the sums of each wave's stretch
-    constexpr int N = Piece<Scalar>::kN;
-    const int part = (V + kWaves * N - 1) / (kWaves * N) * N;
-    const int lo = min(wave * part, V), hi = min(lo + part, V);
-    double rest = 0.0, whole = 0.0;
-    constexpr int kDeep = 4;
-    int at = lo + lane * N;
-    for (; at + (kDeep - 1) * kWave * N + N <= hi; at += kDeep * kWave * N) {
-        Piece<Scalar> a[kDeep], c[kDeep];
+    // the sums of each wave's stretch: whole pieces, and for the last wave the row's
+    // last few elements, one a lane
+    constexpr int N = Piece<Scalar>::kN, kDeep = 4;
+    const int part = (V + kWaves * N - 1) / (kWaves * N) * N, full = V / N * N;
+    const int lo = min(wave * part, full), hi = min(lo + part, full);
+    const bool tail = wave == kWaves - 1 && full + lane < V;
+    auto stretch = [&](auto weight) {
+        double sum = tail ? weight(load_f32(p + full + lane), q ? load_f32(q + full + lane) : 0.f, full + lane) : 0.0;
+        for (int at = lo + lane * N; at < hi; at += kDeep * kWave * N) {
+            Piece<Scalar> x[kDeep], y[kDeep];
 #pragma unroll
-        for (int i = 0; i < kDeep; ++i) {
-            a[i] = load_piece(p + at + i * kWave * N);
-            c[i] = q ? load_piece(q + at + i * kWave * N) : Piece<Scalar>{};
+            for (int i = 0; i < kDeep; ++i) {
+                const int from = at + i * kWave * N;
+                x[i] = from < hi ? load_piece(p + from) : Piece<Scalar>{};
+                y[i] = q && from < hi ? load_piece(q + from) : Piece<Scalar>{};
+            }
+#pragma unroll
+            for (int i = 0; i < kDeep; ++i)
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    sum += weight(x[i][e], y[i][e], at + i * kWave * N + e);
         }
+        sum = wave_sum(sum);
+        if (lane == 0)
+            sums[wave] = sum;
+        __syncthreads();
+        double total = 0.0;
 #pragma unroll
-        for (int i = 0; i < kDeep; ++i)
-#pragma unroll
-            for (int e = 0; e < N; ++e) {
-                rest += left(a[i][e], c[i][e], at + i * kWave * N + e);
-                whole += static_cast<double>(a[i][e]);
-            }
+        for (int w = 0; w < kWaves; ++w)
+            total += sums[w];
+        return total;
+    };
+    double total = stretch(left);
+    const bool own = refused && !(total > 0.0);  // nothing is left (or a NaN): the target's own weights
+    if (own) {
+        __syncthreads();
+        total = stretch([](float pv, float, int) { return static_cast<double>(pv); });
     }
-    for (; at < hi; at += kWave * N) {
-#pragma unroll
-        for (int e = 0; e < N; ++e)
-            if (at + e < hi) {
-                const float pv = load_f32(p + at + e);
-                rest += left(pv, q ? load_f32(q + at + e) : 0.f, at + e);
-                whole += static_cast<double>(pv);
-            }
-    }
-    rest = wave_sum(rest), whole = wave_sum(whole);
-    if (lane == 0)
-        sums[wave][0] = rest, sums[wave][1] = whole;
-    __syncthreads();
-    double total[2] = {0.0, 0.0};
-    for (int w = 0; w < kWaves; ++w)
-        total[0] += sums[w][0], total[1] += sums[w][1];
-    const int kind = total[0] > 0.0 ? 0 : 1;  // (a NaN goes to the target's own weights)
-    const double border = static_cast<double>(job.sample[b]) * total[kind];
+    const double border = static_cast<double>(job.sample[b]) * total;
     double seen = 0.0, before = 0.0;  // the sums before the next stretch, and before at_wave's
     int at_wave = -1;
     for (int w = 0; w < kWaves; ++w) {
-        if (sums[w][kind] > 0.0) {
+        if (sums[w] > 0.0) {
             at_wave = w, before = seen;  // (stays at the last one with a weight where rounding lets none pass)
-            if (seen + sums[w][kind] > border)
+            if (seen + sums[w] > border)
                 break;
         }
-        seen += sums[w][kind];
+        seen += sums[w];
     }
+    int found = V, last = -1;
     if (at_wave >= 0) {
-        seen = before;
-        const int from = min(at_wave * part, V), to = min(from + part, V);
+        const int from = min(at_wave * part, full), to = at_wave == kWaves - 1 ? V : min(from + part, full);
         const int each = (to - from + kThreads - 1) / kThreads;
-        const int first = min(from + tid * each, to), end = min(first + each, to);
+        const int begin = min(from + tid * each, to), end = min(begin + each, to);
         auto weight = [&](int i) {
             const float pv = load_f32(p + i);
-            return kind ? static_cast<double>(pv) : left(pv, q ? load_f32(q + i) : 0.f, i);
+            return own ? static_cast<double>(pv) : left(pv, q ? load_f32(q + i) : 0.f, i);
         };
         double mine = 0.0;
-        for (int i = first; i < end; ++i)
+        for (int i = begin; i < end; ++i)
             mine += weight(i);
         double run = mine;
 #pragma unroll
@@ -161,24 +173,34 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyJob job) {
             scan[wave] = run;
         __syncthreads();
         for (int w = 0; w < wave; ++w)
-            seen += scan[w];
-        run = seen + (run - mine);
-        for (int i = first; i < end; ++i) {
+            before += scan[w];
+        run = before + (run - mine);
+        for (int i = begin; i < end && found == V; ++i) {
             const double x = weight(i);
             run += x;
             if (x > 0.0) {
-                atomicMax(&last_s, i);
-                if (run > border) {
-                    atomicMin(&found_s, i);
-                    break;
-                }
+                last = i;
+                found = run > border ? i : V;
             }
         }
     }
+    // threads have the vocabulary in order: the first that found, the last with a weight
+    const uint64_t finds = __ballot(found < V), any = __ballot(last >= 0);
+    if (finds)
+        found = __shfl(found, __ffsll(static_cast<unsigned long long>(finds)) - 1);
+    if (any)
+        last = __shfl(last, kWave - 1 - __clzll(static_cast<long long>(any)));
+    if (lane == 0)
+        found_s[wave] = finds ? found : V, last_s[wave] = any ? last : -1;
     __syncthreads();
     int64_t *out = job.out + b * (S + 1);
+    int chosen = V, highest = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w)
+        chosen = min(chosen, found_s[w]), highest = max(highest, last_s[w]);
     // (none passes by rounding, or with a sample of 1: the last one with a weight; a NaN gives 0)
-    const int chosen = found_s < V ? found_s : border == border ? max(last_s, 0) : 0;
+    if (chosen == V)
+        chosen = border == border ? highest : 0;
     for (int s = tid; s <= S; s += kThreads)
         out[s] = s < n ? tokens[s] : s == n ? chosen : -1;
     if (tid == 0)
