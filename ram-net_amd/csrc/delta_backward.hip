@@ -460,8 +460,8 @@ __global__ __launch_bounds__(kWave *WAVES, WAVES / 4) void inputs_back_kernel(co
         if (wave == 0) {
             const double own = work.gamma[record * C + lane], end = work.gamma[record * C + C - 1];
             gam[lane] = own;
-            grow[lane] = expf(static_cast<float>(own));
-            left[lane] = expf(static_cast<float>(end - own));
+            grow[lane] = decay_of(own);
+            left[lane] = decay_of(end - own);
         } else if (wave == 1) {
             beta_s[lane] = vec[kVecBeta * C + lane];
             inv_k[lane] = 1.f / vec[kVecSk * C + lane];
@@ -666,7 +666,7 @@ __global__ __launch_bounds__(kWave *WAVES, WAVES / 4) void inputs_back_kernel(co
                 const int i = 16 * ti + 4 * grp + r;
                 float a = 0.f, b = 0.f, both_ij = 0.f;
                 if (i >= j) {
-                    const float decay = expf(static_cast<float>(gam[i] - gam[j])) * beta_s[j];
+                    const float decay = decay_of(gam[i] - gam[j]) * beta_s[j];
                     a = job.scale * decay * r1[n][r];
                     b = i > j ? -decay * r2[n][r] : 0.f;
                     both_ij = p_ij[n][r] * r1[n][r] - bl_ij[n][r] * r2[n][r];

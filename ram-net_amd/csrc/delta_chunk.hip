@@ -110,18 +110,37 @@ __device__ __forceinline__ float line_max(const float *m, int line, int part, bo
     return fmaxf(x, __shfl_xor(x, 2));
 }
 
+// Sum of the lanes up to this one, in 64 bits (DPP moves: a shuffle goes
+// through the LDS).
+template<int CTRL, int ROWS>
+__device__ __forceinline__ double moved(double x) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<uint32_t>(u), CTRL, ROWS, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<uint32_t>(u >> 32), CTRL, ROWS, 0xF, false);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+__device__ __forceinline__ double running_sum(double x) {
+    x += moved<0x111, 0xF>(x);  // from 1, 2, 4 and 8 lanes before within rows of 16
+    x += moved<0x112, 0xF>(x);
+    x += moved<0x114, 0xF>(x);
+    x += moved<0x118, 0xF>(x);
+    x += moved<0x142, 0xA>(x);  // the sum of the row before, in the second and fourth
+    return x + moved<0x143, 0xC>(x);  // and of the first half, in the second
+}
+
 // Y, P, gamma and the scales of one chunk and value head: wave w has the
-// tokens of tile w.
+// tokens of tile w. Latency from end to end, so as many blocks as fit: P's
+// operands and then Y take the place of the keys.
 template<typename Scalar, int DT>
-__global__ __launch_bounds__(256) void prepare_kernel(const DeltaJob job, const DeltaWork work, bool backward) {
+__global__ __launch_bounds__(256, 4) void prepare_kernel(const DeltaJob job, const DeltaWork work, bool backward) {
     constexpr int C = kDeltaChunk, NP = C + 4, wide = 16 * DT, pitch = wide + 16 / static_cast<int>(sizeof(Scalar));
-    constexpr int kSquare = C * NP, kRows = C * pitch * static_cast<int>(sizeof(Scalar)) / 4;
+    constexpr int kSquare = C * NP, kPitchH = C + 8, kHalf = C * kPitchH;
     extern __shared__ __align__(16) float lds[];
-    float *nm = lds, *pm = nm + kSquare;
-    float *ys = pm + kSquare;  // over the keys, once they are done with
+    float *nm = lds, *ys = nm + kSquare;
     Scalar *ks = reinterpret_cast<Scalar *>(ys);
+    uint16_t *ph = reinterpret_cast<uint16_t *>(ys);
     __shared__ double gam[C];
-    __shared__ float beta_s[C], sk_s[C], sq_s[C], scale_y[C], scale_p[C];
+    __shared__ float beta_s[C], sk_s[C], sq_s[C], scale_y[C], p_max[4];
     const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave, wave = uniform(tid / kWave);
     const int row = lane & 15, grp = lane >> 4;
     const int chunk = blockIdx.x, head = blockIdx.y, kh = head / (job.Hv / job.Hk);
@@ -142,26 +161,23 @@ __global__ __launch_bounds__(256) void prepare_kernel(const DeltaJob job, const 
         }
         return;
     }
+    const int64_t record = static_cast<int64_t>(chunk) * job.Hv + head;
+    float g = 0.f, beta = 0.f;
+    if (wave == 0 && lane < at.len) {
+        const int64_t t = at.t0 + lane;
+        g = load_code(job.g, job.g_dtype, at.b * job.g_at[0] + t * job.g_at[1] + head * job.g_at[2]);
+        beta = load_code(job.beta, job.beta_dtype, at.b * job.beta_at[0] + t * job.beta_at[1] + head * job.beta_at[2]);
+    }
     const bool whole = rows_whole<Scalar>(job);
     TileRows<Scalar, DT> kt, qt;
     kt.load(static_cast<const Scalar *>(job.k) + at.b * job.k_at[0] + at.t0 * job.k_at[1] + kh * job.k_at[2], job.k_at[1],
             16 * wave + row, grp, at.len, job.Dk, whole);
     qt.load(static_cast<const Scalar *>(job.q) + at.b * job.q_at[0] + at.t0 * job.q_at[1] + kh * job.q_at[2], job.q_at[1],
             16 * wave + row, grp, at.len, job.Dk, whole);
-    const int64_t record = static_cast<int64_t>(chunk) * job.Hv + head;
     if (wave == 0) {
-        const int64_t t = at.t0 + lane;
-        const bool have = lane < at.len;
-        double x = have ? delta_decay(load_code(job.g, job.g_dtype, at.b * job.g_at[0] + t * job.g_at[1] +
-                                                head * job.g_at[2])) : 0.f;
-        beta_s[lane] = have ? load_code(job.beta, job.beta_dtype,
-                                        at.b * job.beta_at[0] + t * job.beta_at[1] + head * job.beta_at[2]) : 0.f;
-#pragma unroll
-        for (int m = 1; m < kWave; m <<= 1) {
-            const double y = __shfl_up(x, m);
-            x += lane >= m ? y : 0.0;
-        }
+        const double x = running_sum(static_cast<double>(delta_decay(g)) * kLog2e);
         gam[lane] = x;
+        beta_s[lane] = beta;
         work.gamma[record * C + lane] = x;
     }
 #pragma unroll
@@ -177,57 +193,99 @@ __global__ __launch_bounds__(256) void prepare_kernel(const DeltaJob job, const 
     }
     __syncthreads();
 
-    // K K^T and Q K^T, lower tiles
+    // K K^T and Q K^T, lower tiles; P stays in registers
     float *p_out = backward ? work.p + record * C * C : nullptr, *bl_out = backward ? work.bl + record * C * C : nullptr;
+    f32x4 p[4];
+    float largest = 0.f;
+#pragma unroll
     for (int tj = 0; tj < 4; ++tj) {
-        f32x4 a = {0.f, 0.f, 0.f, 0.f}, p = a;
+        p[tj] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (tj > wave)
+            continue;
         const int j = 16 * tj + row;
-        if (tj <= wave) {
-            a = kt.times(ks + j * pitch, grp, a);
-            p = qt.times(ks + j * pitch, grp, p);
-        }
+        const f32x4 a = kt.times(ks + j * pitch, grp, f32x4{0.f, 0.f, 0.f, 0.f});
+        p[tj] = qt.times(ks + j * pitch, grp, p[tj]);
         const double gj = gam[j];
         const float bj = beta_s[j];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int i = 16 * wave + 4 * grp + r;
-            const float decay = i >= j ? expf(static_cast<float>(gam[i] - gj)) : 0.f;
-            const float pij = i >= j ? job.scale * p[r] * decay : 0.f, aij = i > j ? a[r] * decay : 0.f;
-            pm[i * NP + j] = backward ? pij : pij * bj;
+            const float decay = i >= j ? decay_of(gam[i] - gj) : 0.f;
+            const float pij = i >= j ? job.scale * p[tj][r] * decay : 0.f, aij = i > j ? a[r] * decay : 0.f;
+            p[tj][r] = backward ? pij : pij * bj;
+            largest = fmaxf(largest, fabsf(p[tj][r]));
             nm[i * NP + j] = aij * bj;
             if (backward)
                 p_out[i * C + j] = pij, bl_out[i * C + j] = aij;
         }
     }
+#pragma unroll
+    for (int m = 1; m < 16; m <<= 1)
+        largest = fmaxf(largest, __shfl_xor(largest, m));
+    largest = column_max(largest);
+    if (lane == 0)
+        p_max[wave] = largest;
     __syncthreads();
-    for (int i = tid; i < kSquare / 4; i += 256)
-        reinterpret_cast<f32x4 *>(ys)[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 
+    // P (backward: its transpose) as fp16 parts, then as operands to memory. One
+    // scale for all of it: a part is exact to 2^-39 of the largest. (What the chains
+    // do not read is not written: bf16 outputs take the first part.)
+    constexpr bool kBf16 = __is_same(Scalar, bf16_t);
+    const bool both = !kBf16 || backward;
+    float p_inverse;
+    const float scale_p = scale_of(fmaxf(fmaxf(p_max[0], p_max[1]), fmaxf(p_max[2], p_max[3])), p_inverse);
+#pragma unroll
+    for (int tj = 0; tj < 4; ++tj) {
+        const int j = 16 * tj + row;
+        if (tj > (wave | 1))
+            continue;  // (no operand reaches there)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int i = 16 * wave + 4 * grp + r;
+            const _Float16 hi = static_cast<_Float16>(p[tj][r] * scale_p);
+            uint16_t *to = ph + (backward ? j * kPitchH + operand_at(i) : i * kPitchH + operand_at(j));
+            *to = __builtin_bit_cast(uint16_t, hi);
+            if (both)
+                to[kHalf] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(fmaf(p[tj][r], scale_p,
+                                                                                  -static_cast<float>(hi))));
+        }
+    }
+    __syncthreads();
+    for (int i = wave; i < (both ? 2 : 1) * kFrags; i += 4) {
+        const int part = i >= kFrags, f = i - part * kFrags;
+        int tile, block;
+        frag_place(f, backward, tile, block);
+        const u32x4 x = *reinterpret_cast<const u32x4 *>(ph + part * kHalf + (16 * tile + row) * kPitchH + 32 * block + 8 * grp);
+        *reinterpret_cast<u32x4 *>(work.p_frags + record * 2 * kFragWords + part * kFragWords + (f * kWave + lane) * 4) = x;
+    }
     // inverse of the unit lower triangular N: 16-blocks by substitution (lane = column),
     // then pairs of blocks: low part -Yb Nba Ya
+    float x[16];
     {
         const float *block = nm + 16 * wave * NP + 16 * wave;
-        f32x4 rows[16][4];
-#pragma unroll
-        for (int i = 1; i < 16; ++i)
-#pragma unroll
-            for (int j = 0; j < i; j += 4)
-                rows[i][j / 4] = load4(block + i * NP + j);
-        float x[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
+            if (i % 4 == 0)
+                __builtin_amdgcn_sched_barrier(0);  // (four rows at a time: registers)
+            f32x4 n[4];
+#pragma unroll
+            for (int j = 0; j < i; j += 4)
+                n[j / 4] = load4(block + i * NP + j);
             float sum = i == row ? 1.f : 0.f;
 #pragma unroll
             for (int j = 0; j < i; ++j)
-                sum = fmaf(-rows[i][j / 4][j % 4], x[j], sum);
+                sum = fmaf(-n[j / 4][j % 4], x[j], sum);
             x[i] = sum;
         }
-        __syncthreads();
-        if (grp == 0)
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                ys[(16 * wave + i) * NP + 16 * wave + row] = x[i];
     }
+    __syncthreads();
+    for (int i = tid; i < kSquare / 4; i += 256)
+        reinterpret_cast<f32x4 *>(ys)[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    __syncthreads();
+    if (grp == 0)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            ys[(16 * wave + i) * NP + 16 * wave + row] = x[i];
     __syncthreads();
     if (wave < 2) {
         const int a = 32 * wave, b = a + 16;
@@ -260,20 +318,18 @@ __global__ __launch_bounds__(256) void prepare_kernel(const DeltaJob job, const 
     }
     __syncthreads();
 
-    // scales of the rows (backward: the columns) of Y and P, and the vectors
+    // scales of the rows (backward: the columns) of Y, and the vectors
     {
         float inverse;
         const float y_max = line_max(ys, tid / 4, tid % 4, backward, NP);
-        const float p_max = line_max(pm, tid / 4, tid % 4, backward, NP);
         float *vec = work.vec + record * kVecs * C;
         if (tid % 4 == 0) {
             const int i = tid / 4;
             const float sk = sk_s[i], sq = sq_s[i];
             scale_y[i] = scale_of(y_max, inverse);
             vec[kVecInvY * C + i] = inverse;
-            scale_p[i] = scale_of(p_max, inverse);
-            vec[kVecInvP * C + i] = inverse;
-            const float grow = expf(static_cast<float>(gam[i])), left = expf(static_cast<float>(gam[C - 1] - gam[i]));
+            vec[kVecInvP * C + i] = p_inverse;
+            const float grow = decay_of(gam[i]), left = decay_of(gam[C - 1] - gam[i]);
             vec[kVecSk * C + i] = sk;
             vec[kVecSq * C + i] = sq;
             vec[kVecGrowK * C + i] = grow / sk;
@@ -283,31 +339,26 @@ __global__ __launch_bounds__(256) void prepare_kernel(const DeltaJob job, const 
         }
     }
     __syncthreads();
-    for (int i = tid; i < 2 * kFrags * kWave; i += 256) {
-        const bool is_p = i >= kFrags * kWave;
-        const int f = (is_p ? i - kFrags * kWave : i) / kWave;
+    for (int f = wave; f < kFrags; f += 4) {
         int tile, block;
         frag_place(f, backward, tile, block);
-        const float *m = is_p ? pm : ys;
-        const int a = 16 * tile + row, b = 32 * block + 4 * grp;  // (256 is a multiple of a wave: row and grp are i's too)
-        f32x4 x, y;
+        const int a = 16 * tile + row, b = 32 * block + 4 * grp;
+        f32x4 z[2];
         if (backward)
-            x = load4(m + b * NP + a, NP), y = load4(m + (b + 16) * NP + a, NP);
+            z[0] = load4(ys + b * NP + a, NP), z[1] = load4(ys + (b + 16) * NP + a, NP);
         else
-            x = load4(m + a * NP + b), y = load4(m + a * NP + b + 16);
-        const float s = is_p ? scale_p[a] : scale_y[a];
+            z[0] = load4(ys + a * NP + b), z[1] = load4(ys + a * NP + b + 16);
+        const float s = scale_y[a];
         u32x4 hi, lo;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            const f32x4 z = w < 2 ? x : y;
             uint32_t h, l;
-            split2(z[w % 2 * 2], z[w % 2 * 2 + 1], s, h, l);
+            split2(z[w / 2][w % 2 * 2], z[w / 2][w % 2 * 2 + 1], s, h, l);
             hi[w] = h, lo[w] = l;
         }
-        uint32_t *out = (is_p ? work.p_frags : work.y) + record * 2 * kFragWords + (f * kWave + lane) * 4;
+        uint32_t *out = work.y + record * 2 * kFragWords + (f * kWave + lane) * 4;
         *reinterpret_cast<u32x4 *>(out) = hi;
-        if (!__is_same(Scalar, bf16_t) || backward || !is_p)  // (what the chains read)
-            *reinterpret_cast<u32x4 *>(out + kFragWords) = lo;
+        *reinterpret_cast<u32x4 *>(out + kFragWords) = lo;
     }
 }
 
@@ -631,16 +682,18 @@ template<typename Scalar>
 hipError_t prepare_typed(const DeltaJob &job, const DeltaWork &work, bool backward, hipStream_t stream) {
     const int wide = delta_padded(job.Dk);
     const size_t rows = kDeltaChunk * (wide * sizeof(Scalar) + 16), square = kDeltaChunk * (kDeltaChunk + 4) * sizeof(float);
+    const size_t parts = 2 * kDeltaChunk * (kDeltaChunk + 8) * 2;  // of P, in bytes
 #define RAMNET_PREPARE(DT)                                                                                    \
     if (wide == 16 * DT)                                                                                      \
         hipLaunchKernelGGL((prepare_kernel<Scalar, DT>), dim3(work.chunks, job.Hv), dim3(256),                \
-                           2 * square + std::max(rows, square), stream, job, work, backward)
+                           square + std::max({rows, square, parts}), stream, job, work, backward)
     RAMNET_PREPARE(2);
     RAMNET_PREPARE(4);
     RAMNET_PREPARE(6);
     RAMNET_PREPARE(8);
     RAMNET_PREPARE(10);
-    RAMNET_PREPARE(16);
+    if constexpr (sizeof(Scalar) < 4)  // (wider fp32 heads walk their tokens)
+        RAMNET_PREPARE(16);
 #undef RAMNET_PREPARE
     return hipGetLastError();
 }

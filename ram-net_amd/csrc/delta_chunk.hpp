@@ -12,6 +12,11 @@
 
 namespace ramnet {
 
+constexpr double kLog2e = 1.4426950408889634;
+
+// e^x for x in powers of 2: the difference of two sums of decays, rounded once.
+__device__ __forceinline__ float decay_of(double x) { return __builtin_amdgcn_exp2f(static_cast<float>(x)); }
+
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // One 16x16 tile += A (16 x 4 steps) B: lane l gives A[l % 16][4 (l / 16) + r]
