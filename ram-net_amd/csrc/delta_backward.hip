@@ -32,10 +32,11 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
     constexpr int C = kDeltaChunk, BT = DT / 2;
     const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave, wave = uniform(tid / kWave);
     const int row = lane & 15, grp = lane >> 4;
-    const int group = static_cast<int>(blockIdx.x) % groups;
-    const int part = static_cast<int>(blockIdx.x) / groups % (PART ? work.parts - 1 : work.parts);  // from the end
-    const int line = static_cast<int>(blockIdx.x) / groups / (PART ? work.parts - 1 : work.parts);
-    const int head = line % job.Hv, n = line / job.Hv;
+    const int parts = PART ? work.parts - 1 : work.parts;
+    int group, item;
+    split_block(static_cast<int>(blockIdx.x), groups, job.N * job.Hv * parts, group, item);
+    const int part = item % parts, line = item / parts;  // from the end
+    const int head = line % job.Hv, n = delta_line(work, line / job.Hv);
     const int kh = head / (job.Hv / job.Hk);
     DeltaSpan span = delta_span(job, n);
     const int row_end = span.len;
@@ -55,34 +56,38 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
 
     if (wave >= 4) {
         const int at = tid - 256;
-        const bool whole = rows_whole<Scalar>(job);
         const Scalar *k = static_cast<const Scalar *>(job.k) + span.b * job.k_at[0] + kh * job.k_at[2];
         const Scalar *q = static_cast<const Scalar *>(job.q) + span.b * job.q_at[0] + kh * job.q_at[2];
         Stager<Scalar, DT, PIECES, true> stager;
-        auto load = [&](int i) {
-            const int64_t t0 = span.t0 + i * C;
-            stager.load(k + t0 * job.k_at[1], job.k_at[1], q + t0 * job.q_at[1], job.q_at[1], min(C, span.len - i * C),
-                        job.Dk, whole, work.vec + (static_cast<int64_t>(first + i) * job.Hv + head) * kVecs * C, at);
-        };
-        if (count > 0) {
-            load(count - 1);
-            stager.store(buffer(count - 1), at);
-        }
-        __syncthreads();
-        for (int i = count - 1; i >= 0; --i) {
-            if (i > 0)
-                load(i - 1);
-            if constexpr (BUFS == 1)
-                __syncthreads();  // chunk i is done with
-            if (i > 0)
-                stager.store(buffer(i - 1), at);
+        auto bring = [&](auto wide) {
+            auto load = [&](int i) {
+                const int64_t t0 = span.t0 + i * C;
+                stager.template load<decltype(wide)::value, true>(
+                    k + t0 * job.k_at[1], job.k_at[1], q + t0 * job.q_at[1], job.q_at[1], min(C, span.len - i * C), job.Dk,
+                    work.vec + (static_cast<int64_t>(first + i) * job.Hv + head) * kVecs * C, at);
+            };
+            if (count > 0) {
+                load(count - 1);
+                stager.template store<true>(buffer(count - 1), at);
+            }
             __syncthreads();
-        }
+            for (int i = count - 1; i >= 0; --i) {
+                load(max(i - 1, 0));
+                if constexpr (BUFS == 1)
+                    __syncthreads();  // chunk i is done with
+                stager.template store<true>(buffer(i - 1), at);
+                __syncthreads();
+            }
+        };
+        if (rows_whole<Scalar>(job))
+            bring(std::true_type{});
+        else
+            bring(std::false_type{});
         return;
     }
 
     const int c = (group * 4 + wave) * 16 + row;
-    const int64_t matrix = static_cast<int64_t>(line) * job.Dk * job.Dv;
+    const int64_t matrix = (static_cast<int64_t>(n) * job.Hv + head) * job.Dk * job.Dv;
     const int64_t piece = static_cast<int64_t>(line) * work.parts + part;  // of the segments' ends
     const Columns<float> state(job.Dv, job.Dv, grp, c), kept(delta_row(job.Dv), delta_row(job.Dv), grp, c);
     f32x4 s[DT];
@@ -118,7 +123,13 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
         load_o(count - 1);
         load_frags(work.p_frags, count - 1, p_hi, p_lo);
         load_frags(work.y, count - 1, y_hi, y_lo);
+        arrived(o_bits);
+        arrived(p_hi);
+        arrived(p_lo);
+        arrived(y_hi);
+        arrived(y_lo);
     }
+    arrived(s);
     __syncthreads();
 
     for (int i = count - 1; i >= 0; --i) {
@@ -131,31 +142,24 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
             kept.each<DT>([&](int t, int r, int at) { buffer_store<float>(s[t][r], to, at); });
         }
         f32x4 out[4], du[4], x[4];
+        float x_inverse;
 #pragma unroll
         for (int m = 0; m < 4; ++m)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
                 out[m][r] = bits_f32<Scalar>(o_bits[4 * m + r]);
-        if (i > 0)
-            load_o(i - 1);
+        const int then = max(i - 1, 0);  // (the first chunk's once more rather than a branch)
+        load_o(then);
         {
             Operand<4, true> oo;
             oo.set(out);
 #pragma unroll
-            for (int m = 0; m < 4; ++m) {
+            for (int m = 0; m < 4; ++m)
                 x[m] = zero;
-#pragma unroll
-                for (int b = m / 2; b < 2; ++b) {
-                    const int f = m < 2 ? m * 2 + b : m + 2;
-                    x[m] = mfma16(p_hi[f], oo.hi[b], x[m]);
-                    x[m] = mfma16(p_lo[f], oo.hi[b], x[m]);
-                    if constexpr (!__is_same(Scalar, bf16_t))
-                        x[m] = mfma16(p_hi[f], oo.lo[b], x[m]);  // (0 for bf16 but far below a column's largest)
-                }
-                x[m] = x[m] * (load4(vec + kVecInvP * C + 16 * m + 4 * grp) * oo.inverse);
-            }
-            if (i > 0)
-                load_frags(work.p_frags, i - 1, p_hi, p_lo);
+            // (dO's second part is 0 for bf16 but far below a column's largest)
+            triangle<true, true, !__is_same(Scalar, bf16_t)>(p_hi, p_lo, oo.hi, oo.lo, x);
+            x_inverse = vec[kVecInvP * C] * oo.inverse;
+            load_frags(work.p_frags, then, p_hi, p_lo);
         }
         {
             Operand<DT, true> so;
@@ -164,7 +168,7 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
             for (int m = 0; m < 4; ++m)
                 du[m] = zero;
 #pragma unroll
-            for (int b = 0; b < BT; ++b) {
+            for (int b = 0; b < BT; ++b)
 #pragma unroll
                 for (int m = 0; m < 4; ++m) {
                     const u32x4 kf = lds.row_frag(lds.k(0), m, b, lane);
@@ -173,29 +177,23 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
                     if constexpr (PIECES == 2)
                         du[m] = mfma16(lds.row_frag(lds.k(1), m, b, lane), so.hi[b], du[m]);
                 }
-            }
 #pragma unroll
             for (int m = 0; m < 4; ++m)
-                du[m] = (x[m] + du[m] * (load4(vec + kVecLeftK * C + 16 * m + 4 * grp) * so.inverse)) *
+                du[m] = (x[m] * x_inverse + du[m] * (load4(vec + kVecLeftK * C + 16 * m + 4 * grp) * so.inverse)) *
                         load4(vec + kVecBeta * C + 16 * m + 4 * grp);
         }
         {
             Operand<4, true> uo;
             uo.set(du);
 #pragma unroll
-            for (int m = 0; m < 4; ++m) {
+            for (int m = 0; m < 4; ++m)
                 x[m] = zero;
+            triangle<true, true, true>(y_hi, y_lo, uo.hi, uo.lo, x);
+            x_inverse = vec[kVecInvY * C] * uo.inverse;
 #pragma unroll
-                for (int b = m / 2; b < 2; ++b) {
-                    const int f = m < 2 ? m * 2 + b : m + 2;
-                    x[m] = mfma16(y_hi[f], uo.hi[b], x[m]);
-                    x[m] = mfma16(y_hi[f], uo.lo[b], x[m]);
-                    x[m] = mfma16(y_lo[f], uo.hi[b], x[m]);
-                }
-                x[m] = x[m] * (load4(vec + kVecInvY * C + 16 * m + 4 * grp) * uo.inverse);
-            }
-            if (i > 0)
-                load_frags(work.y, i - 1, y_hi, y_lo);
+            for (int m = 0; m < 4; ++m)
+                x[m] = x[m] * x_inverse;
+            load_frags(work.y, then, y_hi, y_lo);
         }
         if constexpr (!PART) {
             const auto to = kept.rows(work.x + record * C * delta_row(job.Dv), C);
@@ -211,6 +209,7 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
         Operand<4, true> xo, oo;
         xo.set(x);
         oo.set(out);
+        // (operands read ahead as in the forward's chain do not fit the registers here)
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
             f32x4 a = zero, z = zero;
@@ -402,9 +401,9 @@ __global__ __launch_bounds__(kWave *WAVES, WAVES / 4) void inputs_back_kernel(co
         const Scalar *q = static_cast<const Scalar *>(job.q) + at.b * job.q_at[0] + at.t0 * job.q_at[1] + kh * job.q_at[2];
         const float *scales = work.vec + (static_cast<int64_t>(chunk) * job.Hv + kh * shared) * kVecs * C + tid % 16 * 4;
         const bool is_q = wave >= 4;
-        keys.load_one(is_q ? q : k, is_q ? job.q_at[1] : job.k_at[1], at.len, Dk, WIDE, tid % 256, keys.raw[0]);
+        keys.template load_one<WIDE>(is_q ? q : k, is_q ? job.q_at[1] : job.k_at[1], at.len, Dk, tid % 256, keys.raw[0]);
         if constexpr (WAVES == 4)
-            keys.load_one(q, job.q_at[1], at.len, Dk, WIDE, tid, keys.raw[1]);
+            keys.template load_one<WIDE>(q, job.q_at[1], at.len, Dk, tid, keys.raw[1]);
         Keys::store_one(keys.raw[0], load4(scales + (is_q ? kVecSq : kVecSk) * C), tid % 256, nullptr, is_q ? qt : kt);
         if constexpr (WAVES == 4)
             Keys::store_one(keys.raw[1], load4(scales + kVecSq * C), tid, nullptr, qt);

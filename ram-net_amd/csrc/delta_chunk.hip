@@ -9,10 +9,14 @@ namespace ramnet {
 
 namespace {
 
-// First chunk of each packed sequence, one block. The sum of the lengths is at
+// First chunk of each packed sequence, and the sequences by their lengths: one
+// starts its whole walk when its block does, the longest had better be first
+// (thirteen sequences of 12345 tokens: chain 214 us in their own order). More
+// than 1024 keep their order. One block. The sum of the lengths is at
 // most T where the bounds are in order; elsewhere it is held to the records
 // there are.
 __global__ __launch_bounds__(1024) void offsets_kernel(const DeltaJob job, const DeltaWork work) {
+    __shared__ int lens[1024];
     __shared__ int wave_sum[16];
     __shared__ int carry;
     const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave, wave = uniform(tid / kWave);
@@ -29,7 +33,18 @@ __global__ __launch_bounds__(1024) void offsets_kernel(const DeltaJob job, const
         }
         if (lane == kWave - 1)
             wave_sum[wave] = x;
+        if (job.N <= 1024)
+            lens[tid] = n < job.N ? delta_span(job, n).len : 0;
         __syncthreads();
+        if (n < job.N) {
+            int rank = n;
+            if (job.N <= 1024) {
+                rank = 0;
+                for (int m = 0; m < job.N; ++m)
+                    rank += lens[m] > lens[tid] || (lens[m] == lens[tid] && m < n);
+            }
+            work.order[rank] = n;
+        }
         int sum = carry;
         for (int w = 0; w < wave; ++w)
             sum = min(sum + wave_sum[w], work.chunks);
@@ -97,19 +112,6 @@ struct TileRows {
     }
 };
 
-// The largest of 64 values of a row (or column), four threads a row.
-__device__ __forceinline__ float line_max(const float *m, int line, int part, bool column, int pitch) {
-    float x = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-        const int at = 4 * part + 4 * i;  // (pieces of the four threads side by side)
-        const f32x4 v = column ? load4(m + at * pitch + line, pitch) : load4(m + line * pitch + at);
-        x = fmaxf(fmaxf(fmaxf(x, fabsf(v[0])), fmaxf(fabsf(v[1]), fabsf(v[2]))), fabsf(v[3]));
-    }
-    x = fmaxf(x, __shfl_xor(x, 1));
-    return fmaxf(x, __shfl_xor(x, 2));
-}
-
 // Sum of the lanes up to this one, in 64 bits (DPP moves: a shuffle goes
 // through the LDS).
 template<int CTRL, int ROWS>
@@ -140,7 +142,7 @@ __global__ __launch_bounds__(256, 4) void prepare_kernel(const DeltaJob job, con
     Scalar *ks = reinterpret_cast<Scalar *>(ys);
     uint16_t *ph = reinterpret_cast<uint16_t *>(ys);
     __shared__ double gam[C];
-    __shared__ float beta_s[C], sk_s[C], sq_s[C], scale_y[C], p_max[4];
+    __shared__ float beta_s[C], sk_s[C], sq_s[C], p_max[4];
     const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave, wave = uniform(tid / kWave);
     const int row = lane & 15, grp = lane >> 4;
     const int chunk = blockIdx.x, head = blockIdx.y, kh = head / (job.Hv / job.Hk);
@@ -318,27 +320,36 @@ __global__ __launch_bounds__(256, 4) void prepare_kernel(const DeltaJob job, con
     }
     __syncthreads();
 
-    // scales of the rows (backward: the columns) of Y, and the vectors
+    // the scale of Y, and the vectors
+    float y_inverse, scale_y;
     {
-        float inverse;
-        const float y_max = line_max(ys, tid / 4, tid % 4, backward, NP);
+        float largest = 0.f;
+        for (int i = tid; i < kSquare / 4; i += 256) {
+            const f32x4 v = reinterpret_cast<const f32x4 *>(ys)[i];
+            largest = fmaxf(fmaxf(largest, fmaxf(fabsf(v[0]), fabsf(v[1]))), fmaxf(fabsf(v[2]), fabsf(v[3])));
+        }
+#pragma unroll
+        for (int m = 1; m < 16; m <<= 1)
+            largest = fmaxf(largest, __shfl_xor(largest, m));
+        largest = column_max(largest);
+        if (lane == 0)
+            p_max[wave] = largest;
+        __syncthreads();
+        scale_y = scale_of(fmaxf(fmaxf(p_max[0], p_max[1]), fmaxf(p_max[2], p_max[3])), y_inverse);
         float *vec = work.vec + record * kVecs * C;
-        if (tid % 4 == 0) {
-            const int i = tid / 4;
-            const float sk = sk_s[i], sq = sq_s[i];
-            scale_y[i] = scale_of(y_max, inverse);
-            vec[kVecInvY * C + i] = inverse;
-            vec[kVecInvP * C + i] = p_inverse;
-            const float grow = decay_of(gam[i]), left = decay_of(gam[C - 1] - gam[i]);
-            vec[kVecSk * C + i] = sk;
-            vec[kVecSq * C + i] = sq;
-            vec[kVecGrowK * C + i] = grow / sk;
-            vec[kVecGrowQ * C + i] = job.scale * grow / sq;
-            vec[kVecLeftK * C + i] = left / sk;
-            vec[kVecBeta * C + i] = beta_s[i];
+        if (wave == 0) {
+            const float sk = sk_s[lane], sq = sq_s[lane], b = beta_s[lane];
+            const float grow = decay_of(gam[lane]), left = decay_of(gam[C - 1] - gam[lane]);
+            vec[kVecSk * C + lane] = sk;
+            vec[kVecSq * C + lane] = sq;
+            vec[kVecGrowK * C + lane] = grow / sk;
+            vec[kVecGrowQ * C + lane] = job.scale * grow / sq;
+            vec[kVecLeftK * C + lane] = (backward ? left : left * b) / sk;
+            vec[kVecBeta * C + lane] = b;
+            vec[kVecInvY * C + lane] = y_inverse;
+            vec[kVecInvP * C + lane] = p_inverse;
         }
     }
-    __syncthreads();
     for (int f = wave; f < kFrags; f += 4) {
         int tile, block;
         frag_place(f, backward, tile, block);
@@ -348,12 +359,11 @@ __global__ __launch_bounds__(256, 4) void prepare_kernel(const DeltaJob job, con
             z[0] = load4(ys + b * NP + a, NP), z[1] = load4(ys + (b + 16) * NP + a, NP);
         else
             z[0] = load4(ys + a * NP + b), z[1] = load4(ys + a * NP + b + 16);
-        const float s = scale_y[a];
         u32x4 hi, lo;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             uint32_t h, l;
-            split2(z[w / 2][w % 2 * 2], z[w / 2][w % 2 * 2 + 1], s, h, l);
+            split2(z[w / 2][w % 2 * 2], z[w / 2][w % 2 * 2 + 1], scale_y, h, l);
             hi[w] = h, lo[w] = l;
         }
         uint32_t *out = work.y + record * 2 * kFragWords + (f * kWave + lane) * 4;
@@ -383,10 +393,11 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
     constexpr int C = kDeltaChunk, BT = DT / 2;
     const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave, wave = uniform(tid / kWave);
     const int row = lane & 15, grp = lane >> 4;
-    const int group = static_cast<int>(blockIdx.x) % groups;
-    const int part = static_cast<int>(blockIdx.x) / groups % (MAP ? work.parts - 1 : work.parts);
-    const int line = static_cast<int>(blockIdx.x) / groups / (MAP ? work.parts - 1 : work.parts);
-    const int head = line % job.Hv, n = line / job.Hv;
+    const int parts = MAP ? work.parts - 1 : work.parts;
+    int group, item;
+    split_block(static_cast<int>(blockIdx.x), groups, job.N * job.Hv * parts, group, item);
+    const int part = item % parts, line = item / parts;
+    const int head = line % job.Hv, n = delta_line(work, line / job.Hv);
     const int kh = head / (job.Hv / job.Hk);
     const int tiles = (job.Dv + 15) / 16;
     if (MAP && part == 0 && group * 4 >= tiles)
@@ -407,36 +418,43 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
 
     if (wave >= 4) {
         const int at = tid - 256;
-        const bool whole = rows_whole<Scalar>(job);
         const Scalar *k = static_cast<const Scalar *>(job.k) + span.b * job.k_at[0] + kh * job.k_at[2];
         const Scalar *q = static_cast<const Scalar *>(job.q) + span.b * job.q_at[0] + kh * job.q_at[2];
         Stager<Scalar, DT, PIECES, false> stager;
-        auto load = [&](int i) {
-            const int64_t t0 = span.t0 + i * C;
-            stager.template load<!MAP>(k + t0 * job.k_at[1], job.k_at[1], q + t0 * job.q_at[1], job.q_at[1], min(C, span.len - i * C),
-                        job.Dk, whole, work.vec + (static_cast<int64_t>(first + i) * job.Hv + head) * kVecs * C, at);
-        };
-        if (count > 0) {
-            load(0);
-            stager.template store<!MAP>(buffer(0), at);
-        }
-        __syncthreads();
-        for (int i = 0; i < count; ++i) {
-            if (i + 1 < count)
-                load(i + 1);
-            if constexpr (BUFS == 1)
-                __syncthreads();  // chunk i is done with
-            if (i + 1 < count)
-                stager.template store<!MAP>(buffer(i + 1), at);
+        // the loads' latency comes first: the chain is in its products of K and Q then, which
+        // the stores to LDS would be in the way of (a chunk more in registers, stored
+        // as soon as a buffer is free: 248 -> 310 us for eight 4096-token prompts)
+        auto bring = [&](auto wide) {
+            auto load = [&](int i) {
+                const int64_t t0 = span.t0 + i * C;
+                stager.template load<decltype(wide)::value, !MAP>(
+                    k + t0 * job.k_at[1], job.k_at[1], q + t0 * job.q_at[1], job.q_at[1], min(C, span.len - i * C), job.Dk,
+                    work.vec + (static_cast<int64_t>(first + i) * job.Hv + head) * kVecs * C, at);
+            };
+            if (count > 0) {
+                load(0);
+                stager.template store<!MAP>(buffer(0), at);
+            }
             __syncthreads();
-        }
+            for (int i = 0; i < count; ++i) {
+                load(min(i + 1, count - 1));
+                if constexpr (BUFS == 1)
+                    __syncthreads();  // chunk i is done with
+                stager.template store<!MAP>(buffer(i + 1), at);
+                __syncthreads();
+            }
+        };
+        if (rows_whole<Scalar>(job))
+            bring(std::true_type{});
+        else
+            bring(std::false_type{});
         return;
     }
 
     const int tile = group * 4 + wave;
     const bool is_map = MAP && tile >= tiles;
     const int c = (is_map ? tile - tiles : tile) * 16 + row;
-    const int64_t matrix = static_cast<int64_t>(line) * job.Dk * job.Dv;
+    const int64_t matrix = (static_cast<int64_t>(n) * job.Hv + head) * job.Dk * job.Dv;
     const int64_t piece = static_cast<int64_t>(line) * work.parts + part;  // of the segments' buffers
     const Columns<float> state(job.Dv, job.Dv, grp, c), kept(delta_row(job.Dv), delta_row(job.Dv), grp, c);
     f32x4 s[DT];
@@ -487,9 +505,17 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
     if (count > 0) {
         load_v(0);
         load_y(0);
-        if constexpr (!MAP)
+        if constexpr (!MAP) {
             load_p(0);
+            arrived(p_hi);
+            if constexpr (LO)
+                arrived(p_lo);
+        }
+        arrived(y_hi);
+        arrived(y_lo);
+        arrived(v_bits);
     }
+    arrived(s);
     __syncthreads();
 
     for (int i = 0; i < count; ++i) {
@@ -511,28 +537,35 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
 #pragma unroll
             for (int m = 0; m < 4; ++m)
                 g[m] = qo[m] = zero;
+            // steps: of each block of 32 rows of S, K's parts and then Q's
+            constexpr int kEach = MAP ? PIECES : 2 * PIECES;
+            pipelined<BT * kEach, 4, 2>(
+                [&](auto step, u32x4(&f)[4]) {
+                    constexpr int at = decltype(step)::value, block = at / kEach, part = at % kEach;
+                    const uint16_t *from = part < PIECES ? lds.k(part) : lds.q(part - PIECES);
 #pragma unroll
-            for (int b = 0; b < BT; ++b) {
+                    for (int m = 0; m < 4; ++m)
+                        f[m] = lds.row_frag(from, m, block, lane);
+                },
+                [&](auto step, const u32x4(&f)[4]) {
+                    constexpr int at = decltype(step)::value, block = at / kEach, part = at % kEach;
+                    constexpr bool is_k = part < PIECES, first_part = part % PIECES == 0;
 #pragma unroll
-                for (int m = 0; m < 4; ++m) {
-                    const u32x4 kf = lds.row_frag(lds.k(0), m, b, lane);
-                    g[m] = mfma16(kf, so.hi[b], g[m]);
-                    g[m] = mfma16(kf, so.lo[b], g[m]);
-                    if constexpr (PIECES == 2)
-                        g[m] = mfma16(lds.row_frag(lds.k(1), m, b, lane), so.hi[b], g[m]);
-                    if constexpr (!MAP) {
-                        const u32x4 qf = lds.row_frag(lds.q(0), m, b, lane);
-                        qo[m] = mfma16(qf, so.hi[b], qo[m]);
-                        if constexpr (LO)
-                            qo[m] = mfma16(qf, so.lo[b], qo[m]);
-                        if constexpr (PIECES == 2)
-                            qo[m] = mfma16(lds.row_frag(lds.q(1), m, b, lane), so.hi[b], qo[m]);
+                    for (int m = 0; m < 4; ++m) {
+                        f32x4 &to = is_k ? g[m] : qo[m];
+                        to = mfma16(f[m], so.hi[block], to);
                     }
-                }
-            }
+                    if constexpr (first_part && (is_k || LO))
+#pragma unroll
+                        for (int m = 0; m < 4; ++m) {
+                            f32x4 &to = is_k ? g[m] : qo[m];
+                            to = mfma16(f[m], so.lo[block], to);
+                        }
+                });
         }
         // what the state gives o, and v - S^T k but for the chunk's own tokens
         f32x4 e[4];
+        float e_inverse;
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
             const f32x4 gr = load4(vec + kVecGrowK * C + 16 * m + 4 * grp) * s_inverse;
@@ -541,72 +574,81 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
             for (int r = 0; r < 4; ++r)
                 g[m][r] = fmaf(-gr[r], g[m][r], bits_f32<Scalar>(v_bits[4 * m + r]));
         }
-        if (i + 1 < count)
-            load_v(i + 1);
+        const int then = min(i + 1, count - 1);  // (the last chunk's once more rather than a branch)
+        load_v(then);
         {
             Operand<4, true> ro;
             ro.set(g);
 #pragma unroll
-            for (int m = 0; m < 4; ++m) {
+            for (int m = 0; m < 4; ++m)
                 e[m] = zero;
-#pragma unroll
-                for (int b = 0; b <= m / 2; ++b) {
-                    const int f = m < 2 ? m : 2 + (m - 2) * 2 + b;
-                    e[m] = mfma16(y_hi[f], ro.hi[b], e[m]);
-                    e[m] = mfma16(y_hi[f], ro.lo[b], e[m]);
-                    e[m] = mfma16(y_lo[f], ro.hi[b], e[m]);
-                }
-                e[m] = e[m] * (load4(vec + kVecInvY * C + 16 * m + 4 * grp) * ro.inverse);
-            }
-            if (i + 1 < count)
-                load_y(i + 1);
+            triangle<false, true, true>(y_hi, y_lo, ro.hi, ro.lo, e);
+            e_inverse = vec[kVecInvY * C] * ro.inverse;
+            load_y(then);
         }
+        // (e without its scale, which is taken into those of the operands made of it)
         if (!MAP && work.e) {
             const auto to = kept.rows(work.e + record * C * delta_row(job.Dv), C);
-            kept.each<4>([&](int m, int r, int at) { buffer_store<float>(e[m][r], to, at); });
+            kept.each<4>([&](int m, int r, int at) { buffer_store<float>(e[m][r] * e_inverse, to, at); });
         }
         if constexpr (!MAP) {
             Operand<4, LO> eo;
             eo.set(e);
+            f32x4 x[4];
 #pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                f32x4 x = zero;
+            for (int m = 0; m < 4; ++m)
+                x[m] = zero;
+            triangle<false, LO, LO>(p_hi, p_lo, eo.hi, eo.lo, x);
+            const float x_inverse = vec[kVecInvP * C] * eo.inverse * e_inverse;
 #pragma unroll
-                for (int b = 0; b <= m / 2; ++b) {
-                    const int f = m < 2 ? m : 2 + (m - 2) * 2 + b;
-                    x = mfma16(p_hi[f], eo.hi[b], x);
-                    if constexpr (LO) {
-                        x = mfma16(p_hi[f], eo.lo[b], x);
-                        x = mfma16(p_lo[f], eo.hi[b], x);
-                    }
-                }
-                qo[m] = qo[m] + x * (load4(vec + kVecInvP * C + 16 * m + 4 * grp) * eo.inverse);
-            }
-            if (i + 1 < count)
-                load_p(i + 1);  // (before the stores: what waits for it does not wait for them)
+            for (int m = 0; m < 4; ++m)
+                qo[m] = qo[m] + x[m] * x_inverse;
+            load_p(then);  // (before the stores: what waits for it does not wait for them)
             const auto to = o_cols.rows(o + static_cast<int64_t>(i) * C * o_step, min(C, span.len - i * C));
             o_cols.template each<4>([&](int m, int r, int at) { buffer_store<Scalar>(qo[m][r], to, at); });
         }
 #pragma unroll
         for (int m = 0; m < 4; ++m)
-            e[m] = e[m] * (load4(vec + kVecLeftK * C + 16 * m + 4 * grp) * load4(vec + kVecBeta * C + 16 * m + 4 * grp));
+            e[m] = e[m] * load4(vec + kVecLeftK * C + 16 * m + 4 * grp);
         Operand<4, true> wo;
         wo.set(e);
+        wo.inverse *= e_inverse;
+        // steps: a part of two tiles of S, the update of the two before beside it
+        f32x4 x[2][2];
+        auto update = [&](int pair, const f32x4(&y)[2]) {
 #pragma unroll
-        for (int t = 0; t < DT; ++t) {
-            f32x4 x = zero;
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const u32x4 kf = lds.col_frag(lds.kt(0), t, b, lane);
-                x = mfma16(kf, wo.hi[b], x);
-                x = mfma16(kf, wo.lo[b], x);
-                if constexpr (PIECES == 2)
-                    x = mfma16(lds.col_frag(lds.kt(1), t, b, lane), wo.hi[b], x);
-            }
+                for (int r = 0; r < 4; ++r)
+                    s[2 * pair + h][r] = fmaf(y[h][r], wo.inverse, total * s[2 * pair + h][r]);
+        };
+        pipelined<DT / 2 * PIECES, 4, 2>(
+            [&](auto step, u32x4(&f)[4]) {
+                constexpr int at = decltype(step)::value, pair = at / PIECES;
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                s[t][r] = fmaf(x[r], wo.inverse, total * s[t][r]);
-        }
+                for (int n = 0; n < 4; ++n)
+                    f[n] = lds.col_frag(lds.kt(at % PIECES), 2 * pair + n / 2, n % 2, lane);
+            },
+            [&](auto step, const u32x4(&f)[4]) {
+                constexpr int at = decltype(step)::value, pair = at / PIECES, part = at % PIECES;
+                f32x4(&y)[2] = x[pair % 2];
+                if constexpr (part == 0)
+                    y[0] = y[1] = zero;
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        y[h] = mfma16(f[2 * h + b], wo.hi[b], y[h]);
+                if constexpr (part == 0)
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+                            y[h] = mfma16(f[2 * h + b], wo.lo[b], y[h]);
+                if constexpr (part == PIECES - 1 && pair > 0)
+                    update(pair - 1, x[(pair - 1) % 2]);
+            });
+        update(DT / 2 - 1, x[(DT / 2 - 1) % 2]);
         __syncthreads();
         if constexpr (BUFS == 1)
             __syncthreads();  // chunk i + 1 is there
@@ -652,29 +694,42 @@ __global__ __launch_bounds__(kWave *DT) void join_kernel(const DeltaJob job, con
         return x;
     };
     *reinterpret_cast<f32x4 *>(&s[0][row][d]) = load(0);
-    f32x4 next = load(1), map[DT];
-    auto load_map = [&](int i) {
+    // maps come two steps ahead of their use: a step is shorter than a load
+    f32x4 next[2], map[2][DT];
+    auto load_step = [&](int i, f32x4 &x, f32x4 (&m)[DT]) {
+        if (i + 1 >= work.parts)
+            return;
+        x = load(i);
         const float *from = work.maps + (piece + (BACK ? work.parts - 1 - i : i)) * wide * wide;
 #pragma unroll
         for (int t = 0; t < DT; ++t)
-            map[t] = BACK ? load4(from + (16 * t + 4 * grp) * wide + 16 * wave + row, wide)
-                          : load4(from + (16 * wave + row) * wide + 4 * grp + 16 * t);
+            m[t] = BACK ? load4(from + (16 * t + 4 * grp) * wide + 16 * wave + row, wide)
+                        : load4(from + (16 * wave + row) * wide + 4 * grp + 16 * t);
     };
-    load_map(1);
+    load_step(1, next[1], map[1]);
+    load_step(2, next[0], map[0]);
+    arrived(next);
+    arrived(map[0]);
+    arrived(map[1]);
     __syncthreads();
-    for (int i = 1; i + 1 < work.parts; ++i) {
-        f32x4 x = next;
+    auto step = [&](int i, f32x4 &x, f32x4 (&m)[DT]) {
+        f32x4 y = {0.f, 0.f, 0.f, 0.f};  // (two sums: half the chain)
 #pragma unroll
-        for (int t = 0; t < DT; ++t)
-            x = mfma4(map[t], load4(&s[(i + 1) & 1][row][16 * t + 4 * grp]), x);
-        if (i + 2 < work.parts) {
-            next = load(i + 1);
-            load_map(i + 1);
+        for (int t = 0; t < DT; t += 2) {
+            x = mfma4(m[t], load4(&s[(i + 1) & 1][row][16 * t + 4 * grp]), x);
+            y = mfma4(m[t + 1], load4(&s[(i + 1) & 1][row][16 * t + 16 + 4 * grp]), y);
         }
+        x = x + y;
         const auto to = state.rows(ends(i), rows);
         state.each<1>([&](int, int r, int at) { buffer_store<float>(x[r], to, at); });
         *reinterpret_cast<f32x4 *>(&s[i & 1][row][d]) = x;
+        load_step(i + 2, x, m);
         __syncthreads();
+    };
+    for (int i = 1; i + 1 < work.parts; i += 2) {
+        step(i, next[1], map[1]);
+        if (i + 2 < work.parts)
+            step(i + 1, next[0], map[0]);
     }
 }
 
@@ -800,6 +855,7 @@ int64_t delta_layout(const DeltaJob &job, bool packed, bool backward, char *base
     Carver carve{base};
     const int64_t records = static_cast<int64_t>(work->chunks) * job.Hv, square = kDeltaChunk * kDeltaChunk;
     work->offsets = packed ? carve.take<int32_t>(job.N + 1) : nullptr;
+    work->order = packed ? carve.take<int32_t>(job.N) : nullptr;
     work->gamma = carve.take<double>(records * kDeltaChunk);
     work->vec = carve.take<float>(records * kVecs * kDeltaChunk);
     work->y = carve.take<uint32_t>(records * 2 * kFragWords);

@@ -10,6 +10,8 @@
 
 #include "delta_rule.hpp"
 
+#include <type_traits>
+
 namespace ramnet {
 
 constexpr double kLog2e = 1.4426950408889634;
@@ -63,6 +65,9 @@ __device__ __forceinline__ DeltaPlace delta_place(const DeltaJob &job, const Del
     const int from = (chunk - first) * kDeltaChunk;
     return {n, span.b, span.t0 + from, max(0, min(kDeltaChunk, span.len - from))};
 }
+
+// The sequence whose states a chain's block walks.
+__device__ __forceinline__ int delta_line(const DeltaWork &work, int at) { return work.order ? work.order[at] : at; }
 
 // First chunk and number of chunks of a sequence.
 __device__ __forceinline__ void delta_chunks(const DeltaJob &job, const DeltaWork &work, int n, const DeltaSpan &span,

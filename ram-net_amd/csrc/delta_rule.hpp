@@ -30,6 +30,7 @@ struct DeltaJob {
 // head, record = chunk * Hv + head), and what a training forward keeps.
 struct DeltaWork {
     int32_t *offsets;  // (N + 1) first chunk of each packed sequence; null where sequences are rows
+    int32_t *order;    // (N) packed sequences, longest first; null likewise
     double *gamma;     // [record][64] running sums of the decays within the chunk, in powers of 2
     float *vec;        // [record][8][64] scales and decays of the tokens (delta_split.hpp)
     uint32_t *y;       // [record][2][6][64][4] N^-1 as matrix operands of fp16 parts (backward: transposed)

@@ -37,15 +37,21 @@ __device__ __forceinline__ float column_max(float m) {
     return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2));
+// Two values times a scale, each rounded once to fp16 (one instruction a value).
+__device__ __forceinline__ uint32_t scaled_f16(float a, float b, float scale) {
+    uint32_t h;
+    asm("v_fma_mixlo_f16 %0, %1, %2, 0 op_sel_hi:[0,0,0]" : "=v"(h) : "v"(a), "v"(scale));
+    asm("v_fma_mixhi_f16 %0, %1, %2, 0 op_sel_hi:[0,0,0]" : "+v"(h) : "v"(b), "v"(scale));
+    return h;
 }
 
 // hi and lo of two values.
 __device__ __forceinline__ void split2(float a, float b, float scale, uint32_t &hi, uint32_t &lo) {
-    const f16x2 h = __builtin_convertvector(f32x2{a * scale, b * scale}, f16x2);
-    hi = __builtin_bit_cast(uint32_t, h);
-    lo = pack_f16(fmaf(a, scale, -static_cast<float>(h[0])), fmaf(b, scale, -static_cast<float>(h[1])));
+    hi = scaled_f16(a, b, scale);
+    uint32_t l;
+    asm("v_fma_mixlo_f16 %0, %1, %2, -%3 op_sel_hi:[0,0,1]" : "=v"(l) : "v"(a), "v"(scale), "v"(hi));
+    asm("v_fma_mixhi_f16 %0, %1, %2, -%3 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "+v"(l) : "v"(b), "v"(scale), "v"(hi));
+    lo = l;
 }
 
 // N tiles of 16 rows (a multiple of 2) as B operands of 32 rows each. Rows go
@@ -75,7 +81,7 @@ struct Operand {
                     split2(x[t][r], x[t][r + 1], scale, h, l);
                     hi[t / 2][w] = h, lo[t / 2][w] = l;
                 } else {
-                    hi[t / 2][w] = pack_f16(x[t][r] * scale, x[t][r + 1] * scale);
+                    hi[t / 2][w] = scaled_f16(x[t][r], x[t][r + 1], scale);
                 }
             }
     }
@@ -125,6 +131,15 @@ struct Columns {
     }
 };
 
+// The values have arrived. A loop that goes on with them, and asks for the next
+// ones itself, would otherwise wait at its head for what it asked for last.
+template<typename T, int N>
+__device__ __forceinline__ void arrived(T (&x)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        asm volatile("" : "+v"(x[i]));
+}
+
 template<typename T>
 __device__ __forceinline__ uint32_t buffer_bits(__amdgpu_buffer_rsrc_t from, int at) {
     if constexpr (sizeof(T) == 4)
@@ -144,13 +159,12 @@ __device__ __forceinline__ void buffer_store(float v, __amdgpu_buffer_rsrc_t to,
 }
 
 // What prepare leaves per record, 64 values each, for the chain kernels: K and
-// Q are scaled by sk and sq a token, the rows of Y and P (backward: their
-// columns) by sy and sp.
+// Q are scaled by sk and sq a token, Y and P by sy and sp as a whole.
 enum : int {
     kVecSk, kVecSq,
     kVecGrowK,   // e^gamma / sk
     kVecGrowQ,   // scale e^gamma / sq
-    kVecLeftK,   // e^(gamma_C - gamma) / sk
+    kVecLeftK,   // e^(gamma_C - gamma) / sk (forward: times beta)
     kVecBeta,
     kVecInvY, kVecInvP,
     kVecs
@@ -202,7 +216,9 @@ struct Stager {
     f32x4 scales[2];  // of this thread's four tokens
     float vecs[2];
 
-    __device__ __forceinline__ void load_one(const Scalar *src, int64_t step, int len, int Dk, bool whole, int tid,
+    // WIDE: in pieces of 16 bytes
+    template<bool WIDE>
+    __device__ __forceinline__ void load_one(const Scalar *src, int64_t step, int len, int Dk, int tid,
                                              uint32_t (&to)[kItems][4][kWords]) {
         constexpr int size = static_cast<int>(sizeof(Scalar));
         const int pitch = static_cast<int>(step) * size;
@@ -214,7 +230,7 @@ struct Stager {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int at = first + e * pitch;
-                if (whole) {  // 16-byte accesses
+                if constexpr (WIDE) {
 #pragma unroll
                     for (int w = 0; w < kWords; w += 4) {
                         const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(rows, at + 4 * w, 0, 0);
@@ -235,15 +251,15 @@ struct Stager {
         }
     }
 
-    template<bool Q = true>
+    template<bool WIDE, bool Q>
     __device__ __forceinline__ void load(const Scalar *k, int64_t k_step, const Scalar *q, int64_t q_step, int len, int Dk,
-                                         bool whole, const float *vec, int tid) {
+                                         const float *vec, int tid) {
         vecs[0] = vec[tid], vecs[1] = vec[tid + 256];
         scales[0] = load4(vec + kVecSk * kDeltaChunk + tid % 16 * 4);
         scales[1] = load4(vec + kVecSq * kDeltaChunk + tid % 16 * 4);
-        load_one(k, k_step, len, Dk, whole, tid, raw[0]);
+        load_one<WIDE>(k, k_step, len, Dk, tid, raw[0]);
         if constexpr (Q)
-            load_one(q, q_step, len, Dk, whole, tid, raw[1]);
+            load_one<WIDE>(q, q_step, len, Dk, tid, raw[1]);
     }
 
     static __device__ __forceinline__ float value(const uint32_t (&w)[kWords], int i) {
@@ -271,7 +287,7 @@ struct Stager {
                     else if constexpr (__is_same(Scalar, _Float16))
                         h[0][e][i / 2] = from[n][e][i / 2];  // as it is
                     else
-                        h[0][e][i / 2] = pack_f16(value(from[n][e], i) * s[e], value(from[n][e], i + 1) * s[e]);
+                        h[0][e][i / 2] = scaled_f16(value(from[n][e], i), value(from[n][e], i + 1), s[e]);
                 }
 #pragma unroll
             for (int p = 0; p < PIECES; ++p) {
@@ -297,7 +313,7 @@ struct Stager {
         }
     }
 
-    template<bool Q = true>
+    template<bool Q>
     __device__ __forceinline__ void store(const Lds &lds, int tid) const {
         lds.vec()[tid] = vecs[0], lds.vec()[tid + 256] = vecs[1];
         store_one(raw[0], scales[0], tid, lds.k(0), lds.kt(0));
@@ -305,6 +321,68 @@ struct Stager {
             store_one(raw[1], scales[1], tid, QT ? nullptr : lds.q(0), QT ? lds.qt(0) : nullptr);
     }
 };
+
+// Products whose A operands come from LDS: a step's are read AHEAD steps before
+// their use, so that the matrix unit does not wait for the LDS (left to itself the
+// compiler keeps one or two reads under way). read(step, operands), use(step,
+// operands).
+template<int STEPS, int EACH, int AHEAD, int STEP = 0, typename Read, typename Use>
+__device__ __forceinline__ void pipelined_step(u32x4 (&f)[AHEAD + 1][EACH], Read read, Use use) {
+    if constexpr (STEP < STEPS) {
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (STEP + AHEAD < STEPS)
+            read(std::integral_constant<int, STEP + AHEAD>{}, f[(STEP + AHEAD) % (AHEAD + 1)]);
+        use(std::integral_constant<int, STEP>{}, f[STEP % (AHEAD + 1)]);
+        pipelined_step<STEPS, EACH, AHEAD, STEP + 1>(f, read, use);
+    }
+}
+
+template<int STEPS, int EACH, int AHEAD, typename Read, typename Use>
+__device__ __forceinline__ void pipelined(Read read, Use use) {
+    u32x4 f[AHEAD + 1][EACH];
+    read(std::integral_constant<int, 0>{}, f[0]);
+    if constexpr (AHEAD == 2 && STEPS > 1)
+        read(std::integral_constant<int, 1>{}, f[1]);
+    pipelined_step<STEPS, EACH, AHEAD>(f, read, use);
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// Which of `items` (and which of its `groups` column groups) block `at` has: an
+// item's groups read the same keys and queries, so they go to one of the eight
+// compute dies, which take blocks in turn, at one time.
+__device__ __forceinline__ void split_block(int at, int groups, int items, int &group, int &item) {
+    const int even = items / 8 * 8 * groups;
+    if (at < even) {
+        group = at / 8 % groups;
+        item = at / 8 / groups * 8 + at % 8;
+    } else {
+        group = (at - even) % groups;
+        item = items / 8 * 8 + (at - even) / groups;
+    }
+}
+
+// A lower (forward) or upper triangular 64 x 64 of fragments times an operand:
+// e += hi hi + hi lo + lo hi, the four row tiles' sums in turn.
+template<bool UPPER, bool LO, bool LO_B>
+__device__ __forceinline__ void triangle(const u32x4 (&hi)[kFrags], const u32x4 *lo, const u32x4 (&b_hi)[2],
+                                         const u32x4 *b_lo, f32x4 (&e)[4]) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int kind = 0; kind < 3; ++kind)
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                if (UPPER ? b < m / 2 : b > m / 2)
+                    continue;
+                const int f = UPPER ? (m < 2 ? m * 2 + b : m + 2) : (m < 2 ? m : 2 + (m - 2) * 2 + b);
+                if (kind == 0)
+                    e[m] = mfma16(hi[f], b_hi[b], e[m]);
+                else if (kind == 1 && LO_B)
+                    e[m] = mfma16(hi[f], b_lo[b], e[m]);
+                else if (kind == 2 && LO)
+                    e[m] = mfma16(lo[f], b_hi[b], e[m]);
+            }
+}
 
 // The segments' ends put together (work.parts > 1); backward: from the last
 // segment on, with the maps transposed.
