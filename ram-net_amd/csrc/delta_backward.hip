@@ -43,9 +43,12 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
     int first, count;
     delta_chunks(job, work, n, span, first, count);
     int skipped = 0;
-    if (work.parts > 1) {
+    const int segments = delta_segments(work, count);
+    if (part >= segments || (PART && part + 1 == segments))
+        return;
+    if (segments > 1) {
         const int to = count;
-        skipped = min((work.parts - 1 - part) * work.part_chunks, to);
+        skipped = (segments - 1 - part) * work.part_chunks;
         first += skipped;
         count = min(to - skipped, work.part_chunks);
         span.t0 += skipped * C, span.len = min(span.len - skipped * C, count * C);
@@ -234,7 +237,7 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
             __syncthreads();  // chunk i - 1 is there
     }
     float *const before = PART ? work.ends + piece * job.Dk * job.Dv
-                          : part + 1 < work.parts || !grads.dinit ? nullptr
+                          : part + 1 < segments || !grads.dinit ? nullptr
                                                                    : grads.dinit + matrix;
     if (before) {
         const auto to = state.rows(before, job.Dk);

@@ -406,8 +406,11 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
     const int row_end = span.len;
     int first, count;
     delta_chunks(job, work, n, span, first, count);
-    if (work.parts > 1) {
-        const int from = min(part * work.part_chunks, count);
+    const int segments = delta_segments(work, count);
+    if (part >= segments || (MAP && part + 1 == segments))
+        return;
+    if (segments > 1) {
+        const int from = part * work.part_chunks;
         first += from;
         count = min(count - from, work.part_chunks);
         span.t0 += from * C, span.len -= from * C;
@@ -465,11 +468,19 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
             for (int r = 0; r < 4; ++r)
                 s[t][r] = 16 * t + 4 * grp + r == c && c < job.Dk ? 1.f : 0.f;
     } else {
-        const float *init = part == 0 ? job.init ? job.init + matrix : nullptr
+        // A row that is cut has its first state twice: the last segment may write where it
+        // came from (in place) before the first one has started, so it reads a copy, in the
+        // last segment's place.
+        float *const copy = work.ends + (piece - part + work.parts - 1) * job.Dk * job.Dv;
+        const float *init = part == 0 ? !job.init ? nullptr : !MAP && segments > 1 ? copy : job.init + matrix
                             : MAP     ? nullptr
                                       : work.ends + (piece - 1) * job.Dk * job.Dv;
         const auto from = state.rows(init, init ? job.Dk : 0);
         state.each<DT>([&](int t, int r, int at) { s[t][r] = __uint_as_float(buffer_bits<float>(from, at)); });
+        if (MAP && init) {
+            const auto to = state.rows(copy, job.Dk);
+            state.each<DT>([&](int t, int r, int at) { buffer_store<float>(s[t][r], to, at); });
+        }
     }
     const Scalar *v = static_cast<const Scalar *>(job.v) + span.b * job.v_at[0] + head * job.v_at[2] +
                       span.t0 * job.v_at[1];
@@ -662,7 +673,7 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
         }
         return;
     }
-    if (!MAP && part + 1 < work.parts)
+    if (!MAP && part + 1 < segments)
         return;
     const auto to = state.rows(MAP ? work.ends + piece * job.Dk * job.Dv : job.state + matrix, job.Dk);
     state.each<DT>([&](int t, int r, int at) { buffer_store<float>(s[t][r], to, at); });
@@ -683,6 +694,12 @@ __global__ __launch_bounds__(kWave *DT) void join_kernel(const DeltaJob job, con
     const int row = lane & 15, grp = lane >> 4;
     const int group = static_cast<int>(blockIdx.x) % groups, line = static_cast<int>(blockIdx.x) / groups;
     const int c = group * 16 + row, d = 16 * wave + 4 * grp;
+    const int n = delta_line(work, line / job.Hv);
+    int first, count;
+    delta_chunks(job, work, n, delta_span(job, n), first, count);
+    const int segments = delta_segments(work, count);
+    if (segments <= 2)
+        return;  // (the first segment's end is whole)
     const int64_t piece = static_cast<int64_t>(line) * work.parts, size = static_cast<int64_t>(job.Dk) * job.Dv;
     const Columns<float> state(job.Dv, job.Dv, grp, c);
     auto ends = [&](int i) { return work.ends + (piece + i) * size + static_cast<int64_t>(16 * wave) * job.Dv; };
@@ -697,10 +714,10 @@ __global__ __launch_bounds__(kWave *DT) void join_kernel(const DeltaJob job, con
     // maps come two steps ahead of their use: a step is shorter than a load
     f32x4 next[2], map[2][DT];
     auto load_step = [&](int i, f32x4 &x, f32x4 (&m)[DT]) {
-        if (i + 1 >= work.parts)
+        if (i + 1 >= segments)
             return;
         x = load(i);
-        const float *from = work.maps + (piece + (BACK ? work.parts - 1 - i : i)) * wide * wide;
+        const float *from = work.maps + (piece + (BACK ? segments - 1 - i : i)) * wide * wide;
 #pragma unroll
         for (int t = 0; t < DT; ++t)
             m[t] = BACK ? load4(from + (16 * t + 4 * grp) * wide + 16 * wave + row, wide)
@@ -726,9 +743,9 @@ __global__ __launch_bounds__(kWave *DT) void join_kernel(const DeltaJob job, con
         load_step(i + 2, x, m);
         __syncthreads();
     };
-    for (int i = 1; i + 1 < work.parts; i += 2) {
+    for (int i = 1; i + 1 < segments; i += 2) {
         step(i, next[1], map[1]);
-        if (i + 2 < work.parts)
+        if (i + 2 < segments)
             step(i + 1, next[0], map[0]);
     }
 }
@@ -802,9 +819,12 @@ hipError_t chain_typed(const DeltaJob &job, const DeltaWork &work, hipStream_t s
 }  // namespace
 
 // Short calls, and those whose chunks (two fp16 parts of each fp32 key and
-// query) do not fit the LDS.
+// query) do not fit the LDS. A chunk costs the same however few its tokens: with
+// 8 tokens of 128 x 128 heads in bf16, token by token and in chunks take 15.4 and
+// 19.2 us for 8 heads, 47.6 and 47.5 for 32 rows of 16 heads, 83 and 78 for 64;
+// with 16 tokens 26.5 and 19.4, 82 and 46, 153 and 77.
 bool delta_is_recurrent(const DeltaJob &job) {
-    return job.T <= 32 || (job.dtype == kF32 && delta_padded(job.Dk) > 160);
+    return job.T <= 8 || (job.dtype == kF32 && delta_padded(job.Dk) > 160);
 }
 
 namespace {
@@ -827,19 +847,34 @@ void count_chunks(const DeltaJob &job, bool packed, DeltaWork *work) {
     work->chunks = packed ? work->per_row + job.N : job.N * work->per_row;
 }
 
-// Segments of a row: as many as fill the GPU's 256 compute units with blocks of
-// 64 columns, each at least kPartChunks long. A segment's map costs its state
-// columns once more, so half full is left as it is: one row of 32768 tokens, 8
-// heads of 128 x 128 (16 blocks), takes 1.59 ms in one segment.
+// Segments of a row: what costs least, in times of a chunk of the chain. A pass
+// walks a segment's chunks (and starts, about two) once for every 256 blocks of 64
+// columns; the first pass, 0.6 of the time, has the columns of the maps too; the
+// join takes 0.6 a segment. One row of 32768 tokens, 8 heads of 128 x 128 (16
+// blocks): 1.59 ms in one segment, 0.36 ms in 16. 4096 tokens: 16 blocks 210 us in
+// one segment, 85 in 8, 95 in 16; 64 blocks 228 in one, 177 in 4; 128 blocks 272
+// in one, 249 in 2.
+// Packed rows may be one long one or all alike: segments are sized as for one, and
+// a row is cut where it has more than two.
 void count_parts(const DeltaJob &job, bool packed, DeltaWork *work) {
-    constexpr int kUnits = 256, kPartChunks = 8;
-    const int64_t blocks = static_cast<int64_t>(job.N) * job.Hv * ((job.Dv + 63) / 64);
-    work->parts = 1, work->part_chunks = work->per_row;
-    if (packed || blocks > kUnits / 4 || work->per_row < 2 * kPartChunks)
+    constexpr int kUnits = 256, kMost = 64, kLeast = 4;
+    const int64_t columns = static_cast<int64_t>(job.Hv) * ((job.Dv + 63) / 64);
+    work->parts = 1, work->part_chunks = work->uncut = work->per_row;
+    if (columns * job.N > kUnits / 2)
         return;
-    const int parts = std::min(static_cast<int>(kUnits / blocks), work->per_row / kPartChunks);
-    work->part_chunks = (work->per_row + parts - 1) / parts;
-    work->parts = (work->per_row + work->part_chunks - 1) / work->part_chunks;
+    const int64_t blocks = packed ? columns : columns * job.N;
+    const int64_t map_blocks = blocks / ((job.Dv + 63) / 64) * ((delta_padded(job.Dk) + job.Dv + 63) / 64);
+    float least = static_cast<float>(work->per_row + 2);
+    for (int parts = 2; parts <= std::min(work->per_row / kLeast, kMost); ++parts) {
+        const int chunks = (work->per_row + parts - 1) / parts;
+        const int64_t first = (blocks + (parts - 2) * map_blocks + kUnits - 1) / kUnits;
+        const int64_t second = (blocks * parts + kUnits - 1) / kUnits;
+        const float cost = static_cast<float>(chunks + 2) * (0.6f * static_cast<float>(first) + static_cast<float>(second)) +
+                           0.6f * static_cast<float>(parts - 2) + 2.f;
+        if (cost < least)
+            least = cost, work->part_chunks = chunks, work->parts = (work->per_row + chunks - 1) / chunks;
+    }
+    work->uncut = packed ? 2 * work->part_chunks : work->part_chunks;
 }
 
 int64_t map_floats(const DeltaJob &job, const DeltaWork &work) {

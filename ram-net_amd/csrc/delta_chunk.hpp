@@ -81,6 +81,11 @@ __device__ __forceinline__ void delta_chunks(const DeltaJob &job, const DeltaWor
     }
 }
 
+// Segments of a row of `count` chunks.
+__device__ __forceinline__ int delta_segments(const DeltaWork &work, int count) {
+    return count > work.uncut ? (count + work.part_chunks - 1) / work.part_chunks : 1;
+}
+
 constexpr int kLdsBytes = 160 * 1024;
 
 // Whether rows of q and k are whole pieces of 16 bytes at 16-byte addresses.
@@ -90,18 +95,6 @@ __host__ __device__ inline bool rows_whole(const DeltaJob &job) {
     const int64_t steps = job.q_at[0] | job.q_at[1] | job.q_at[2] | job.k_at[0] | job.k_at[1] | job.k_at[2];
     const uintptr_t starts = reinterpret_cast<uintptr_t>(job.q) | reinterpret_cast<uintptr_t>(job.k);
     return job.Dk % 8 == 0 && steps % V == 0 && starts % 16 == 0;
-}
-
-// 64 rows of D values into fp32 rows of `pitch`, zeros after `len` rows and up
-// to `wide` columns; `step` between rows of the source.
-template<typename Scalar>
-__device__ __forceinline__ void stage_rows(const Scalar *src, int64_t step, int len, int D, int wide, float *dst,
-                                           int pitch) {
-    const int total = kDeltaChunk * wide;
-    for (int i = threadIdx.x; i < total; i += blockDim.x) {
-        const int t = i / wide, d = i - t * wide;
-        dst[t * pitch + d] = t < len && d < D ? load_f32(src + t * step + d) : 0.f;
-    }
 }
 
 }  // namespace ramnet

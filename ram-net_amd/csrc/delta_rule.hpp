@@ -44,9 +44,10 @@ struct DeltaWork {
     float *states;     // [record][Dk][..] state before the chunk    (kept)
     // where the time axis of a row is cut into segments that run side by side (parts > 1),
     // per row, value head and segment:
-    float *ends;       // [Dk][Dv] state after the segment: first from zeros (the first from init), then in full
+    float *ends;       // [Dk][Dv] state after the segment: first from zeros (the first from init), then in full;
+                       //   in the last place the row's init
     float *maps;       // [wide][wide] what the segment makes of the state before it (kept)
-    int parts, part_chunks;
+    int parts, part_chunks, uncut;  // (at most; chunks of one; the most chunks that a row is not cut at)
     int per_row;       // chunks of a row where sequences are rows
     int chunks;        // records / Hv
 };

@@ -503,3 +503,46 @@ def test_gradients_compiled_and_selected():
     x = [t.detach().requires_grad_(i == 2) for i, t in enumerate(case)]
     loss(*x).backward()
     assert torch.equal(x[2].grad, want[2]) and all(t.grad is None for i, t in enumerate(x) if i != 2)
+
+
+# ---- rows cut into segments: packed ones, ones whose tokens do not all count, in place
+
+@pytest.mark.parametrize("lens", [[1600], [30, 1500, 0, 70], [700, 700, 600], [1] * 6 + [1994], [1024] + [0] * 5])
+def test_long_packed(lens):
+    case = _case(T=sum(lens), Hk=1, Hv=2, Dk=40, Dv=24, N=len(lens), seed=len(lens))
+    cu = torch.tensor([0] + lens).cumsum(0).to(DEV, torch.int32)
+    _check(case, _call(case, cu_seqlens=cu), lens, packed=True)
+    case[5] = None
+    _check(case, _call(case, cu_seqlens=cu), lens, packed=True)
+
+
+def test_long_packed_tokens_of_no_sequence_are_zero():
+    case = _case(T=2000, Dk=16, Dv=16, N=3, seed=5)
+    cu = torch.tensor([100, 110, 1800, 1801], dtype=torch.int32, device=DEV)
+    o, state = _call(case, cu_seqlens=cu)
+    part = [t[:, 100:1801] for t in case[:5]] + [case[5]]
+    _check(part, (o[:, 100:1801].contiguous(), state), [10, 1690, 1], packed=True)
+    assert o[:, :100].abs().max() == 0 and o[:, 1801:].abs().max() == 0
+
+
+@pytest.mark.parametrize("lens", [[1100], [20, 1500, 0, 70], [1] * 3 + [1200]])
+def test_long_packed_gradients(lens):
+    case = _case(T=sum(lens), Hk=1, Hv=2, Dk=24, Dv=40, N=len(lens), seed=len(lens))
+    cu = torch.tensor([0] + lens).cumsum(0).to(DEV, torch.int32)
+    _check_grads(case, kw=dict(cu_seqlens=cu), lens=lens, packed=True)
+
+
+def test_long_rows_counted_lengths_gradients():
+    lens = [1100, 0, 1, 600, 320]
+    case = _case(B=5, T=1100, Hk=1, Hv=1, Dk=24, Dv=40, seed=8)
+    _check_grads(case, kw=dict(lengths=torch.tensor(lens, device=DEV)), lens=lens)
+
+
+@pytest.mark.parametrize("T,packed", [(1024, False), (4000, False), (4000, True)])
+def test_long_rows_in_place(T, packed):
+    """The first segment's state is what the last one writes over."""
+    case = _case(T=T, Hk=2, Hv=2, Dk=64, Dv=64, dtype="bf16", seed=T)
+    kw = dict(cu_seqlens=torch.tensor([0, T], dtype=torch.int32, device=DEV)) if packed else {}
+    want = _call(case, **kw)
+    got = _call(case, inplace=True, **kw)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
