@@ -5,7 +5,7 @@
 // four columns to a thread where Dv and the addresses allow 16-byte accesses.
 // A token costs one reduction over rows: with S the state before it,
 //     S_new^T q = e^g S^T q + (k.q) u,
-// so S^T k, S^T q and k.q are summed together, within a wave by shuffles and
+// so S^T k, S^T q and k.q are summed together, within a wave by lane swaps and
 // over the four waves through LDS, in a fixed order. The next token's inputs
 // are on their way meanwhile.
 //
@@ -27,10 +27,25 @@ struct Token {
     float g, beta;
 };
 
+// a and b, each summed over the two halves of the wave (or of each 32 lanes): a
+// in the first of the two, b in the second. No LDS is in it, as in a shuffle.
+__device__ __forceinline__ float fold32(float a, float b) {
+    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return __uint_as_float(x[0]) + __uint_as_float(x[1]);
+}
+__device__ __forceinline__ float fold16(float a, float b) {
+    const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return __uint_as_float(x[0]) + __uint_as_float(x[1]);
+}
+// Each lane's and that of the lane 8 further in its row of 16.
+__device__ __forceinline__ float fold8(float a) {
+    return a + __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(a), 0x128, 0xF, 0xF, false));
+}
+
 template<typename Scalar, int VEC, int R>
 __global__ __launch_bounds__(kThreads) void recurrent_kernel(const DeltaJob job, int slices) {
     constexpr int CL = kSlice / VEC, RG = kThreads / CL;  // column lanes, row groups
-    __shared__ float part[2][kThreads / kWave][kSlice][2];
+    __shared__ __align__(16) float part[2][kThreads / kWave][2][kSlice];  // [k, q]
     __shared__ float part_kq[2][kThreads / kWave];
     const int tid = static_cast<int>(threadIdx.x), wave = tid / kWave;
     const int cl = tid % CL, rg = tid / CL;
@@ -99,24 +114,22 @@ __global__ __launch_bounds__(kThreads) void recurrent_kernel(const DeltaJob job,
                 sq[e] = fmaf(qr, s[j][e], sq[e]);
             }
         }
-#pragma unroll
-        for (int m = CL; m < kWave; m <<= 1) {
-            kq += __shfl_xor(kq, m);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                sk[e] += __shfl_xor(sk[e], m);
-                sq[e] += __shfl_xor(sq[e], m);
+        const int lane = tid % kWave;
+        if constexpr (VEC == 4) {
+            const float x = fold8(fold16(fold32(sk[0], sq[0]), fold32(sk[1], sq[1])));
+            const float y = fold8(fold16(fold32(sk[2], sq[2]), fold32(sk[3], sq[3])));
+            kq = fold8(kq);
+            kq = fold16(kq, kq);
+            if (lane % 16 < CL) {  // rows of 16 lanes: columns e and e + 2 of k, e = 0, 1; then of q
+                float *to = &part[buf][wave][lane / 32][cl * 4 + lane / 16 % 2];
+                to[0] = x, to[2] = y;
             }
+        } else {
+            part[buf][wave][lane / 32][cl] = fold32(sk[0], sq[0]);
         }
-        if (tid % kWave < CL) {
-            if (cl == 0)
-                part_kq[buf][wave] = kq;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                part[buf][wave][cl * VEC + e][0] = sk[e];
-                part[buf][wave][cl * VEC + e][1] = sq[e];
-            }
-        }
+        kq = fold32(kq, kq);
+        if (lane == 0)
+            part_kq[buf][wave] = kq;
         __syncthreads();  // (the other buffer is written next: one barrier a token)
         kq = 0.f;
 #pragma unroll
@@ -129,8 +142,8 @@ __global__ __launch_bounds__(kThreads) void recurrent_kernel(const DeltaJob job,
             float a = 0.f, b = 0.f;
 #pragma unroll
             for (int w = 0; w < kThreads / kWave; ++w) {
-                a += part[buf][w][cl * VEC + e][0];
-                b += part[buf][w][cl * VEC + e][1];
+                a += part[buf][w][0][cl * VEC + e];
+                b += part[buf][w][1][cl * VEC + e];
             }
             const float u = now.beta * (bits_f32<Scalar>(now.v[e]) - alpha * a);
             out[e] = job.scale * (alpha * b + kq * u);
