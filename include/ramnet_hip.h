@@ -508,8 +508,8 @@ int ramnet_delta_rule_forward(const ramnet_delta_rule_call *call, void *stream);
  * Its gradients, from d_o (B, T, Hv, Dv) `dtype`, of strides d_o_strides (batch
  * row, token, head), and d_state (N, Hv, Dk, Dv) fp32 (or NULL: zeros): dq, dk,
  * dv, dg, dbeta in their inputs' shapes and types, dense, and dinit (N, Hv, Dk,
- * Dv) fp32 (or NULL). `call` is the forward's, with a workspace of kind 2; its
- * init_state, state and o are not read. Value heads that share a key head add
+ * Dv) fp32 (or NULL; not d_state). `call` is the forward's, with a workspace of
+ * kind 2; its init_state, state and o are not read. Value heads that share a key head add
  * to its gradient in one order: results do not change from call to call.
  * float32 inputs take Dk up to 160 here.
  */

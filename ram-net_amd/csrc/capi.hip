@@ -1259,6 +1259,7 @@ int ramnet_delta_rule_backward(const ramnet_delta_rule_call *call, const void *d
     if (job.N == 0)
         return RAMNET_OK;
     RAMNET_REQUIRE(d_o && d_o_strides && dq && dk && dv && dg && dbeta && call->kept, "null tensor pointer");
+    RAMNET_REQUIRE(!dinit || dinit != d_state, "delta rule: dinit must not be d_state");
     ramnet::DeltaWork work{};
     if (int rc = delta_regions(job, *call, true, work))
         return rc;

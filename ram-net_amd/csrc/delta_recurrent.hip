@@ -9,7 +9,11 @@
 // over the four waves through LDS, in a fixed order. The next token's inputs
 // are on their way meanwhile.
 //
-// A decode step is bound by reading and writing the state once.
+// A decode step is bound by reading and writing the state once: one token of 64
+// rows, 16 heads of 128 x 128 moves 134 MB in 25 us (5.3 TB/s, a large copy's
+// rate). Several tokens add their latency: six of 32 rows take 22 us a call, 27
+// with shuffles for the sums. More blocks at a time by fewer registers (80 and 64
+// of the 90) spill: 24.6 and 45 us.
 #include "delta_rule.hpp"
 #include "ramnet_kernels.hpp"
 

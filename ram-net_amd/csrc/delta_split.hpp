@@ -322,28 +322,28 @@ struct Stager {
     }
 };
 
-// Products whose A operands come from LDS: a step's are read AHEAD steps before
+// Products whose A operands come from LDS: a step's are read two steps before
 // their use, so that the matrix unit does not wait for the LDS (left to itself the
 // compiler keeps one or two reads under way). read(step, operands), use(step,
 // operands).
-template<int STEPS, int EACH, int AHEAD, int STEP = 0, typename Read, typename Use>
-__device__ __forceinline__ void pipelined_step(u32x4 (&f)[AHEAD + 1][EACH], Read read, Use use) {
+template<int STEPS, int EACH, int STEP, typename Read, typename Use>
+__device__ __forceinline__ void pipelined_step(u32x4 (&f)[3][EACH], Read read, Use use) {
     if constexpr (STEP < STEPS) {
         __builtin_amdgcn_sched_barrier(0);
-        if constexpr (STEP + AHEAD < STEPS)
-            read(std::integral_constant<int, STEP + AHEAD>{}, f[(STEP + AHEAD) % (AHEAD + 1)]);
-        use(std::integral_constant<int, STEP>{}, f[STEP % (AHEAD + 1)]);
-        pipelined_step<STEPS, EACH, AHEAD, STEP + 1>(f, read, use);
+        if constexpr (STEP + 2 < STEPS)
+            read(std::integral_constant<int, STEP + 2>{}, f[(STEP + 2) % 3]);
+        use(std::integral_constant<int, STEP>{}, f[STEP % 3]);
+        pipelined_step<STEPS, EACH, STEP + 1>(f, read, use);
     }
 }
 
-template<int STEPS, int EACH, int AHEAD, typename Read, typename Use>
+template<int STEPS, int EACH, typename Read, typename Use>
 __device__ __forceinline__ void pipelined(Read read, Use use) {
-    u32x4 f[AHEAD + 1][EACH];
+    u32x4 f[3][EACH];
     read(std::integral_constant<int, 0>{}, f[0]);
-    if constexpr (AHEAD == 2 && STEPS > 1)
+    if constexpr (STEPS > 1)
         read(std::integral_constant<int, 1>{}, f[1]);
-    pipelined_step<STEPS, EACH, AHEAD>(f, read, use);
+    pipelined_step<STEPS, EACH, 0>(f, read, use);
     __builtin_amdgcn_sched_barrier(0);
 }
 

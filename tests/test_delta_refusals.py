@@ -150,3 +150,9 @@ def test_native_verify_drafts():
     call("dtype", dtype=5)
     call("null tensor", tokens=None)
     call("null tensor", sample=None)
+
+
+def test_native_delta_rule_backward_in_place():
+    nat = _native()
+    _einval("ramnet_delta_rule_backward",
+            (_packed(kept=FAKE, kept_bytes=1 << 30), FAKE, nat.strides(64, 64, 64), FAKE, *(FAKE,) * 6, None), "dinit")
