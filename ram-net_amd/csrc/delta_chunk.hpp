@@ -81,6 +81,21 @@ __device__ __forceinline__ void delta_chunks(const DeltaJob &job, const DeltaWor
     }
 }
 
+// Which of `items` (and which of its `groups` column groups) block `at` has: an
+// item's groups read the same keys and queries (and write parts of the same cache
+// lines), so they go to one of the eight compute dies, which take blocks in turn, at
+// one time.
+__device__ __forceinline__ void split_block(int at, int groups, int items, int &group, int &item) {
+    const int even = items / 8 * 8 * groups;
+    if (at < even) {
+        group = at / 8 % groups;
+        item = at / 8 / groups * 8 + at % 8;
+    } else {
+        group = (at - even) % groups;
+        item = items / 8 * 8 + (at - even) / groups;
+    }
+}
+
 // Segments of a row of `count` chunks.
 __device__ __forceinline__ int delta_segments(const DeltaWork &work, int count) {
     return count > work.uncut ? (count + work.part_chunks - 1) / work.part_chunks : 1;

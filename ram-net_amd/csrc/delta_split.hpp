@@ -347,20 +347,6 @@ __device__ __forceinline__ void pipelined(Read read, Use use) {
     __builtin_amdgcn_sched_barrier(0);
 }
 
-// Which of `items` (and which of its `groups` column groups) block `at` has: an
-// item's groups read the same keys and queries, so they go to one of the eight
-// compute dies, which take blocks in turn, at one time.
-__device__ __forceinline__ void split_block(int at, int groups, int items, int &group, int &item) {
-    const int even = items / 8 * 8 * groups;
-    if (at < even) {
-        group = at / 8 % groups;
-        item = at / 8 / groups * 8 + at % 8;
-    } else {
-        group = (at - even) % groups;
-        item = items / 8 * 8 + (at - even) / groups;
-    }
-}
-
 // A lower (forward) or upper triangular 64 x 64 of fragments times an operand:
 // e += hi hi + hi lo + lo hi, the four row tiles' sums in turn.
 template<bool UPPER, bool LO, bool LO_B>

@@ -546,3 +546,36 @@ def test_long_rows_in_place(T, packed):
     want = _call(case, **kw)
     got = _call(case, inplace=True, **kw)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("T", [70, 1100])
+def test_gradients_graph_replays(T):
+    """A forward and its backward captured together, on leaves that no eager graph holds then."""
+    from ramnet_ops import gated_delta_rule
+
+    def leaves(seed):
+        return [t.to(DEV) for t in _case(T=T, Hk=1, Hv=2, Dk=40, Dv=32, dtype="bf16", seed=seed)]
+
+    def grads(x, w):
+        o, state = gated_delta_rule(*x[:5], init_state=x[5])
+        return torch.autograd.grad([o, state], x, [w, torch.ones_like(state)])
+    x = [t.requires_grad_() for t in leaves(1)]
+    w = torch.randn(1, T, 2, 32, device=DEV).to(torch.bfloat16)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        grads(x, w)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = grads(x, w)
+    for step in range(3):
+        new = leaves(2 + step)
+        with torch.no_grad():
+            for t, s in zip(x, new):
+                t.copy_(s)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, grads([t.requires_grad_() for t in new], w)):
+            assert torch.equal(a, b)
