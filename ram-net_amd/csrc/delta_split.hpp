@@ -182,6 +182,8 @@ __device__ __forceinline__ void frag_place(int f, bool upper, int &tile, int &bl
 // The K and Q of a chunk as A operands in LDS, PIECES fp16 parts of each:
 //   k, q  [64 tokens][wide]   contraction over Dk
 //   kt    [wide][64 tokens]   contraction over the tokens (and qt, backward)
+// A row's pieces of 16 bytes lie in another order, by fours, in each 16 tokens: the
+// tokens that 16 lanes store at a time, four apart, would else share four banks.
 template<int DT, int PIECES, bool QT>
 struct ChunkLds {
     static constexpr int kWide = 16 * DT, kPitch = kWide + 8, kPitchT = kDeltaChunk + 8;
@@ -197,7 +199,7 @@ struct ChunkLds {
     __device__ __forceinline__ float *vec() const { return reinterpret_cast<float *>(base + kHalves); }
 
     __device__ __forceinline__ u32x4 row_frag(const uint16_t *m, int tile, int block, int lane) const {
-        return *reinterpret_cast<const u32x4 *>(m + (16 * tile + (lane & 15)) * kPitch + 32 * block + 8 * (lane >> 4));
+        return *reinterpret_cast<const u32x4 *>(m + (16 * tile + (lane & 15)) * kPitch + 32 * block + 8 * (lane >> 4 ^ (tile & 3)));
     }
     __device__ __forceinline__ u32x4 col_frag(const uint16_t *m, int tile, int block, int lane) const {
         return *reinterpret_cast<const u32x4 *>(m + (16 * tile + (lane & 15)) * kPitchT + 32 * block + 8 * (lane >> 4));
@@ -295,8 +297,8 @@ struct Stager {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         uint16_t *to = rows + p * Lds::kRows + (4 * quad + e) * Lds::kPitch;
-                        *reinterpret_cast<u32x2 *>(to + operand_at(d)) = u32x2{h[p][e][0], h[p][e][1]};
-                        *reinterpret_cast<u32x2 *>(to + operand_at(d + 4)) = u32x2{h[p][e][2], h[p][e][3]};
+                        *reinterpret_cast<u32x2 *>(to + (operand_at(d) ^ quad / 4 * 8)) = u32x2{h[p][e][0], h[p][e][1]};
+                        *reinterpret_cast<u32x2 *>(to + (operand_at(d + 4) ^ quad / 4 * 8)) = u32x2{h[p][e][2], h[p][e][3]};
                     }
                 if (cols)
 #pragma unroll
