@@ -133,7 +133,7 @@ __device__ __forceinline__ double running_sum(double x) {
 // Y, P, gamma and the scales of one chunk and value head: wave w has the
 // tokens of tile w. Latency from end to end, so as many blocks as fit: P's
 // operands and then Y take the place of the keys. Eight rows of 4096 tokens, 16
-// heads of 128 in bf16 (420 MB in and out): 125 us, 3.4 TB/s.
+// heads of 128 in bf16 (461 MB in and out): 125 us, 3.7 TB/s.
 template<typename Scalar, int DT>
 __global__ __launch_bounds__(256, 4) void prepare_kernel(const DeltaJob job, const DeltaWork work, bool backward) {
     constexpr int C = kDeltaChunk, NP = C + 4, wide = 16 * DT, pitch = wide + 16 / static_cast<int>(sizeof(Scalar));
@@ -384,9 +384,9 @@ __global__ __launch_bounds__(256, 4) void prepare_kernel(const DeltaJob job, con
 // join_kernel puts the states at the segments' ends together, and the chain
 // proper starts each segment from there.
 //
-// Latency of the matrix products that depend on one another binds a chunk (64 blocks
-// a time step and more: what they read, keys and queries once for each 64 columns).
-// Eight rows of 4096 tokens, 16 heads of 128 x 128 in bf16: 247 us.
+// What binds a chunk is the latency of products that depend on one another: eight
+// rows of 4096 tokens, 16 heads of 128 x 128 in bf16, take 248 us at 3.1 TB/s, the
+// matrix units 23% and the LDS 33% busy.
 //
 // DT: Dk in tiles of 16; PIECES: fp16 parts of q and k; LO: whether products
 // that go to o alone take the second parts too (bf16 outputs do not show them:

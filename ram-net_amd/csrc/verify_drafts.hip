@@ -14,7 +14,7 @@
 // fixed order: a draw next to a border of the running sum would go by the
 // rounding of 32. What waves find is put together by ballots: LDS atomics on one
 // word go lane by lane (20 us of a call). 192 rows of 128257 in fp32 (197 MB): 45 us,
-// 4.4 TB/s; one row of 32000: 5 us of latency.
+// 4.4 TB/s; one row of 32000: 9 us of latency.
 #include "ramnet_device.hpp"
 #include "ramnet_kernels.hpp"
 
