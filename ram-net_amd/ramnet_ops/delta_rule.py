@@ -81,7 +81,8 @@ def gated_delta_rule(
                                    init_state)[:2]
         return _delta.gated_delta_rule_(q, k, v, g, beta, init_state, cu_seqlens, lengths, scale), init_state
     if grad:
-        return _delta.gated_delta_rule_kept(q, k, v, g, beta, init_state, cu_seqlens, lengths, scale)[:2]
+        run = _delta.Trained.apply if eager else _delta.gated_delta_rule_kept
+        return run(q, k, v, g, beta, init_state, cu_seqlens, lengths, scale)[:2]
     if eager:
         return _delta._forward("gated_delta_rule", q, k, v, g, beta, init_state, cu_seqlens, lengths, scale)[:2]
     return _delta.gated_delta_rule(q, k, v, g, beta, init_state, cu_seqlens, lengths, scale)
