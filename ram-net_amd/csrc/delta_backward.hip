@@ -154,18 +154,18 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
         const int then = max(i - 1, 0);  // (the first chunk's once more rather than a branch)
         load_o(then);
         {
-            Operand<4, true> oo;
+            Operand<4> oo;
             oo.set(out);
 #pragma unroll
             for (int m = 0; m < 4; ++m)
                 x[m] = zero;
             // (dO's second part is 0 for bf16 but far below a column's largest)
-            triangle<true, true, !__is_same(Scalar, bf16_t)>(p_hi, p_lo, oo.hi, oo.lo, x);
+            triangle<true, !__is_same(Scalar, bf16_t)>(p_hi, p_lo, oo.hi, oo.lo, x);
             x_inverse = vec[kVecInvP * C] * oo.inverse;
             load_frags(work.p_frags, then, p_hi, p_lo);
         }
         {
-            Operand<DT, true> so;
+            Operand<DT> so;
             so.set(s);
 #pragma unroll
             for (int m = 0; m < 4; ++m)
@@ -186,12 +186,12 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
                         load4(vec + kVecBeta * C + 16 * m + 4 * grp);
         }
         {
-            Operand<4, true> uo;
+            Operand<4> uo;
             uo.set(du);
 #pragma unroll
             for (int m = 0; m < 4; ++m)
                 x[m] = zero;
-            triangle<true, true, true>(y_hi, y_lo, uo.hi, uo.lo, x);
+            triangle<true>(y_hi, y_lo, uo.hi, uo.lo, x);
             x_inverse = vec[kVecInvY * C] * uo.inverse;
 #pragma unroll
             for (int m = 0; m < 4; ++m)
@@ -209,7 +209,7 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
             x[m] = -(load4(vec + kVecGrowK * C + 16 * m + 4 * grp) * x[m]);
             out[m] = out[m] * load4(vec + kVecGrowQ * C + 16 * m + 4 * grp);
         }
-        Operand<4, true> xo, oo;
+        Operand<4> xo, oo;
         xo.set(x);
         oo.set(out);
         // (operands read ahead as in the forward's chain do not fit the registers here)
@@ -325,12 +325,12 @@ __device__ __forceinline__ void split8(const Eight<Scalar> &x, float scale, u32x
 // LDS of inputs_back_kernel, in halves: K and Q by element, then 64 columns of
 // dO, X and E by token; where the products of these are done with, the token by
 // token matrices of the second stage take their place.
-template<int DT, int PIECES, bool LO>
+template<int DT, int PIECES>
 struct BackLds {
     static constexpr int kSlab = 64, kPitch = kSlab + 8, kPart = kDeltaChunk * kPitch;
     static constexpr int kCols = 16 * DT * (kDeltaChunk + 8);  // of K or Q, a part
     static constexpr int kKeys = 2 * PIECES * kCols;
-    static constexpr int kParts = PIECES + 4, kSquares = 3 * (LO ? 2 : 1);
+    static constexpr int kParts = PIECES + 4, kSquares = 3 * 2;
     static constexpr int kBytes = 2 * (kKeys + kPart * (kParts > kSquares ? kParts : kSquares));
 };
 
@@ -343,11 +343,11 @@ struct BackLds {
 // loads hide behind another's products (bf16, 4 rows of 2048 tokens, 8 heads of
 // 128 x 128: a training step takes 360 us, 385 with 4), or 4 of twice the registers
 // where 8 spill (fp32, 3001 tokens, 6 heads of 72 x 96: 58 us, 116 with 8).
-template<typename Scalar, int DT, int PIECES, bool LO, bool WIDE, int WAVES>
+template<typename Scalar, int DT, int PIECES, bool WIDE, int WAVES>
 __global__ __launch_bounds__(kWave *WAVES, WAVES / 4) void inputs_back_kernel(const DeltaJob job, const DeltaWork work,
                                                           const DeltaGrads grads) {
     extern __shared__ __align__(16) float lds_base[];
-    using Lds = BackLds<DT, PIECES, LO>;
+    using Lds = BackLds<DT, PIECES>;
     constexpr int C = kDeltaChunk, kPitchT = C + 8, kThreads = kWave * WAVES;
     constexpr int TW = (DT + WAVES - 1) / WAVES, NR = (10 + WAVES - 1) / WAVES, NI = 512 / kThreads;
     uint16_t *const halves = reinterpret_cast<uint16_t *>(lds_base);
@@ -750,8 +750,7 @@ __global__ __launch_bounds__(kWave *WAVES, WAVES / 4) void inputs_back_kernel(co
             const _Float16 hi = static_cast<_Float16>(v * scale);
             uint16_t *to = parts + matrix * Lds::kPart + i * Lds::kPitch + j;
             *to = __builtin_bit_cast(uint16_t, hi);
-            if constexpr (LO)
-                to[3 * Lds::kPart] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(fmaf(v, scale, -static_cast<float>(hi))));
+            to[3 * Lds::kPart] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(fmaf(v, scale, -static_cast<float>(hi))));
         };
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
@@ -808,8 +807,7 @@ __global__ __launch_bounds__(kWave *WAVES, WAVES / 4) void inputs_back_kernel(co
                     auto product = [&](int matrix, const u32x4 (&f)[PIECES][2], f32x4 acc) {
                         const u32x4 hi = square(matrix, m, b);
                         acc = mfma16(hi, f[0][b], acc);
-                        if constexpr (LO)
-                            acc = mfma16(square(matrix + 3, m, b), f[0][b], acc);
+                        acc = mfma16(square(matrix + 3, m, b), f[0][b], acc);
                         if constexpr (PIECES == 2)
                             acc = mfma16(hi, f[PIECES - 1][b], acc);
                         return acc;
@@ -842,7 +840,7 @@ __global__ __launch_bounds__(kWave *WAVES, WAVES / 4) void inputs_back_kernel(co
 // Whether a chunk's operands and the gradients' products fit the LDS.
 template<int DT, int PIECES>
 constexpr bool delta_trains = ChunkLds<DT, PIECES, true>::kBytes <= kLdsBytes &&
-                              BackLds<DT, PIECES, true>::kBytes + 12288 <= kLdsBytes;
+                              BackLds<DT, PIECES>::kBytes + 12288 <= kLdsBytes;
 static_assert(delta_trains<16, 1> && delta_trains<10, 2> && !delta_trains<16, 2>);  // as delta_kept has it
 
 template<typename Scalar>
@@ -858,7 +856,6 @@ hipError_t backward_typed(const DeltaJob &job, const DeltaWork &work, const Delt
     const dim3 part_grid(static_cast<unsigned>(lines * (work.parts - 1) * groups));
     const dim3 grid(static_cast<unsigned>(lines * work.parts * groups));
     constexpr int PIECES = sizeof(Scalar) == 4 ? 2 : 1;
-    constexpr bool LO = !__is_same(Scalar, bf16_t);
     constexpr int V = 16 / static_cast<int>(sizeof(Scalar));
     const bool pieces = rows_whole<Scalar>(job) && job.Dv % V == 0 && reinterpret_cast<uintptr_t>(grads.d_o) % 16 == 0 &&
                         (grads.d_o_at[0] | grads.d_o_at[1] | grads.d_o_at[2]) % V == 0;
@@ -866,7 +863,7 @@ hipError_t backward_typed(const DeltaJob &job, const DeltaWork &work, const Delt
     if constexpr (delta_trains<DT, PIECES>) {                                                                                   \
         if (wide == 16 * DT) {                                                                                                  \
             constexpr int each = ChunkLds<DT, PIECES, true>::kBytes, bufs = 2 * each <= kLdsBytes ? 2 : 1;                      \
-            constexpr int back = BackLds<DT, PIECES, LO>::kBytes;                                                               \
+            constexpr int back = BackLds<DT, PIECES>::kBytes;                                                                   \
             if (work.parts > 1) {                                                                                               \
                 hipLaunchKernelGGL((chain_back_kernel<Scalar, DT, PIECES, bufs, true>), part_grid, dim3(512), bufs * each,      \
                                    stream, job, work, grads, groups);                                                           \
@@ -880,10 +877,10 @@ hipError_t backward_typed(const DeltaJob &job, const DeltaWork &work, const Delt
             constexpr int waves = DT == 2 || (DT <= 8 && PIECES == 1) ? 8 : 4;                                                  \
             const dim3 in_grid(work.chunks, job.Hk), in_block(kWave * waves);                                                   \
             if (pieces)                                                                                                         \
-                hipLaunchKernelGGL((inputs_back_kernel<Scalar, DT, PIECES, LO, true, waves>), in_grid, in_block, back, stream,  \
+                hipLaunchKernelGGL((inputs_back_kernel<Scalar, DT, PIECES, true, waves>), in_grid, in_block, back, stream,      \
                                    job, work, grads);                                                                           \
             else                                                                                                                \
-                hipLaunchKernelGGL((inputs_back_kernel<Scalar, DT, PIECES, LO, false, waves>), in_grid, in_block, back, stream, \
+                hipLaunchKernelGGL((inputs_back_kernel<Scalar, DT, PIECES, false, waves>), in_grid, in_block, back, stream,     \
                                    job, work, grads);                                                                           \
         }                                                                                                                       \
     }

@@ -231,10 +231,7 @@ __global__ __launch_bounds__(256, 4) void prepare_kernel(const DeltaJob job, con
     __syncthreads();
 
     // P (backward: its transpose) as fp16 parts, then as operands to memory. One
-    // scale for all of it: a part is exact to 2^-39 of the largest. (What the chains
-    // do not read is not written: bf16 outputs take the first part.)
-    constexpr bool kBf16 = __is_same(Scalar, bf16_t);
-    const bool both = !kBf16 || backward;
+    // scale for all of it: both parts are exact to 2^-39 of the largest.
     float p_inverse;
     const float scale_p = scale_of(fmaxf(fmaxf(p_max[0], p_max[1]), fmaxf(p_max[2], p_max[3])), p_inverse);
 #pragma unroll
@@ -248,13 +245,11 @@ __global__ __launch_bounds__(256, 4) void prepare_kernel(const DeltaJob job, con
             const _Float16 hi = static_cast<_Float16>(p[tj][r] * scale_p);
             uint16_t *to = ph + (backward ? j * kPitchH + operand_at(i) : i * kPitchH + operand_at(j));
             *to = __builtin_bit_cast(uint16_t, hi);
-            if (both)
-                to[kHalf] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(fmaf(p[tj][r], scale_p,
-                                                                                  -static_cast<float>(hi))));
+            to[kHalf] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(fmaf(p[tj][r], scale_p, -static_cast<float>(hi))));
         }
     }
     __syncthreads();
-    for (int i = wave; i < (both ? 2 : 1) * kFrags; i += 4) {
+    for (int i = wave; i < 2 * kFrags; i += 4) {
         const int part = i >= kFrags, f = i - part * kFrags;
         int tile, block;
         frag_place(f, backward, tile, block);
@@ -388,10 +383,8 @@ __global__ __launch_bounds__(256, 4) void prepare_kernel(const DeltaJob job, con
 // rows of 4096 tokens, 16 heads of 128 x 128 in bf16, take 248 us at 3.1 TB/s, the
 // matrix units 23% and the LDS 33% busy.
 //
-// DT: Dk in tiles of 16; PIECES: fp16 parts of q and k; LO: whether products
-// that go to o alone take the second parts too (bf16 outputs do not show them:
-// their rounding is 2^-9, what is left out 2^-12).
-template<typename Scalar, int DT, int PIECES, bool LO, int BUFS, bool MAP>
+// DT: Dk in tiles of 16; PIECES: fp16 parts of q and k.
+template<typename Scalar, int DT, int PIECES, int BUFS, bool MAP>
 __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const DeltaWork work, int groups) {
     extern __shared__ __align__(16) float lds_base[];
     using Lds = ChunkLds<DT, PIECES, false>;
@@ -500,7 +493,7 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
         v_cols.template each<4>([&](int m, int r, int at) { v_bits[4 * m + r] = buffer_bits<Scalar>(from, at); });
     };
     // the next chunk's operands are asked for as soon as this one's have been used
-    u32x4 y_hi[kFrags], y_lo[kFrags], p_hi[kFrags], p_lo[LO ? kFrags : 1];
+    u32x4 y_hi[kFrags], y_lo[kFrags], p_hi[kFrags];
     auto load_y = [&](int i) {
         const int64_t record = static_cast<int64_t>(first + i) * job.Hv + head;
         const u32x4 *yf = reinterpret_cast<const u32x4 *>(work.y + record * 2 * kFragWords);
@@ -508,24 +501,19 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
         for (int f = 0; f < kFrags; ++f)
             y_hi[f] = yf[f * kWave + lane], y_lo[f] = yf[(kFrags + f) * kWave + lane];
     };
-    auto load_p = [&](int i) {
+    auto load_p = [&](int i, int part, u32x4 (&p)[kFrags]) {
         const int64_t record = static_cast<int64_t>(first + i) * job.Hv + head;
-        const u32x4 *pf = reinterpret_cast<const u32x4 *>(work.p_frags + record * 2 * kFragWords);
+        const u32x4 *pf = reinterpret_cast<const u32x4 *>(work.p_frags + (record * 2 + part) * kFragWords);
 #pragma unroll
-        for (int f = 0; f < kFrags; ++f) {
-            p_hi[f] = pf[f * kWave + lane];
-            if constexpr (LO)
-                p_lo[f] = pf[(kFrags + f) * kWave + lane];
-        }
+        for (int f = 0; f < kFrags; ++f)
+            p[f] = pf[f * kWave + lane];
     };
     if (count > 0) {
         load_v(0);
         load_y(0);
         if constexpr (!MAP) {
-            load_p(0);
+            load_p(0, 0, p_hi);
             arrived(p_hi);
-            if constexpr (LO)
-                arrived(p_lo);
         }
         arrived(y_hi);
         arrived(y_lo);
@@ -547,7 +535,7 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
         f32x4 g[4], qo[4];
         float s_inverse;
         {
-            Operand<DT, true> so;
+            Operand<DT> so;
             so.set(s);
             s_inverse = so.inverse;
 #pragma unroll
@@ -565,13 +553,13 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
                 },
                 [&](auto step, const u32x4(&f)[4]) {
                     constexpr int at = decltype(step)::value, block = at / kEach, part = at % kEach;
-                    constexpr bool is_k = part < PIECES, first_part = part % PIECES == 0;
+                    constexpr bool is_k = part < PIECES;
 #pragma unroll
                     for (int m = 0; m < 4; ++m) {
                         f32x4 &to = is_k ? g[m] : qo[m];
                         to = mfma16(f[m], so.hi[block], to);
                     }
-                    if constexpr (first_part && (is_k || LO))
+                    if constexpr (part % PIECES == 0)
 #pragma unroll
                         for (int m = 0; m < 4; ++m) {
                             f32x4 &to = is_k ? g[m] : qo[m];
@@ -579,6 +567,12 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
                         }
                 });
         }
+        // P's second part comes now, in the registers of the first products' operands (asked
+        // for a chunk ahead like its first one it makes the loop spill: eight 4096-token
+        // prompts take 477 us a call, 368 so)
+        u32x4 p_lo[kFrags];
+        if constexpr (!MAP)
+            load_p(i, 1, p_lo);
         // what the state gives o, and v - S^T k but for the chunk's own tokens
         f32x4 e[4];
         float e_inverse;
@@ -593,12 +587,12 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
         const int then = min(i + 1, count - 1);  // (the last chunk's once more rather than a branch)
         load_v(then);
         {
-            Operand<4, true> ro;
+            Operand<4> ro;
             ro.set(g);
 #pragma unroll
             for (int m = 0; m < 4; ++m)
                 e[m] = zero;
-            triangle<false, true, true>(y_hi, y_lo, ro.hi, ro.lo, e);
+            triangle<false>(y_hi, y_lo, ro.hi, ro.lo, e);
             e_inverse = vec[kVecInvY * C] * ro.inverse;
             load_y(then);
         }
@@ -608,25 +602,25 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
             kept.each<4>([&](int m, int r, int at) { buffer_store<float>(e[m][r] * e_inverse, to, at); });
         }
         if constexpr (!MAP) {
-            Operand<4, LO> eo;
+            Operand<4> eo;
             eo.set(e);
             f32x4 x[4];
 #pragma unroll
             for (int m = 0; m < 4; ++m)
                 x[m] = zero;
-            triangle<false, LO, LO>(p_hi, p_lo, eo.hi, eo.lo, x);
+            triangle<false>(p_hi, p_lo, eo.hi, eo.lo, x);
             const float x_inverse = vec[kVecInvP * C] * eo.inverse * e_inverse;
 #pragma unroll
             for (int m = 0; m < 4; ++m)
                 qo[m] = qo[m] + x[m] * x_inverse;
-            load_p(then);  // (before the stores: what waits for it does not wait for them)
+            load_p(then, 0, p_hi);  // (before the stores: what waits for it does not wait for them)
             const auto to = o_cols.rows(o + static_cast<int64_t>(i) * C * o_step, min(C, span.len - i * C));
             o_cols.template each<4>([&](int m, int r, int at) { buffer_store<Scalar>(qo[m][r], to, at); });
         }
 #pragma unroll
         for (int m = 0; m < 4; ++m)
             e[m] = e[m] * load4(vec + kVecLeftK * C + 16 * m + 4 * grp);
-        Operand<4, true> wo;
+        Operand<4> wo;
         wo.set(e);
         wo.inverse *= e_inverse;
         // steps: a part of two tiles of S, the update of the two before beside it
@@ -782,7 +776,6 @@ constexpr bool kChainFits = ChunkLds<DT, sizeof(Scalar) == 4 ? 2 : 1, false>::kB
 template<typename Scalar, int DT>
 hipError_t chain_launch(const DeltaJob &job, const DeltaWork &work, hipStream_t stream, const char **why) {
     constexpr int PIECES = sizeof(Scalar) == 4 ? 2 : 1;
-    constexpr bool LO = !__is_same(Scalar, bf16_t);
     constexpr int bytes = ChunkLds<DT, PIECES, false>::kBytes;
     constexpr int BUFS = 2 * bytes <= kLdsBytes ? 2 : 1;  // (128 x 128 in bf16, eight 4096-token prompts: 345 us, 419)
     const int tiles = (job.Dv + 15) / 16, groups = (tiles + 3) / 4, map_groups = (tiles + DT + 3) / 4;
@@ -793,14 +786,14 @@ hipError_t chain_launch(const DeltaJob &job, const DeltaWork &work, hipStream_t 
     }
     auto blocks = [&](int64_t n) { return dim3(static_cast<unsigned>(n)); };
     if (work.parts > 1) {
-        hipLaunchKernelGGL((chain_kernel<Scalar, DT, PIECES, LO, BUFS, true>), blocks(lines * (work.parts - 1) * map_groups),
+        hipLaunchKernelGGL((chain_kernel<Scalar, DT, PIECES, BUFS, true>), blocks(lines * (work.parts - 1) * map_groups),
                            dim3(512), BUFS * bytes, stream, job, work, map_groups);
         if (const hipError_t err = hipGetLastError())
             return err;
         if (const hipError_t err = launch_delta_join(job, work, false, stream))
             return err;
     }
-    hipLaunchKernelGGL((chain_kernel<Scalar, DT, PIECES, LO, BUFS, false>), blocks(lines * work.parts * groups), dim3(512),
+    hipLaunchKernelGGL((chain_kernel<Scalar, DT, PIECES, BUFS, false>), blocks(lines * work.parts * groups), dim3(512),
                        BUFS * bytes, stream, job, work, groups);
     return hipGetLastError();
 }

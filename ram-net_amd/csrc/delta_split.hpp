@@ -58,9 +58,9 @@ __device__ __forceinline__ void split2(float a, float b, float scale, uint32_t &
 // in the order a result tile holds them: position 8 g + j of a block is row
 // 4 g + j of its first tile for j < 4, of its second one else; A operands are
 // laid out to match.
-template<int N, bool LO>
+template<int N>
 struct Operand {
-    u32x4 hi[N / 2], lo[LO ? N / 2 : 1];
+    u32x4 hi[N / 2], lo[N / 2];
     float inverse;  // of the column's scale
 
     __device__ __forceinline__ void set(const f32x4 (&x)[N]) {
@@ -76,13 +76,9 @@ struct Operand {
 #pragma unroll
             for (int r = 0; r < 4; r += 2) {
                 const int w = t % 2 * 2 + r / 2;
-                if constexpr (LO) {
-                    uint32_t h, l;
-                    split2(x[t][r], x[t][r + 1], scale, h, l);
-                    hi[t / 2][w] = h, lo[t / 2][w] = l;
-                } else {
-                    hi[t / 2][w] = scaled_f16(x[t][r], x[t][r + 1], scale);
-                }
+                uint32_t h, l;
+                split2(x[t][r], x[t][r + 1], scale, h, l);
+                hi[t / 2][w] = h, lo[t / 2][w] = l;
             }
     }
 };
@@ -350,14 +346,15 @@ __device__ __forceinline__ void pipelined(Read read, Use use) {
 }
 
 // A lower (forward) or upper triangular 64 x 64 of fragments times an operand:
-// e += hi hi + hi lo + lo hi, the four row tiles' sums in turn.
-template<bool UPPER, bool LO, bool LO_B>
-__device__ __forceinline__ void triangle(const u32x4 (&hi)[kFrags], const u32x4 *lo, const u32x4 (&b_hi)[2],
-                                         const u32x4 *b_lo, f32x4 (&e)[4]) {
+// e += hi hi + hi lo + lo hi, the four row tiles' sums in turn. LO_B: whether the
+// operand has a second part.
+template<bool UPPER, bool LO_B = true>
+__device__ __forceinline__ void triangle(const u32x4 (&hi)[kFrags], const u32x4 (&lo)[kFrags], const u32x4 (&b_hi)[2],
+                                         const u32x4 (&b_lo)[2], f32x4 (&e)[4]) {
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int kind = 0; kind < 3; ++kind)
 #pragma unroll
-        for (int kind = 0; kind < 3; ++kind)
+        for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
                 if (UPPER ? b < m / 2 : b > m / 2)
@@ -367,7 +364,7 @@ __device__ __forceinline__ void triangle(const u32x4 (&hi)[kFrags], const u32x4 
                     e[m] = mfma16(hi[f], b_hi[b], e[m]);
                 else if (kind == 1 && LO_B)
                     e[m] = mfma16(hi[f], b_lo[b], e[m]);
-                else if (kind == 2 && LO)
+                else if (kind == 2)
                     e[m] = mfma16(lo[f], b_hi[b], e[m]);
             }
 }
