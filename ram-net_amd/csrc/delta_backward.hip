@@ -139,7 +139,7 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
         const int64_t record = static_cast<int64_t>(first + i) * job.Hv + head;
         const Lds lds = buffer(i);
         const float *vec = lds.vec();
-        const float total = vec[kVecGrowK * C + C - 1] * vec[kVecSk * C + C - 1];  // (a power of two: e^gamma_C)
+        const float total = vec[kVecTotal * C];
         if constexpr (!PART) {
             const auto to = kept.rows(work.dstate + record * job.Dk * delta_row(job.Dv), job.Dk);
             kept.each<DT>([&](int t, int r, int at) { buffer_store<float>(s[t][r], to, at); });
@@ -161,7 +161,7 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
                 x[m] = zero;
             // (dO's second part is 0 for bf16 but far below a column's largest)
             triangle<true, !__is_same(Scalar, bf16_t)>(p_hi, p_lo, oo.hi, oo.lo, x);
-            x_inverse = vec[kVecInvP * C] * oo.inverse;
+            x_inverse = vec[kVecInv * C + 1] * oo.inverse;
             load_frags(work.p_frags, then, p_hi, p_lo);
         }
         {
@@ -192,7 +192,7 @@ __global__ __launch_bounds__(512, 2) void chain_back_kernel(const DeltaJob job, 
             for (int m = 0; m < 4; ++m)
                 x[m] = zero;
             triangle<true>(y_hi, y_lo, uo.hi, uo.lo, x);
-            x_inverse = vec[kVecInvY * C] * uo.inverse;
+            x_inverse = vec[kVecInv * C] * uo.inverse;
 #pragma unroll
             for (int m = 0; m < 4; ++m)
                 x[m] = x[m] * x_inverse;

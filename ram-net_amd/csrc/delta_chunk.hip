@@ -342,8 +342,8 @@ __global__ __launch_bounds__(256, 4) void prepare_kernel(const DeltaJob job, con
             vec[kVecGrowQ * C + lane] = job.scale * grow / sq;
             vec[kVecLeftK * C + lane] = (backward ? left : left * b) / sk;
             vec[kVecBeta * C + lane] = b;
-            vec[kVecInvY * C + lane] = y_inverse;
-            vec[kVecInvP * C + lane] = p_inverse;
+            vec[kVecTotal * C + lane] = decay_of(gam[C - 1]);
+            vec[kVecInv * C + lane] = lane == 0 ? y_inverse : p_inverse;
         }
     }
     for (int f = wave; f < kFrags; f += 4) {
@@ -526,7 +526,7 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
         const int64_t record = static_cast<int64_t>(first + i) * job.Hv + head;
         const Lds lds = buffer(i);
         const float *vec = lds.vec();
-        const float total = vec[kVecGrowK * C + C - 1] * vec[kVecSk * C + C - 1];  // (a power of two: e^gamma_C)
+        const float total = vec[kVecTotal * C];
         if (!MAP && work.states) {
             const auto to = kept.rows(work.states + record * job.Dk * delta_row(job.Dv), job.Dk);
             kept.each<DT>([&](int t, int r, int at) { buffer_store<float>(s[t][r], to, at); });
@@ -593,7 +593,7 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
             for (int m = 0; m < 4; ++m)
                 e[m] = zero;
             triangle<false>(y_hi, y_lo, ro.hi, ro.lo, e);
-            e_inverse = vec[kVecInvY * C] * ro.inverse;
+            e_inverse = vec[kVecInv * C] * ro.inverse;
             load_y(then);
         }
         // (e without its scale, which is taken into those of the operands made of it)
@@ -609,7 +609,7 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
             for (int m = 0; m < 4; ++m)
                 x[m] = zero;
             triangle<false>(p_hi, p_lo, eo.hi, eo.lo, x);
-            const float x_inverse = vec[kVecInvP * C] * eo.inverse * e_inverse;
+            const float x_inverse = vec[kVecInv * C + 1] * eo.inverse * e_inverse;
 #pragma unroll
             for (int m = 0; m < 4; ++m)
                 qo[m] = qo[m] + x[m] * x_inverse;

@@ -162,9 +162,11 @@ enum : int {
     kVecGrowQ,   // scale e^gamma / sq
     kVecLeftK,   // e^(gamma_C - gamma) / sk (forward: times beta)
     kVecBeta,
-    kVecInvY, kVecInvP,
+    kVecTotal,   // e^gamma_C (GrowK of token 63 times its sk is not: a key of zeros has sk = 2^126)
+    kVecInv,     // 1 / sy and then 1 / sp
     kVecs
 };
+static_assert(kVecs * kDeltaChunk == 512);  // two for each of a group's 256 threads (Stager)
 enum : int { kFrags = 6, kFragWords = kFrags * kWave * 4 };  // operands of 16 x 32 of a triangular 64 x 64
 
 // The row tile and block of 32 of fragment f.
