@@ -77,8 +77,10 @@ def gated_delta_rule(
             raise ValueError("`inplace` has no gradients.")
         if eager:
             _delta._require_state("gated_delta_rule", init_state)
-            return _delta._forward("gated_delta_rule", q, k, v, g, beta, init_state, cu_seqlens, lengths, scale,
-                                   init_state)[:2]
+            out = _delta._forward("gated_delta_rule", q, k, v, g, beta, init_state, cu_seqlens, lengths, scale,
+                                  init_state)[:2]
+            torch.autograd.graph.increment_version(init_state)  # (as the dispatcher does)
+            return out
         return _delta.gated_delta_rule_(q, k, v, g, beta, init_state, cu_seqlens, lengths, scale), init_state
     if grad:
         run = _delta.Trained.apply if eager else _delta.gated_delta_rule_kept
