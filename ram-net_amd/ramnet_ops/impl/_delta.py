@@ -22,14 +22,16 @@ _FLOATS = tuple(nat.DTYPE_CODES)
 
 
 _peek, _modes = torch._C._functorch.peek_interpreter_stack, torch._C._len_torch_dispatch_stack
+_jit_trace = torch._C._get_tracing_state
 _PLAIN = {Tensor, torch.nn.Parameter, type(None)}
 
 
 def is_eager(*tensors: Tensor | None) -> bool:
     """Whether a call on these tensors loses nothing beside the dispatcher: no
-    tracing, mode, transform, forward-mode level or tensor subclass."""
-    return (not torch.compiler.is_compiling() and _peek() is None and _modes() == 0 and forward_ad._current_level < 0
-            and _PLAIN.issuperset(map(type, tensors)))
+    tracing (by torch.compile or torch.jit.trace), mode, transform, forward-mode
+    level or tensor subclass."""
+    return (not torch.compiler.is_compiling() and _jit_trace() is None and _peek() is None and _modes() == 0
+            and forward_ad._current_level < 0 and _PLAIN.issuperset(map(type, tensors)))
 
 
 def wants_grad(*tensors: Tensor | None) -> bool:
