@@ -23,15 +23,21 @@ _FLOATS = tuple(nat.DTYPE_CODES)
 
 _peek, _modes = torch._C._functorch.peek_interpreter_stack, torch._C._len_torch_dispatch_stack
 _jit_trace = torch._C._get_tracing_state
-_PLAIN = {Tensor, torch.nn.Parameter, type(None)}
+_PLAIN = {Tensor, torch.nn.Parameter}
 
 
 def is_eager(*tensors: Tensor | None) -> bool:
     """Whether a call on these tensors loses nothing beside the dispatcher: no
     tracing (by torch.compile or torch.jit.trace), mode, transform, forward-mode
-    level or tensor subclass."""
-    return (not torch.compiler.is_compiling() and _jit_trace() is None and _peek() is None and _modes() == 0
-            and forward_ad._current_level < 0 and _PLAIN.issuperset(map(type, tensors)))
+    level, tensor subclass or view whose memory holds the negated values (the
+    imaginary part of a conjugated tensor)."""
+    if (torch.compiler.is_compiling() or _jit_trace() is not None or _peek() is not None or _modes()
+            or forward_ad._current_level >= 0):
+        return False
+    for t in tensors:
+        if t is not None and (type(t) not in _PLAIN or t.is_neg()):
+            return False
+    return True
 
 
 def wants_grad(*tensors: Tensor | None) -> bool:
@@ -249,9 +255,9 @@ def _gradients(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, cu_seql
     plan, q, k, v = _plan(op, q, k, v, g, beta, None, cu_seqlens, lengths)
     B, T, N, Hk, Hv, Dk, Dv = plan.sizes
     _check_shapes(op, d_o=(d_o, (B, T, Hv, Dv)), d_state=(d_state, plan.state_shape))
-    d_o = _rows(d_o.to(q.dtype))
+    d_o = _rows(d_o.resolve_neg().to(q.dtype))
     if d_state is not None:
-        d_state = d_state.to(torch.float32).contiguous()
+        d_state = d_state.resolve_neg().to(torch.float32).contiguous()
     grads = [torch.empty(t.shape, dtype=t.dtype, device=q.device) for t in (q, k, v, g, beta)]
     dinit = q.new_empty(plan.state_shape, dtype=torch.float32)
     n = _bytes(op, plan.workspace[2], plan.sizes)
