@@ -1140,6 +1140,8 @@ int ramnet_readout_stepwise(const void *y, const void *gate, const void *weight,
 // tokens is then a range of addresses.
 constexpr int64_t kDeltaRow = 1LL << 22;
 
+static int64_t dtype_bytes(int dtype) { return dtype == RAMNET_F32 ? 4 : 2; }
+
 static int check_delta_rows(const char *name, int64_t T, int64_t step, int64_t width) {
     RAMNET_REQUIRE(T <= 1 || (step >= width && step < kDeltaRow),
                    std::string("delta rule: tokens of ") + name + " must lie one row to 2**22 elements apart");
@@ -1232,11 +1234,14 @@ int ramnet_delta_rule_forward(const ramnet_delta_rule_call *call, void *stream) 
     ramnet::DeltaJob job{};
     if (int rc = delta_job(job, *call))
         return rc;
-    if (job.N == 0)
-        return RAMNET_OK;
-    RAMNET_REQUIRE(job.state && (job.T == 0 || job.o), "null tensor pointer");
     const char *why = nullptr;
     const hipStream_t on = static_cast<hipStream_t>(stream);
+    if (job.N == 0) {  // (tokens of no sequence, where there are any)
+        const int64_t values = static_cast<int64_t>(job.B) * job.T * job.Hv * job.Dv;
+        RAMNET_REQUIRE(values == 0 || job.o, "null tensor pointer");
+        return finish(ramnet::launch_delta_zero(job.o, values * dtype_bytes(job.dtype), on), why, "delta rule launch");
+    }
+    RAMNET_REQUIRE(job.state && (job.T == 0 || job.o), "null tensor pointer");
     if (job.T == 0 || (!call->kept && ramnet::delta_is_recurrent(job)))
         return finish(ramnet::launch_delta_recurrent(job, on, &why), why, "delta rule launch");
     ramnet::DeltaWork work{};
@@ -1256,8 +1261,20 @@ int ramnet_delta_rule_backward(const ramnet_delta_rule_call *call, const void *d
     if (int rc = delta_job(job, *call))
         return rc;
     RAMNET_REQUIRE(job.T > 0, "delta rule: a backward call needs tokens");
-    if (job.N == 0)
-        return RAMNET_OK;
+    const char *why = nullptr;
+    const hipStream_t on = static_cast<hipStream_t>(stream);
+    if (job.N == 0) {
+        const int64_t tokens = static_cast<int64_t>(job.B) * job.T, keys = tokens * job.Hk * job.Dk, heads = tokens * job.Hv;
+        RAMNET_REQUIRE(tokens == 0 || (dq && dk && dv && dg && dbeta), "null tensor pointer");
+        const int64_t size = dtype_bytes(job.dtype);
+        void *const to[5] = {dq, dk, dv, dg, dbeta};
+        const int64_t bytes[5] = {keys * size, keys * size, heads * job.Dv * size, heads * dtype_bytes(job.g_dtype),
+                                  heads * dtype_bytes(job.beta_dtype)};
+        hipError_t err = hipSuccess;
+        for (int i = 0; i < 5 && err == hipSuccess; ++i)
+            err = ramnet::launch_delta_zero(to[i], bytes[i], on);
+        return finish(err, why, "delta rule backward launch");
+    }
     RAMNET_REQUIRE(d_o && d_o_strides && dq && dk && dv && dg && dbeta && call->kept, "null tensor pointer");
     RAMNET_REQUIRE(!dinit || dinit != d_state, "delta rule: dinit must not be d_state");
     ramnet::DeltaWork work{};
@@ -1267,8 +1284,6 @@ int ramnet_delta_rule_backward(const ramnet_delta_rule_call *call, const void *d
                              {d_o_strides[0], job.T == 1 ? job.Dv : d_o_strides[1], d_o_strides[2]}};
     if (int rc = check_delta_rows("d_o", job.T, grads.d_o_at[1], job.Dv))
         return rc;
-    const char *why = nullptr;
-    const hipStream_t on = static_cast<hipStream_t>(stream);
     hipError_t err = ramnet::launch_delta_prepare(job, work, true, on, &why);
     if (err == hipSuccess)
         err = ramnet::launch_delta_backward(job, work, grads, on, &why);

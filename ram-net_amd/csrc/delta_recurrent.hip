@@ -209,6 +209,12 @@ __global__ __launch_bounds__(kThreads) void recurrent_kernel(const DeltaJob job,
     }
 }
 
+__global__ __launch_bounds__(kThreads) void zero_kernel(uint16_t *p, int64_t count) {
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < count; i += step)
+        p[i] = 0;
+}
+
 template<typename Scalar>
 hipError_t launch_typed(const DeltaJob &job, hipStream_t stream, const char **why) {
     const int slices = (job.Dv + kSlice - 1) / kSlice;
@@ -236,6 +242,15 @@ hipError_t launch_typed(const DeltaJob &job, hipStream_t stream, const char **wh
 }
 
 }  // namespace
+
+hipError_t launch_delta_zero(void *p, int64_t bytes, hipStream_t stream) {
+    if (bytes > 0) {
+        const int64_t count = bytes / 2, blocks = (count + kThreads - 1) / kThreads;
+        hipLaunchKernelGGL(zero_kernel, dim3(static_cast<unsigned>(blocks < 1024 ? blocks : 1024)), dim3(kThreads), 0, stream,
+                           static_cast<uint16_t *>(p), count);
+    }
+    return hipGetLastError();
+}
 
 hipError_t launch_delta_recurrent(const DeltaJob &job, hipStream_t stream, const char **why) {
     switch (job.dtype) {

@@ -324,6 +324,8 @@ hipError_t launch_segment_backward(const SegmentBwdJob &job, hipStream_t stream,
 // `base`, or sizes them (null base); kept: what a training forward leaves for
 // its backward (a second region, delta_kept).
 hipError_t launch_delta_recurrent(const DeltaJob &job, hipStream_t stream, const char **why);
+// Zeros, for tokens where there are no sequences at all (an even number of bytes).
+hipError_t launch_delta_zero(void *p, int64_t bytes, hipStream_t stream);
 int64_t delta_layout(const DeltaJob &job, bool packed, bool backward, char *base, DeltaWork *work);
 int64_t delta_kept(const DeltaJob &job, bool packed, char *base, DeltaWork *work);
 // Whether a call without gradients walks its tokens.
