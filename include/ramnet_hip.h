@@ -486,7 +486,7 @@ int ramnet_segment_call_form(int64_t B, int64_t H, int64_t T, int64_t A, int64_t
  *                   (ramnet_delta_rule_kept_bytes), or NULL
  *   workspace       ramnet_delta_rule_workspace_bytes, kind 0, or 1 with `kept`
  * Sums, states and norms are fp32, decays' sums within a chunk fp64.
- * Requires Dk <= 256, Hv a multiple of Hk.
+ * Requires Dk <= 256, Hv a multiple of Hk, Hv Dv < 2**22.
  */
 typedef struct ramnet_delta_rule_call {
     const void *q, *k, *v, *g, *beta;
@@ -511,7 +511,8 @@ int ramnet_delta_rule_forward(const ramnet_delta_rule_call *call, void *stream);
  * Dv) fp32 (or NULL; not d_state). `call` is the forward's, with a workspace of
  * kind 2; its init_state, state and o are not read. Value heads that share a key head add
  * to its gradient in one order: results do not change from call to call.
- * float32 inputs take Dk up to 160 here.
+ * float32 inputs take Dk up to 160 here; Hk Dk is below 2**22, and Dk Dv (Dk at
+ * the next of 32, 64, 96, 128, 160, 256, Dv at a multiple of 8) at most 2**28.
  */
 int ramnet_delta_rule_backward(const ramnet_delta_rule_call *call, const void *d_o, const int64_t *d_o_strides,
                                const float *d_state, void *dq, void *dk, void *dv, void *dg, void *dbeta, float *dinit,

@@ -1174,6 +1174,8 @@ int64_t ramnet_delta_rule_workspace_bytes(int64_t B, int64_t T, int64_t N, int64
     job.dtype = dtype;
     if (kind == 0 && ramnet::delta_is_recurrent(job))
         return 0;
+    if (kind > 0 && !ramnet::delta_trains(job))
+        return -1;
     return ramnet::delta_layout(job, packed != 0, kind == 2, nullptr, &work);
 }
 
@@ -1220,7 +1222,8 @@ static int delta_regions(const ramnet::DeltaJob &job, const ramnet_delta_rule_ca
     const bool packed = job.cu != nullptr;
     if (c.kept) {
         const int64_t need = ramnet::delta_kept(job, packed, static_cast<char *>(c.kept), &work);
-        RAMNET_REQUIRE(need >= 0, "delta rule: gradients of float32 take Dk up to 160");
+        RAMNET_REQUIRE(need >= 0, "delta rule: gradients take Dk up to 160 in float32, Hk Dk below 2**22, and Dk Dv "
+                                  "(Dk padded) up to 2**28");
         RAMNET_REQUIRE(c.kept_bytes >= need, "delta rule: kept region too small");
     }
     RAMNET_REQUIRE(c.workspace && c.workspace_bytes >= ramnet::delta_layout(job, packed, backward,

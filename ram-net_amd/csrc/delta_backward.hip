@@ -839,9 +839,9 @@ __global__ __launch_bounds__(kWave *WAVES, WAVES / 4) void inputs_back_kernel(co
 
 // Whether a chunk's operands and the gradients' products fit the LDS.
 template<int DT, int PIECES>
-constexpr bool delta_trains = ChunkLds<DT, PIECES, true>::kBytes <= kLdsBytes &&
+constexpr bool kTrains = ChunkLds<DT, PIECES, true>::kBytes <= kLdsBytes &&
                               BackLds<DT, PIECES>::kBytes + 12288 <= kLdsBytes;
-static_assert(delta_trains<16, 1> && delta_trains<10, 2> && !delta_trains<16, 2>);  // as delta_kept has it
+static_assert(kTrains<16, 1> && kTrains<10, 2> && !kTrains<16, 2>);  // as delta_trains has it
 
 template<typename Scalar>
 hipError_t backward_typed(const DeltaJob &job, const DeltaWork &work, const DeltaGrads &grads, hipStream_t stream,
@@ -860,7 +860,7 @@ hipError_t backward_typed(const DeltaJob &job, const DeltaWork &work, const Delt
     const bool pieces = rows_whole<Scalar>(job) && job.Dv % V == 0 && reinterpret_cast<uintptr_t>(grads.d_o) % 16 == 0 &&
                         (grads.d_o_at[0] | grads.d_o_at[1] | grads.d_o_at[2]) % V == 0;
 #define RAMNET_BACK(DT)                                                                                                         \
-    if constexpr (delta_trains<DT, PIECES>) {                                                                                   \
+    if constexpr (kTrains<DT, PIECES>) {                                                                                        \
         if (wide == 16 * DT) {                                                                                                  \
             constexpr int each = ChunkLds<DT, PIECES, true>::kBytes, bufs = 2 * each <= kLdsBytes ? 2 : 1;                      \
             constexpr int back = BackLds<DT, PIECES>::kBytes;                                                                   \

@@ -818,12 +818,18 @@ hipError_t chain_typed(const DeltaJob &job, const DeltaWork &work, hipStream_t s
 }  // namespace
 
 // Short calls, and those whose chunks (two fp16 parts of each fp32 key and
-// query) do not fit the LDS. A chunk costs the same however few its tokens: with
+// query) do not fit the LDS or whose matrices are out of reach. A chunk costs the same however few its tokens: with
 // 8 tokens of 128 x 128 heads in bf16, token by token and in chunks take 15.4 and
 // 19.2 us for 8 heads, 47.6 and 47.5 for 32 rows of 16 heads, 83 and 78 for 64;
 // with 16 tokens 26.5 and 19.4, 82 and 46, 153 and 77.
 bool delta_is_recurrent(const DeltaJob &job) {
-    return job.T <= 8 || (job.dtype == kF32 && delta_padded(job.Dk) > 160);
+    return job.T <= 8 || (job.dtype == kF32 && delta_padded(job.Dk) > 160) || !delta_within_reach(job);
+}
+
+bool delta_trains(const DeltaJob &job) {
+    // (64 tokens of dq and dk, too, are within reach)
+    return !(job.dtype == kF32 && delta_padded(job.Dk) > 160) && delta_within_reach(job) &&
+           static_cast<int64_t>(job.Hk) * job.Dk < kDeltaReach / (4 * kDeltaChunk);
 }
 
 namespace {
@@ -910,7 +916,7 @@ int64_t delta_layout(const DeltaJob &job, bool packed, bool backward, char *base
 }
 
 int64_t delta_kept(const DeltaJob &job, bool packed, char *base, DeltaWork *work) {
-    if (job.dtype == kF32 && delta_padded(job.Dk) > 160)
+    if (!delta_trains(job))
         return -1;
     count_chunks(job, packed, work);
     Carver carve{base};

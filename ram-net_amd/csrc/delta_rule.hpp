@@ -8,7 +8,7 @@
 
 namespace ramnet {
 
-enum : int { kDeltaMaxDk = 256, kDeltaChunk = 64 };
+enum : int { kDeltaMaxDk = 256, kDeltaChunk = 64, kDeltaReach = 1 << 30 };
 
 // Tensors of one call; strides in elements, of batch row, token and head (the
 // last dimension is dense). Value head h reads key head h / (Hv / Hk).
@@ -93,6 +93,12 @@ inline int delta_padded(int Dk) {
 
 // Length of a row of Dv values in the workspace.
 __host__ __device__ inline int delta_row(int Dv) { return (Dv + 7) / 8 * 8; }
+
+// Whether a head's matrix in the workspace, its rows padded, ends within the reach of
+// the chunked kernels' 32-bit offsets (delta_split.hpp: kNowhere lies past every window).
+inline bool delta_within_reach(const DeltaJob &job) {
+    return static_cast<int64_t>(delta_padded(job.Dk)) * delta_row(job.Dv) * 4 <= kDeltaReach;
+}
 
 // A decay of one step. e^-200 is 0 in fp32 as e^-inf is; held there, sums of
 // decays stay finite and differences of them free of inf - inf. (A NaN stays.)

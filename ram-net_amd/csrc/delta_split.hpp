@@ -99,7 +99,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t window(const void *base, int64
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, static_cast<int>(bytes), kBufWord3);
 }
 
-constexpr int kNowhere = 1 << 30;  // past every window, with any row's offset on top
+constexpr int kNowhere = kDeltaReach;  // past every window, with any row's offset on top
 
 // A wave's 16 columns of a matrix whose rows are `step` elements apart (at
 // least its width): rows 16 m + 4 (lane / 16) + r, in order of m and r.

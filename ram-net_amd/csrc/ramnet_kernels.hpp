@@ -330,6 +330,8 @@ int64_t delta_layout(const DeltaJob &job, bool packed, bool backward, char *base
 int64_t delta_kept(const DeltaJob &job, bool packed, char *base, DeltaWork *work);
 // Whether a call without gradients walks its tokens.
 bool delta_is_recurrent(const DeltaJob &job);
+// Whether the kernels take gradients of a call of these sizes.
+bool delta_trains(const DeltaJob &job);
 hipError_t launch_delta_prepare(const DeltaJob &job, const DeltaWork &work, bool backward, hipStream_t stream,
                                 const char **why);
 hipError_t launch_delta_chain(const DeltaJob &job, const DeltaWork &work, hipStream_t stream, const char **why);

@@ -114,7 +114,8 @@ def _whole(t: Tensor | None) -> Tensor | None:
 def _bytes(op: str, count: int, sizes) -> int:
     if count < 0:
         raise RuntimeError(f"{op}: sizes (B, T, N, Hk, Hv, Dk, Dv) = {tuple(sizes)} are not supported "
-                           "(Dk up to 256, up to 160 for gradients of float32; tokens within int32)")
+                           "(Dk up to 256, up to 160 for gradients of float32; Hk Dk below 2**22 and Dk Dv up to "
+                           "2**28 for gradients; tokens within int32)")
     return count
 
 
