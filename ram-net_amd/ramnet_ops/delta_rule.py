@@ -51,7 +51,7 @@ def gated_delta_rule(
     :param g: Logarithm of the decay (B, T, Hv), any float type; -inf clears the state.
     :param beta: Write strength (B, T, Hv).
     :param scale: Factor of o; default ``Dk ** -0.5``.
-    :param init_state: State before the first token (N, Hv, Dk, Dv); default zeros.
+    :param init_state: State before the first token (N, Hv, Dk, Dv), a float type of 32 bits or fewer; default zeros.
     :param cu_seqlens: (N + 1) bounds of N sequences packed one after the other in a batch of one.
     :param lengths: (B) tokens of each row that count; the others leave the state and have o = 0.
     :param inplace: Update init_state in place (contiguous float32, no gradients).
@@ -108,8 +108,8 @@ def verify_drafts(
     :param target: The target's probabilities after each of 0 .. S drafts (B, S + 1, V).
     :param draft: Probabilities the drafts were drawn from (B, S, V), in target's type; None for drafts without
         (looked up, or greedy): 1 at the drafted token.
-    :param accept: Uniform numbers in [0, 1) (B, S).
-    :param sample: Uniform numbers in [0, 1) (B).
+    :param accept: Uniform numbers in [0, 1) (B, S), any float type; used in 32 bits.
+    :param sample: Uniform numbers in [0, 1) (B), likewise.
     :param draft_lens: Drafts of each row (B); default S.
     :return: ``(tokens, taken)``: (B, S + 1) int64 -- the drafts that stay, the drawn token, then -1 -- and (B) int32.
     """

@@ -77,6 +77,8 @@ def _check(op: str, q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, in
             or beta.dtype not in _FLOATS:
         raise RuntimeError(f"{op}: q, k and v must share one of {_FLOATS}, g and beta have one of them, got "
                            f"{q.dtype}, {k.dtype}, {v.dtype}, {g.dtype} and {beta.dtype}")
+    if init_state is not None and init_state.dtype not in _FLOATS:
+        raise RuntimeError(f"{op}: init_state must be one of {_FLOATS}, got {init_state.dtype}")
     device = q.device
     for t in (q, k, v, g, beta, init_state, cu_seqlens, lengths):
         if t is not None and t.device != device:
@@ -138,7 +140,7 @@ def _plan(op: str, q, k, v, g, beta, init_state, cu_seqlens, lengths):
     """The call's plan, with q, k and v as the native calls read them."""
     key = (q.shape, k.shape, v.shape, g.shape, beta.shape, q.stride(), k.stride(), v.stride(), g.stride(),
            beta.stride(), q.dtype, k.dtype, v.dtype, g.dtype, beta.dtype, q.device, k.device, v.device, g.device,
-           beta.device, None if init_state is None else (init_state.shape, init_state.device),
+           beta.device, None if init_state is None else (init_state.shape, init_state.dtype, init_state.device),
            None if cu_seqlens is None else (cu_seqlens.shape, cu_seqlens.dtype, cu_seqlens.device),
            None if lengths is None else (lengths.shape, lengths.dtype, lengths.device))
     plan = _plans.get(key)
@@ -346,6 +348,9 @@ def _verify_plan(key, tokens, target, draft, accept, sample, draft_lens):
     if target.dtype not in _FLOATS or draft is not None and draft.dtype != target.dtype:
         raise RuntimeError(f"{op}: target and draft must share one of {_FLOATS}, got {target.dtype} and "
                            f"{None if draft is None else draft.dtype}")
+    for name, t in (("accept", accept), ("sample", sample)):
+        if not t.dtype.is_floating_point:
+            raise RuntimeError(f"{op}: {name} must be floating-point, got {t.dtype}")
     _require_gpu(op, target)
     for name, t in (("tokens", tokens), ("draft_lens", draft_lens)):
         if t is not None and t.dtype not in (torch.int32, torch.int64):
@@ -365,7 +370,7 @@ def _verify(tokens: Tensor, target: Tensor, draft: Tensor | None, accept: Tensor
     if draft is not None and draft.dim() == 3:
         draft = _dense(draft)
     key = (tokens.shape, target.shape, accept.shape, sample.shape, target.stride(), target.dtype, tokens.dtype,
-           tokens.device, target.device, accept.device, sample.device,
+           tokens.device, target.device, accept.device, sample.device, accept.dtype, sample.dtype,
            None if draft is None else (draft.shape, draft.stride(), draft.dtype, draft.device),
            None if draft_lens is None else (draft_lens.shape, draft_lens.dtype, draft_lens.device))
     plan = _verify_plans.get(key) or _verify_plan(key, tokens, target, draft, accept, sample, draft_lens)
