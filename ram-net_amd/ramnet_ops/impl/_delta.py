@@ -113,6 +113,26 @@ def _whole(t: Tensor | None) -> Tensor | None:
     return t.to(torch.int32).contiguous()
 
 
+def _kept_bytes(op: str, sizes, dtype: torch.dtype, packed: bool):
+    """Bytes of what a training forward keeps, in arithmetic that tracing leaves
+    symbolic: ramnet_delta_rule_kept_bytes, but room for the maps of the most
+    segments that rows of these sizes can be cut into."""
+    B, T, N, Hk, Hv, Dk, Dv = sizes
+    wide = next((w for w in (32, 64, 96, 128, 160, 256) if Dk <= w), 0)
+    row = (Dv + 7) // 8 * 8
+    if wide == 0 or dtype == torch.float32 and wide > 160 or wide * row > 2 ** 28 or Hk * Dk >= 2 ** 22:
+        _bytes(op, -1, sizes)
+    per_row = (T + 63) // 64
+    records = (per_row + N if packed else N * per_row) * Hv
+
+    def region(floats):
+        return (floats * 4 + 255) // 256 * 256
+    count = region(records * 64 * row) + region(records * Dk * row)
+    if N * Hv * ((Dv + 63) // 64) <= 128:
+        count += region(N * Hv * torch.sym_min(per_row // 4, 64) * wide * wide)
+    return count
+
+
 def _bytes(op: str, count: int, sizes) -> int:
     if count < 0:
         raise RuntimeError(f"{op}: sizes (B, T, N, Hk, Hv, Dk, Dv) = {tuple(sizes)} are not supported "
@@ -162,8 +182,9 @@ def _plan(op: str, q, k, v, g, beta, init_state, cu_seqlens, lengths):
 
 def _forward(op: str, q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, init_state: Tensor | None,
              cu_seqlens: Tensor | None, lengths: Tensor | None, scale: float, state: Tensor | None = None,
-             keep: bool = False) -> tuple[Tensor, Tensor, Tensor | None]:
-    """(o, state, kept). ``state``: where the state goes (init_state itself in place)."""
+             keep: bool = False, kept: Tensor | None = None) -> tuple[Tensor, Tensor, Tensor | None]:
+    """(o, state, kept). ``state``: where the state goes (init_state itself in place);
+    ``kept``: where what is kept goes."""
     plan, q, k, v = _plan(op, q, k, v, g, beta, init_state, cu_seqlens, lengths)
     if init_state is not None and init_state is not state and not (init_state.dtype == torch.float32
                                                                    and init_state.is_contiguous()):
@@ -172,10 +193,11 @@ def _forward(op: str, q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, 
         state = q.new_empty(plan.state_shape, dtype=torch.float32)
     o = q.new_empty(v.shape)
     n = _bytes(op, plan.workspace[keep], plan.sizes)
-    kept, kept_bytes = None, 0
+    kept_bytes = 0
     if keep:
-        kept_bytes = _bytes(op, plan.kept, plan.sizes)
-        kept = q.new_empty((kept_bytes,), dtype=torch.uint8)
+        if kept is None:
+            kept = q.new_empty((_bytes(op, plan.kept, plan.sizes),), dtype=torch.uint8)
+        kept_bytes = kept.numel()
     ws = q.new_empty((n,), dtype=torch.uint8) if n else None
     if plan.sizes[2] == 0:
         return o.zero_(), state, kept
@@ -233,14 +255,18 @@ def gated_delta_rule_kept(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tens
                           scale: float) -> tuple[Tensor, Tensor, Tensor]:
     """(o, state, kept): ``gated_delta_rule`` that leaves its backward the state
     before each chunk of 64 tokens and each token's v - S^T k."""
-    return _forward("gated_delta_rule_kept", q, k, v, g, beta, init_state, cu_seqlens, lengths, scale, keep=True)
+    op = "gated_delta_rule_kept"
+    sizes = _check(op, q, k, v, g, beta, init_state, cu_seqlens, lengths)
+    kept = q.new_empty((_kept_bytes(op, sizes, q.dtype, cu_seqlens is not None),), dtype=torch.uint8)
+    return _forward(op, q, k, v, g, beta, init_state, cu_seqlens, lengths, scale, keep=True, kept=kept)
 
 
 @gated_delta_rule_kept.register_fake
 def _(q, k, v, g, beta, init_state, cu_seqlens, lengths, scale):
     B, T, Hk, Dk = q.shape
     N = B if cu_seqlens is None else cu_seqlens.shape[0] - 1
-    n = nat.lib().ramnet_delta_rule_kept_bytes(B, T, N, Hk, v.shape[2], Dk, v.shape[3], _code(q), cu_seqlens is not None)
+    n = _kept_bytes("gated_delta_rule_kept", (B, T, N, Hk, v.shape[2], Dk, v.shape[3]), q.dtype,
+                    cu_seqlens is not None)
     return *_out_shapes(q, k, v, cu_seqlens), q.new_empty((n,), dtype=torch.uint8)
 
 
