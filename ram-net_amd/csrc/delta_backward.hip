@@ -367,28 +367,23 @@ __global__ __launch_bounds__(kWave *WAVES, WAVES / 4) void inputs_back_kernel(co
     Scalar *dk = static_cast<Scalar *>(grads.dk) + static_cast<int64_t>(kh) * Dk;
     // tokens of no sequence or past a row's length
     auto clear = [&](int64_t from, int64_t to) {
-        for (int64_t t = from; t < to; ++t) {
-            for (int d = tid; d < Dk; d += kThreads) {
+        for (int64_t t = from + wave; t < to; t += WAVES) {
+            for (int d = lane; d < Dk; d += kWave) {
                 store_f32(dq + t * dk_step + d, 0.f);
                 store_f32(dk + t * dk_step + d, 0.f);
             }
-            for (int h = tid; h < shared; h += kThreads) {
+            for (int h = lane; h < shared; h += kWave) {
                 store_code(grads.dg, job.g_dtype, t * job.Hv + kh * shared + h, 0.f);
                 store_code(grads.dbeta, job.beta_dtype, t * job.Hv + kh * shared + h, 0.f);
             }
             if (job.cu)
-                for (int i = tid; i < shared * Dv; i += kThreads)
+                for (int i = lane; i < shared * Dv; i += kWave)
                     store_f32(static_cast<Scalar *>(grads.dv) + (t * job.Hv + kh * shared) * Dv + i, 0.f);
         }
     };
     if (job.cu) {
         if (at.n < 0) {
-            if (chunk == work.offsets[job.N]) {
-                const int start = delta_span(job, 0).t0;
-                const DeltaSpan last = delta_span(job, job.N - 1);
-                clear(0, start);
-                clear(max(start, last.t0 + last.len), job.T);
-            }
+            delta_outside(job, work, chunk, clear);
             return;
         }
     } else if (at.len < C) {

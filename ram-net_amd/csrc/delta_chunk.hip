@@ -150,17 +150,13 @@ __global__ __launch_bounds__(256, 4) void prepare_kernel(const DeltaJob job, con
     const DeltaPlace at = delta_place(job, work, chunk);
     if (at.len == 0) {
         // a record of no sequence: the tokens that no sequence covers have output 0
-        if (at.n < 0 && chunk == work.offsets[job.N] && !backward) {
-            const int first = delta_span(job, 0).t0;
-            const DeltaSpan last = delta_span(job, job.N - 1);
+        if (at.n < 0 && !backward) {
             Scalar *o = static_cast<Scalar *>(job.o) + static_cast<int64_t>(head) * job.Dv;
-            auto clear = [&](int from, int to) {
-                for (int64_t t = from; t < to; ++t)
-                    for (int c = tid; c < job.Dv; c += 256)
+            delta_outside(job, work, chunk, [&](int from, int to) {
+                for (int64_t t = from + wave; t < to; t += 4)
+                    for (int c = lane; c < job.Dv; c += kWave)
                         store_f32(o + t * job.Hv * job.Dv + c, 0.f);
-            };
-            clear(0, first);
-            clear(max(first, last.t0 + last.len), job.T);
+            });
         }
         return;
     }
