@@ -485,7 +485,12 @@ int ramnet_segment_call_form(int64_t B, int64_t H, int64_t T, int64_t A, int64_t
  *   kept            what ramnet_delta_rule_backward takes of this call
  *                   (ramnet_delta_rule_kept_bytes), or NULL
  *   workspace       ramnet_delta_rule_workspace_bytes, kind 0, or 1 with `kept`
- * Sums, states and norms are fp32, decays' sums within a chunk fp64.
+ * Sums, states and norms are fp32, decays' sums within a chunk fp64; 16-bit outputs
+ * are rounded once. Calls of more than 8 tokens run in chunks of 64 (but float32
+ * with Dk > 160, and Dk Dv above 2**28): there a token's values are exact to 2^-24
+ * down to 2^-15 of the largest of their column in the chunk and to 2^-39 of that
+ * below, and a NaN or infinity reaches the chunk's other tokens, earlier ones too
+ * (one in v: those of its column). Token by token it reaches only those after it.
  * Requires Dk <= 256, Hv a multiple of Hk, Hv Dv < 2**22.
  */
 typedef struct ramnet_delta_rule_call {

@@ -341,7 +341,7 @@ struct BackLds {
 // memory is asked for one step ahead of its use.
 // WIDE: q, k and d_o are read in pieces of 16 bytes. WAVES: 8, so that one's
 // loads hide behind another's products (bf16, 4 rows of 2048 tokens, 8 heads of
-// 128 x 128: a training step takes 360 us, 385 with 4), or 4 of twice the registers
+// 128 x 128: 115 us of a training step's 377, 25 more with 4), or 4 of twice the registers
 // where 8 spill (fp32, 3001 tokens, 6 heads of 72 x 96: 58 us, 116 with 8).
 template<typename Scalar, int DT, int PIECES, bool WIDE, int WAVES>
 __global__ __launch_bounds__(kWave *WAVES, WAVES / 4) void inputs_back_kernel(const DeltaJob job, const DeltaWork work,

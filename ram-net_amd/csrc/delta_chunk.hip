@@ -11,7 +11,7 @@ namespace {
 
 // First chunk of each packed sequence, and the sequences by their lengths: one
 // starts its whole walk when its block does, the longest had better be first
-// (thirteen sequences of 12345 tokens: chain 214 us in their own order, 145 so).
+// (thirteen sequences of 12345 tokens: chain 125 us; in their own order half as long again).
 // More than 1024 keep their order. One block. The sum of the lengths is at
 // most T where the bounds are in order; elsewhere it is held to the records
 // there are.
@@ -133,7 +133,7 @@ __device__ __forceinline__ double running_sum(double x) {
 // Y, P, gamma and the scales of one chunk and value head: wave w has the
 // tokens of tile w. Latency from end to end, so as many blocks as fit: P's
 // operands and then Y take the place of the keys. Eight rows of 4096 tokens, 16
-// heads of 128 in bf16 (461 MB in and out): 125 us, 3.7 TB/s.
+// heads of 128 in bf16 (518 MB in and out): 127 us, 4.1 TB/s.
 template<typename Scalar, int DT>
 __global__ __launch_bounds__(256, 4) void prepare_kernel(const DeltaJob job, const DeltaWork work, bool backward) {
     constexpr int C = kDeltaChunk, NP = C + 4, wide = 16 * DT, pitch = wide + 16 / static_cast<int>(sizeof(Scalar));
@@ -376,8 +376,8 @@ __global__ __launch_bounds__(256, 4) void prepare_kernel(const DeltaJob job, con
 // proper starts each segment from there.
 //
 // What binds a chunk is the latency of products that depend on one another: eight
-// rows of 4096 tokens, 16 heads of 128 x 128 in bf16, take 248 us at 3.1 TB/s, the
-// matrix units 23% and the LDS 33% busy.
+// rows of 4096 tokens, 16 heads of 128 x 128 in bf16, take 259 us at 3.0 TB/s, the
+// matrix units 27% and the LDS 31% busy.
 //
 // DT: Dk in tiles of 16; PIECES: fp16 parts of q and k.
 template<typename Scalar, int DT, int PIECES, int BUFS, bool MAP>
@@ -420,7 +420,7 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(const DeltaJob job, const
         Stager<Scalar, DT, PIECES, false> stager;
         // the loads' latency comes first: the chain is in its products of K and Q then, which
         // the stores to LDS would be in the way of (a chunk more in registers, stored
-        // as soon as a buffer is free: 248 -> 310 us for eight 4096-token prompts)
+        // as soon as a buffer is free: a quarter longer for eight 4096-token prompts)
         auto bring = [&](auto wide) {
             auto load = [&](int i) {
                 const int64_t t0 = span.t0 + i * C;
@@ -773,7 +773,7 @@ template<typename Scalar, int DT>
 hipError_t chain_launch(const DeltaJob &job, const DeltaWork &work, hipStream_t stream, const char **why) {
     constexpr int PIECES = sizeof(Scalar) == 4 ? 2 : 1;
     constexpr int bytes = ChunkLds<DT, PIECES, false>::kBytes;
-    constexpr int BUFS = 2 * bytes <= kLdsBytes ? 2 : 1;  // (128 x 128 in bf16, eight 4096-token prompts: 345 us, 419)
+    constexpr int BUFS = 2 * bytes <= kLdsBytes ? 2 : 1;  // (128 x 128 in bf16, eight 4096-token prompts: a fifth longer with one)
     const int tiles = (job.Dv + 15) / 16, groups = (tiles + 3) / 4, map_groups = (tiles + DT + 3) / 4;
     const int64_t lines = static_cast<int64_t>(job.N) * job.Hv;
     if (lines * work.parts * map_groups > 0x7fffffff || lines * tiles > 0x7fffffff) {
@@ -814,10 +814,10 @@ hipError_t chain_typed(const DeltaJob &job, const DeltaWork &work, hipStream_t s
 }  // namespace
 
 // Short calls, and those whose chunks (two fp16 parts of each fp32 key and
-// query) do not fit the LDS or whose matrices are out of reach. A chunk costs the same however few its tokens: with
-// 8 tokens of 128 x 128 heads in bf16, token by token and in chunks take 15.4 and
-// 19.2 us for 8 heads, 47.6 and 47.5 for 32 rows of 16 heads, 83 and 78 for 64;
-// with 16 tokens 26.5 and 19.4, 82 and 46, 153 and 77.
+// query) do not fit the LDS or whose matrices are out of reach. A chunk costs the
+// same however few its tokens: with 128 x 128 heads in bf16, 8 heads, 32 rows of 16
+// heads and 64 rows of them take 20, 48 and 78 us in chunks, and token by token 15, 35
+// and 60 with 8 tokens, 17, 47 and 83 with 12, 22, 59 and 105 with 16.
 bool delta_is_recurrent(const DeltaJob &job) {
     return job.T <= 8 || (job.dtype == kF32 && delta_padded(job.Dk) > 160) || !delta_within_reach(job);
 }

@@ -8,6 +8,11 @@
 // significant bits and lie within fp16's once their token's largest is at
 // 2^14: only elements below 2^-31 of it lose digits. fp32 matrix instructions
 // run at 1/16 of the 16-bit rate, so three products are five times faster.
+//
+// A column of values or errors has one scale over a chunk's 64 tokens: a token's
+// own are exact to 2^-24 down to 2^-15 of the column's largest there, to 2^-39 of
+// that below. An infinity or a NaN reaches the chunk's other tokens, those before its
+// own among them (zeros of a triangle times it): one in v, those of its column alone.
 #pragma once
 
 #include "delta_chunk.hpp"

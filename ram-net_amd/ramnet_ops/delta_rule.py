@@ -43,7 +43,10 @@ def gated_delta_rule(
 
     Per token: ``S = exp(g) S``, ``S = S + k (beta (v - S^T k))^T``, ``o = scale S^T q``.
     Differentiable in q, k, v, g, beta and init_state. Whole prompts run in
-    chunks of 64 tokens, decode steps and short prompts token by token.
+    chunks of 64 tokens, decode steps and short prompts (up to 8 tokens) token by
+    token. In chunks, values far below the largest of their column of v within a
+    chunk (2^-15 and less) have fewer than 24 bits, and a NaN or infinity reaches
+    the tokens of its chunk before it as well as those after (one in v: its column).
 
     :param q: Queries (B, T, Hk, Dk), Dk up to 256; their last dimension dense, any other strides.
     :param k: Keys (B, T, Hk, Dk), as a rule of norm 1.
