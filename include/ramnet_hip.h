@@ -552,6 +552,129 @@ int ramnet_verify_drafts(const int64_t *tokens, const void *target, const void *
                          const float *sample, const int32_t *draft_lens, int64_t B, int64_t S, int64_t V,
                          const int64_t *strides, int64_t *out, int32_t *taken, void *stream);
 
+/*
+ * Short causal convolution of each channel over its last W tokens. No
+ * counterpart in the reference.
+ *     s[t, d] = bias[d] + sum_j weight[d, j] x[t - (W - 1) + j, d];   y = s, or silu(s)
+ * `call` holds, all in `dtype`:
+ *   x              (B, T, D), last dimension dense, strides (elements): batch row, token
+ *   weight, bias   (D, W), (D) or NULL; W from 1 to 8
+ *   init_state     (N, W - 1, D) inputs before the first token, or NULL: zeros
+ *   state          (N, W - 1, D) the last W - 1 inputs of a sequence and its
+ *                  init_state; may be init_state
+ *   y              (B, T, D), dense; 0 where a token does not count
+ *   cu_seqlens     (N + 1) int32 bounds of sequences packed in a batch of one, or
+ *                  NULL: N = B. A bound below the one before it, or outside [0, T], is
+ *                  held to these
+ *   lengths        (B) int32 tokens that count, held to [0, T], or NULL: all
+ *   workspace      ramnet_causal_conv_workspace_bytes
+ */
+typedef struct ramnet_causal_conv_call {
+    const void *x, *weight, *bias, *init_state;
+    void *state, *y;
+    const int32_t *cu_seqlens, *lengths;
+    void *workspace;
+    int64_t workspace_bytes;
+    int64_t B, T, N, D, W;
+    int64_t strides[2];
+    int64_t dtype, silu;
+} ramnet_causal_conv_call;
+
+int ramnet_causal_conv_forward(const ramnet_causal_conv_call *call, void *stream);
+
+/*
+ * Its gradients, from dy (B, T, D), strides dy_strides (batch row, token), and
+ * dstate (N, W - 1, D) dense (or NULL: zeros): dx, dweight, dbias (or NULL) and
+ * dinit (or NULL), dense, all in `dtype`. `call` is the forward's; its state and
+ * y are not read. Sums are in one order: results do not change from call to call.
+ */
+int ramnet_causal_conv_backward(const ramnet_causal_conv_call *call, const void *dy, const int64_t *dy_strides,
+                                const void *dstate, void *dx, void *dweight, void *dbias, void *dinit, void *stream);
+
+/* Bytes of the device workspace of either; -1 for sizes they do not take. */
+int64_t ramnet_causal_conv_workspace_bytes(int64_t B, int64_t T, int64_t N, int64_t D, int64_t W, int dtype, int packed,
+                                           int backward);
+
+/*
+ * Selective scan: S numbers of state per sequence and channel, each with a decay
+ * of its own. No counterpart in the reference. Per token, channel d of group g:
+ *     dt = softplus(dt + dt_bias)   (or dt + dt_bias)
+ *     h_n <- exp(dt A_dn) h_n + dt x B_gn;   s = sum_n C_gn h_n + skip x
+ *     y = s silu(gate)              (or s)
+ * `call` holds
+ *   x, dt, gate    (B, T, D) `dtype`, last dimension dense; gate may be NULL
+ *   Bm, Cm         (B, T, G, S) `dtype`, last dimension dense; channel d reads group d / (D / G)
+ *   A              (D, S) fp32, dense; S from 1 to 64
+ *   skip, dt_bias  (D) fp32, or NULL
+ *   init_state     (N, D, S) fp32, or NULL: zeros
+ *   state          (N, D, S) fp32; may be init_state
+ *   y              (B, T, D) `dtype`, dense; 0 where a token does not count
+ *   cu_seqlens, lengths  as above
+ *   kept           NULL, or ramnet_selective_scan_kept_bytes for the backward
+ *   workspace      ramnet_selective_scan_workspace_bytes
+ *   strides        12: of x, dt, gate batch row and token, of Bm, Cm batch row, token and group
+ */
+typedef struct ramnet_selective_scan_call {
+    const void *x, *dt, *gate, *Bm, *Cm;
+    const float *A, *skip, *dt_bias, *init_state;
+    float *state;
+    void *y;
+    const int32_t *cu_seqlens, *lengths;
+    void *kept, *workspace;
+    int64_t kept_bytes, workspace_bytes;
+    int64_t B, T, N, D, S, G;
+    int64_t strides[12];
+    int64_t dtype, softplus;
+} ramnet_selective_scan_call;
+
+int ramnet_selective_scan_forward(const ramnet_selective_scan_call *call, void *stream);
+
+/*
+ * Its gradients, from dy (B, T, D) `dtype`, strides dy_strides (batch row,
+ * token), and dstate (N, D, S) fp32 dense (or NULL: zeros): dx, ddt, dgate (where
+ * there is a gate), dB and dC in `dtype`, dA, dskip, dbias and dinit in fp32 (the
+ * last three may be NULL), dense. `call` is the forward's with what it kept; its
+ * init_state, state and y are not read. Sums are in one order.
+ */
+int ramnet_selective_scan_backward(const ramnet_selective_scan_call *call, const void *dy, const int64_t *dy_strides,
+                                   const float *dstate, void *dx, void *ddt, void *dgate, void *dB, void *dC, float *dA,
+                                   float *dskip, float *dbias, float *dinit, void *stream);
+
+/* Bytes of the device workspace (kind 0: forward, 1: forward that keeps, 2:
+ * backward) and of what a forward keeps; -1 for sizes they do not take. */
+int64_t ramnet_selective_scan_workspace_bytes(int64_t B, int64_t T, int64_t N, int64_t D, int64_t S, int64_t G, int packed,
+                                              int kind);
+int64_t ramnet_selective_scan_kept_bytes(int64_t B, int64_t T, int64_t N, int64_t D, int64_t S, int64_t G, int packed);
+
+/*
+ * One token a row, from a uniform number. No counterpart in the reference. Weights
+ * are w_i = exp((l_i - max) / temperature), of a NaN logit 0; tokens are ordered by
+ * descending logit, equal ones by index. Each filter keeps a prefix of that order:
+ * the first top_k; of these, tokens with less than top_p times their sum before
+ * them (at least one); tokens of w >= min_p. The token is the lowest index of a kept one
+ * whose running sum, by index, passes random * sum.
+ *   logits         (R, V) `dtype`, rows row_stride elements apart
+ *   random         (R) fp32 uniform in [0, 1), or NULL where tokens is
+ *   temperature, top_p, min_p  (R) fp32, or NULL: the value of all rows beside it;
+ *                  temperature 0 (or below) takes the greatest logit, top_p of 1 and
+ *                  min_p of 0 keep all
+ *   top_k          (R) int32, or NULL: that of all; 0 (or below) keeps all
+ *   tokens         (R) int64, or NULL
+ *   probs          (R, V) fp32 kept weights over their sum, or NULL
+ * A row without a logit above -inf gives token 0 and probabilities of 0. Sums are in 64 bits.
+ */
+typedef struct ramnet_sample_tokens_call {
+    const void *logits;
+    const float *random, *temperature, *top_p, *min_p;
+    const int32_t *top_k;
+    int64_t *tokens;
+    float *probs;
+    double temperature_of_all, top_p_of_all, min_p_of_all;
+    int64_t top_k_of_all, R, V, row_stride, dtype;
+} ramnet_sample_tokens_call;
+
+int ramnet_sample_tokens(const ramnet_sample_tokens_call *call, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -2,9 +2,11 @@
 // stream. Errors never abort: they set a thread-local message and return a
 // nonzero code (the reference raises RuntimeError from the same checks,
 // csrc/cuda_utils.cuh:375-391 and ram_attn_topk_addr.cu:241-246).
+#include "causal_conv.hpp"
 #include "ramnet_hip.h"
 #include "ramnet_kernels.hpp"
 #include "ramnet_search.hpp"
+#include "selective_scan.hpp"
 
 #include <algorithm>
 #include <atomic>
@@ -1308,6 +1310,191 @@ int ramnet_verify_drafts(const int64_t *tokens, const void *target, const void *
     const char *why = nullptr;
     const hipError_t err = ramnet::launch_verify_drafts(job, static_cast<hipStream_t>(stream), &why);
     return finish(err, why, "verify_drafts launch");
+}
+
+// Sequences of a call that walks time, and its batch.
+static int check_sequences(ramnet::SequenceJob &seq, const char *what, int64_t B, int64_t T, int64_t N, bool packed) {
+    RAMNET_REQUIRE(B >= 0 && T >= 0 && N >= 0, std::string(what) + " shape must have B, T, N >= 0");
+    RAMNET_REQUIRE(packed ? B == 1 : N == B,
+                   std::string(what) + ": packed sequences lie in a batch of one, others one to a row");
+    RAMNET_REQUIRE(fits_int({B, T, N, B * T, T + N + 64}), std::string(what) + ": index overflow");
+    seq.B = static_cast<int>(B), seq.T = static_cast<int>(T), seq.N = static_cast<int>(N);
+    return RAMNET_OK;
+}
+
+static int check_conv(ramnet::ConvJob &job, int64_t B, int64_t T, int64_t N, int64_t D, int64_t W, bool packed) {
+    if (int rc = check_sequences(job.seq, "causal_conv", B, T, N, packed))
+        return rc;
+    RAMNET_REQUIRE(D > 0 && W > 0 && W <= ramnet::kConvMaxWidth, "causal_conv: D must be above 0 and W from 1 to 8");
+    RAMNET_REQUIRE(D < (1LL << 24), "causal_conv: index overflow");
+    // (threads of a launch: a piece of 16 tokens and 16 bytes of channels each)
+    RAMNET_REQUIRE((B * (T / 16 + 1) + N + 2) * ((D + 3) / 4) < (1LL << 36), "causal_conv: index overflow");
+    job.D = static_cast<int>(D), job.W = static_cast<int>(W);
+    return RAMNET_OK;
+}
+
+static const int32_t kSomeBounds = 0;  // (marks sizes as of packed sequences where only they are asked for)
+
+int64_t ramnet_causal_conv_workspace_bytes(int64_t B, int64_t T, int64_t N, int64_t D, int64_t W, int dtype, int packed,
+                                           int backward) {
+    ramnet::ConvJob job{};
+    if (!valid_dtype(dtype) || check_conv(job, B, T, N, D, W, packed != 0) != RAMNET_OK)
+        return -1;
+    job.dtype = dtype, job.seq.cu = packed ? &kSomeBounds : nullptr;
+    return ramnet::conv_layout(job, backward != 0, nullptr, nullptr);
+}
+
+// What forward and backward check alike.
+static int conv_job(ramnet::ConvJob &job, const ramnet_causal_conv_call &c, bool backward, ramnet::ConvGrads *grads) {
+    if (int rc = check_conv(job, c.B, c.T, c.N, c.D, c.W, c.cu_seqlens != nullptr))
+        return rc;
+    RAMNET_REQUIRE(valid_dtype(static_cast<int>(c.dtype)), "causal_conv dtype must be float32, float16 or bfloat16");
+    RAMNET_REQUIRE(!(c.cu_seqlens && c.lengths), "causal_conv: packed sequences have no lengths beside their bounds");
+    job.seq.cu = c.cu_seqlens, job.seq.lengths = c.lengths;
+    job.x = c.x, job.weight = c.weight, job.bias = c.bias, job.init = c.init_state, job.y = c.y, job.state = c.state;
+    job.dtype = static_cast<int>(c.dtype), job.silu = c.silu != 0;
+    job.x_at[0] = c.strides[0], job.x_at[1] = c.strides[1];
+    RAMNET_REQUIRE(c.weight && (c.B * c.T == 0 || c.x), "null tensor pointer");
+    const int64_t need = ramnet::conv_layout(job, backward, static_cast<char *>(c.workspace), grads);
+    RAMNET_REQUIRE(need == 0 || (c.workspace && c.workspace_bytes >= need), "causal_conv: workspace too small");
+    return RAMNET_OK;
+}
+
+int ramnet_causal_conv_forward(const ramnet_causal_conv_call *call, void *stream) {
+    RAMNET_REQUIRE(call, "null call");
+    ramnet::ConvJob job{};
+    if (int rc = conv_job(job, *call, false, nullptr))
+        return rc;
+    RAMNET_REQUIRE((call->B * call->T == 0 || job.y) && (call->N * (call->W - 1) == 0 || job.state), "null tensor pointer");
+    if (job.seq.B == 0)
+        return RAMNET_OK;
+    const char *why = nullptr;
+    return finish(ramnet::launch_conv(job, static_cast<hipStream_t>(stream), &why), why, "causal_conv launch");
+}
+
+int ramnet_causal_conv_backward(const ramnet_causal_conv_call *call, const void *dy, const int64_t *dy_strides,
+                                const void *dstate, void *dx, void *dweight, void *dbias, void *dinit, void *stream) {
+    RAMNET_REQUIRE(call, "null call");
+    ramnet::ConvJob job{};
+    ramnet::ConvGrads grads{};
+    if (int rc = conv_job(job, *call, true, &grads))
+        return rc;
+    RAMNET_REQUIRE(dweight && (call->B * call->T == 0 || (dy && dy_strides && dx)), "null tensor pointer");
+    RAMNET_REQUIRE(!dinit || dinit != dstate, "causal_conv: dinit must not be dstate");
+    RAMNET_REQUIRE(job.seq.B > 0, "causal_conv: a backward call needs rows");
+    grads.dy = dy, grads.dstate = dstate, grads.dx = dx, grads.dinit = dinit, grads.dweight = dweight, grads.dbias = dbias;
+    if (dy_strides)
+        grads.dy_at[0] = dy_strides[0], grads.dy_at[1] = dy_strides[1];
+    const char *why = nullptr;
+    return finish(ramnet::launch_conv_backward(job, grads, static_cast<hipStream_t>(stream), &why), why,
+                  "causal_conv backward launch");
+}
+
+static int check_scan(ramnet::ScanJob &job, int64_t B, int64_t T, int64_t N, int64_t D, int64_t S, int64_t G, bool packed) {
+    if (int rc = check_sequences(job.seq, "selective_scan", B, T, N, packed))
+        return rc;
+    RAMNET_REQUIRE(D > 0 && G > 0 && D % G == 0, "selective_scan: D must be a multiple of G, both above 0");
+    RAMNET_REQUIRE(S > 0 && S <= ramnet::kScanMaxStates, "selective_scan: S must be from 1 to 64");
+    RAMNET_REQUIRE(D < (1LL << 24), "selective_scan: index overflow");
+    job.D = static_cast<int>(D), job.S = static_cast<int>(S), job.G = static_cast<int>(G);
+    // blocks of a launch (64 channels of a piece of 64 tokens or more, or of a row) are counted in 32 bits
+    RAMNET_REQUIRE((B * (T / 64 + 1) + N + 2) * G * ((D / G + 63) / 64) < kIntMax, "selective_scan: index overflow");
+    return RAMNET_OK;
+}
+
+int64_t ramnet_selective_scan_workspace_bytes(int64_t B, int64_t T, int64_t N, int64_t D, int64_t S, int64_t G, int packed,
+                                              int kind) {
+    ramnet::ScanJob job{};
+    if (kind < 0 || kind > 2 || check_scan(job, B, T, N, D, S, G, packed != 0) != RAMNET_OK)
+        return -1;
+    job.seq.cu = packed ? &kSomeBounds : nullptr;
+    float some = 0.f;
+    job.kept = kind ? &some : nullptr;
+    return ramnet::scan_layout(job, kind == 2, nullptr, nullptr);
+}
+
+int64_t ramnet_selective_scan_kept_bytes(int64_t B, int64_t T, int64_t N, int64_t D, int64_t S, int64_t G, int packed) {
+    ramnet::ScanJob job{};
+    if (check_scan(job, B, T, N, D, S, G, packed != 0) != RAMNET_OK)
+        return -1;
+    job.seq.cu = packed ? &kSomeBounds : nullptr;
+    return ramnet::scan_kept_bytes(job);
+}
+
+static int scan_job(ramnet::ScanJob &job, const ramnet_selective_scan_call &c, bool backward, ramnet::ScanGrads *grads) {
+    if (int rc = check_scan(job, c.B, c.T, c.N, c.D, c.S, c.G, c.cu_seqlens != nullptr))
+        return rc;
+    RAMNET_REQUIRE(valid_dtype(static_cast<int>(c.dtype)), "selective_scan dtype must be float32, float16 or bfloat16");
+    RAMNET_REQUIRE(!(c.cu_seqlens && c.lengths), "selective_scan: packed sequences have no lengths beside their bounds");
+    job.seq.cu = c.cu_seqlens, job.seq.lengths = c.lengths;
+    job.x = c.x, job.dt = c.dt, job.gate = c.gate, job.B = c.Bm, job.C = c.Cm, job.A = c.A, job.skip = c.skip;
+    job.bias = c.dt_bias, job.init = c.init_state, job.y = c.y, job.state = c.state;
+    job.dtype = static_cast<int>(c.dtype), job.softplus = c.softplus != 0;
+    int64_t *to[5] = {job.x_at, job.dt_at, job.gate_at, job.B_at, job.C_at};
+    for (int i = 0; i < 6; ++i)
+        to[i / 2][i % 2] = c.strides[i];
+    for (int i = 0; i < 6; ++i)
+        to[3 + i / 3][i % 3] = c.strides[6 + i];
+    RAMNET_REQUIRE(c.A && (c.B * c.T == 0 || (c.x && c.dt && c.Bm && c.Cm)), "null tensor pointer");
+    job.kept = static_cast<float *>(c.kept);
+    if (c.kept)
+        RAMNET_REQUIRE(c.kept_bytes >= ramnet::scan_kept_bytes(job), "selective_scan: kept region too small");
+    const int64_t need = ramnet::scan_layout(job, backward, static_cast<char *>(c.workspace), grads);
+    RAMNET_REQUIRE(need == 0 || (c.workspace && c.workspace_bytes >= need), "selective_scan: workspace too small");
+    return RAMNET_OK;
+}
+
+int ramnet_selective_scan_forward(const ramnet_selective_scan_call *call, void *stream) {
+    RAMNET_REQUIRE(call, "null call");
+    ramnet::ScanJob job{};
+    if (int rc = scan_job(job, *call, false, nullptr))
+        return rc;
+    RAMNET_REQUIRE((call->B * call->T == 0 || job.y) && (call->N == 0 || job.state), "null tensor pointer");
+    if (job.seq.B == 0)
+        return RAMNET_OK;
+    const char *why = nullptr;
+    return finish(ramnet::launch_scan(job, static_cast<hipStream_t>(stream), &why), why, "selective_scan launch");
+}
+
+int ramnet_selective_scan_backward(const ramnet_selective_scan_call *call, const void *dy, const int64_t *dy_strides,
+                                   const float *dstate, void *dx, void *ddt, void *dgate, void *dB, void *dC, float *dA,
+                                   float *dskip, float *dbias, float *dinit, void *stream) {
+    RAMNET_REQUIRE(call, "null call");
+    ramnet::ScanJob job{};
+    ramnet::ScanGrads grads{};
+    if (int rc = scan_job(job, *call, true, &grads))
+        return rc;
+    RAMNET_REQUIRE(dA && (call->B * call->T == 0 || (dy && dy_strides && dx && ddt && dB && dC && call->kept &&
+                                                     (dgate || !call->gate))),
+                   "null tensor pointer");
+    RAMNET_REQUIRE(!dinit || dinit != dstate, "selective_scan: dinit must not be dstate");
+    RAMNET_REQUIRE(call->B * call->T > 0, "selective_scan: a backward call needs tokens");
+    grads.dy = dy, grads.dstate = dstate, grads.dx = dx, grads.ddt = ddt, grads.dgate = dgate, grads.dB = dB, grads.dC = dC;
+    grads.dA = dA, grads.dskip = dskip, grads.dbias = dbias, grads.dinit = dinit;
+    grads.dy_at[0] = dy_strides[0], grads.dy_at[1] = dy_strides[1];
+    const char *why = nullptr;
+    return finish(ramnet::launch_scan_backward(job, grads, static_cast<hipStream_t>(stream), &why), why,
+                  "selective_scan backward launch");
+}
+
+int ramnet_sample_tokens(const ramnet_sample_tokens_call *call, void *stream) {
+    RAMNET_REQUIRE(call, "null call");
+    const ramnet_sample_tokens_call &c = *call;
+    RAMNET_REQUIRE(c.R >= 0 && c.V > 0, "sample_tokens shape must have R >= 0 and V > 0");
+    RAMNET_REQUIRE(c.R < kIntMax && c.V < (1LL << 30), "sample_tokens: index overflow");
+    RAMNET_REQUIRE(valid_dtype(static_cast<int>(c.dtype)), "sample_tokens dtype must be float32, float16 or bfloat16");
+    if (c.R == 0)
+        return RAMNET_OK;
+    RAMNET_REQUIRE(c.logits && (c.tokens || c.probs) && (!c.tokens || c.random), "null tensor pointer");
+    int bits = 0;
+    while ((1LL << bits) < c.V)
+        ++bits;
+    const ramnet::SampleJob job{c.logits, c.random, c.temperature, c.top_p, c.min_p, c.top_k, c.temperature_of_all,
+                                c.top_p_of_all, c.min_p_of_all, c.top_k_of_all, c.tokens, c.probs,
+                                static_cast<double>(1LL << (62 - bits)), c.row_stride, static_cast<int>(c.dtype),
+                                static_cast<int>(c.R), static_cast<int>(c.V)};
+    const char *why = nullptr;
+    return finish(ramnet::launch_sample_tokens(job, static_cast<hipStream_t>(stream), &why), why, "sample_tokens launch");
 }
 
 // The query has no token count: it answers for a call of kPlanQueryTokens

@@ -354,4 +354,20 @@ struct VerifyJob {
 };
 hipError_t launch_verify_drafts(const VerifyJob &job, hipStream_t stream, const char **why);
 
+// Sampling; a filter's values are of each row (R) or, where that is null, of all.
+struct SampleJob {
+    const void *logits;         // (R, V), rows row_at elements apart
+    const float *random;        // (R), where tokens are drawn
+    const float *temperature, *top_p, *min_p;
+    const int32_t *top_k;
+    double temperature_of_all, top_p_of_all, min_p_of_all;
+    int64_t top_k_of_all;
+    int64_t *tokens;            // (R), or null
+    float *probs;               // (R, V), or null
+    double unit;                // weights are added up in parts of 1 / unit
+    int64_t row_at;
+    int dtype, R, V;
+};
+hipError_t launch_sample_tokens(const SampleJob &job, hipStream_t stream, const char **why);
+
 }  // namespace ramnet

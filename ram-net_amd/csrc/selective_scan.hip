@@ -1,0 +1,353 @@
+// Selective scan, forward: whole and packed prompts, decode steps, and what a training call keeps.
+#include "ramnet_kernels.hpp"
+#include "selective_scan.hpp"
+
+namespace ramnet {
+
+namespace {
+
+constexpr int kThreads = 256, kChannels = kThreads / 4, kTile = kScanKept;
+
+// A wave's B and C of a tile of tokens as fp32, [token][B, C][4 NR], those past S zero.
+template<typename Scalar, int NR>
+struct GroupTile {
+    static constexpr int kRow = 8 * NR, kFloats = kTile * kRow, kLoads = kFloats / kWave;
+    uint32_t raw[kLoads];
+
+    __device__ __forceinline__ void load(const ScanJob &job, const TimePiece &piece, int group, int t, int lane) {
+        const Scalar *B = static_cast<const Scalar *>(job.B) + piece.row * job.B_at[0] + group * job.B_at[2];
+        const Scalar *C = static_cast<const Scalar *>(job.C) + piece.row * job.C_at[0] + group * job.C_at[2];
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int e = i * kWave + lane, n = e % (4 * NR);
+            const int64_t token = piece.t0 + min(t + e / kRow, piece.len - 1);
+            const bool second = e % kRow >= 4 * NR;
+            raw[i] = n < job.S ? load_bits(second ? C + token * job.C_at[1] + n : B + token * job.B_at[1] + n) : 0u;
+        }
+    }
+    __device__ __forceinline__ void store(float *to, int lane) const {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i)
+            to[i * kWave + lane] = bits_f32<Scalar>(raw[i]);
+    }
+};
+
+// Which channel a lane holds a quarter of; where there is none, the group's last one, which it does not write.
+struct ScanPlace {
+    int piece, group, channel, sub;
+    bool valid;
+
+    __device__ __forceinline__ ScanPlace(const ScanJob &job) {
+        const int wide = job.D / job.G, per_group = (wide + kChannels - 1) / kChannels;
+        const int block = static_cast<int>(blockIdx.x), per_piece = per_group * job.G;
+        piece = block / per_piece;
+        const int at = block - piece * per_piece;
+        group = at / per_group;
+        const int c = (at - group * per_group) * kChannels + static_cast<int>(threadIdx.x) / 4;
+        valid = c < wide;
+        channel = group * wide + min(c, wide - 1);
+        sub = static_cast<int>(threadIdx.x) % 4;
+    }
+};
+
+enum : int { kEnds, kWhole };
+
+// kEnds: the state after each piece but a sequence's last, from zeros, and the sum of its dt.
+// kWhole: y, and the state after the sequence.
+template<typename Scalar, int NR, int kMode>
+__global__ __launch_bounds__(kThreads) void scan_kernel(const ScanJob job) {
+    using Groups = GroupTile<Scalar, NR>;
+    __shared__ __align__(16) float lds[kThreads / kWave][2][Groups::kFloats];
+    const ScanPlace at(job);
+    TimePiece piece;
+    if (!time_piece(job.seq, job.step, at.piece, piece))
+        return;
+    const int lane = static_cast<int>(threadIdx.x) % kWave, sub = at.sub, channel = at.channel, n0 = sub * NR;
+    float(*tile)[Groups::kFloats] = lds[threadIdx.x / kWave];
+    const int count = job.S - n0;
+    const int64_t wide = static_cast<int64_t>(job.D) * 4 * NR;  // floats of a workspace row
+    const int64_t mine = static_cast<int64_t>(channel) * 4 * NR + n0;
+    const int64_t row = static_cast<int64_t>(piece.row) * job.seq.T + piece.t0;
+    Scalar *y = static_cast<Scalar *>(job.y) + row * job.D + channel;
+    if (piece.seq >= 0 && piece.at < piece.count) {
+        float h[NR], A2[NR];
+        load_states<NR>(A2, job.A + static_cast<int64_t>(channel) * job.S + n0, count);
+#pragma unroll
+        for (int j = 0; j < NR; ++j)
+            h[j] = 0.f, A2[j] *= kLog2e;
+        const float *init = job.init ? job.init + (static_cast<int64_t>(piece.seq) * job.D + channel) * job.S + n0 : nullptr;
+        if constexpr (kMode == kEnds) {
+            if (piece.at == piece.count - 1) {
+                // The sequence's state, for its first piece: the last one writes over it in place.
+                if (piece.count > 1 && job.init && at.valid) {
+                    load_states<NR>(h, init, count);
+                    store_states<NR>(job.ends + at.piece * wide + mine, h, NR);
+                }
+                return;
+            }
+        } else {
+            const int64_t first = at.piece - piece.at;
+            if (job.init && piece.count == 1)
+                load_states<NR>(h, init, count);
+            else if (job.init)
+                load_states<NR>(h, job.ends + (first + piece.count - 1) * wide + mine, NR);
+            for (int k = 0; k < piece.at; ++k) {
+                float end[NR];
+                load_states<NR>(end, job.ends + (first + k) * wide + mine, NR);
+                const double span = job.spans[(first + k) * job.D + channel];
+#pragma unroll
+                for (int j = 0; j < NR; ++j)
+                    h[j] = fmaf(__builtin_amdgcn_exp2f(static_cast<float>(A2[j] * span)), h[j], end[j]);
+            }
+        }
+        const float bias = job.bias ? job.bias[channel] : 0.f, skip = job.skip ? job.skip[channel] : 0.f;
+        const Scalar *x = static_cast<const Scalar *>(job.x) + piece.row * job.x_at[0] + channel;
+        const Scalar *dt = static_cast<const Scalar *>(job.dt) + piece.row * job.dt_at[0] + channel;
+        const Scalar *gate = job.gate ? static_cast<const Scalar *>(job.gate) + piece.row * job.gate_at[0] + channel : nullptr;
+        double span = 0.0;
+
+        Groups groups;
+        uint32_t xs[kTile / 4], ds[kTile / 4], gs[kTile / 4];
+        auto load = [&](int t) {
+            groups.load(job, piece, at.group, t, lane);
+#pragma unroll
+            for (int g = 0; g < kTile / 4; ++g) {
+                const int64_t token = piece.t0 + min(t + 4 * g + sub, piece.len - 1);
+                xs[g] = load_bits(x + token * job.x_at[1]);
+                ds[g] = load_bits(dt + token * job.dt_at[1]);
+                gs[g] = kMode == kWhole && gate ? load_bits(gate + token * job.gate_at[1]) : 0u;
+            }
+        };
+        auto walk = [&](int t, const float *bc, auto whole) {
+            float xv[kTile / 4], dv[kTile / 4], gv[kTile / 4];
+#pragma unroll
+            for (int g = 0; g < kTile / 4; ++g) {
+                xv[g] = bits_f32<Scalar>(xs[g]), gv[g] = bits_f32<Scalar>(gs[g]);
+                const float raw = bits_f32<Scalar>(ds[g]) + bias;
+                float e;
+                dv[g] = job.softplus ? softplus(raw, e) : raw;
+            }
+            if (t + kTile < piece.len)
+                load(t + kTile);
+#pragma unroll
+            for (int g = 0; g < kTile / 4; ++g) {
+                const bool live = decltype(whole)::value || t + 4 * g + sub < piece.len;
+                if constexpr (kMode == kEnds)
+                    span += live ? static_cast<double>(dv[g]) : 0.0;
+                const float ux = dv[g] * xv[g];
+                float sums[4];
+                auto token = [&](auto k_) {
+                    constexpr int k = decltype(k_)::value;
+                    sums[k] = 0.f;
+                    if (!decltype(whole)::value && t + 4 * g + k >= piece.len)
+                        return;
+                    const float d = quad_lane<k>(dv[g]), u = quad_lane<k>(ux);
+                    const float *b = bc + (4 * g + k) * Groups::kRow + n0, *c = b + 4 * NR;
+#pragma unroll
+                    for (int j = 0; j < NR; ++j) {
+                        h[j] = fmaf(__builtin_amdgcn_exp2f(d * A2[j]), h[j], u * b[j]);
+                        if constexpr (kMode == kWhole)
+                            sums[k] = fmaf(c[j], h[j], sums[k]);
+                    }
+                };
+                token(std::integral_constant<int, 0>{});
+                token(std::integral_constant<int, 1>{});
+                token(std::integral_constant<int, 2>{});
+                token(std::integral_constant<int, 3>{});
+                if constexpr (kMode == kWhole) {
+                    float s = fmaf(skip, xv[g], quad_sums(sums, sub));
+                    if (gate)
+                        s *= gv[g] * sigmoid(gv[g]);
+                    if (live && at.valid)
+                        store_vec<Scalar, 1>(y + static_cast<int64_t>(t + 4 * g + sub) * job.D, {{round_bits<Scalar>(s)}});
+                }
+            }
+        };
+        float *kept = nullptr;
+        if (kMode == kWhole && job.kept)
+            kept = job.kept + (scan_slot(job.seq, piece.seq, piece.lo) + (piece.t0 - piece.lo) / kScanKept) * wide + mine;
+        if (piece.len > 0)
+            load(0);
+        for (int t = 0, turn = 0; t < piece.len; t += kTile, turn ^= 1) {
+            groups.store(tile[turn], lane);
+            wave_sync();
+            if (kMode == kWhole && job.kept && at.valid) {
+                store_states<NR>(kept, h, NR);
+                kept += wide;
+            }
+            if (t + kTile <= piece.len)
+                walk(t, tile[turn], std::true_type{});
+            else
+                walk(t, tile[turn], std::false_type{});
+        }
+        if constexpr (kMode == kEnds) {
+            span += __shfl_xor(span, 1);
+            span += __shfl_xor(span, 2);
+            if (at.valid) {
+                store_states<NR>(job.ends + at.piece * wide + mine, h, NR);
+                if (sub == 0)
+                    job.spans[static_cast<int64_t>(at.piece) * job.D + channel] = span;
+            }
+        } else if (piece.at == piece.count - 1 && at.valid) {
+            store_states<NR>(job.state + (static_cast<int64_t>(piece.seq) * job.D + channel) * job.S + n0, h, count);
+        }
+    }
+    if (kMode == kWhole && at.valid)
+        for (int i = sub; i < piece.rest; i += 4)
+            store_vec<Scalar, 1>(y + static_cast<int64_t>(piece.len + i) * job.D, {{0u}});
+}
+
+// Decode steps of up to kScanStepTokens tokens, bound by reading and writing the states: no staging, one wave
+// 16 channels of one sequence.
+template<typename Scalar, int NR>
+__global__ __launch_bounds__(kThreads) void scan_step_kernel(const ScanJob job) {
+    const ScanPlace at(job);
+    const int b = at.piece, sub = at.sub, channel = at.channel, n0 = sub * NR, count = job.S - n0;
+    const int T = job.seq.T, len = job.seq.lengths ? clamped(job.seq.lengths[b], 0, T) : T;
+    float h[NR], A2[NR];
+    const int64_t where = (static_cast<int64_t>(b) * job.D + channel) * job.S + n0;
+    if (job.init) {
+        load_states<NR>(h, job.init + where, count);
+    } else {
+#pragma unroll
+        for (int j = 0; j < NR; ++j)
+            h[j] = 0.f;
+    }
+    load_states<NR>(A2, job.A + static_cast<int64_t>(channel) * job.S + n0, count);
+#pragma unroll
+    for (int j = 0; j < NR; ++j)
+        A2[j] *= kLog2e;
+    const float bias = job.bias ? job.bias[channel] : 0.f, skip = job.skip ? job.skip[channel] : 0.f;
+    const Scalar *x = static_cast<const Scalar *>(job.x) + b * job.x_at[0] + channel;
+    const Scalar *dt = static_cast<const Scalar *>(job.dt) + b * job.dt_at[0] + channel;
+    const Scalar *gate = job.gate ? static_cast<const Scalar *>(job.gate) + b * job.gate_at[0] + channel : nullptr;
+    const Scalar *B = static_cast<const Scalar *>(job.B) + b * job.B_at[0] + at.group * job.B_at[2];
+    const Scalar *C = static_cast<const Scalar *>(job.C) + b * job.C_at[0] + at.group * job.C_at[2];
+    Scalar *y = static_cast<Scalar *>(job.y) + static_cast<int64_t>(b) * T * job.D + channel;
+    for (int t = 0; t < T; ++t) {
+        float out = 0.f;
+        if (t < len) {
+            const float xv = load_f32(x + t * job.x_at[1]);
+            float d = load_f32(dt + t * job.dt_at[1]) + bias, e, s = 0.f;
+            d = job.softplus ? softplus(d, e) : d;
+            const float u = d * xv;
+#pragma unroll
+            for (int j = 0; j < NR; ++j) {
+                const bool on = j < count;
+                const float bv = on ? load_f32(B + t * job.B_at[1] + n0 + j) : 0.f;
+                const float cv = on ? load_f32(C + t * job.C_at[1] + n0 + j) : 0.f;
+                h[j] = fmaf(__builtin_amdgcn_exp2f(d * A2[j]), h[j], u * bv);
+                s = fmaf(cv, h[j], s);
+            }
+            s += quad_swap<1>(s);
+            s += quad_swap<2>(s);
+            out = fmaf(skip, xv, s);
+            if (gate) {
+                const float g = load_f32(gate + t * job.gate_at[1]);
+                out *= g * sigmoid(g);
+            }
+        }
+        if (sub == 0 && at.valid)
+            store_vec<Scalar, 1>(y + static_cast<int64_t>(t) * job.D, {{round_bits<Scalar>(out)}});
+    }
+    if (at.valid)
+        store_states<NR>(job.state + where, h, count);
+}
+
+// Blocks of a launch over `pieces` pieces.
+unsigned blocks_of(const ScanJob &job, int64_t pieces) {
+    return static_cast<unsigned>(pieces * job.G * ((job.D / job.G + kChannels - 1) / kChannels));
+}
+
+template<typename Scalar, int NR>
+hipError_t launch_states(const ScanJob &job, hipStream_t stream) {
+    const dim3 block(kThreads);
+    if (scan_is_step(job)) {
+        hipLaunchKernelGGL((scan_step_kernel<Scalar, NR>), dim3(blocks_of(job, job.seq.B)), block, 0, stream, job);
+        return hipGetLastError();
+    }
+    const dim3 grid(blocks_of(job, most_pieces(job.seq, job.step)));
+    if (job.seq.T > job.step)
+        hipLaunchKernelGGL((scan_kernel<Scalar, NR, kEnds>), grid, block, 0, stream, job);
+    hipLaunchKernelGGL((scan_kernel<Scalar, NR, kWhole>), grid, block, 0, stream, job);
+    return hipGetLastError();
+}
+
+template<typename Scalar>
+hipError_t launch_type(const ScanJob &job, hipStream_t stream) {
+    switch (scan_lane_states(job.S)) {
+        case 1: return launch_states<Scalar, 1>(job, stream);
+        case 2: return launch_states<Scalar, 2>(job, stream);
+        case 4: return launch_states<Scalar, 4>(job, stream);
+        case 8: return launch_states<Scalar, 8>(job, stream);
+        default: return launch_states<Scalar, 16>(job, stream);
+    }
+}
+
+}  // namespace
+
+bool scan_is_step(const ScanJob &job) { return !job.seq.cu && !job.kept && job.seq.T <= kScanStepTokens; }
+
+// Rows are cut into pieces where their channels alone leave compute units idle: the state after each
+// piece from zeros is a pass of its own, of five sixths of the work, so that two pieces of a row
+// take about as long as the row in one, and more than two less.
+int scan_step_tokens(const ScanJob &job) {
+    const int64_t rows = job.seq.B > 0 ? job.seq.B : 1;
+    const int64_t waves = rows * job.G * ((job.D / job.G + 15) / 16);
+    const int64_t parts = waves >= 1024 ? 1 : (2048 + waves - 1) / waves;
+    const int64_t tokens = (job.seq.T + parts - 1) / parts;
+    const int64_t step = (tokens + kScanKept - 1) / kScanKept * kScanKept;
+    return static_cast<int>(step < 64 ? 64 : step);
+}
+
+int64_t scan_layout(ScanJob &job, bool backward, char *base, ScanGrads *grads) {
+    int64_t size = 0;
+    auto region = [&](int64_t bytes) {
+        char *at = base ? base + size : nullptr;
+        size += (bytes + 255) / 256 * 256;
+        return at;
+    };
+    if (!backward && scan_is_step(job))
+        return 0;
+    job.step = scan_step_tokens(job);
+    const int64_t pieces = most_pieces(job.seq, job.step), wide = 4LL * scan_lane_states(job.S);
+    if (job.seq.cu) {
+        job.seq.bounds = reinterpret_cast<int32_t *>(region((job.seq.N + 1) * 4LL));
+        job.seq.first = reinterpret_cast<int32_t *>(region((job.seq.N + 1) * 4LL));
+    }
+    const bool cut = job.seq.T > job.step;
+    if (cut) {
+        job.spans = reinterpret_cast<double *>(region(pieces * job.D * 8));
+        float *ends = reinterpret_cast<float *>(region(pieces * job.D * wide * 4));
+        if (backward && grads)
+            grads->backs = ends;
+        else
+            job.ends = ends;
+    }
+    if (backward) {
+        const int64_t blocks = blocks_of(job, 1) / job.G;  // of a group
+        float *groups = reinterpret_cast<float *>(region(blocks * job.seq.B * job.seq.T * job.G * 2 * wide * 4));
+        float *sums = reinterpret_cast<float *>(region(pieces * job.D * (wide + 2) * 4));
+        if (grads)
+            grads->groups = groups, grads->sums = sums;
+    }
+    return size;
+}
+
+int64_t scan_kept_bytes(const ScanJob &job) { return scan_slots(job.seq) * job.D * 16 * scan_lane_states(job.S); }
+
+hipError_t launch_scan(const ScanJob &job, hipStream_t stream, const char **why) {
+    if (job.seq.cu) {
+        const hipError_t err = launch_sequences(job.seq, job.step, stream);
+        if (err != hipSuccess)
+            return err;
+    }
+    switch (job.dtype) {
+        case kF32: return launch_type<float>(job, stream);
+        case kF16: return launch_type<_Float16>(job, stream);
+        case kBF16: return launch_type<bf16_t>(job, stream);
+        default: *why = "selective_scan: unsupported dtype"; return hipErrorInvalidValue;
+    }
+}
+
+}  // namespace ramnet

@@ -1,0 +1,140 @@
+// The selective scan: jobs of its launches and device helpers they share.
+//
+// S numbers h of state (fp32) per sequence and channel, per token and channel d of group g:
+//     dt = softplus(raw + dt_bias)          (or raw + dt_bias)
+//     h_n <- e^(dt A_dn) h_n + dt x B_gn;   s = sum_n C_gn h_n + skip x;   y = s silu(gate)   (or s)
+//
+// Four adjacent lanes hold a channel, NR = S / 4 (rounded up to 1, 2, 4, 8 or 16) states each; a wave
+// holds 16 channels. Tokens are taken four at a time: what a token needs once (its softplus, its gate)
+// is done by one of the four lanes, and given to the others within vector instructions.
+#pragma once
+
+#include "sequences.hpp"
+#include "vector16.hpp"
+
+#include <type_traits>
+
+namespace ramnet {
+
+enum : int { kScanMaxStates = 64, kScanKept = 16, kScanStepTokens = 8 };
+
+struct ScanJob {
+    SequenceJob seq;
+    const void *x, *dt, *gate;  // (B, T, D), strides of batch row and token; gate may be null
+    const void *B, *C;          // (B, T, G, S), strides of batch row, token and group
+    const float *A;             // (D, S)
+    const float *skip, *bias;   // (D), or null
+    const float *init;          // (N, D, S), or null: zeros
+    void *y;                    // (B, T, D) dense
+    float *state;               // (N, D, S); may be init
+    int dtype, softplus, D, S, G;
+    int64_t x_at[2], dt_at[2], gate_at[2], B_at[3], C_at[3];
+    int step;                   // tokens of a piece, a multiple of kScanKept
+    // workspace, [piece][D][4 NR] and [piece][D]
+    float *ends;                // state after each piece from zeros
+    double *spans;              // sum of a piece's dt
+    // of a training call: the state before every kScanKept tokens of a sequence, [slot][D][4 NR]
+    float *kept;
+};
+
+// Gradients: of x, dt, gate, B and C in their types, of the others fp32; dense.
+struct ScanGrads {
+    const void *dy;       // (B, T, D), strides dy_at
+    const float *dstate;  // (N, D, S), or null: zeros
+    void *dx, *ddt, *dgate, *dB, *dC;
+    float *dA, *dskip, *dbias, *dinit;  // (dskip, dbias and dinit may be null)
+    int64_t dy_at[2];
+    // workspace
+    float *backs;    // [piece][D][4 NR] gradient of the state before each piece, from its own outputs
+    float *groups;   // [channel block][B T][2][4 NR] sums of dB and dC over the block's channels
+    float *sums;     // [piece][D][4 NR + 2] sums of dA, dskip and dbias over the piece's tokens
+};
+
+__host__ __device__ inline int scan_lane_states(int S) { return S <= 4 ? 1 : S <= 8 ? 2 : S <= 16 ? 4 : S <= 32 ? 8 : 16; }
+
+// The place of a sequence's kept states: sequence `seq` from token lo on, one for every kScanKept tokens.
+__host__ __device__ inline int64_t scan_slot(const SequenceJob &job, int seq, int lo) {
+    return job.cu ? static_cast<int64_t>(lo / kScanKept) + seq
+                  : static_cast<int64_t>(seq) * ((job.T + kScanKept - 1) / kScanKept);
+}
+__host__ __device__ inline int64_t scan_slots(const SequenceJob &job) {
+    return job.cu ? static_cast<int64_t>(job.T) / kScanKept + job.N + 1
+                  : static_cast<int64_t>(job.B) * ((job.T + kScanKept - 1) / kScanKept);
+}
+
+// Value of lane K of each four.
+template<int K>
+__device__ __forceinline__ float quad_lane(float x) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), K * 0x55, 0xF, 0xF, true));
+}
+template<int XOR>
+__device__ __forceinline__ float quad_swap(float x) {
+    constexpr int kControl = XOR == 1 ? 0xB1 : 0x4E;  // lanes 1 0 3 2, 2 3 0 1
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), kControl, 0xF, 0xF, true));
+}
+
+// Of four values a lane, each summed over the four lanes: lane i has the sum of v[i].
+__device__ __forceinline__ float quad_sums(const float (&v)[4], int lane) {
+    const bool odd = lane & 1, high = lane & 2;
+    const float a = (odd ? v[1] : v[0]) + quad_swap<1>(odd ? v[0] : v[1]);
+    const float b = (odd ? v[3] : v[2]) + quad_swap<1>(odd ? v[2] : v[3]);
+    return (high ? b : a) + quad_swap<2>(high ? a : b);
+}
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// log(1 + e^x) = max(x, 0) + log(1 + e), e = e^-|x| in (0, 1], the latter as 2 atanh(e / (2 + e)): the
+// series of atanh on (0, 1/3], to 2e-9 of its value. `e` comes out for the derivative.
+__device__ __forceinline__ float softplus(float x, float &e) {
+    e = __builtin_amdgcn_exp2f(-fabsf(x) * kLog2e);
+    const float s = e * __builtin_amdgcn_rcpf(2.f + e), q = s * s;
+    float sum = 1.f / 17.f;
+#pragma unroll
+    for (int k = 15; k >= 1; k -= 2)
+        sum = fmaf(sum, q, 1.f / static_cast<float>(k));
+    return fmaxf(x, 0.f) + 2.f * s * sum;
+}
+
+// Writes of some lanes of a wave to LDS before reads of others.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// NR states of a channel, those past S zero. `p`: state n0 of it.
+template<int NR>
+__device__ __forceinline__ void load_states(float (&h)[NR], const float *p, int count) {
+    if (count >= NR) {
+#pragma unroll
+        for (int j = 0; j < NR; ++j)
+            h[j] = p[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < NR; ++j)
+            h[j] = j < count ? p[j] : 0.f;
+    }
+}
+template<int NR>
+__device__ __forceinline__ void store_states(float *p, const float (&h)[NR], int count) {
+    if (count >= NR) {
+#pragma unroll
+        for (int j = 0; j < NR; ++j)
+            p[j] = h[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < NR; ++j)
+            if (j < count)
+                p[j] = h[j];
+    }
+}
+
+// Whether a call walks its few tokens without staging (it then needs no workspace).
+bool scan_is_step(const ScanJob &job);
+// Places the buffers of a call in `base`, or sizes them (null base); chooses its pieces.
+int64_t scan_layout(ScanJob &job, bool backward, char *base, ScanGrads *grads);
+int64_t scan_kept_bytes(const ScanJob &job);
+hipError_t launch_scan(const ScanJob &job, hipStream_t stream, const char **why);
+hipError_t launch_scan_backward(const ScanJob &job, const ScanGrads &grads, hipStream_t stream, const char **why);
+
+}  // namespace ramnet

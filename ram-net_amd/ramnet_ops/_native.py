@@ -137,6 +137,14 @@ SIGNATURES: dict[str, tuple[type, list]] = {
     "ramnet_verify_drafts": (_c_int, [
         _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64s, _c_ptr, _c_ptr,
         _c_ptr]),
+    "ramnet_causal_conv_forward": (_c_int, [ctypes.c_char_p, _c_ptr]),
+    "ramnet_causal_conv_backward": (_c_int, [ctypes.c_char_p, _c_ptr, _c_i64s] + [_c_ptr] * 6),
+    "ramnet_causal_conv_workspace_bytes": (_c_i64, [_c_i64] * 5 + [_c_int] * 3),
+    "ramnet_selective_scan_forward": (_c_int, [ctypes.c_char_p, _c_ptr]),
+    "ramnet_selective_scan_backward": (_c_int, [ctypes.c_char_p, _c_ptr, _c_i64s] + [_c_ptr] * 11),
+    "ramnet_selective_scan_workspace_bytes": (_c_i64, [_c_i64] * 6 + [_c_int] * 2),
+    "ramnet_selective_scan_kept_bytes": (_c_i64, [_c_i64] * 6 + [_c_int]),
+    "ramnet_sample_tokens": (_c_int, [ctypes.c_char_p, _c_ptr]),
     "ramnet_segment_plan": (_c_int, [
         _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_int, ctypes.POINTER(_c_int), ctypes.POINTER(_c_int),
         ctypes.POINTER(_c_int)]),
