@@ -1326,7 +1326,7 @@ static int check_conv(ramnet::ConvJob &job, int64_t B, int64_t T, int64_t N, int
     if (int rc = check_sequences(job.seq, "causal_conv", B, T, N, packed))
         return rc;
     RAMNET_REQUIRE(D > 0 && W > 0 && W <= ramnet::kConvMaxWidth, "causal_conv: D must be above 0 and W from 1 to 8");
-    RAMNET_REQUIRE(D < (1LL << 24), "causal_conv: index overflow");
+    RAMNET_REQUIRE(D < (1LL << 22), "causal_conv: index overflow");
     // (threads of a launch: a piece of 16 tokens and 16 bytes of channels each)
     RAMNET_REQUIRE((B * (T / 16 + 1) + N + 2) * ((D + 3) / 4) < (1LL << 36), "causal_conv: index overflow");
     job.D = static_cast<int>(D), job.W = static_cast<int>(W);
@@ -1395,7 +1395,7 @@ static int check_scan(ramnet::ScanJob &job, int64_t B, int64_t T, int64_t N, int
         return rc;
     RAMNET_REQUIRE(D > 0 && G > 0 && D % G == 0, "selective_scan: D must be a multiple of G, both above 0");
     RAMNET_REQUIRE(S > 0 && S <= ramnet::kScanMaxStates, "selective_scan: S must be from 1 to 64");
-    RAMNET_REQUIRE(D < (1LL << 24), "selective_scan: index overflow");
+    RAMNET_REQUIRE(D < ramnet::kScanStride && G * S < ramnet::kScanStride, "selective_scan: index overflow");
     job.D = static_cast<int>(D), job.S = static_cast<int>(S), job.G = static_cast<int>(G);
     // blocks of a launch (64 channels of a piece of 64 tokens or more, or of a row) are counted in 32 bits
     RAMNET_REQUIRE((B * (T / 64 + 1) + N + 2) * G * ((D / G + 63) / 64) < kIntMax, "selective_scan: index overflow");
@@ -1435,6 +1435,13 @@ static int scan_job(ramnet::ScanJob &job, const ramnet_selective_scan_call &c, b
         to[i / 2][i % 2] = c.strides[i];
     for (int i = 0; i < 6; ++i)
         to[3 + i / 3][i % 3] = c.strides[6 + i];
+    if (job.seq.T > 1)
+        for (const int64_t *at : to)
+            RAMNET_REQUIRE(at[1] >= 0 && at[1] < ramnet::kScanStride,
+                           "selective_scan: tokens must lie less than 2**22 elements apart");
+    else
+        for (int64_t *at : to)  // (any, there is no second token)
+            at[1] = 0;
     RAMNET_REQUIRE(c.A && (c.B * c.T == 0 || (c.x && c.dt && c.Bm && c.Cm)), "null tensor pointer");
     job.kept = static_cast<float *>(c.kept);
     if (c.kept)
@@ -1471,7 +1478,9 @@ int ramnet_selective_scan_backward(const ramnet_selective_scan_call *call, const
     RAMNET_REQUIRE(call->B * call->T > 0, "selective_scan: a backward call needs tokens");
     grads.dy = dy, grads.dstate = dstate, grads.dx = dx, grads.ddt = ddt, grads.dgate = dgate, grads.dB = dB, grads.dC = dC;
     grads.dA = dA, grads.dskip = dskip, grads.dbias = dbias, grads.dinit = dinit;
-    grads.dy_at[0] = dy_strides[0], grads.dy_at[1] = dy_strides[1];
+    grads.dy_at[0] = dy_strides[0], grads.dy_at[1] = job.seq.T > 1 ? dy_strides[1] : 0;
+    RAMNET_REQUIRE(grads.dy_at[1] >= 0 && grads.dy_at[1] < ramnet::kScanStride,
+                   "selective_scan: tokens must lie less than 2**22 elements apart");
     const char *why = nullptr;
     return finish(ramnet::launch_scan_backward(job, grads, static_cast<hipStream_t>(stream), &why), why,
                   "selective_scan backward launch");

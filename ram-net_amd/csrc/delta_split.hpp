@@ -15,6 +15,7 @@
 // own among them (zeros of a triangle times it): one in v, those of its column alone.
 #pragma once
 
+#include "buffer_window.hpp"
 #include "delta_chunk.hpp"
 
 namespace ramnet {
@@ -99,12 +100,7 @@ __device__ __forceinline__ int operand_at(int k) {
     return (k & ~31) | ((quad < 4 ? 2 * quad : 2 * quad - 7) << 2) | (k & 3);
 }
 
-// A window of rows in memory: loads past it give 0, stores past it are dropped.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t window(const void *base, int64_t bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, static_cast<int>(bytes), kBufWord3);
-}
-
-constexpr int kNowhere = kDeltaReach;  // past every window, with any row's offset on top
+static_assert(kNowhere == kDeltaReach, "offsets of a window end before");
 
 // A wave's 16 columns of a matrix whose rows are `step` elements apart (at
 // least its width): rows 16 m + 4 (lane / 16) + r, in order of m and r.
@@ -139,24 +135,6 @@ __device__ __forceinline__ void arrived(T (&x)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
         asm volatile("" : "+v"(x[i]));
-}
-
-template<typename T>
-__device__ __forceinline__ uint32_t buffer_bits(__amdgpu_buffer_rsrc_t from, int at) {
-    if constexpr (sizeof(T) == 4)
-        return __builtin_amdgcn_raw_buffer_load_b32(from, at, 0, 0);
-    else
-        return __builtin_amdgcn_raw_buffer_load_b16(from, at, 0, 0);
-}
-
-template<typename T>
-__device__ __forceinline__ void buffer_store(float v, __amdgpu_buffer_rsrc_t to, int at) {
-    if constexpr (sizeof(T) == 4)
-        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), to, at, 0, 0);
-    else if constexpr (__is_same(T, bf16_t))
-        __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, static_cast<__bf16>(v)), to, at, 0, 0);
-    else
-        __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, static_cast<_Float16>(v)), to, at, 0, 0);
 }
 
 // What prepare leaves per record, 64 values each, for the chain kernels: K and

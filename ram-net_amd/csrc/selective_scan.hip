@@ -6,64 +6,22 @@ namespace ramnet {
 
 namespace {
 
-constexpr int kThreads = 256, kChannels = kThreads / 4, kTile = kScanKept;
-
-// A wave's B and C of a tile of tokens as fp32, [token][B, C][4 NR], those past S zero.
-template<typename Scalar, int NR>
-struct GroupTile {
-    static constexpr int kRow = 8 * NR, kFloats = kTile * kRow, kLoads = kFloats / kWave;
-    uint32_t raw[kLoads];
-
-    __device__ __forceinline__ void load(const ScanJob &job, const TimePiece &piece, int group, int t, int lane) {
-        const Scalar *B = static_cast<const Scalar *>(job.B) + piece.row * job.B_at[0] + group * job.B_at[2];
-        const Scalar *C = static_cast<const Scalar *>(job.C) + piece.row * job.C_at[0] + group * job.C_at[2];
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int e = i * kWave + lane, n = e % (4 * NR);
-            const int64_t token = piece.t0 + min(t + e / kRow, piece.len - 1);
-            const bool second = e % kRow >= 4 * NR;
-            raw[i] = n < job.S ? load_bits(second ? C + token * job.C_at[1] + n : B + token * job.B_at[1] + n) : 0u;
-        }
-    }
-    __device__ __forceinline__ void store(float *to, int lane) const {
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i)
-            to[i * kWave + lane] = bits_f32<Scalar>(raw[i]);
-    }
-};
-
-// Which channel a lane holds a quarter of; where there is none, the group's last one, which it does not write.
-struct ScanPlace {
-    int piece, group, channel, sub;
-    bool valid;
-
-    __device__ __forceinline__ ScanPlace(const ScanJob &job) {
-        const int wide = job.D / job.G, per_group = (wide + kChannels - 1) / kChannels;
-        const int block = static_cast<int>(blockIdx.x), per_piece = per_group * job.G;
-        piece = block / per_piece;
-        const int at = block - piece * per_piece;
-        group = at / per_group;
-        const int c = (at - group * per_group) * kChannels + static_cast<int>(threadIdx.x) / 4;
-        valid = c < wide;
-        channel = group * wide + min(c, wide - 1);
-        sub = static_cast<int>(threadIdx.x) % 4;
-    }
-};
+constexpr int kThreads = kScanThreads, kTile = kScanKept, kQuads = kTile / 4;
 
 enum : int { kEnds, kWhole };
 
 // kEnds: the state after each piece but a sequence's last, from zeros, and the sum of its dt.
 // kWhole: y, and the state after the sequence.
-template<typename Scalar, int NR, int kMode>
+template<typename Scalar, int NR, int kMode, bool kGate>
 __global__ __launch_bounds__(kThreads) void scan_kernel(const ScanJob job) {
-    using Groups = GroupTile<Scalar, NR>;
-    __shared__ __align__(16) float lds[kThreads / kWave][2][Groups::kFloats];
+    using Groups = ScanGroups<Scalar, NR>;
+    __shared__ __align__(16) float lds[kThreads / kWave][2][2 * Groups::kFloats];
     const ScanPlace at(job);
     TimePiece piece;
     if (!time_piece(job.seq, job.step, at.piece, piece))
         return;
     const int lane = static_cast<int>(threadIdx.x) % kWave, sub = at.sub, channel = at.channel, n0 = sub * NR;
-    float(*tile)[Groups::kFloats] = lds[threadIdx.x / kWave];
+    float(*tile)[2 * Groups::kFloats] = lds[threadIdx.x / kWave];
     const int count = job.S - n0;
     const int64_t wide = static_cast<int64_t>(job.D) * 4 * NR;  // floats of a workspace row
     const int64_t mine = static_cast<int64_t>(channel) * 4 * NR + n0;
@@ -101,39 +59,65 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(const ScanJob job) {
             }
         }
         const float bias = job.bias ? job.bias[channel] : 0.f, skip = job.skip ? job.skip[channel] : 0.f;
-        const Scalar *x = static_cast<const Scalar *>(job.x) + piece.row * job.x_at[0] + channel;
-        const Scalar *dt = static_cast<const Scalar *>(job.dt) + piece.row * job.dt_at[0] + channel;
-        const Scalar *gate = job.gate ? static_cast<const Scalar *>(job.gate) + piece.row * job.gate_at[0] + channel : nullptr;
         double span = 0.0;
-
-        Groups groups;
-        uint32_t xs[kTile / 4], ds[kTile / 4], gs[kTile / 4];
+        // Windows over the 16 tokens of a tile: tokens that are not there read 0 and are not written
+        const int64_t token = piece.t0, xr = piece.row * job.x_at[0], dr = piece.row * job.dt_at[0],
+                      gr = piece.row * job.gate_at[0], Br = piece.row * job.B_at[0] + at.group * job.B_at[2],
+                      Cr = piece.row * job.C_at[0] + at.group * job.C_at[2];
+        const ScanRows<Scalar> x_rows(at, job.x_at[1], true), dt_rows(at, job.dt_at[1], true), gate_rows(at, job.gate_at[1], true),
+            y_rows(at, job.D, at.valid);
+        const Groups B_rows(lane, job.B_at[1], job.S), C_rows(lane, job.C_at[1], job.S);
+        uint32_t xs[kQuads], ds[kQuads], gs[kQuads], Bs[NR], Cs[NR];
         auto load = [&](int t) {
-            groups.load(job, piece, at.group, t, lane);
-#pragma unroll
-            for (int g = 0; g < kTile / 4; ++g) {
-                const int64_t token = piece.t0 + min(t + 4 * g + sub, piece.len - 1);
-                xs[g] = load_bits(x + token * job.x_at[1]);
-                ds[g] = load_bits(dt + token * job.dt_at[1]);
-                gs[g] = kMode == kWhole && gate ? load_bits(gate + token * job.gate_at[1]) : 0u;
+            const int left = piece.len - t;
+            dt_rows.load(ds, dt_rows.over(job.dt, dr + (token + t) * job.dt_at[1], job.dt_at[1], job.D, left));
+            x_rows.load(xs, x_rows.over(job.x, xr + (token + t) * job.x_at[1], job.x_at[1], job.D, left));
+            B_rows.load(Bs, dt_rows.over(job.B, Br + (token + t) * job.B_at[1], job.B_at[1], job.S, left));
+            if constexpr (kMode == kWhole) {
+                C_rows.load(Cs, dt_rows.over(job.C, Cr + (token + t) * job.C_at[1], job.C_at[1], job.S, left));
+                if constexpr (kGate)
+                    gate_rows.load(gs, gate_rows.over(job.gate, gr + (token + t) * job.gate_at[1], job.gate_at[1], job.D, left));
             }
         };
         auto walk = [&](int t, const float *bc, auto whole) {
-            float xv[kTile / 4], dv[kTile / 4], gv[kTile / 4];
+            float xv[kQuads], dv[kQuads], gv[kQuads];
 #pragma unroll
-            for (int g = 0; g < kTile / 4; ++g) {
-                xv[g] = bits_f32<Scalar>(xs[g]), gv[g] = bits_f32<Scalar>(gs[g]);
-                const float raw = bits_f32<Scalar>(ds[g]) + bias;
+            for (int g = 0; g < kQuads; ++g) {
+                xv[g] = bits_f32<Scalar>(xs[g]), dv[g] = bits_f32<Scalar>(ds[g]) + bias;
+                if constexpr (kGate && kMode == kWhole)
+                    gv[g] = bits_f32<Scalar>(gs[g]);
+            }
+            if (job.softplus) {
                 float e;
-                dv[g] = job.softplus ? softplus(raw, e) : raw;
+#pragma unroll
+                for (int g = 0; g < kQuads; ++g)
+                    dv[g] = softplus(dv[g], e);
             }
             if (t + kTile < piece.len)
                 load(t + kTile);
+            const __amdgpu_buffer_rsrc_t out = y_rows.over(job.y, (row + t) * job.D, job.D, job.D, piece.len - t);
+            // B and C of four tokens at a time, read from LDS while the four before are walked
+            float b[2][4][NR], c[2][4][NR];
+            auto fetch = [&](int g) {
 #pragma unroll
-            for (int g = 0; g < kTile / 4; ++g) {
-                const bool live = decltype(whole)::value || t + 4 * g + sub < piece.len;
+                for (int k = 0; k < 4; ++k) {
+                    const float *from = bc + (4 * g + k) * Groups::kRow + n0;
+#pragma unroll
+                    for (int j = 0; j < NR; ++j) {
+                        b[g & 1][k][j] = from[j];
+                        if constexpr (kMode == kWhole)
+                            c[g & 1][k][j] = from[Groups::kFloats + j];
+                    }
+                }
+            };
+            fetch(0);
+#pragma unroll
+            for (int g = 0; g < kQuads; ++g) {
+                if (g + 1 < kQuads)
+                    fetch(g + 1);
+                __builtin_amdgcn_sched_barrier(0);
                 if constexpr (kMode == kEnds)
-                    span += live ? static_cast<double>(dv[g]) : 0.0;
+                    span += decltype(whole)::value || t + 4 * g + sub < piece.len ? static_cast<double>(dv[g]) : 0.0;
                 const float ux = dv[g] * xv[g];
                 float sums[4];
                 auto token = [&](auto k_) {
@@ -142,12 +126,11 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(const ScanJob job) {
                     if (!decltype(whole)::value && t + 4 * g + k >= piece.len)
                         return;
                     const float d = quad_lane<k>(dv[g]), u = quad_lane<k>(ux);
-                    const float *b = bc + (4 * g + k) * Groups::kRow + n0, *c = b + 4 * NR;
 #pragma unroll
                     for (int j = 0; j < NR; ++j) {
-                        h[j] = fmaf(__builtin_amdgcn_exp2f(d * A2[j]), h[j], u * b[j]);
+                        h[j] = fmaf(__builtin_amdgcn_exp2f(d * A2[j]), h[j], u * b[g & 1][k][j]);
                         if constexpr (kMode == kWhole)
-                            sums[k] = fmaf(c[j], h[j], sums[k]);
+                            sums[k] = j ? fmaf(c[g & 1][k][j], h[j], sums[k]) : c[g & 1][k][j] * h[j];
                     }
                 };
                 token(std::integral_constant<int, 0>{});
@@ -156,10 +139,9 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(const ScanJob job) {
                 token(std::integral_constant<int, 3>{});
                 if constexpr (kMode == kWhole) {
                     float s = fmaf(skip, xv[g], quad_sums(sums, sub));
-                    if (gate)
+                    if constexpr (kGate)
                         s *= gv[g] * sigmoid(gv[g]);
-                    if (live && at.valid)
-                        store_vec<Scalar, 1>(y + static_cast<int64_t>(t + 4 * g + sub) * job.D, {{round_bits<Scalar>(s)}});
+                    buffer_store<Scalar>(s, out, y_rows.at + g * y_rows.step);
                 }
             }
         };
@@ -169,7 +151,9 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(const ScanJob job) {
         if (piece.len > 0)
             load(0);
         for (int t = 0, turn = 0; t < piece.len; t += kTile, turn ^= 1) {
-            groups.store(tile[turn], lane);
+            Groups::store(tile[turn], Bs, lane);
+            if constexpr (kMode == kWhole)
+                Groups::store(tile[turn] + Groups::kFloats, Cs, lane);
             wave_sync();
             if (kMode == kWhole && job.kept && at.valid) {
                 store_states<NR>(kept, h, NR);
@@ -256,7 +240,7 @@ __global__ __launch_bounds__(kThreads) void scan_step_kernel(const ScanJob job) 
 
 // Blocks of a launch over `pieces` pieces.
 unsigned blocks_of(const ScanJob &job, int64_t pieces) {
-    return static_cast<unsigned>(pieces * job.G * ((job.D / job.G + kChannels - 1) / kChannels));
+    return static_cast<unsigned>(pieces * job.G * ((job.D / job.G + kScanChannels - 1) / kScanChannels));
 }
 
 template<typename Scalar, int NR>
@@ -268,8 +252,11 @@ hipError_t launch_states(const ScanJob &job, hipStream_t stream) {
     }
     const dim3 grid(blocks_of(job, most_pieces(job.seq, job.step)));
     if (job.seq.T > job.step)
-        hipLaunchKernelGGL((scan_kernel<Scalar, NR, kEnds>), grid, block, 0, stream, job);
-    hipLaunchKernelGGL((scan_kernel<Scalar, NR, kWhole>), grid, block, 0, stream, job);
+        hipLaunchKernelGGL((scan_kernel<Scalar, NR, kEnds, false>), grid, block, 0, stream, job);
+    if (job.gate)
+        hipLaunchKernelGGL((scan_kernel<Scalar, NR, kWhole, true>), grid, block, 0, stream, job);
+    else
+        hipLaunchKernelGGL((scan_kernel<Scalar, NR, kWhole, false>), grid, block, 0, stream, job);
     return hipGetLastError();
 }
 

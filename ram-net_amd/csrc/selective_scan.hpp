@@ -9,6 +9,7 @@
 // is done by one of the four lanes, and given to the others within vector instructions.
 #pragma once
 
+#include "buffer_window.hpp"
 #include "sequences.hpp"
 #include "vector16.hpp"
 
@@ -16,7 +17,7 @@
 
 namespace ramnet {
 
-enum : int { kScanMaxStates = 64, kScanKept = 16, kScanStepTokens = 8 };
+enum : int { kScanMaxStates = 64, kScanKept = 16, kScanStepTokens = 8, kScanStride = 1 << 22 };
 
 struct ScanJob {
     SequenceJob seq;
@@ -28,7 +29,7 @@ struct ScanJob {
     void *y;                    // (B, T, D) dense
     float *state;               // (N, D, S); may be init
     int dtype, softplus, D, S, G;
-    int64_t x_at[2], dt_at[2], gate_at[2], B_at[3], C_at[3];
+    int64_t x_at[2], dt_at[2], gate_at[2], B_at[3], C_at[3];  // (of tokens below kScanStride)
     int step;                   // tokens of a piece, a multiple of kScanKept
     // workspace, [piece][D][4 NR] and [piece][D]
     float *ends;                // state after each piece from zeros
@@ -101,6 +102,70 @@ __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
+
+enum : int { kScanThreads = 256, kScanChannels = kScanThreads / 4 };
+
+// Which channel a lane holds a quarter of; where there is none, the group's last one, which it does not write.
+struct ScanPlace {
+    int piece, group, channel, sub, block;  // (block: which 64 channels of the group)
+    bool valid;
+
+    __device__ __forceinline__ ScanPlace(const ScanJob &job) {
+        const int wide = job.D / job.G, per_group = (wide + kScanChannels - 1) / kScanChannels;
+        const int id = static_cast<int>(blockIdx.x), per_piece = per_group * job.G;
+        piece = id / per_piece;
+        const int at = id - piece * per_piece;
+        group = at / per_group;
+        block = at - group * per_group;
+        const int c = block * kScanChannels + static_cast<int>(threadIdx.x) / 4;
+        valid = c < wide;
+        channel = group * wide + min(c, wide - 1);
+        sub = static_cast<int>(threadIdx.x) % 4;
+    }
+};
+
+// One value of a lane's channel for each four tokens of a tile, through a window over the tile's tokens that
+// are there.
+template<typename Scalar>
+struct ScanRows {
+    int at, step;  // bytes: the lane's place in the first four tokens; four tokens on
+
+    __device__ __forceinline__ ScanRows(const ScanPlace &place, int64_t stride, bool on) {
+        step = 4 * static_cast<int>(stride) * static_cast<int>(sizeof(Scalar));
+        at = on ? (place.sub * static_cast<int>(stride) + place.channel) * static_cast<int>(sizeof(Scalar)) : kNowhere;
+    }
+    __device__ static __forceinline__ __amdgpu_buffer_rsrc_t over(const void *p, int64_t from, int64_t stride, int D, int tokens) {
+        return window(static_cast<const Scalar *>(p) + from, ((min(tokens, kScanKept) - 1) * stride + D) * static_cast<int>(sizeof(Scalar)));
+    }
+    __device__ __forceinline__ void load(uint32_t (&to)[kScanKept / 4], __amdgpu_buffer_rsrc_t rows) const {
+#pragma unroll
+        for (int g = 0; g < kScanKept / 4; ++g)
+            to[g] = buffer_bits<Scalar>(rows, at + g * step);
+    }
+};
+
+// A wave's share of B or C of a tile, which it keeps in LDS as fp32, [token][4 NR], those past S zero.
+template<typename Scalar, int NR>
+struct ScanGroups {
+    static constexpr int kRow = 4 * NR, kFloats = kScanKept * kRow;
+    static constexpr int kSpan = kWave / kRow;  // tokens that a load of the wave spans
+    int at, step;
+
+    __device__ __forceinline__ ScanGroups(int lane, int64_t stride, int S) {
+        step = kSpan * static_cast<int>(stride) * static_cast<int>(sizeof(Scalar));
+        at = lane % kRow < S ? (lane / kRow * static_cast<int>(stride) + lane % kRow) * static_cast<int>(sizeof(Scalar)) : kNowhere;
+    }
+    __device__ __forceinline__ void load(uint32_t (&to)[NR], __amdgpu_buffer_rsrc_t rows) const {
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+            to[i] = buffer_bits<Scalar>(rows, at + i * step);
+    }
+    __device__ static __forceinline__ void store(float *to, const uint32_t (&from)[NR], int lane) {
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+            to[i * kWave + lane] = bits_f32<Scalar>(from[i]);
+    }
+};
 
 // NR states of a channel, those past S zero. `p`: state n0 of it.
 template<int NR>

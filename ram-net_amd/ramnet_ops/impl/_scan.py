@@ -52,6 +52,12 @@ def _rows_of(t: Tensor) -> Tensor:
     return _dense(t) if t.dim() else t
 
 
+def _near_rows_of(t: Tensor) -> Tensor:
+    """Likewise, its tokens (dimension 1) within the scan's reach of each other."""
+    t = _rows_of(t)
+    return t.contiguous() if t.dim() > 2 and t.stride(1) >= 2 ** 22 and t.shape[1] > 1 else t
+
+
 # --------------------------------------------------------------------------
 # short causal convolution
 
@@ -99,7 +105,7 @@ def _conv_plan(op: str, x, weight, bias, init_state, cu_seqlens, lengths) -> _Co
 
 def _bytes_of(op: str, count: int, sizes) -> int:
     if count < 0:
-        raise RuntimeError(f"{op}: sizes {tuple(sizes)} are not supported (tokens within int32, channels below 2**24)")
+        raise RuntimeError(f"{op}: sizes {tuple(sizes)} are not supported (tokens within int32, channels below 2**22)")
     return count
 
 
@@ -313,8 +319,8 @@ def _scan(op: str, x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, skip:
           dt_bias: Tensor | None, init_state: Tensor | None, cu_seqlens: Tensor | None, lengths: Tensor | None,
           softplus: bool, state: Tensor | None = None, keep: bool = False) -> tuple[Tensor, Tensor, Tensor | None]:
     """(y, state, kept). ``state``: where the state goes (init_state itself in place)."""
-    x, dt, B, C = _rows_of(x), _rows_of(dt), _rows_of(B), _rows_of(C)
-    gate = None if gate is None else _rows_of(gate)
+    x, dt, B, C = _near_rows_of(x), _near_rows_of(dt), _near_rows_of(B), _near_rows_of(C)
+    gate = None if gate is None else _near_rows_of(gate)
     plan = _scan_plan(op, x, dt, A, B, C, skip, gate, dt_bias, init_state, cu_seqlens, lengths)
     batch, T, N, D, S, G = plan.sizes
     A, skip, dt_bias = _parameter(A), _parameter(skip), _parameter(dt_bias)
@@ -402,12 +408,12 @@ def selective_scan_backward(
 def _scan_gradients(x, dt, A, B, C, skip, gate, dt_bias, cu_seqlens, lengths, softplus, sequences, kept, d_y,
                     d_state) -> tuple:
     op = "selective_scan_backward"
-    x, dt, B, C = _rows_of(x), _rows_of(dt), _rows_of(B), _rows_of(C)
-    gate = None if gate is None else _rows_of(gate)
+    x, dt, B, C = _near_rows_of(x), _near_rows_of(dt), _near_rows_of(B), _near_rows_of(C)
+    gate = None if gate is None else _near_rows_of(gate)
     plan = _scan_plan(op, x, dt, A, B, C, skip, gate, dt_bias, None, cu_seqlens, lengths)
     batch, T, N, D, S, G = plan.sizes
     _check_shapes(op, d_y=(d_y, (batch, T, D)), d_state=(d_state, (N, D, S)))
-    d_y = _rows_of(d_y.resolve_neg().to(x.dtype))
+    d_y = _near_rows_of(d_y.resolve_neg().to(x.dtype))
     if d_state is not None:
         d_state = d_state.resolve_neg().to(torch.float32).contiguous()
     dx, ddt, dgate = (x.new_empty((batch, T, D)) for _ in range(3))
