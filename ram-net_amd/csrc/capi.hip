@@ -1500,7 +1500,7 @@ int ramnet_sample_tokens(const ramnet_sample_tokens_call *call, void *stream) {
         ++bits;
     const ramnet::SampleJob job{c.logits, c.random, c.temperature, c.top_p, c.min_p, c.top_k, c.temperature_of_all,
                                 c.top_p_of_all, c.min_p_of_all, c.top_k_of_all, c.tokens, c.probs,
-                                static_cast<double>(1LL << (62 - bits)), c.row_stride, static_cast<int>(c.dtype),
+                                static_cast<double>(1LL << std::min(51, 62 - bits)), c.row_stride, static_cast<int>(c.dtype),
                                 static_cast<int>(c.R), static_cast<int>(c.V)};
     const char *why = nullptr;
     return finish(ramnet::launch_sample_tokens(job, static_cast<hipStream_t>(stream), &why), why, "sample_tokens launch");

@@ -9,9 +9,9 @@
 // and a token next to a border does not go by the rounding of 32 bits.
 //
 // One block a row, which it reads from memory once and from the caches after that. Where few tokens are kept they
-// are gathered in LDS together with some more, by a limit that each wave's greatest logits give, and compared
-// with each other. Otherwise the end of the prefix is found by counts and sums of the weights in 2048 bins, even
-// in the logit, and in the bin where it lies as before; then a pass adds up what is kept by stretches of the index.
+// are gathered in LDS and compared with each other: with some more, by a limit that each wave's greatest logits
+// give, or with the bin where the prefix ends, which counts (by top_k) or sums of the weights (by top_p) in 2048
+// bins tell. Otherwise the end is found within that bin, and a pass adds up what is kept by stretches of the index.
 #include "ramnet_kernels.hpp"
 #include "vector16.hpp"
 
@@ -19,45 +19,46 @@ namespace ramnet {
 
 namespace {
 
-constexpr int kThreads = 1024, kWaves = kThreads / kWave, kBins = 2048, kList = kThreads;
-// The most tokens that top_k keeps on the way by lists: a limit that 16 lanes of each wave reach lets in some 400
+constexpr int kThreads = 1024, kWaves = kThreads / kWave, kBins = 2 * kThreads, kList = kThreads;
+// The most tokens of top_k that are gathered by a limit: one that 16 lanes of each wave reach lets in some 400
 // of a language model's.
 constexpr int kListCount = 256;
+// Bins of a sum for each halving of the weight: what lies past 2^-32 is in the last bin.
+constexpr float kBinsAHalving = 64.f;
 
-// A token's place in the order as one number, greater for earlier ones.
-__device__ __forceinline__ uint64_t order_of(float l, int index) {
+// A token's place in the order as one number, greater for earlier ones; its upper half goes by the logit alone.
+__device__ __forceinline__ uint32_t key_of(float l) {
     const uint32_t bits = __float_as_uint(l);
-    const uint32_t key = bits ^ (static_cast<uint32_t>(static_cast<int32_t>(bits) >> 31) | 0x80000000u);
-    return static_cast<uint64_t>(key) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>(index));
+    return bits ^ (static_cast<uint32_t>(static_cast<int32_t>(bits) >> 31) | 0x80000000u);
 }
-__device__ __forceinline__ float logit_of(uint64_t order) {
-    const uint32_t key = static_cast<uint32_t>(order >> 32);
+__device__ __forceinline__ float logit_of_key(uint32_t key) {
     return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
-
-template<typename T, typename Op>
-__device__ __forceinline__ T wave_reduce(T x, Op op) {
-#pragma unroll
-    for (int m = 1; m < kWave; m <<= 1)
-        x = op(x, __shfl_xor(x, m));
-    return x;
+__device__ __forceinline__ uint64_t order_of(float l, int index) {
+    return static_cast<uint64_t>(key_of(l)) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>(index));
+}
+__device__ __forceinline__ float logit_of(uint64_t order) { return logit_of_key(static_cast<uint32_t>(order >> 32)); }
+__device__ __forceinline__ int index_of(uint64_t order) {
+    return static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(order));
 }
 
 struct Shared {
     uint32_t counts[kBins];
     uint64_t sums[kBins];
-    uint64_t list[kList], weights[kList];
+    uint64_t list[kList];
     uint64_t scan[2][kWaves];
-    float tops[kWaves], lows[kWaves];
-    uint64_t before, through;  // results that one thread finds
-    int count_before, bin, listed;
-    uint64_t order;
+    double powers[32];       // 2^(i / 32)
+    uint64_t before, order;  // results that one thread finds
+    int count_before, count_through, bin, listed;
 };
 
 // The block's LDS, by one name: through a pointer it would be read as memory of any kind.
 __device__ __forceinline__ Shared &lds() {
     __shared__ Shared shared;
     return shared;
+}
+__device__ __forceinline__ void add(uint64_t &to, uint64_t x) {
+    atomicAdd(reinterpret_cast<unsigned long long *>(&to), static_cast<unsigned long long>(x));
 }
 
 struct Least {
@@ -70,32 +71,70 @@ struct Sum {
     template<typename T> __device__ T operator()(T a, T b) const { return a + b; }
 };
 
-// 2^x for x <= 0, to 1e-14: the series of e^(f ln 2) for the fraction f of x, in [-1/2, 1/2], to its 11th power.
-__device__ __forceinline__ double power_of_2(double x) {
-    const double whole = __builtin_rint(x), f = (x - whole) * 0.693147180559945309417;
-    double sum = 1.0 / 39916800.0;
-    constexpr double kTerms[] = {1.0 / 3628800.0, 1.0 / 362880.0, 1.0 / 40320.0, 1.0 / 5040.0, 1.0 / 720.0, 1.0 / 120.0,
-                                 1.0 / 24.0,      1.0 / 6.0,      0.5,           1.0,          1.0};
+// The value of the lane whose number differs in one bit.
+template<int XOR>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t x) {
+    if constexpr (XOR == 1) {
+        return __builtin_amdgcn_mov_dpp(x, 0xB1, 0xF, 0xF, true);  // quad_perm 1 0 3 2
+    } else if constexpr (XOR == 2) {
+        return __builtin_amdgcn_mov_dpp(x, 0x4E, 0xF, 0xF, true);  // quad_perm 2 3 0 1
+    } else if constexpr (XOR == 4) {
+        const uint32_t up = __builtin_amdgcn_update_dpp(0u, x, 0x104, 0xF, 0x5, false);  // row_shl:4, lanes without bit 2
+        return __builtin_amdgcn_update_dpp(up, x, 0x114, 0xF, 0xA, false);               // row_shr:4, lanes with it
+    } else if constexpr (XOR == 8) {
+        return __builtin_amdgcn_mov_dpp(x, 0x128, 0xF, 0xF, true);  // row_ror:8
+    } else {
+        const auto r = XOR == 16 ? __builtin_amdgcn_permlane16_swap(x, x, false, false)
+                                 : __builtin_amdgcn_permlane32_swap(x, x, false, false);
+        return __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)) & XOR ? r[0] : r[1];
+    }
+}
+
+template<typename T, typename Op>
+__device__ __forceinline__ T wave_reduce(T x, Op op) {
 #pragma unroll
-    for (double term : kTerms)
-        sum = fma(sum, f, term);
-    return __builtin_amdgcn_ldexp(sum, static_cast<int>(whole));
+    for (int m = 1; m < kWave; m <<= 1)
+        x = op(x, __shfl_xor(x, m));
+    return x;
+}
+
+// 2^x for x in [-1000, 0], to 2e-15: of x in parts of 1/32, which adding 3 2^46 leaves in the lowest bits of the
+// sum, the last five bits by a table (whose 32 values lie in as many pairs of LDS banks), those above into the
+// exponent, and what is left, up to 1/64, by the series of e^(f ln 2) to its 5th power.
+constexpr int kParts = 32;
+__device__ __forceinline__ double power_of_2(double x) {
+    constexpr double kRound = 3.0 * 70368744177664.0, kLn2 = 0.693147180559945309417;
+    const double shifted = x + kRound, f = x - (shifted - kRound);
+    double terms[] = {kLn2 * kLn2 * kLn2 * kLn2 * kLn2 / 120.0, kLn2 * kLn2 * kLn2 * kLn2 / 24.0, kLn2 * kLn2 * kLn2 / 6.0,
+                      kLn2 * kLn2 / 2.0, kLn2};
+    const int part = static_cast<int>(__builtin_bit_cast(uint64_t, shifted));
+    double sum = terms[0];
+#pragma unroll
+    for (int i = 1; i < 5; ++i) {
+        asm("" : "+s"(terms[i]));  // (in scalar registers: from vector registers each would be copied first)
+        sum = fma(sum, f, terms[i]);
+    }
+    const double of_part = lds().powers[part & (kParts - 1)];
+    sum = fma(sum * f, of_part, of_part);
+    return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, sum) +
+                                          (static_cast<uint64_t>(static_cast<uint32_t>(part >> 5)) << 52));
 }
 
 template<typename Scalar>
 struct Sampler {
     const Scalar *row;
     int V, tid, lane, wave;
-    float top, low;         // the greatest logit, the smallest finite one
+    float top;              // the greatest logit
     float scale;            // bins per unit of the logit
     double rate, unit;      // log2(e) / temperature, 2^F
     double least;           // min_p
-    uint64_t border;        // order of the last token kept
+    float last_logit;       // the last token kept: of its logit those up to its index, of greater ones all
+    int last_index;
 
     __device__ __forceinline__ float clean(float l) const { return l != l ? -INFINITY : l + 0.f; }
 
     // f(logit, index) for all tokens, 16 bytes a thread, all threads of the block side by side.
-    template<int kDeep = 2, typename F>
+    template<int kDeep = 4, typename F>
     __device__ __forceinline__ void sweep(F f) const {
         constexpr int N = 16 / sizeof(Scalar);
         const int full = V / N * N;
@@ -120,28 +159,54 @@ struct Sampler {
             f(clean(load_f32(row + full + tid)), full + tid);
     }
 
-    // (a difference of -inf, or of nothing times 0, is held to where the weight is 0)
-    __device__ __forceinline__ double weight(float l) const {
-        const double x = (static_cast<double>(l) - static_cast<double>(top)) * rate;
-        return l == top ? 1.0 : power_of_2(x > -2000.0 ? x : -2000.0);
-    }
-    __device__ __forceinline__ uint64_t whole(double w) const { return static_cast<uint64_t>(w * unit + 0.5); }
-    __device__ __forceinline__ int bin(float l) const {
-        if (l == top)
-            return 0;
-        const float at = (top - l) * scale;  // (descending with l, whatever it rounds to)
-        return at < static_cast<float>(kBins - 1) ? static_cast<int>(at) : kBins - 1;
-    }
-    // Whether a token is drawn from.
-    __device__ __forceinline__ bool kept(float l, int index, double &w) const {
-        if (order_of(l, index) < border)
-            return false;
-        w = weight(l);
-        return w >= least && l > -INFINITY;  // (order_of(-inf) is greater than that of no token)
+    // The same with one piece ahead, for an f that takes longer than the read.
+    template<typename F>
+    __device__ __forceinline__ void sweep_ahead(F f) const {
+        constexpr int N = 16 / sizeof(Scalar), kStep = kThreads * N;
+        const int full = V / N * N;
+        Vec<Scalar, N> next{};
+        if (tid * N < full)
+            next = load_vec<Scalar, N>(row + tid * N);
+        for (int at = tid * N; at < full; at += kStep) {
+            const Vec<Scalar, N> x = next;
+            if (at + kStep < full)
+                next = load_vec<Scalar, N>(row + at + kStep);
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                f(x[e], at + e);
+        }
+        if (full + tid < V)
+            f(load_f32(row + full + tid), full + tid);
     }
 
-    // The sums of x over the threads before, and over all.
-    __device__ __forceinline__ uint64_t block_scan(uint64_t x, uint64_t &total, int which) {
+    // (what is no number, as a difference of -inf or nothing times 0, is held to where no part of the sum is left)
+    __device__ __forceinline__ double weight(float l) const {
+        const double x = (static_cast<double>(l) - static_cast<double>(top)) * rate;
+        return power_of_2(l == top ? 0.0 : __builtin_fmax(x, -1000.0));
+    }
+    // A weight in whole parts of 1 / unit, below 2^52: they are the last bits of its sum with 2^52.
+    __device__ __forceinline__ uint64_t whole(double w) const {
+        return __builtin_bit_cast(uint64_t, fma(w, unit, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
+    }
+    __device__ __forceinline__ int bin(float l) const {
+        const float at = l == top ? 0.f : (top - l) * scale;  // (descending with l, whatever it rounds to; a NaN last)
+        return static_cast<int>(__builtin_fminf(at, static_cast<float>(kBins - 1)));
+    }
+    // Whether a token is in the prefix kept (a NaN is not).
+    __device__ __forceinline__ bool within(float l, int index) const {
+        return l > last_logit || (l == last_logit && index <= last_index);
+    }
+    __device__ __forceinline__ void end_with(uint64_t order) { last_logit = logit_of(order), last_index = index_of(order); }
+    // Whether a token is drawn from.
+    __device__ __forceinline__ bool kept(float l, int index, double &w) const {
+        if (!within(l, index))
+            return false;
+        w = weight(l);
+        return w >= least;
+    }
+
+    // The sum of x over the threads before.
+    __device__ __forceinline__ uint64_t block_scan(uint64_t x, int which) {
         uint64_t run = x;
 #pragma unroll
         for (int m = 1; m < kWave; m <<= 1) {
@@ -153,32 +218,27 @@ struct Sampler {
             lds().scan[which][wave] = run;
         __syncthreads();
         uint64_t before = 0;
-        total = 0;
-        for (int w = 0; w < kWaves; ++w) {
-            before += w < wave ? lds().scan[which][w] : 0;
-            total += lds().scan[which][w];
-        }
+        for (int w = 0; w < wave; ++w)
+            before += lds().scan[which][w];
         return before + run - x;
     }
 
     template<typename T, typename Op>
-    __device__ __forceinline__ T block_reduce(T x, Op op) {
-        auto put = [&](T v) {
-            if constexpr (sizeof(T) == 8)
-                lds().scan[0][wave] = __builtin_bit_cast(uint64_t, v);
-            else
-                lds().scan[0][wave] = __builtin_bit_cast(uint32_t, v);
-        };
+    __device__ __forceinline__ T block_reduce(T x, Op op, int which = 0) {
         auto get = [&](int w) {
             if constexpr (sizeof(T) == 8)
-                return __builtin_bit_cast(T, lds().scan[0][w]);
+                return __builtin_bit_cast(T, lds().scan[which][w]);
             else
-                return __builtin_bit_cast(T, static_cast<uint32_t>(lds().scan[0][w]));
+                return __builtin_bit_cast(T, static_cast<uint32_t>(lds().scan[which][w]));
         };
         x = wave_reduce(x, op);
         __syncthreads();
-        if (lane == 0)
-            put(x);
+        if (lane == 0) {
+            if constexpr (sizeof(T) == 8)
+                lds().scan[which][wave] = __builtin_bit_cast(uint64_t, x);
+            else
+                lds().scan[which][wave] = __builtin_bit_cast(uint32_t, x);
+        }
         __syncthreads();
         x = get(0);
         for (int w = 1; w < kWaves; ++w)
@@ -187,92 +247,116 @@ struct Sampler {
     }
 
     // A limit that at least `count` logits reach, from the greatest one of each lane: the waves whose lanes have
-    // logits all give their share of it.
+    // logits all give their share of it, each to the 16 upper bits.
     __device__ __forceinline__ float limit_of(float mine, int count) {
         const int waves = min(V / static_cast<int>(16 / sizeof(Scalar)) / kWave, kWaves), each = (count + waves - 1) / max(waves, 1);
         if (waves == 0 || each > kWave)
             return -INFINITY;
-        int ahead = 0;
+        const uint32_t key = key_of(mine);
+        uint32_t reached = 0;
 #pragma unroll
-        for (int i = 0; i < kWave; ++i) {
-            const float other = readlane_f(mine, i);
-            ahead += other > mine || (other == mine && i < lane) ? 1 : 0;
-        }
-        const int at = __ffsll(static_cast<unsigned long long>(__ballot(ahead == each - 1))) - 1;
-        return block_reduce(wave < waves ? readlane_f(mine, at) : INFINITY, Least{});
+        for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1)
+            reached |= __popcll(__ballot(key >= (reached | bit))) >= each ? bit : 0;
+        reached = block_reduce(wave < waves ? reached : ~0u, Least{});
+        return reached > key_of(-INFINITY) ? logit_of_key(reached) : -INFINITY;
     }
 
-    // The tokens that reach `limit`, and their weights, in the list, in any order; more than kList in `found` if
-    // they are too many. `sum`: the weights of all tokens, where they are wanted.
-    __device__ __forceinline__ void gather(float limit, bool wanted, int &found, uint64_t &sum) {
+    // The tokens of which `wanted` is true in the list, in any order. How many they are: where
+    // more than kList the list has some of them.
+    template<typename F>
+    __device__ __forceinline__ int gather(F wanted) {
         __syncthreads();
         if (tid == 0)
             lds().listed = 0;
         __syncthreads();
-        uint64_t total = 0;
         sweep([&](float l, int i) {
-            if (wanted)
-                total += whole(weight(l));
-            if (l >= limit) {
+            if (wanted(l, i)) {
                 const int at = atomicAdd(&lds().listed, 1);
                 if (at < kList)
                     lds().list[at] = order_of(l, i);
             }
         });
-        sum = wanted ? block_reduce(total, Sum{}) : 0;
         __syncthreads();
-        found = lds().listed;
-        if (tid < min(found, kList))
-            lds().weights[tid] = whole(weight(logit_of(lds().list[tid])));
-        __syncthreads();
+        return lds().listed;
     }
 
-    // The rest of the way where the list has all tokens that can be kept. `all`: the sum that top_p is a share of,
-    // where it is not that of the first k. False if the list ends before that share does.
-    __device__ __forceinline__ bool finish(int members, uint64_t k, bool by_sum, double p, uint64_t all, double u, int64_t *token, float *probs) {
-        const bool mine = tid < members;
-        const uint64_t order = mine ? lds().list[tid] : 0;
-        uint64_t weights = mine ? lds().weights[tid] : 0, before = 0;
-        int rank = 0;
-        if (mine) {
-            for (int j = 0; j < members; ++j) {
-                const bool ahead = lds().list[j] > order;
-                rank += ahead, before += ahead ? lds().weights[j] : 0;
+    // One step of a bitonic sort within a wave.
+    template<int STRIDE>
+    __device__ __forceinline__ uint64_t step(uint64_t x, int size) const {
+        const uint32_t low = lane_xor<STRIDE>(static_cast<uint32_t>(x)), high = lane_xor<STRIDE>(static_cast<uint32_t>(x >> 32));
+        const uint64_t other = static_cast<uint64_t>(high) << 32 | low;
+        const bool greater = ((tid & STRIDE) == 0) == ((tid & size) == 0);
+        return (other > x) == greater ? other : x;
+    }
+    template<int STRIDE>
+    __device__ __forceinline__ uint64_t steps(uint64_t x, int size) const {
+        x = step<STRIDE>(x, size);
+        if constexpr (STRIDE > 1)
+            return steps<STRIDE / 2>(x, size);
+        return x;
+    }
+
+    // The numbers of the first `count` threads, one each, the greatest to the first thread, zeros behind them: a
+    // bitonic sort, by lane swaps within a wave and through LDS across waves.
+    __device__ __forceinline__ uint64_t sorted(uint64_t x, int count) const {
+        x = steps<1>(x, 2), x = steps<2>(x, 4), x = steps<4>(x, 8);
+        x = steps<8>(x, 16), x = steps<16>(x, 32), x = steps<32>(x, 64);
+        for (int size = 2 * kWave; size < 2 * count; size *= 2) {
+            for (int stride = size / 2; stride >= kWave; stride /= 2) {
+                __syncthreads();
+                lds().sums[tid] = x;
+                __syncthreads();
+                const uint64_t other = lds().sums[tid ^ stride];
+                const bool greater = ((tid & stride) == 0) == ((tid & size) == 0);
+                x = (other > x) == greater ? other : x;
             }
+            x = steps<32>(x, size);
         }
-        if (by_sum) {
-            if (k < static_cast<uint64_t>(V))
-                all = block_reduce(static_cast<uint64_t>(rank) < k ? weights : 0, Sum{});
-            else if (static_cast<double>(block_reduce(weights, Sum{})) < p * static_cast<double>(all) && members < V)
-                return false;
+        return x;
+    }
+
+    // The rest of the way where the list has all tokens that can be kept: of these the first k, and those with less
+    // than the share p of `all` before them (0: of the first k).
+    __device__ __forceinline__ void finish(int members, uint64_t k, bool by_sum, double p, uint64_t all, double u, int64_t *token,
+                                           float *probs) {
+        if (probs) {
+            constexpr int N = 4;
+            for (int i = tid * N; i < V / N * N; i += kThreads * N)
+                store_vec<float, N>(probs + i, {});
+            if (V / N * N + tid < V)
+                probs[V / N * N + tid] = 0.f;
         }
-        const double target = by_sum ? p * static_cast<double>(all) : INFINITY;
+        const uint64_t order = sorted(tid < members ? lds().list[tid] : 0, members);
+        const bool mine = tid < members;
         const float l = logit_of(order);
         const double exact = mine ? weight(l) : 0.0;
-        const bool stays = mine && l > -INFINITY &&
-                           (rank == 0 || (static_cast<uint64_t>(rank) < k && static_cast<double>(before) < target && exact >= least));
-        weights = stays ? weights : 0;
-        const uint64_t total = block_reduce(weights, Sum{});  // (nobody reads the list's weights any more)
-        const double threshold = u * static_cast<double>(total);
-        const int index = static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(order));
-        if (probs && stays)
-            probs[index] = static_cast<float>(exact * unit / static_cast<double>(total));
+        uint64_t part = mine ? whole(exact) : 0;
+        const uint64_t before = block_scan(part, 0);
+        if (by_sum && all == 0)
+            all = block_reduce(static_cast<uint64_t>(tid) < k ? part : 0, Sum{}, 1);
+        const double target = by_sum ? p * static_cast<double>(all) : INFINITY;
+        const bool stays = mine && within(l, index_of(order)) &&
+                           (tid == 0 || (static_cast<uint64_t>(tid) < k && static_cast<double>(before) < target && exact >= least));
+        part = stays ? part : 0;
+        const double total = static_cast<double>(block_reduce(part, Sum{}, 1));
+        if (probs && stays)  // (the zeros are behind the barriers of that sum)
+            probs[index_of(order)] = static_cast<float>(exact * unit / total);
         if (token) {
-            if (mine)
-                lds().weights[tid] = weights;
+            // by index, each with its place among the weights
+            const int drawn = block_reduce(part > 0 ? tid + 1 : 0, Most{});
+            lds().list[tid] = part;
+            const uint64_t at = sorted(part > 0 ? order << 32 | static_cast<uint32_t>(tid) : 0, drawn);
             __syncthreads();
+            const uint64_t own = tid < drawn ? lds().list[static_cast<uint32_t>(at)] : 0;
+            const uint64_t run = block_scan(own, 0) + own;
+            const int index = index_of(at >> 32);
             int first = V, last = -1;
-            if (weights > 0) {
-                uint64_t run = 0;
-                for (int j = 0; j < members; ++j)
-                    run += static_cast<uint32_t>(lds().list[j]) >= static_cast<uint32_t>(order) ? lds().weights[j] : 0;
-                first = static_cast<double>(run) > threshold ? index : V, last = index;
-            }
-            first = block_reduce(first, Least{}), last = block_reduce(last, Most{});
-            if (tid == 0)
+            if (own > 0)
+                first = static_cast<double>(run) > u * total ? index : V, last = index;
+            first = block_reduce(first, Least{}, 1), last = block_reduce(last, Most{});
+            if (tid == 0)  // (none passes by rounding: the last one with a weight)
                 *token = first < V ? first : last;
         }
-        return true;
     }
 
     __device__ __forceinline__ void clear_bins() {
@@ -282,110 +366,85 @@ struct Sampler {
         __syncthreads();
     }
 
-    // The first bin where tokens, or their weights, reach what is asked for: k tokens (target 0), or a sum of
-    // `target` beyond `base`. False (in all threads) if none does.
-    __device__ __forceinline__ bool find_bin(uint64_t k, double target, uint64_t base, int first_count) {
-        static_assert(kBins == 2 * kThreads, "two bins a thread");
+    // The first bin where the tokens reach k of them or, where there is a target, the weights reach it; the counts
+    // and sums of the bins before it come on top of `count` and `sum`.
+    __device__ __forceinline__ bool find_bin(uint64_t k, double target, uint64_t sum, int count) {
         if (tid == 0)
             lds().bin = -1;
-        const uint64_t c0 = lds().counts[2 * tid], c1 = lds().counts[2 * tid + 1], w0 = lds().sums[2 * tid], w1 = lds().sums[2 * tid + 1];
-        uint64_t all_c, all_w;
-        uint64_t c = block_scan(c0 + c1, all_c, 0) + static_cast<uint64_t>(first_count), w = block_scan(w0 + w1, all_w, 1) + base;
+        const bool by_sum = target > 0.0;
+        uint64_t of[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            of[i] = by_sum ? lds().sums[2 * tid + i] : lds().counts[2 * tid + i];
+        uint64_t before = block_scan(of[0] + of[1], 0) + (by_sum ? sum : static_cast<uint64_t>(count));
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const uint64_t ci = i ? c1 : c0, wi = i ? w1 : w0;
-            const bool here = ci > 0 && (target > 0.0 ? static_cast<double>(w) < target && static_cast<double>(w + wi) >= target
-                                                      : c < k && c + ci >= k);
-            if (here)
-                lds().bin = 2 * tid + i, lds().before = w, lds().count_before = static_cast<int>(c);
-            c += ci, w += wi;
+            const uint64_t through = before + of[i];
+            if (by_sum ? static_cast<double>(before) < target && static_cast<double>(through) >= target : before < k && through >= k) {
+                lds().bin = 2 * tid + i, lds().before = before;
+                lds().count_before = static_cast<int>(before), lds().count_through = static_cast<int>(through);
+            }
+            before = through;
         }
         __syncthreads();
         return lds().bin >= 0;
     }
 
-    // The order of the k-th token, or of the last one with less than `target` before it; `through`: the weights
-    // up to it. The bins hold what find_bin needs.
-    __device__ __forceinline__ bool find_border(uint64_t k, double target, uint64_t &order, uint64_t &through) {
-        if (!find_bin(k, target, 0, 0))
-            return false;
+    // The order of the k-th token, or of the last one with less than `target` before it, in the bin that find_bin
+    // has found: as long as it holds more tokens than the list, it is cut into 2048 parts again, now by the order.
+    __device__ __forceinline__ uint64_t find_border(uint64_t k, double target) {
         const int level = lds().bin;
-        uint64_t base = lds().before, lo = 0, hi = ~0ull;
-        int count_before = lds().count_before, members = static_cast<int>(lds().counts[level]);
-        bool narrowed = false;
-        auto member = [&](float l, uint64_t o) { return narrowed ? o >= lo && o <= hi : bin(l) == level; };
+        const bool by_sum = target > 0.0;
+        uint64_t base = by_sum ? lds().before : 0, lo = 0, hi = ~0ull;
+        int count = by_sum ? 0 : lds().count_before;
+        int members = gather([&](float l, int i) { return bin(l) == level && within(l, i); });
+        if (members > kList) {
+            uint64_t least_o = ~0ull, most_o = 0;
+            sweep([&](float l, int i) {
+                const uint64_t o = order_of(l, i);
+                if (bin(l) == level && within(l, i))
+                    least_o = min(least_o, o), most_o = max(most_o, o);
+            });
+            lo = block_reduce(least_o, Least{}), hi = block_reduce(most_o, Most{}, 1);
+        }
         while (members > kList) {
-            if (!narrowed) {
-                uint64_t least_o = ~0ull, most_o = 0;
-                sweep([&](float l, int i) {
-                    if (bin(l) == level) {
-                        const uint64_t o = order_of(l, i);
-                        least_o = min(least_o, o), most_o = max(most_o, o);
-                    }
-                });
-                least_o = wave_reduce(least_o, Least{}), most_o = wave_reduce(most_o, Most{});
-                __syncthreads();
-                if (lane == 0)
-                    lds().scan[0][wave] = least_o, lds().scan[1][wave] = most_o;
-                __syncthreads();
-                lo = ~0ull, hi = 0;
-                for (int w = 0; w < kWaves; ++w)
-                    lo = min(lo, lds().scan[0][w]), hi = max(hi, lds().scan[1][w]);
-                narrowed = true;
-            }
-            // bins of equal width in the order, the greatest first
             int shift = 0;
             while (((hi - lo) >> shift) >= kBins)
                 ++shift;
             clear_bins();
-            sweep([&](float l, int i) {
+            sweep_ahead([&](float raw, int i) {
+                const float l = clean(raw);
                 const uint64_t o = order_of(l, i);
                 if (o >= lo && o <= hi) {
                     const int b = static_cast<int>((hi - o) >> shift);
-                    atomicAdd(&lds().counts[b], 1u);
-                    atomicAdd(reinterpret_cast<unsigned long long *>(&lds().sums[b]), whole(weight(l)));
+                    if (by_sum)
+                        add(lds().sums[b], whole(weight(l)));
+                    else
+                        atomicAdd(&lds().counts[b], 1u);
                 }
             });
             __syncthreads();
-            if (!find_bin(k, target, base, count_before))
-                return false;
-            base = lds().before, count_before = lds().count_before;
-            const int at = lds().bin;
-            members = static_cast<int>(lds().counts[at]);
-            const uint64_t most = hi - (static_cast<uint64_t>(at) << shift);
+            if (!find_bin(k, target, base, count))
+                return lo;  // (not met: the parts' sums are the bin's)
+            base = by_sum ? lds().before : 0, count = by_sum ? 0 : lds().count_before;
+            hi -= static_cast<uint64_t>(lds().bin) << shift;
             const uint64_t width = (1ull << shift) - 1;
-            lo = most - lo > width ? most - width : lo;
-            hi = most;
+            lo = hi - lo > width ? hi - width : lo;
+            members = gather([&](float l, int i) {
+                const uint64_t o = order_of(l, i);
+                return o >= lo && o <= hi;
+            });
         }
-        __syncthreads();
-        if (tid == 0)
-            lds().listed = 0;
-        __syncthreads();
-        sweep([&](float l, int i) {
-            const uint64_t o = order_of(l, i);
-            if (member(l, o)) {
-                const int at = atomicAdd(&lds().listed, 1);
-                lds().list[at] = o, lds().weights[at] = whole(weight(l));
-            }
-        });
-        __syncthreads();
+        const uint64_t own = sorted(tid < members ? lds().list[tid] : 0, members);
+        const uint64_t part = tid < members ? whole(weight(logit_of(own))) : 0;
+        const uint64_t before = base + block_scan(part, 0);
         if (tid < members) {
-            const uint64_t o = lds().list[tid], w = lds().weights[tid];
-            uint64_t before = base;
-            int rank = 0;
-            for (int j = 0; j < members; ++j) {
-                const bool ahead = lds().list[j] > o;
-                rank += ahead, before += ahead ? lds().weights[j] : 0;
-            }
-            const bool last = target > 0.0 ? static_cast<double>(before) < target &&
-                                                 (static_cast<double>(before + w) >= target || rank == members - 1)
-                                           : static_cast<uint64_t>(count_before + rank + 1) == k;
-            if (last)
-                lds().order = o, lds().through = before + w;
+            const double from = static_cast<double>(before), to = static_cast<double>(before + part);
+            if (by_sum ? from < target && (to >= target || tid == members - 1) : static_cast<uint64_t>(count + tid + 1) == k)
+                lds().order = own;
         }
         __syncthreads();
-        order = lds().order, through = lds().through;
-        return true;
+        return lds().order;
     }
 };
 
@@ -396,149 +455,151 @@ __device__ __forceinline__ double setting(const float *of_rows, double of_all, i
 template<typename Scalar>
 __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleJob job) {
     const int64_t r = blockIdx.x;
-    const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave, wave = tid / kWave, V = job.V;
+    const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave, V = job.V;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     Sampler<Scalar> me{static_cast<const Scalar *>(job.logits) + r * job.row_at, V, tid, lane, wave};
     float *probs = job.probs ? job.probs + r * V : nullptr;
+    int64_t *token = job.tokens ? job.tokens + r : nullptr;
 
-    me.top = -INFINITY, me.low = INFINITY;
-    me.template sweep<4>([&](float l, int) {
-        me.top = l > me.top ? l : me.top;
-        me.low = l > -INFINITY && l < me.low ? l : me.low;
+    if (tid < kParts)
+        lds().powers[tid] = exp2(tid * (1.0 / kParts));
+    float mine = -INFINITY, low = INFINITY;
+    me.sweep([&](float l, int) {
+        mine = l > mine ? l : mine;
+        low = l > -INFINITY && l < low ? l : low;
     });
-    const float mine = me.top;
-    me.low = wave_reduce(me.low, Least{});
-    const float top = wave_reduce(mine, Most{});
-    if (lane == 0)
-        lds().tops[wave] = top, lds().lows[wave] = me.low;
-    __syncthreads();
-    for (int w = 0; w < kWaves; ++w) {
-        me.top = w ? fmaxf(me.top, lds().tops[w]) : lds().tops[0];
-        me.low = fminf(me.low, lds().lows[w]);
-    }
+    me.top = me.block_reduce(mine, Most{});
     if (me.top == -INFINITY) {  // nothing to draw from
-        if (tid == 0 && job.tokens)
-            job.tokens[r] = 0;
+        if (tid == 0 && token)
+            *token = 0;
         for (int i = tid; probs && i < V; i += kThreads)
             probs[i] = 0.f;
         return;
     }
     const double temperature = setting(job.temperature, job.temperature_of_all, r);
+    const double p = setting(job.top_p, job.top_p_of_all, r), least = setting(job.min_p, job.min_p_of_all, r);
     int64_t k = job.top_k ? job.top_k[r] : job.top_k_of_all;
-    const double p = setting(job.top_p, job.top_p_of_all, r);
     me.rate = 1.4426950408889634074 / temperature;
-    if (!(temperature > 0.0))  // the greatest alone
-        k = 1, me.rate = 1.0;
-    const double least = setting(job.min_p, job.min_p_of_all, r);
+    if (!(temperature > 0.0))
+        me.rate = 1.0;
+    if (!(temperature > 0.0) || p <= 0.0)  // the greatest alone
+        k = 1;
+    const bool by_count = k > 0 && k < V, by_sum = p < 1.0 && k != 1;
+    const uint64_t first = by_count ? static_cast<uint64_t>(k) : static_cast<uint64_t>(V);
     me.least = least > 0.0 ? (least < 1.0 ? least : 1.0) : 0.0;
-    me.unit = job.unit;
-    const float range = me.top - me.low;
-    me.scale = range > 0.f && range < INFINITY ? static_cast<float>(kBins - 1) / range : 0.f;
-    me.border = 0;
-    const bool by_count = k > 0 && k < V, by_sum = p < 1.0;
-    const double u = job.tokens ? static_cast<double>(job.random[r]) : 0.0;
-    if (by_count ? k <= kListCount : by_sum || me.least > 0.0) {
-        float limit;
-        if (by_count || by_sum) {
-            // (for a share, some more than a language model's usually has)
-            limit = me.limit_of(mine, by_count ? static_cast<int>(k) : 256);
-        } else {
+    me.unit = job.unit, me.last_logit = -INFINITY, me.last_index = -1;
+    const double u = token ? static_cast<double>(job.random[r]) : 0.0;
+    if (by_count ? k <= kListCount : !by_sum && me.least > 0.0) {
+        float limit = me.top;
+        if (by_count && k > 1) {
+            limit = me.limit_of(mine, static_cast<int>(k));
+        } else if (!by_count) {
             // below the logit of weight min_p by more than the roundings on the way
             const double cut = static_cast<double>(me.top) + log2(me.least) / me.rate;
             limit = static_cast<float>(cut - (fabs(cut) + fabs(static_cast<double>(me.top))) * 1e-6 - 1e-37);
             limit = limit < me.top ? limit : -INFINITY;
         }
-        int members;
-        uint64_t all;
-        me.gather(limit, !by_count && by_sum, members, all);
+        const int members = me.gather([&](float l, int) { return l >= limit; });
         if (members <= kList) {
-            if (probs) {
-                constexpr int N = 4;
-                for (int i = tid * N; i < V / N * N; i += kThreads * N)
-                    store_vec<float, N>(probs + i, {});
-                if (V / N * N + tid < V)
-                    probs[V / N * N + tid] = 0.f;
-                __syncthreads();
-            }
-            if (me.finish(members, by_count ? static_cast<uint64_t>(k) : static_cast<uint64_t>(V), by_sum, p > 0.0 ? p : 0.0, all, u,
-                          job.tokens ? job.tokens + r : nullptr, probs))
-                return;
+            me.finish(members, first, by_sum, p, 0, u, token, probs);
+            return;
         }
     }
-    if (by_count || by_sum) {
+    if (by_count) {
+        const float range = me.top - me.block_reduce(low, Least{});
+        me.scale = range > 0.f && range < INFINITY ? static_cast<float>(kBins - 1) / range : 0.f;
         me.clear_bins();
-        uint64_t total = 0;
-        me.sweep([&](float l, int) {
+        me.sweep([&](float l, int) { atomicAdd(&lds().counts[me.bin(l)], 1u); });
+        __syncthreads();
+        me.find_bin(first, 0.0, 0, 0);
+        const int level = lds().bin;
+        if (lds().count_through <= kList) {
+            const int members = me.gather([&](float l, int) { return me.bin(l) <= level; });
+            me.finish(members, first, by_sum, p, 0, u, token, probs);
+            return;
+        }
+        me.end_with(me.find_border(first, 0.0));
+    }
+    if (by_sum) {
+        me.scale = static_cast<float>(me.rate) * kBinsAHalving;
+        me.clear_bins();
+        uint64_t all = 0, last = 0;
+        auto count = [&](float l) {
+            const uint64_t w = me.whole(me.weight(l));
             const int b = me.bin(l);
-            atomicAdd(&lds().counts[b], 1u);
-            if (by_sum) {
-                const uint64_t w = me.whole(me.weight(l));
-                atomicAdd(reinterpret_cast<unsigned long long *>(&lds().sums[b]), w);
-                total += w;
+            all += w;
+            if (b < kBins - 1)
+                add(lds().sums[b], w);
+            else
+                last += w;
+        };
+        if (by_count)
+            me.sweep_ahead([&](float l, int i) {
+                if (me.within(l, i))
+                    count(l);
+            });
+        else  // (a NaN has neither weight nor bin as it is)
+            me.sweep_ahead([&](float l, int) { count(l); });
+        all = me.block_reduce(all, Sum{}), last = me.block_reduce(last, Sum{}, 1);
+        if (tid == 0)
+            lds().sums[kBins - 1] = last;
+        __syncthreads();
+        const double target = p * static_cast<double>(all);
+        if (me.find_bin(0, target, 0, 0)) {
+            const int level = lds().bin;
+            // No weight is above its bin's first: a sum takes so many tokens at least. Where these fit the list, so
+            // may all of them.
+            double tokens = 0.0;
+            for (int i = tid; i <= level; i += kThreads)
+                tokens += static_cast<double>(lds().sums[i]) * exp2(i / static_cast<double>(kBinsAHalving));
+            if (me.block_reduce(tokens, Sum{}) < kList * me.unit) {
+                const int members = me.gather([&](float l, int i) { return me.bin(l) <= level && me.within(l, i); });
+                if (members <= kList) {
+                    me.finish(members, static_cast<uint64_t>(V), true, p, all, u, token, probs);
+                    return;
+                }
             }
-        });
-        uint64_t all = 0;
-        me.block_scan(total, all, 0);
-        uint64_t order = 0, through = 0;
-        if (by_count && me.find_border(static_cast<uint64_t>(k), 0.0, order, through))
-            me.border = order, all = through;
-        if (by_sum) {
-            // (a narrowed search by count has used the bins for its own)
-            if (by_count) {
-                me.clear_bins();
-                me.sweep([&](float l, int i) {
-                    if (order_of(l, i) >= me.border) {
-                        const int b = me.bin(l);
-                        atomicAdd(&lds().counts[b], 1u);
-                        atomicAdd(reinterpret_cast<unsigned long long *>(&lds().sums[b]), me.whole(me.weight(l)));
-                    }
-                });
-                __syncthreads();
-            }
-            const double target = p > 0.0 ? p * static_cast<double>(all) : 0.0;
-            if (!(target > 0.0)) {
-                if (me.find_border(1, 0.0, order, through))
-                    me.border = order > me.border ? order : me.border;
-            } else if (me.find_border(0, target, order, through)) {
-                me.border = order > me.border ? order : me.border;
-            }
+            me.end_with(me.find_border(0, target));
         }
     }
     // The kept weights by stretches of the vocabulary, a wave each, in order of the index: whole pieces of 16 bytes,
     // and for the last wave the row's last few elements
-    constexpr int N = 16 / sizeof(Scalar), kDeep = 2;
+    constexpr int N = 16 / sizeof(Scalar);
     const int full = V / N * N, part = (V + kWaves * N - 1) / (kWaves * N) * N;
     const int lo = min(wave * part, full), hi = min(lo + part, full);
-    uint64_t sum = 0;
-    for (int at = lo + lane * N; at < hi; at += kDeep * kWave * N) {
-        Vec<Scalar, N> x[kDeep];
-#pragma unroll
-        for (int i = 0; i < kDeep; ++i)
-            x[i] = at + i * kWave * N < hi ? load_vec<Scalar, N>(me.row + at + i * kWave * N) : Vec<Scalar, N>{};
-#pragma unroll
-        for (int i = 0; i < kDeep; ++i) {
-            if (at + i * kWave * N < hi) {
-#pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    double w;
-                    sum += me.kept(me.clean(x[i][e]), at + i * kWave * N + e, w) ? me.whole(w) : 0;
-                }
-            }
-        }
-    }
-    if (wave == kWaves - 1 && full + lane < V) {
+    auto share = [&](float l, int i) -> uint64_t {
         double w;
-        sum += me.kept(me.clean(load_f32(me.row + full + lane)), full + lane, w) ? me.whole(w) : 0;
-    }
+        return me.kept(l, i, w) ? me.whole(w) : 0;
+    };
+    uint64_t sum = wave == kWaves - 1 && full + lane < V ? share(load_f32(me.row + full + lane), full + lane) : 0;
+    auto stretch = [&](auto of) {
+        Vec<Scalar, N> next{};
+        if (lo + lane * N < hi)
+            next = load_vec<Scalar, N>(me.row + lo + lane * N);
+        for (int at = lo + lane * N; at < hi; at += kWave * N) {
+            const Vec<Scalar, N> x = next;
+            if (at + kWave * N < hi)
+                next = load_vec<Scalar, N>(me.row + at + kWave * N);
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                sum += of(x[e], at + e);
+        }
+    };
+    if (!by_count && !by_sum && me.least == 0.0)
+        stretch([&](float l, int) { return me.whole(me.weight(l)); });
+    else
+        stretch(share);
     sum = wave_reduce(sum, Sum{});
     __syncthreads();
     if (lane == 0)
         lds().scan[0][wave] = sum;
     __syncthreads();
-    uint64_t total = 0;
+    uint64_t parts = 0;
     for (int w = 0; w < kWaves; ++w)
-        total += lds().scan[0][w];
-    if (job.tokens) {
-        const double threshold = u * static_cast<double>(total);
+        parts += lds().scan[0][w];
+    const double total = static_cast<double>(parts);
+    if (token) {
+        const double threshold = u * total;
         uint64_t seen = 0, before = 0;
         int at = 0;
         for (int w = 0; w < kWaves; ++w) {
@@ -552,32 +613,28 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleJob job) {
         }
         const int from = min(at * part, full), to = at == kWaves - 1 ? V : min(from + part, full);
         const int each = (to - from + kThreads - 1) / kThreads, begin = min(from + tid * each, to), end = min(begin + each, to);
-        uint64_t mine = 0;
-        for (int i = begin; i < end; ++i) {
-            double w;
-            mine += me.kept(me.clean(load_f32(me.row + i)), i, w) ? me.whole(w) : 0;
-        }
-        uint64_t all;
-        uint64_t run = before + me.block_scan(mine, all, 1);
+        uint64_t own = 0;
+        for (int i = begin; i < end; ++i)
+            own += share(load_f32(me.row + i), i);
+        uint64_t run = before + me.block_scan(own, 1);
         int found = V, last = -1;
         for (int i = begin; i < end && found == V; ++i) {
-            double w;
-            const uint64_t x = me.kept(me.clean(load_f32(me.row + i)), i, w) ? me.whole(w) : 0;
+            const uint64_t x = share(load_f32(me.row + i), i);
             run += x;
             if (x > 0) {
                 last = i;
                 found = static_cast<double>(run) > threshold ? i : V;
             }
         }
-        found = me.block_reduce(found, Least{}), last = me.block_reduce(last, Most{});
+        found = me.block_reduce(found, Least{}), last = me.block_reduce(last, Most{}, 1);
         if (tid == 0)
-            job.tokens[r] = found < V ? found : last;
+            *token = found < V ? found : last;
     }
     if (probs) {
-        const double inv = me.unit / static_cast<double>(total);
+        const double inv = me.unit / total;
         auto value = [&](float l, int i) {
             double w;
-            return me.kept(me.clean(l), i, w) ? static_cast<float>(w * inv) : 0.f;
+            return me.kept(l, i, w) ? static_cast<float>(w * inv) : 0.f;
         };
         for (int at = tid * N; at < full; at += kThreads * N) {
             const Vec<Scalar, N> x = load_vec<Scalar, N>(me.row + at);
