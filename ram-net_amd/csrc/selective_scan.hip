@@ -67,7 +67,7 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(const ScanJob job) {
         const ScanRows<Scalar> x_rows(at, job.x_at[1], true), dt_rows(at, job.dt_at[1], true), gate_rows(at, job.gate_at[1], true),
             y_rows(at, job.D, at.valid);
         const Groups B_rows(lane, job.B_at[1], job.S), C_rows(lane, job.C_at[1], job.S);
-        uint32_t xs[kQuads], ds[kQuads], gs[kQuads], Bs[NR], Cs[NR];
+        uint32_t xs[kQuads], ds[kQuads], gs[kQuads], Bs[Groups::kLoads], Cs[Groups::kLoads];
         auto load = [&](int t) {
             const int left = piece.len - t;
             dt_rows.load(ds, dt_rows.over(job.dt, dr + (token + t) * job.dt_at[1], job.dt_at[1], job.D, left));
@@ -151,9 +151,9 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(const ScanJob job) {
         if (piece.len > 0)
             load(0);
         for (int t = 0, turn = 0; t < piece.len; t += kTile, turn ^= 1) {
-            Groups::store(tile[turn], Bs, lane);
+            B_rows.store(tile[turn], Bs);
             if constexpr (kMode == kWhole)
-                Groups::store(tile[turn] + Groups::kFloats, Cs, lane);
+                C_rows.store(tile[turn] + Groups::kFloats, Cs);
             wave_sync();
             if (kMode == kWhole && job.kept && at.valid) {
                 store_states<NR>(kept, h, NR);
@@ -265,8 +265,11 @@ hipError_t launch_type(const ScanJob &job, hipStream_t stream) {
     switch (scan_lane_states(job.S)) {
         case 1: return launch_states<Scalar, 1>(job, stream);
         case 2: return launch_states<Scalar, 2>(job, stream);
+        case 3: return launch_states<Scalar, 3>(job, stream);
         case 4: return launch_states<Scalar, 4>(job, stream);
+        case 6: return launch_states<Scalar, 6>(job, stream);
         case 8: return launch_states<Scalar, 8>(job, stream);
+        case 12: return launch_states<Scalar, 12>(job, stream);
         default: return launch_states<Scalar, 16>(job, stream);
     }
 }
@@ -275,13 +278,16 @@ hipError_t launch_type(const ScanJob &job, hipStream_t stream) {
 
 bool scan_is_step(const ScanJob &job) { return !job.seq.cu && !job.kept && job.seq.T <= kScanStepTokens; }
 
-// Rows are cut into pieces where their channels alone leave compute units idle: the state after each
-// piece from zeros is a pass of its own, of five sixths of the work, so that two pieces of a row
-// take about as long as the row in one, and more than two less.
-int scan_step_tokens(const ScanJob &job) {
+// Rows are cut into pieces where their channels alone leave compute units idle. The state after each piece from zeros
+// is a pass of its own that costs two thirds of the other, so a row in many pieces takes as long as 1.35 in one do
+// where the waves of either fill the machine: 4096 tokens of 1024 waves take 395 us in one piece, 550 in two
+// (336 + 230) and 515 in four. From 768 waves on, three quarters of what runs at once, rows stay whole. Below that
+// 4096 waves (four a SIMD) hide each other's latencies: 32768 tokens of 64 waves take 277 us in 32 pieces, 266 in 64.
+// The backward has registers for two waves a SIMD, and keeps to 2048.
+int scan_step_tokens(const ScanJob &job, bool backward) {
     const int64_t rows = job.seq.B > 0 ? job.seq.B : 1;
-    const int64_t waves = rows * job.G * ((job.D / job.G + 15) / 16);
-    const int64_t parts = waves >= 1024 ? 1 : (2048 + waves - 1) / waves;
+    const int64_t waves = rows * job.G * ((job.D / job.G + 15) / 16), most = backward ? 2048 : 4096;
+    const int64_t parts = waves >= 768 ? 1 : (most + waves - 1) / waves;
     const int64_t tokens = (job.seq.T + parts - 1) / parts;
     const int64_t step = (tokens + kScanKept - 1) / kScanKept * kScanKept;
     return static_cast<int>(step < 64 ? 64 : step);
@@ -296,7 +302,7 @@ int64_t scan_layout(ScanJob &job, bool backward, char *base, ScanGrads *grads) {
     };
     if (!backward && scan_is_step(job))
         return 0;
-    job.step = scan_step_tokens(job);
+    job.step = scan_step_tokens(job, backward);
     const int64_t pieces = most_pieces(job.seq, job.step), wide = 4LL * scan_lane_states(job.S);
     if (job.seq.cu) {
         job.seq.bounds = reinterpret_cast<int32_t *>(region((job.seq.N + 1) * 4LL));

@@ -4,7 +4,7 @@
 //     dt = softplus(raw + dt_bias)          (or raw + dt_bias)
 //     h_n <- e^(dt A_dn) h_n + dt x B_gn;   s = sum_n C_gn h_n + skip x;   y = s silu(gate)   (or s)
 //
-// Four adjacent lanes hold a channel, NR = S / 4 (rounded up to 1, 2, 4, 8 or 16) states each; a wave
+// Four adjacent lanes hold a channel, NR = S / 4 (rounded up to 1, 2, 3, 4, 6, 8, 12 or 16) states each; a wave
 // holds 16 channels. Tokens are taken four at a time: what a token needs once (its softplus, its gate)
 // is done by one of the four lanes, and given to the others within vector instructions.
 #pragma once
@@ -51,7 +51,13 @@ struct ScanGrads {
     float *sums;     // [piece][D][4 NR + 2] sums of dA, dskip and dbias over the piece's tokens
 };
 
-__host__ __device__ inline int scan_lane_states(int S) { return S <= 4 ? 1 : S <= 8 ? 2 : S <= 16 ? 4 : S <= 32 ? 8 : 16; }
+// NR of S states.
+__host__ __device__ inline int scan_lane_states(int S) {
+    for (const int states : {1, 2, 3, 4, 6, 8, 12})
+        if (S <= 4 * states)
+            return states;
+    return 16;
+}
 
 // The place of a sequence's kept states: sequence `seq` from token lo on, one for every kScanKept tokens.
 __host__ __device__ inline int64_t scan_slot(const SequenceJob &job, int seq, int lo) {
@@ -124,6 +130,11 @@ struct ScanPlace {
     }
 };
 
+__device__ __forceinline__ int anew(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
 // One value of a lane's channel for each four tokens of a tile, through a window over the tile's tokens that
 // are there.
 template<typename Scalar>
@@ -137,10 +148,13 @@ struct ScanRows {
     __device__ static __forceinline__ __amdgpu_buffer_rsrc_t over(const void *p, int64_t from, int64_t stride, int D, int tokens) {
         return window(static_cast<const Scalar *>(p) + from, ((min(tokens, kScanKept) - 1) * stride + D) * static_cast<int>(sizeof(Scalar)));
     }
+    // (kAnew: offsets are made for each load; kept over a loop they fill registers)
+    template<bool kAnew = false>
     __device__ __forceinline__ void load(uint32_t (&to)[kScanKept / 4], __amdgpu_buffer_rsrc_t rows) const {
+        const int from = kAnew ? anew(at) : at;
 #pragma unroll
         for (int g = 0; g < kScanKept / 4; ++g)
-            to[g] = buffer_bits<Scalar>(rows, at + g * step);
+            to[g] = buffer_bits<Scalar>(rows, from + g * step);
     }
 };
 
@@ -148,22 +162,30 @@ struct ScanRows {
 template<typename Scalar, int NR>
 struct ScanGroups {
     static constexpr int kRow = 4 * NR, kFloats = kScanKept * kRow;
-    static constexpr int kSpan = kWave / kRow;  // tokens that a load of the wave spans
-    int at, step;
+    // tokens that a load of the wave spans (lanes past them have no part), and loads of a tile
+    static constexpr int kSpan = kWave / kRow >= 4 ? kWave / kRow / 4 * 4 : kWave / kRow >= 2 ? 2 : 1, kLoads = kScanKept / kSpan;
+    static_assert(kLoads * kSpan == kScanKept, "whole loads");
+    int at, step, to;
 
     __device__ __forceinline__ ScanGroups(int lane, int64_t stride, int S) {
+        const bool on = lane / kRow < kSpan;
         step = kSpan * static_cast<int>(stride) * static_cast<int>(sizeof(Scalar));
-        at = lane % kRow < S ? (lane / kRow * static_cast<int>(stride) + lane % kRow) * static_cast<int>(sizeof(Scalar)) : kNowhere;
+        at = on && lane % kRow < S ? (lane / kRow * static_cast<int>(stride) + lane % kRow) * static_cast<int>(sizeof(Scalar)) : kNowhere;
+        to = on ? lane : -1;
     }
-    __device__ __forceinline__ void load(uint32_t (&to)[NR], __amdgpu_buffer_rsrc_t rows) const {
+    template<bool kAnew = false>
+    __device__ __forceinline__ void load(uint32_t (&to)[kLoads], __amdgpu_buffer_rsrc_t rows) const {
+        const int from = kAnew ? anew(at) : at;
 #pragma unroll
-        for (int i = 0; i < NR; ++i)
-            to[i] = buffer_bits<Scalar>(rows, at + i * step);
+        for (int i = 0; i < kLoads; ++i)
+            to[i] = buffer_bits<Scalar>(rows, from + i * step);
     }
-    __device__ static __forceinline__ void store(float *to, const uint32_t (&from)[NR], int lane) {
+    __device__ __forceinline__ void store(float *tile, const uint32_t (&from)[kLoads]) const {
+        if (kSpan * kRow == kWave || to >= 0) {
 #pragma unroll
-        for (int i = 0; i < NR; ++i)
-            to[i * kWave + lane] = bits_f32<Scalar>(from[i]);
+            for (int i = 0; i < kLoads; ++i)
+                tile[i * kSpan * kRow + to] = bits_f32<Scalar>(from[i]);
+        }
     }
 };
 

@@ -13,7 +13,7 @@ namespace ramnet {
 
 namespace {
 
-constexpr int kThreads = 256, kWaves = kThreads / kWave, kChannels = kThreads / 4, kTile = kScanKept;
+constexpr int kThreads = kScanThreads, kWaves = kThreads / kWave, kTile = kScanKept, kQuads = kTile / 4;
 
 template<int CONTROL, int BANKS>
 __device__ __forceinline__ float row_move(float old, float x) {
@@ -43,63 +43,6 @@ __device__ __forceinline__ float channel_sums(float (&v)[16], int lane) {
     return keep + row_move<0x114, 0xA>(up, give);           // row_shr:4, lanes with it
 }
 
-// Which channel a lane holds a quarter of; where there is none, the group's last one, which it does not write.
-struct BackPlace {
-    int piece, group, channel, sub, block;
-    bool valid;
-
-    __device__ __forceinline__ BackPlace(const ScanJob &job) {
-        const int wide = job.D / job.G, per_group = (wide + kChannels - 1) / kChannels;
-        const int id = static_cast<int>(blockIdx.x), per_piece = per_group * job.G;
-        piece = id / per_piece;
-        const int at = id - piece * per_piece;
-        group = at / per_group;
-        block = at - group * per_group;
-        const int c = block * kChannels + static_cast<int>(threadIdx.x) / 4;
-        valid = c < wide;
-        channel = group * wide + min(c, wide - 1);
-        sub = static_cast<int>(threadIdx.x) % 4;
-    }
-};
-
-// What a lane reads of a tile: its channel's values of one token of each four, and its share of B and C.
-template<typename Scalar, int NR>
-struct BackTile {
-    static constexpr int kRow = 8 * NR, kFloats = kTile * kRow, kLoads = kFloats / kWave;
-    uint32_t x[kTile / 4], dt[kTile / 4], gate[kTile / 4], dy[kTile / 4], groups[kLoads];
-
-    __device__ __forceinline__ void load(const ScanJob &job, const ScanGrads &grads, const TimePiece &piece,
-                                         const BackPlace &at, int t, int lane, bool with_b) {
-        const int64_t row = piece.row;
-#pragma unroll
-        for (int g = 0; g < kTile / 4; ++g) {
-            const int64_t token = piece.t0 + min(t + 4 * g + at.sub, piece.len - 1);
-            auto value = [&](const void *p, const int64_t *stride) {
-                return load_bits(static_cast<const Scalar *>(p) + row * stride[0] + token * stride[1] + at.channel);
-            };
-            x[g] = with_b ? value(job.x, job.x_at) : 0u;
-            dt[g] = value(job.dt, job.dt_at);
-            gate[g] = job.gate ? value(job.gate, job.gate_at) : 0u;
-            dy[g] = value(grads.dy, grads.dy_at);
-        }
-        const Scalar *B = static_cast<const Scalar *>(job.B) + row * job.B_at[0] + at.group * job.B_at[2];
-        const Scalar *C = static_cast<const Scalar *>(job.C) + row * job.C_at[0] + at.group * job.C_at[2];
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int e = i * kWave + lane, n = e % (4 * NR);
-            const int64_t token = piece.t0 + min(t + e / kRow, piece.len - 1);
-            const bool second = e % kRow >= 4 * NR;
-            groups[i] = n < job.S && (second || with_b)
-                            ? load_bits(second ? C + token * job.C_at[1] + n : B + token * job.B_at[1] + n) : 0u;
-        }
-    }
-    __device__ __forceinline__ void store_groups(float *to, int lane) const {
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i)
-            to[i * kWave + lane] = bits_f32<Scalar>(groups[i]);
-    }
-};
-
 // A decay of -inf is held to a finite one: times a dt of 0 (of a token that does not count) it gives 1.
 template<int NR>
 __device__ __forceinline__ void load_decays(float (&A2)[NR], const ScanJob &job, int channel, int n0) {
@@ -115,14 +58,14 @@ __device__ __forceinline__ void load_decays(float (&A2)[NR], const ScanJob &job,
 // its dt.
 template<typename Scalar, int NR>
 __global__ __launch_bounds__(kThreads) void scan_backs_kernel(const ScanJob job, const ScanGrads grads) {
-    using Tile = BackTile<Scalar, NR>;
-    __shared__ __align__(16) float lds[kWaves][2][Tile::kFloats];
-    const BackPlace at(job);
+    using Groups = ScanGroups<Scalar, NR>;
+    __shared__ __align__(16) float lds[kWaves][2][Groups::kFloats];
+    const ScanPlace at(job);
     TimePiece piece;
     if (!time_piece(job.seq, job.step, at.piece, piece) || piece.seq < 0 || piece.at == 0 || piece.len == 0)
         return;
     const int lane = static_cast<int>(threadIdx.x) % kWave, sub = at.sub, n0 = sub * NR;
-    float(*tile)[Tile::kFloats] = lds[threadIdx.x / kWave];
+    float(*tile)[Groups::kFloats] = lds[threadIdx.x / kWave];
     float A2[NR], carry[NR];
     load_decays<NR>(A2, job, at.channel, n0);
 #pragma unroll
@@ -130,34 +73,62 @@ __global__ __launch_bounds__(kThreads) void scan_backs_kernel(const ScanJob job,
         carry[j] = 0.f;
     const float bias = job.bias ? job.bias[at.channel] : 0.f;
     double span = 0.0;
-    Tile next;
+    const int64_t token = piece.t0, dr = piece.row * job.dt_at[0], gr = piece.row * job.gate_at[0],
+                  yr = piece.row * grads.dy_at[0], Cr = piece.row * job.C_at[0] + at.group * job.C_at[2];
+    const ScanRows<Scalar> dt_rows(at, job.dt_at[1], true), gate_rows(at, job.gate_at[1], true), dy_rows(at, grads.dy_at[1], true);
+    const Groups C_rows(lane, job.C_at[1], job.S);
+    uint32_t dts[kQuads], gates[kQuads], dys[kQuads], Cs[Groups::kLoads];
+    auto load = [&](int t) {
+        const int left = piece.len - t;
+        dt_rows.load(dts, dt_rows.over(job.dt, dr + (token + t) * job.dt_at[1], job.dt_at[1], job.D, left));
+        dy_rows.load(dys, dy_rows.over(grads.dy, yr + (token + t) * grads.dy_at[1], grads.dy_at[1], job.D, left));
+        if (job.gate)
+            gate_rows.load(gates, gate_rows.over(job.gate, gr + (token + t) * job.gate_at[1], job.gate_at[1], job.D, left));
+        C_rows.load(Cs, dt_rows.over(job.C, Cr + (token + t) * job.C_at[1], job.C_at[1], job.S, left));
+    };
     int t = (piece.len - 1) / kTile * kTile;
-    next.load(job, grads, piece, at, t, lane, false);
+    load(t);
     for (int turn = 0; t >= 0; t -= kTile, turn ^= 1) {
-        float dv[kTile / 4], ds[kTile / 4];
+        float dv[kQuads], sv[kQuads];
 #pragma unroll
-        for (int g = 0; g < kTile / 4; ++g) {
-            const bool live = t + 4 * g + sub < piece.len;
-            const float raw = bits_f32<Scalar>(next.dt[g]) + bias, z = bits_f32<Scalar>(next.gate[g]);
-            float e;
-            dv[g] = live ? (job.softplus ? softplus(raw, e) : raw) : 0.f;
-            ds[g] = bits_f32<Scalar>(next.dy[g]) * (job.gate ? z * sigmoid(z) : 1.f);
-            ds[g] = live ? ds[g] : 0.f;
+        for (int g = 0; g < kQuads; ++g) {
+            dv[g] = bits_f32<Scalar>(dts[g]) + bias, sv[g] = bits_f32<Scalar>(dys[g]);
+            if (job.softplus) {
+                float e;
+                dv[g] = softplus(dv[g], e);
+            }
+            if (job.gate) {
+                const float z = bits_f32<Scalar>(gates[g]);
+                sv[g] *= z * sigmoid(z);
+            }
+            const bool live = t + 4 * g + sub < piece.len;  // (rows may lie on each other: what is past the end may be read)
+            dv[g] = live ? dv[g] : 0.f, sv[g] = live ? sv[g] : 0.f;
             span += static_cast<double>(dv[g]);
         }
-        next.store_groups(tile[turn], lane);
+        C_rows.store(tile[turn], Cs);
         wave_sync();
         if (t > 0)
-            next.load(job, grads, piece, at, t - kTile, lane, false);
+            load(t - kTile);
+        float c[2][4][NR];
+        auto fetch = [&](int g) {
 #pragma unroll
-        for (int g = kTile / 4 - 1; g >= 0; --g) {
-            auto token = [&](auto k_) {
-                constexpr int k = decltype(k_)::value;
-                const float d = quad_lane<k>(dv[g]), s = quad_lane<k>(ds[g]);
-                const float *c = tile[turn] + (4 * g + k) * Tile::kRow + 4 * NR + n0;
+            for (int k = 0; k < 4; ++k)
 #pragma unroll
                 for (int j = 0; j < NR; ++j)
-                    carry[j] = __builtin_amdgcn_exp2f(d * A2[j]) * fmaf(c[j], s, carry[j]);
+                    c[g & 1][k][j] = tile[turn][(4 * g + k) * Groups::kRow + n0 + j];
+        };
+        fetch(kQuads - 1);
+#pragma unroll
+        for (int g = kQuads - 1; g >= 0; --g) {
+            if (g > 0)
+                fetch(g - 1);
+            __builtin_amdgcn_sched_barrier(0);
+            auto token = [&](auto k_) {
+                constexpr int k = decltype(k_)::value;
+                const float d = quad_lane<k>(dv[g]), s = quad_lane<k>(sv[g]);
+#pragma unroll
+                for (int j = 0; j < NR; ++j)
+                    carry[j] = __builtin_amdgcn_exp2f(d * A2[j]) * fmaf(c[g & 1][k][j], s, carry[j]);
             };
             token(std::integral_constant<int, 3>{});
             token(std::integral_constant<int, 2>{});
@@ -174,25 +145,34 @@ __global__ __launch_bounds__(kThreads) void scan_backs_kernel(const ScanJob job,
     }
 }
 
-template<typename Scalar, int NR>
-__global__ __launch_bounds__(kThreads) void scan_backward_kernel(const ScanJob job, const ScanGrads grads) {
-    using Tile = BackTile<Scalar, NR>;
-    // Tokens whose decays fit the registers; a tile is walked in so many parts.
-    constexpr int kPart = NR <= 4 ? kTile : 4 * kTile / NR, kParts = kTile / kPart;
-    __shared__ __align__(16) float lds[kWaves][Tile::kFloats], out[kWaves][Tile::kFloats];
-    const BackPlace at(job);
+// What is read from LDS before is not kept in registers for after: B and C of a whole tile would fill them.
+__device__ __forceinline__ void reread() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// Tokens whose decays fit the registers beside the rest: a tile is walked in parts of so many, and but for the last
+// one twice. (16 states, 4 x 2048 x 2048 channels: parts of 16 spill, 545 us; of 8 283, of 4 280.)
+template<int NR>
+constexpr int scan_part() { return NR <= 2 ? kTile : NR <= 4 ? kTile / 2 : kTile / 4; }
+
+template<typename Scalar, int NR, bool kGate>
+__global__ __launch_bounds__(kThreads, 2) void scan_backward_kernel(const ScanJob job, const ScanGrads grads) {
+    using Groups = ScanGroups<Scalar, NR>;
+    constexpr int kPart = scan_part<NR>(), kParts = kTile / kPart, kRow = Groups::kRow, kFloats = Groups::kFloats;
+    constexpr int kSpread = 2 * kRow;  // dB and dC of a token
+    __shared__ __align__(16) float lds[kWaves][2 * kFloats], out[2][kWaves][2 * kFloats];
+    const ScanPlace at(job);
     TimePiece piece;
     if (!time_piece(job.seq, job.step, at.piece, piece))
         return;
-    const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave, wave = tid / kWave, sub = at.sub, n0 = sub * NR;
+    const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave, sub = at.sub, n0 = sub * NR;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int channel = at.channel, D = job.D;
-    const int64_t wide = static_cast<int64_t>(D) * 4 * NR, mine = static_cast<int64_t>(channel) * 4 * NR + n0;
+    const int64_t wide = static_cast<int64_t>(D) * kRow, mine = static_cast<int64_t>(channel) * kRow + n0;
     const int64_t row = static_cast<int64_t>(piece.row) * job.seq.T + piece.t0;
-    Scalar *dx = static_cast<Scalar *>(grads.dx) + row * D + channel;
-    Scalar *ddt = static_cast<Scalar *>(grads.ddt) + row * D + channel;
-    Scalar *dgate = job.gate ? static_cast<Scalar *>(grads.dgate) + row * D + channel : nullptr;
     const int64_t tokens = static_cast<int64_t>(job.seq.B) * job.seq.T;
-    float *groups = grads.groups + ((at.block * tokens + row) * job.G + at.group) * Tile::kRow;
+    float *groups = grads.groups + ((at.block * tokens + row) * job.G + at.group) * kSpread;
     float dA[NR], dskip = 0.f, dbias = 0.f;
 #pragma unroll
     for (int j = 0; j < NR; ++j)
@@ -217,36 +197,56 @@ __global__ __launch_bounds__(kThreads) void scan_backward_kernel(const ScanJob j
         }
         const float bias = job.bias ? job.bias[channel] : 0.f, skip = job.skip ? job.skip[channel] : 0.f;
         const float *kept = job.kept + (scan_slot(job.seq, piece.seq, piece.lo) + (piece.t0 - piece.lo) / kScanKept) * wide + mine;
-        Tile next;
-        int t = (piece.len - 1) / kTile * kTile;
-        if (piece.len > 0) {
-            next.load(job, grads, piece, at, t, lane, true);
+        const int64_t token = piece.t0, xr = piece.row * job.x_at[0], dr = piece.row * job.dt_at[0],
+                      gr = piece.row * job.gate_at[0], yr = piece.row * grads.dy_at[0],
+                      Br = piece.row * job.B_at[0] + at.group * job.B_at[2], Cr = piece.row * job.C_at[0] + at.group * job.C_at[2];
+        // (lanes without a channel read an x and a dy of 0, and so add nothing to the sums over channels)
+        const ScanRows<Scalar> x_rows(at, job.x_at[1], at.valid), dt_rows(at, job.dt_at[1], true), gate_rows(at, job.gate_at[1], true),
+            dy_rows(at, grads.dy_at[1], at.valid), d_rows(at, D, at.valid);
+        const Groups B_rows(lane, job.B_at[1], job.S), C_rows(lane, job.C_at[1], job.S);
+        uint32_t xs[kQuads], dts[kQuads], gates[kQuads], dys[kQuads], Bs[Groups::kLoads], Cs[Groups::kLoads];
+        auto load = [&](int t) {
+            const int left = piece.len - t;
+            dt_rows.template load<true>(dts, dt_rows.over(job.dt, dr + (token + t) * job.dt_at[1], job.dt_at[1], D, left));
+            x_rows.template load<true>(xs, x_rows.over(job.x, xr + (token + t) * job.x_at[1], job.x_at[1], D, left));
+            dy_rows.template load<true>(dys, dy_rows.over(grads.dy, yr + (token + t) * grads.dy_at[1], grads.dy_at[1], D, left));
+            if constexpr (kGate)
+                gate_rows.template load<true>(gates, gate_rows.over(job.gate, gr + (token + t) * job.gate_at[1], job.gate_at[1], D, left));
+            B_rows.template load<true>(Bs, dt_rows.over(job.B, Br + (token + t) * job.B_at[1], job.B_at[1], job.S, left));
+            C_rows.template load<true>(Cs, dt_rows.over(job.C, Cr + (token + t) * job.C_at[1], job.C_at[1], job.S, left));
             load_states<NR>(h_next, kept + t / kTile * wide, NR);
-        }
-        for (; piece.len > 0 && t >= 0; t -= kTile) {
-            float xv[kTile / 4], dv[kTile / 4], ev[kTile / 4], rv[kTile / 4], zv[kTile / 4], gv[kTile / 4], sv[kTile / 4];
+        };
+        int t = (piece.len - 1) / kTile * kTile;
+        if (piece.len > 0)
+            load(t);
+        for (int turn = 0; piece.len > 0 && t >= 0; t -= kTile, turn ^= 1) {
+            float xv[kQuads], dv[kQuads], ev[kQuads], rv[kQuads], zv[kQuads], gv[kQuads], sv[kQuads];
 #pragma unroll
-            for (int g = 0; g < kTile / 4; ++g) {
+            for (int g = 0; g < kQuads; ++g) {
                 const bool live = t + 4 * g + sub < piece.len;
-                const float raw = bits_f32<Scalar>(next.dt[g]) + bias;
-                float e = 0.f;
-                const float d = job.softplus ? softplus(raw, e) : raw;
-                xv[g] = live ? bits_f32<Scalar>(next.x[g]) : 0.f;
-                dv[g] = live ? d : 0.f, ev[g] = e, rv[g] = raw;
-                zv[g] = bits_f32<Scalar>(next.gate[g]);
-                gv[g] = live ? bits_f32<Scalar>(next.dy[g]) : 0.f;            // gradient of y
-                sv[g] = job.gate ? gv[g] * zv[g] * sigmoid(zv[g]) : gv[g];    // of s
-                sv[g] = live ? sv[g] : 0.f;
+                rv[g] = bits_f32<Scalar>(dts[g]) + bias, ev[g] = 0.f;
+                const float d = job.softplus ? softplus(rv[g], ev[g]) : rv[g];
+                dv[g] = live ? d : 0.f;
+                xv[g] = live ? bits_f32<Scalar>(xs[g]) : 0.f;
+                gv[g] = live ? bits_f32<Scalar>(dys[g]) : 0.f;  // gradient of y
+                sv[g] = gv[g];                                  // of s
+                if constexpr (kGate) {
+                    zv[g] = bits_f32<Scalar>(gates[g]);
+                    sv[g] = live ? gv[g] * zv[g] * sigmoid(zv[g]) : 0.f;
+                }
             }
 #pragma unroll
             for (int j = 0; j < NR; ++j)
                 h[j] = h_next[j];
-            next.store_groups(lds[wave], lane);
+            B_rows.store(lds[wave], Bs);
+            C_rows.store(lds[wave] + kFloats, Cs);
             wave_sync();
-            if (t > 0) {
-                next.load(job, grads, piece, at, t - kTile, lane, true);
-                load_states<NR>(h_next, kept + (t / kTile - 1) * wide, NR);
-            }
+            if (t > 0)
+                load(t - kTile);
+            const int left = piece.len - t;
+            const int64_t first = (row + t) * D;
+            const auto dx_rows = d_rows.over(grads.dx, first, D, D, left), ddt_rows = d_rows.over(grads.ddt, first, D, D, left);
+            const auto dgate_rows = d_rows.over(kGate ? grads.dgate : grads.dx, first, D, D, left);
             // the states before each part of the tile
             float from[kParts][NR];
 #pragma unroll
@@ -257,11 +257,12 @@ __global__ __launch_bounds__(kThreads) void scan_backward_kernel(const ScanJob j
                 if (part + 1 < kParts) {
 #pragma unroll
                     for (int g = part * kPart / 4; g < (part + 1) * kPart / 4; ++g) {
+                        reread();
                         const float ux = dv[g] * xv[g];
                         auto token = [&](auto k_) {
                             constexpr int k = decltype(k_)::value;
                             const float d = quad_lane<k>(dv[g]), u = quad_lane<k>(ux);
-                            const float *b = lds[wave] + (4 * g + k) * Tile::kRow + n0;
+                            const float *b = lds[wave] + (4 * g + k) * kRow + n0;
 #pragma unroll
                             for (int j = 0; j < NR; ++j)
                                 h[j] = fmaf(__builtin_amdgcn_exp2f(d * A2[j]), h[j], u * b[j]);
@@ -275,47 +276,55 @@ __global__ __launch_bounds__(kThreads) void scan_backward_kernel(const ScanJob j
             }
 #pragma unroll
             for (int part = kParts - 1; part >= 0; --part) {
+#pragma unroll
+                for (int j = 0; j < NR; ++j)  // (nor are the decays of the parts to come)
+                    asm volatile("" : "+v"(A2[j]));
                 float a[kPart][NR], ah[kPart][NR], ys[kPart / 4];
 #pragma unroll
                 for (int j = 0; j < NR; ++j)
                     h[j] = from[part][j];
 #pragma unroll
                 for (int i = 0; i < kPart / 4; ++i) {
+                    reread();
                     const int g = part * kPart / 4 + i;
                     const float ux = dv[g] * xv[g];
                     float sums[4];
                     auto token = [&](auto k_) {
                         constexpr int k = decltype(k_)::value;
                         const float d = quad_lane<k>(dv[g]), u = quad_lane<k>(ux);
-                        const float *b = lds[wave] + (4 * g + k) * Tile::kRow + n0, *c = b + 4 * NR;
+                        const float *b = lds[wave] + (4 * g + k) * kRow + n0, *c = b + kFloats;
                         sums[k] = 0.f;
 #pragma unroll
                         for (int j = 0; j < NR; ++j) {
                             a[4 * i + k][j] = __builtin_amdgcn_exp2f(d * A2[j]);
                             ah[4 * i + k][j] = a[4 * i + k][j] * h[j];
                             h[j] = fmaf(u, b[j], ah[4 * i + k][j]);
-                            sums[k] = fmaf(c[j], h[j], sums[k]);
+                            if constexpr (kGate)
+                                sums[k] = j ? fmaf(c[j], h[j], sums[k]) : c[j] * h[j];
                         }
                     };
                     token(std::integral_constant<int, 0>{});
                     token(std::integral_constant<int, 1>{});
                     token(std::integral_constant<int, 2>{});
                     token(std::integral_constant<int, 3>{});
-                    ys[i] = quad_sums(sums, sub);
+                    if constexpr (kGate)
+                        ys[i] = quad_sums(sums, sub);
                 }
                 float sums[16] = {};  // of dB and dC, as many tokens of a group as it holds
 #pragma unroll
                 for (int i = kPart / 4 - 1; i >= 0; --i) {
+                    reread();
                     const int g = part * kPart / 4 + i;
                     const float ux = dv[g] * xv[g];
                     float dus[4], das[4];
                     auto token = [&](auto k_) {
                         constexpr int k = decltype(k_)::value;
                         const float d = quad_lane<k>(dv[g]), u = quad_lane<k>(ux), s = quad_lane<k>(sv[g]);
-                        const float *b = lds[wave] + (4 * g + k) * Tile::kRow + n0, *c = b + 4 * NR;
-                        constexpr int kFill = NR == 1 ? 4 : NR <= 8 ? 8 / NR : 1;
+                        const float *b = lds[wave] + (4 * g + k) * kRow + n0, *c = b + kFloats;
+                        constexpr int kFill = NR <= 2 ? 4 : NR <= 4 ? 2 : 1;
                         constexpr int place = k % kFill * 2 * NR;
-                        dus[k] = 0.f, das[k] = 0.f;
+                        if constexpr (NR > 4)
+                            reread();
                         float db[NR], dc[NR];
 #pragma unroll
                         for (int j = 0; j < NR; ++j) {
@@ -323,30 +332,31 @@ __global__ __launch_bounds__(kThreads) void scan_backward_kernel(const ScanJob j
                             dc[j] = s * fmaf(u, b[j], kept_h);
                             const float G = fmaf(c[j], s, carry[j]);
                             db[j] = u * G;
-                            dus[k] = fmaf(b[j], G, dus[k]);
                             const float through = G * kept_h;
-                            das[k] = fmaf(through, A2[j], das[k]);
+                            dus[k] = j ? fmaf(b[j], G, dus[k]) : b[j] * G;
+                            das[k] = j ? fmaf(through, A2[j], das[k]) : through * A2[j];
                             dA[j] = fmaf(through, d, dA[j]);
                             carry[j] = G * a[4 * i + k][j];
                         }
                         if constexpr (NR <= 8) {
-                            // (lanes of channels that are not there hold copies of another's)
 #pragma unroll
                             for (int j = 0; j < NR; ++j)
-                                sums[place + j] = at.valid ? db[j] : 0.f, sums[place + NR + j] = at.valid ? dc[j] : 0.f;
+                                sums[place + j] = db[j], sums[place + NR + j] = dc[j];
                             if constexpr (k % kFill == 0) {
                                 const float v = channel_sums(sums, lane);
                                 const int q = lane / 4, which = q % (2 * NR) / NR, j = q % NR;
-                                if (q < kFill * 2 * NR)
-                                    out[wave][(4 * g + k + q / (2 * NR)) * Tile::kRow + which * 4 * NR + n0 + j] = v;
+                                if (kFill * 2 * NR == 16 || q < kFill * 2 * NR)
+                                    out[turn][wave][(4 * g + k + q / (2 * NR)) * kSpread + which * kRow + n0 + j] = v;
                             }
                         } else {
 #pragma unroll
                             for (int which = 0; which < 2; ++which) {
 #pragma unroll
                                 for (int j = 0; j < NR; ++j)
-                                    sums[j] = at.valid ? (which ? dc[j] : db[j]) : 0.f;
-                                out[wave][(4 * g + k) * Tile::kRow + which * 4 * NR + n0 + lane / 4] = channel_sums(sums, lane);
+                                    sums[j] = which ? dc[j] : db[j];
+                                const float v = channel_sums(sums, lane);
+                                if (NR == 16 || lane / 4 < NR)
+                                    out[turn][wave][(4 * g + k) * kSpread + which * kRow + n0 + lane / 4] = v;
                             }
                         }
                     };
@@ -360,57 +370,51 @@ __global__ __launch_bounds__(kThreads) void scan_backward_kernel(const ScanJob j
                         const float inv = __builtin_amdgcn_rcpf(1.f + ev[g]);
                         draw *= rv[g] >= 0.f ? inv : ev[g] * inv;
                     }
-                    const int token_at = t + 4 * g + sub;
-                    if (token_at < piece.len) {
-                        dskip = fmaf(sv[g], xv[g], dskip);
-                        dbias += draw;
-                        const int64_t where = static_cast<int64_t>(token_at) * D;
-                        if (at.valid) {
-                            store_vec<Scalar, 1>(dx + where, {{round_bits<Scalar>(fmaf(dv[g], du, skip * sv[g]))}});
-                            store_vec<Scalar, 1>(ddt + where, {{round_bits<Scalar>(draw)}});
-                            if (dgate) {
-                                const float sig = sigmoid(zv[g]), y = fmaf(skip, xv[g], ys[i]);
-                                store_vec<Scalar, 1>(dgate + where, {{round_bits<Scalar>(
-                                                                        gv[g] * y * sig * (1.f + zv[g] * (1.f - sig)))}});
-                            }
-                        }
+                    draw = t + 4 * g + sub < piece.len ? draw : 0.f;
+                    dskip = fmaf(sv[g], xv[g], dskip);
+                    dbias += draw;
+                    const int where = anew(d_rows.at) + g * d_rows.step;
+                    buffer_store<Scalar>(fmaf(dv[g], du, skip * sv[g]), dx_rows, where);
+                    buffer_store<Scalar>(draw, ddt_rows, where);
+                    if constexpr (kGate) {
+                        const float sig = sigmoid(zv[g]), y = fmaf(skip, xv[g], ys[i]);
+                        buffer_store<Scalar>(gv[g] * y * sig * (1.f + zv[g] * (1.f - sig)), dgate_rows, where);
                     }
                 }
             }
-            // dB and dC over the block's channels
+            // dB and dC over the block's channels; the next tile's are put beside them
             __syncthreads();
-            for (int i = tid; i < Tile::kFloats; i += kThreads) {
-                const int token_at = t + i / Tile::kRow;
+            for (int i = tid; i < 2 * kFloats; i += kThreads) {
+                const int token_at = t + i / kSpread;
                 float sum = 0.f;
 #pragma unroll
                 for (int w = 0; w < kWaves; ++w)
-                    sum += out[w][i];
+                    sum += out[turn][w][i];
                 if (token_at < piece.len)
-                    groups[static_cast<int64_t>(token_at) * job.G * Tile::kRow + i % Tile::kRow] = sum;
+                    groups[static_cast<int64_t>(token_at) * job.G * kSpread + i % kSpread] = sum;
             }
-            __syncthreads();
         }
         if (piece.at == 0 && grads.dinit && at.valid)
             store_states<NR>(grads.dinit + state, carry, job.S - n0);
     }
     for (int i = sub; i < piece.rest; i += 4) {
-        const int64_t where = static_cast<int64_t>(piece.len + i) * D;
+        const int64_t where = (row + piece.len + i) * D + channel;
         if (at.valid) {
-            store_vec<Scalar, 1>(dx + where, {{0u}});
-            store_vec<Scalar, 1>(ddt + where, {{0u}});
-            if (dgate)
-                store_vec<Scalar, 1>(dgate + where, {{0u}});
+            store_vec<Scalar, 1>(static_cast<Scalar *>(grads.dx) + where, {{0u}});
+            store_vec<Scalar, 1>(static_cast<Scalar *>(grads.ddt) + where, {{0u}});
+            if (kGate)
+                store_vec<Scalar, 1>(static_cast<Scalar *>(grads.dgate) + where, {{0u}});
         }
     }
-    for (int i = tid; i < piece.rest * Tile::kRow; i += kThreads)
-        groups[static_cast<int64_t>(piece.len + i / Tile::kRow) * job.G * Tile::kRow + i % Tile::kRow] = 0.f;
+    for (int i = tid; i < piece.rest * kSpread; i += kThreads)
+        groups[static_cast<int64_t>(piece.len + i / kSpread) * job.G * kSpread + i % kSpread] = 0.f;
     dskip += quad_swap<1>(dskip), dbias += quad_swap<1>(dbias);
     dskip += quad_swap<2>(dskip), dbias += quad_swap<2>(dbias);
     if (at.valid) {
-        float *to = grads.sums + (static_cast<int64_t>(at.piece) * D + channel) * (4 * NR + 2);
+        float *to = grads.sums + (static_cast<int64_t>(at.piece) * D + channel) * (kRow + 2);
         store_states<NR>(to + n0, dA, NR);
         if (sub == 0)
-            to[4 * NR] = dskip, to[4 * NR + 1] = dbias;
+            to[kRow] = dskip, to[kRow + 1] = dbias;
     }
 }
 
@@ -460,11 +464,14 @@ __global__ __launch_bounds__(1024) void scan_sums_kernel(const ScanJob job, cons
 template<typename Scalar, int NR>
 hipError_t launch_states(const ScanJob &job, const ScanGrads &grads, hipStream_t stream) {
     const int64_t pieces = most_pieces(job.seq, job.step);
-    const int blocks = (job.D / job.G + kChannels - 1) / kChannels;
+    const int blocks = (job.D / job.G + kScanChannels - 1) / kScanChannels;
     const dim3 grid(static_cast<unsigned>(pieces * job.G * blocks)), block(kThreads);
     if (job.seq.T > job.step)
         hipLaunchKernelGGL((scan_backs_kernel<Scalar, NR>), grid, block, 0, stream, job, grads);
-    hipLaunchKernelGGL((scan_backward_kernel<Scalar, NR>), grid, block, 0, stream, job, grads);
+    if (job.gate)
+        hipLaunchKernelGGL((scan_backward_kernel<Scalar, NR, true>), grid, block, 0, stream, job, grads);
+    else
+        hipLaunchKernelGGL((scan_backward_kernel<Scalar, NR, false>), grid, block, 0, stream, job, grads);
     const int64_t values = static_cast<int64_t>(job.seq.B) * job.seq.T * job.G * 8 * NR;
     hipLaunchKernelGGL(scan_groups_kernel<Scalar>, dim3(static_cast<unsigned>((values + kThreads - 1) / kThreads)), block, 0,
                        stream, job, grads, blocks, 8 * NR);
@@ -480,8 +487,11 @@ hipError_t launch_type(const ScanJob &job, const ScanGrads &grads, hipStream_t s
     switch (scan_lane_states(job.S)) {
         case 1: return launch_states<Scalar, 1>(job, grads, stream);
         case 2: return launch_states<Scalar, 2>(job, grads, stream);
+        case 3: return launch_states<Scalar, 3>(job, grads, stream);
         case 4: return launch_states<Scalar, 4>(job, grads, stream);
+        case 6: return launch_states<Scalar, 6>(job, grads, stream);
         case 8: return launch_states<Scalar, 8>(job, grads, stream);
+        case 12: return launch_states<Scalar, 12>(job, grads, stream);
         default: return launch_states<Scalar, 16>(job, grads, stream);
     }
 }

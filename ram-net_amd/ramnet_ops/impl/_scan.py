@@ -301,7 +301,7 @@ def _kept_bytes(sizes, packed: bool):
     """ramnet_selective_scan_kept_bytes in arithmetic that tracing leaves symbolic."""
     batch, T, N, D, S, _ = sizes
     slots = T // _KEPT + N + 1 if packed else batch * ((T + _KEPT - 1) // _KEPT)
-    return slots * D * 16 * next(w for w in (1, 2, 4, 8, 16) if S <= 4 * w)
+    return slots * D * 16 * next(w for w in (1, 2, 3, 4, 6, 8, 12, 16) if S <= 4 * w)
 
 
 def _head(x, dt, gate, B, C, A, skip, dt_bias, init_state, state, y, cu_seqlens, lengths, kept, ws) -> bytes:
