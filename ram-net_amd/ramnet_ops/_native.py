@@ -251,7 +251,8 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 
 def stream_of(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+    """The handle of the current stream of t's device (without an object of it: a tenth of the time)."""
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
 _here = contextlib.nullcontext()

@@ -44,7 +44,17 @@ def _check_devices(op: str, first: Tensor, *others: Tensor | None) -> None:
 
 
 def _key(*tensors: Tensor | None) -> tuple:
-    return tuple(None if t is None else (t.shape, t.stride(), t.dtype, t.device) for t in tensors)
+    return tuple([None if t is None else (t.shape, t.stride(), t.dtype, t.device) for t in tensors])
+
+
+def _as_read(t: Tensor | None, dtype: torch.dtype) -> bool:
+    """Whether a tensor that is read whole, as `dtype`, needs no copy."""
+    return t is None or t.dtype == dtype and t.is_contiguous()
+
+
+def _gradient(t: Tensor, dtype: torch.dtype) -> Tensor:
+    """An output's gradient in the type and with the sign that memory has."""
+    return t if t.dtype == dtype and not t.is_neg() else t.resolve_neg().to(dtype)
 
 
 def _rows_of(t: Tensor) -> Tensor:
@@ -68,6 +78,7 @@ class _ConvPlan(NamedTuple):
     sizes: tuple[int, ...]       # B, T, N, D, W
     tails: tuple[bytes, bytes]   # without and with silu
     workspace: tuple[int, int]   # bytes of forward and backward
+    plain: bool                  # whether all but x are read as they are
 
 
 _conv_plans = _Plans()
@@ -90,17 +101,30 @@ def _conv_sizes(op: str, x, weight, bias, init_state, cu_seqlens, lengths) -> tu
     return B, T, N, D, W
 
 
-def _conv_plan(op: str, x, weight, bias, init_state, cu_seqlens, lengths) -> _ConvPlan:
+def _conv_plan(op: str, x, weight, bias, init_state, cu_seqlens, lengths) -> tuple[_ConvPlan, Tensor]:
+    """The call's plan, with x as the native calls read it."""
     key = _key(x, weight, bias, init_state, cu_seqlens, lengths)
     plan = _conv_plans.get(key)
     if plan is not None:
-        return plan
+        return plan, x
     sizes = _conv_sizes(op, x, weight, bias, init_state, cu_seqlens, lengths)
+    rows = _rows_of(x)
+    if rows is not x:
+        return _conv_plan(op, rows, weight, bias, init_state, cu_seqlens, lengths)
     code, lib, packed = _code(x), nat.lib(), cu_seqlens is not None
     return _conv_plans.keep(key, _ConvPlan(
         sizes, tuple(_CONV_TAIL.pack(*sizes, *x.stride()[:2], code, silu) for silu in (0, 1)),
         tuple(_bytes_of(op, lib.ramnet_causal_conv_workspace_bytes(*sizes, code, packed, back), sizes)
-              for back in (0, 1))))
+              for back in (0, 1)),
+        all(_as_read(t, x.dtype) for t in (weight, bias, init_state))
+        and all(_as_read(t, torch.int32) for t in (cu_seqlens, lengths)))), x
+
+
+def _conv_inputs(weight, bias, init_state, cu_seqlens, lengths, state=None) -> tuple:
+    """Those that are read whole, as the native calls read them (a state updated in place as it is)."""
+    return (weight.contiguous(), None if bias is None else bias.contiguous(),
+            init_state if init_state is None or init_state is state else _as(init_state, weight.dtype),
+            _whole(cu_seqlens), _whole(lengths))
 
 
 def _bytes_of(op: str, count: int, sizes) -> int:
@@ -113,16 +137,13 @@ def _conv(op: str, x: Tensor, weight: Tensor, bias: Tensor | None, init_state: T
           cu_seqlens: Tensor | None, lengths: Tensor | None, silu: bool,
           state: Tensor | None = None) -> tuple[Tensor, Tensor]:
     """(y, state). ``state``: where the state goes (init_state itself in place)."""
-    x = _rows_of(x)
-    plan = _conv_plan(op, x, weight, bias, init_state, cu_seqlens, lengths)
+    plan, x = _conv_plan(op, x, weight, bias, init_state, cu_seqlens, lengths)
     B, T, N, D, W = plan.sizes
-    weight, bias = weight.contiguous(), None if bias is None else bias.contiguous()
-    if init_state is not None and init_state is not state:
-        init_state = _as(init_state, x.dtype)
+    if not plan.plain:
+        weight, bias, init_state, cu_seqlens, lengths = _conv_inputs(weight, bias, init_state, cu_seqlens, lengths, state)
     if state is None:
         state = x.new_empty((N, W - 1, D))
     y = x.new_empty((B, T, D))
-    cu_seqlens, lengths = _whole(cu_seqlens), _whole(lengths)
     n = plan.workspace[0]
     ws = x.new_empty((n,), dtype=torch.uint8) if n else None
     with nat.on_device(x):
@@ -178,20 +199,17 @@ def causal_conv_backward(x: Tensor, weight: Tensor, bias: Tensor | None, init_st
 
 def _conv_gradients(x, weight, bias, init_state, cu_seqlens, lengths, silu, d_y, d_state) -> tuple:
     op = "causal_conv_backward"
-    x = _rows_of(x)
-    plan = _conv_plan(op, x, weight, bias, init_state, cu_seqlens, lengths)
+    plan, x = _conv_plan(op, x, weight, bias, init_state, cu_seqlens, lengths)
     B, T, N, D, W = plan.sizes
     _check_shapes(op, d_y=(d_y, (B, T, D)), d_state=(d_state, (N, W - 1, D)))
-    d_y = _rows_of(d_y.resolve_neg().to(x.dtype))
+    d_y = _rows_of(_gradient(d_y, x.dtype))
     if d_state is not None:
-        d_state = d_state.resolve_neg().to(x.dtype).contiguous()
+        d_state = _gradient(d_state, x.dtype).contiguous()
     dx, dweight, dbias, dinit = x.new_empty((B, T, D)), x.new_empty((D, W)), x.new_empty((D,)), x.new_empty((N, W - 1, D))
     if B == 0:
         return dx, dweight.zero_(), dbias.zero_(), dinit
-    weight, bias = weight.contiguous(), None if bias is None else bias.contiguous()
-    if init_state is not None:
-        init_state = _as(init_state, x.dtype)
-    cu_seqlens, lengths = _whole(cu_seqlens), _whole(lengths)
+    if not plan.plain:
+        weight, bias, init_state, cu_seqlens, lengths = _conv_inputs(weight, bias, init_state, cu_seqlens, lengths)
     n = plan.workspace[1]
     ws = x.new_empty((n,), dtype=torch.uint8)
     with nat.on_device(x):
@@ -256,6 +274,7 @@ class _ScanPlan(NamedTuple):
     tails: tuple[bytes, bytes]         # without and with softplus
     workspace: tuple[int, int, int]    # bytes of kinds 0 to 2
     kept: int
+    plain: bool                        # whether all but x, dt, B, C and gate are read as they are
 
 
 _scan_plans = _Plans()
@@ -281,12 +300,17 @@ def _scan_sizes(op: str, x, dt, A, B, C, skip, gate, dt_bias, init_state, cu_seq
     return batch, T, N, D, S, G
 
 
-def _scan_plan(op: str, x, dt, A, B, C, skip, gate, dt_bias, init_state, cu_seqlens, lengths) -> _ScanPlan:
+def _scan_plan(op: str, x, dt, A, B, C, skip, gate, dt_bias, init_state, cu_seqlens, lengths) -> tuple[_ScanPlan, tuple]:
+    """The call's plan, with x, dt, B, C and gate as the native calls read them."""
     key = _key(x, dt, A, B, C, skip, gate, dt_bias, init_state, cu_seqlens, lengths)
     plan = _scan_plans.get(key)
     if plan is not None:
-        return plan
+        return plan, (x, dt, B, C, gate)
     sizes = _scan_sizes(op, x, dt, A, B, C, skip, gate, dt_bias, init_state, cu_seqlens, lengths)
+    rows = tuple(None if t is None else _near_rows_of(t) for t in (x, dt, B, C, gate))
+    if any(a is not b for a, b in zip(rows, (x, dt, B, C, gate))):
+        x, dt, B, C, gate = rows
+        return _scan_plan(op, x, dt, A, B, C, skip, gate, dt_bias, init_state, cu_seqlens, lengths)
     lib, packed = nat.lib(), cu_seqlens is not None
     strides = (*x.stride()[:2], *dt.stride()[:2], *(gate.stride()[:2] if gate is not None else (0, 0)),
                *B.stride()[:3], *C.stride()[:3])
@@ -294,7 +318,9 @@ def _scan_plan(op: str, x, dt, A, B, C, skip, gate, dt_bias, init_state, cu_seql
         sizes, tuple(_SCAN_TAIL.pack(*sizes, *strides, _code(x), softplus) for softplus in (0, 1)),
         tuple(_bytes_of(op, lib.ramnet_selective_scan_workspace_bytes(*sizes, packed, kind), sizes)
               for kind in range(3)),
-        _bytes_of(op, lib.ramnet_selective_scan_kept_bytes(*sizes, packed), sizes)))
+        _bytes_of(op, lib.ramnet_selective_scan_kept_bytes(*sizes, packed), sizes),
+        all(_as_read(t, torch.float32) for t in (A, skip, dt_bias, init_state))
+        and all(_as_read(t, torch.int32) for t in (cu_seqlens, lengths)))), rows
 
 
 def _kept_bytes(sizes, packed: bool):
@@ -319,20 +345,18 @@ def _scan(op: str, x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, skip:
           dt_bias: Tensor | None, init_state: Tensor | None, cu_seqlens: Tensor | None, lengths: Tensor | None,
           softplus: bool, state: Tensor | None = None, keep: bool = False) -> tuple[Tensor, Tensor, Tensor | None]:
     """(y, state, kept). ``state``: where the state goes (init_state itself in place)."""
-    x, dt, B, C = _near_rows_of(x), _near_rows_of(dt), _near_rows_of(B), _near_rows_of(C)
-    gate = None if gate is None else _near_rows_of(gate)
-    plan = _scan_plan(op, x, dt, A, B, C, skip, gate, dt_bias, init_state, cu_seqlens, lengths)
+    plan, (x, dt, B, C, gate) = _scan_plan(op, x, dt, A, B, C, skip, gate, dt_bias, init_state, cu_seqlens, lengths)
     batch, T, N, D, S, G = plan.sizes
-    A, skip, dt_bias = _parameter(A), _parameter(skip), _parameter(dt_bias)
-    if init_state is not None and init_state is not state:
-        init_state = _parameter(init_state)
+    if not plan.plain:
+        A, skip, dt_bias = _parameter(A), _parameter(skip), _parameter(dt_bias)
+        init_state = init_state if init_state is state else _parameter(init_state)
+        cu_seqlens, lengths = _whole(cu_seqlens), _whole(lengths)
     if state is None:
         state = x.new_empty((N, D, S), dtype=torch.float32)
     y = x.new_empty((batch, T, D))
     kept = x.new_empty((plan.kept,), dtype=torch.uint8) if keep else None
     n = plan.workspace[keep]
     ws = x.new_empty((n,), dtype=torch.uint8) if n else None
-    cu_seqlens, lengths = _whole(cu_seqlens), _whole(lengths)
     with nat.on_device(x):
         nat.call("ramnet_selective_scan_forward", _head(
             x, dt, gate, B, C, A, skip, dt_bias, init_state, state, y, cu_seqlens, lengths, kept, ws)
@@ -408,18 +432,18 @@ def selective_scan_backward(
 def _scan_gradients(x, dt, A, B, C, skip, gate, dt_bias, cu_seqlens, lengths, softplus, sequences, kept, d_y,
                     d_state) -> tuple:
     op = "selective_scan_backward"
-    x, dt, B, C = _near_rows_of(x), _near_rows_of(dt), _near_rows_of(B), _near_rows_of(C)
-    gate = None if gate is None else _near_rows_of(gate)
-    plan = _scan_plan(op, x, dt, A, B, C, skip, gate, dt_bias, None, cu_seqlens, lengths)
+    plan, (x, dt, B, C, gate) = _scan_plan(op, x, dt, A, B, C, skip, gate, dt_bias, None, cu_seqlens, lengths)
     batch, T, N, D, S, G = plan.sizes
     _check_shapes(op, d_y=(d_y, (batch, T, D)), d_state=(d_state, (N, D, S)))
-    d_y = _near_rows_of(d_y.resolve_neg().to(x.dtype))
+    d_y = _near_rows_of(_gradient(d_y, x.dtype))
     if d_state is not None:
-        d_state = d_state.resolve_neg().to(torch.float32).contiguous()
-    dx, ddt, dgate = (x.new_empty((batch, T, D)) for _ in range(3))
-    dB, dC = (x.new_empty((batch, T, G, S)) for _ in range(2))
-    A, skip, dt_bias = _parameter(A), _parameter(skip), _parameter(dt_bias)
-    dA, dskip, dbias = (A.new_empty(s) for s in ((D, S), (D,), (D,)))
+        d_state = _gradient(d_state, torch.float32).contiguous()
+    dx, ddt, dgate = x.new_empty((batch, T, D)), x.new_empty((batch, T, D)), x.new_empty((batch, T, D))
+    dB, dC = x.new_empty((batch, T, G, S)), x.new_empty((batch, T, G, S))
+    if not plan.plain:
+        A, skip, dt_bias = _parameter(A), _parameter(skip), _parameter(dt_bias)
+        cu_seqlens, lengths = _whole(cu_seqlens), _whole(lengths)
+    dA, dskip, dbias = A.new_empty((D, S)), A.new_empty((D,)), A.new_empty((D,))
     dinit = A.new_empty((N, D, S))
     if batch * T == 0 or N == 0:
         for t in (dx, ddt, dgate, dB, dC, dA, dskip, dbias):
@@ -430,7 +454,6 @@ def _scan_gradients(x, dt, A, B, C, skip, gate, dt_bias, cu_seqlens, lengths, so
         dgate.zero_()
     n = plan.workspace[2]
     ws = x.new_empty((n,), dtype=torch.uint8)
-    cu_seqlens, lengths = _whole(cu_seqlens), _whole(lengths)
     with nat.on_device(x):
         nat.call("ramnet_selective_scan_backward", _head(
             x, dt, gate, B, C, A, skip, dt_bias, None, None, None, cu_seqlens, lengths, kept, ws)
