@@ -90,12 +90,36 @@ __device__ __forceinline__ uint32_t lane_xor(uint32_t x) {
     }
 }
 
+template<int XOR, typename T>
+__device__ __forceinline__ T lane_xor_of(T x) {
+    if constexpr (sizeof(T) == 8) {
+        const uint64_t bits = __builtin_bit_cast(uint64_t, x);
+        return __builtin_bit_cast(T, static_cast<uint64_t>(lane_xor<XOR>(static_cast<uint32_t>(bits >> 32))) << 32 |
+                                         lane_xor<XOR>(static_cast<uint32_t>(bits)));
+    } else {
+        return __builtin_bit_cast(T, lane_xor<XOR>(__builtin_bit_cast(uint32_t, x)));
+    }
+}
+
 template<typename T, typename Op>
 __device__ __forceinline__ T wave_reduce(T x, Op op) {
-#pragma unroll
-    for (int m = 1; m < kWave; m <<= 1)
-        x = op(x, __shfl_xor(x, m));
-    return x;
+    x = op(x, lane_xor_of<1>(x)), x = op(x, lane_xor_of<2>(x)), x = op(x, lane_xor_of<4>(x));
+    x = op(x, lane_xor_of<8>(x)), x = op(x, lane_xor_of<16>(x));
+    return op(x, lane_xor_of<32>(x));
+}
+
+// x and the values of the lanes before it, added up: within rows of 16 by shifts, then row by row.
+template<int CONTROL, int ROWS>
+__device__ __forceinline__ uint64_t shifted(uint64_t x) {
+    const uint32_t low = __builtin_amdgcn_update_dpp(0u, static_cast<uint32_t>(x), CONTROL, ROWS, 0xF, false);
+    const uint32_t high = __builtin_amdgcn_update_dpp(0u, static_cast<uint32_t>(x >> 32), CONTROL, ROWS, 0xF, false);
+    return static_cast<uint64_t>(high) << 32 | low;
+}
+__device__ __forceinline__ uint64_t wave_scan(uint64_t x) {
+    x += shifted<0x111, 0xF>(x), x += shifted<0x112, 0xF>(x);  // row_shr:1, 2, 4, 8
+    x += shifted<0x114, 0xF>(x), x += shifted<0x118, 0xF>(x);
+    x += shifted<0x142, 0xA>(x);                               // row_bcast:15, to rows 1 and 3
+    return x + shifted<0x143, 0xC>(x);                         // row_bcast:31, to rows 2 and 3
 }
 
 // 2^x for x in [-1000, 0], to 2e-15: of x in parts of 1/32, which adding 3 2^46 leaves in the lowest bits of the
@@ -205,45 +229,59 @@ struct Sampler {
         return w >= least;
     }
 
+    // What op makes of the 16 waves' values, from a value a lane that goes by the lane's place in its row of 16.
+    template<typename T, typename Op>
+    __device__ __forceinline__ static T row_reduce(T x, Op op) {
+        static_assert(kWaves == 16, "a row of lanes");
+        x = op(x, lane_xor_of<1>(x)), x = op(x, lane_xor_of<2>(x)), x = op(x, lane_xor_of<4>(x));
+        return op(x, lane_xor_of<8>(x));
+    }
+
     // The sum of x over the threads before.
     __device__ __forceinline__ uint64_t block_scan(uint64_t x, int which) {
-        uint64_t run = x;
-#pragma unroll
-        for (int m = 1; m < kWave; m <<= 1) {
-            const uint64_t y = __shfl_up(run, m);
-            run += lane >= m ? y : 0;
-        }
+        const uint64_t run = wave_scan(x);
         __syncthreads();
         if (lane == kWave - 1)
             lds().scan[which][wave] = run;
         __syncthreads();
-        uint64_t before = 0;
-        for (int w = 0; w < wave; ++w)
-            before += lds().scan[which][w];
-        return before + run - x;
+        const uint64_t of_wave = lds().scan[which][lane % kWaves];
+        return row_reduce(lane % kWaves < wave ? of_wave : 0, Sum{}) + run - x;
     }
 
+    template<typename T>
+    __device__ __forceinline__ static uint64_t as_word(T x) {
+        if constexpr (sizeof(T) == 8)
+            return __builtin_bit_cast(uint64_t, x);
+        else
+            return __builtin_bit_cast(uint32_t, x);
+    }
+    template<typename T>
+    __device__ __forceinline__ static T of_word(uint64_t x) {
+        if constexpr (sizeof(T) == 8)
+            return __builtin_bit_cast(T, x);
+        else
+            return __builtin_bit_cast(T, static_cast<uint32_t>(x));
+    }
+
+    // Over the block; of two values at once.
     template<typename T, typename Op>
-    __device__ __forceinline__ T block_reduce(T x, Op op, int which = 0) {
-        auto get = [&](int w) {
-            if constexpr (sizeof(T) == 8)
-                return __builtin_bit_cast(T, lds().scan[which][w]);
-            else
-                return __builtin_bit_cast(T, static_cast<uint32_t>(lds().scan[which][w]));
-        };
+    __device__ __forceinline__ T block_reduce(T x, Op op) {
         x = wave_reduce(x, op);
         __syncthreads();
-        if (lane == 0) {
-            if constexpr (sizeof(T) == 8)
-                lds().scan[which][wave] = __builtin_bit_cast(uint64_t, x);
-            else
-                lds().scan[which][wave] = __builtin_bit_cast(uint32_t, x);
-        }
+        if (lane == 0)
+            lds().scan[0][wave] = as_word(x);
         __syncthreads();
-        x = get(0);
-        for (int w = 1; w < kWaves; ++w)
-            x = op(x, get(w));
-        return x;
+        return row_reduce(of_word<T>(lds().scan[0][lane % kWaves]), op);
+    }
+    template<typename T, typename OpT, typename U, typename OpU>
+    __device__ __forceinline__ void block_reduce(T &x, OpT op_x, U &y, OpU op_y) {
+        x = wave_reduce(x, op_x), y = wave_reduce(y, op_y);
+        __syncthreads();
+        if (lane == 0)
+            lds().scan[0][wave] = as_word(x), lds().scan[1][wave] = as_word(y);
+        __syncthreads();
+        x = row_reduce(of_word<T>(lds().scan[0][lane % kWaves]), op_x);
+        y = row_reduce(of_word<U>(lds().scan[1][lane % kWaves]), op_y);
     }
 
     // A limit that at least `count` logits reach, from the greatest one of each lane: the waves whose lanes have
@@ -333,29 +371,29 @@ struct Sampler {
         uint64_t part = mine ? whole(exact) : 0;
         const uint64_t before = block_scan(part, 0);
         if (by_sum && all == 0)
-            all = block_reduce(static_cast<uint64_t>(tid) < k ? part : 0, Sum{}, 1);
+            all = block_reduce(static_cast<uint64_t>(tid) < k ? part : 0, Sum{});
         const double target = by_sum ? p * static_cast<double>(all) : INFINITY;
         const bool stays = mine && within(l, index_of(order)) &&
                            (tid == 0 || (static_cast<uint64_t>(tid) < k && static_cast<double>(before) < target && exact >= least));
         part = stays ? part : 0;
-        const double total = static_cast<double>(block_reduce(part, Sum{}, 1));
+        int drawn = part > 0 ? tid + 1 : 0;  // (those with a weight are a prefix)
+        uint64_t parts = part;
+        block_reduce(parts, Sum{}, drawn, Most{});
+        const double total = static_cast<double>(parts);
         if (probs && stays)  // (the zeros are behind the barriers of that sum)
             probs[index_of(order)] = static_cast<float>(exact * unit / total);
         if (token) {
             // by index, each with its place among the weights
-            const int drawn = block_reduce(part > 0 ? tid + 1 : 0, Most{});
             lds().list[tid] = part;
             const uint64_t at = sorted(part > 0 ? order << 32 | static_cast<uint32_t>(tid) : 0, drawn);
             __syncthreads();
             const uint64_t own = tid < drawn ? lds().list[static_cast<uint32_t>(at)] : 0;
-            const uint64_t run = block_scan(own, 0) + own;
-            const int index = index_of(at >> 32);
-            int first = V, last = -1;
-            if (own > 0)
-                first = static_cast<double>(run) > u * total ? index : V, last = index;
-            first = block_reduce(first, Least{}, 1), last = block_reduce(last, Most{});
-            if (tid == 0)  // (none passes by rounding: the last one with a weight)
-                *token = first < V ? first : last;
+            const uint64_t run = block_scan(own, 0);
+            const double threshold = u * total;
+            // (the first that passes or, where by rounding none does, the last)
+            if (tid < drawn && !(static_cast<double>(run) > threshold) &&
+                (static_cast<double>(run + own) > threshold || tid == drawn - 1))
+                *token = index_of(at >> 32);
         }
     }
 
@@ -405,7 +443,8 @@ struct Sampler {
                 if (bin(l) == level && within(l, i))
                     least_o = min(least_o, o), most_o = max(most_o, o);
             });
-            lo = block_reduce(least_o, Least{}), hi = block_reduce(most_o, Most{}, 1);
+            block_reduce(least_o, Least{}, most_o, Most{});
+            lo = least_o, hi = most_o;
         }
         while (members > kList) {
             int shift = 0;
@@ -540,7 +579,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleJob job) {
             });
         else  // (a NaN has neither weight nor bin as it is)
             me.sweep_ahead([&](float l, int) { count(l); });
-        all = me.block_reduce(all, Sum{}), last = me.block_reduce(last, Sum{}, 1);
+        me.block_reduce(all, Sum{}, last, Sum{});
         if (tid == 0)
             lds().sums[kBins - 1] = last;
         __syncthreads();
@@ -626,7 +665,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleJob job) {
                 found = static_cast<double>(run) > threshold ? i : V;
             }
         }
-        found = me.block_reduce(found, Least{}), last = me.block_reduce(last, Most{}, 1);
+        me.block_reduce(found, Least{}, last, Most{});
         if (tid == 0)
             *token = found < V ? found : last;
     }
