@@ -5,17 +5,21 @@ Layer stack:
     x -> x + DeltaLayer(RMSNorm(x)) -> x + SwiGLU(RMSNorm(x))
 
 DeltaLayer: queries, keys (each of norm 1), values, a decay and a write
-strength per value head from Linear maps of x; the operator
-``gated_delta_rule``; a head-wise RMSNorm of what it reads, a sigmoid gate and
-the output projection, as RamLayer has them. The only state is the operator's,
-one (key_dim, value_dim) matrix per sequence and value head.
+strength per value head from Linear maps of x; where ``conv_width`` is set, a
+short causal convolution with silu of the queries, keys and values
+(``causal_conv``); the operator ``gated_delta_rule``; a head-wise RMSNorm of what
+it reads, a sigmoid gate and the output projection, as RamLayer has them. The
+state is the operator's, one (key_dim, value_dim) matrix per sequence and value
+head, and with a convolution also its last inputs: a pair of the two.
 
 ``speculative_generate`` decodes with a smaller model that drafts: the target
 scores all drafts of a sequence in one call, ``verify_drafts`` says which stay,
 and the states move over those alone. A matrix state cannot be cut back the way
 a cache of tokens can, so the scoring call leaves the states as they are, each
-layer keeps its operator's inputs (a few rows), and the operator runs over them
-once more in place with the number of tokens that stayed.
+layer keeps its operators' inputs (a few rows), and the operators run over them
+once more in place with the number of tokens that stayed. With ``top_k``,
+``top_p`` or ``min_p`` both models' tokens come from what these leave of their
+distributions (``sample_tokens``, ``token_probabilities``).
 """
 from __future__ import annotations
 
@@ -25,7 +29,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from ramnet_ops import gated_delta_rule, verify_drafts
+from ramnet_ops import causal_conv, gated_delta_rule, sample_tokens, token_probabilities, verify_drafts
 
 from .lm import SwiGLU
 
@@ -41,6 +45,7 @@ class DeltaConfig:
     value_dim: int = 128
     mlp_width: int = 2816
     norm_eps: float = 1e-6
+    conv_width: int = 0      # taps of the convolution before the operator; 0: none
 
 
 class DeltaLayer(nn.Module):
@@ -58,6 +63,8 @@ class DeltaLayer(nn.Module):
         self.gate = nn.Linear(d, values)
         self.out = nn.Linear(values, d, bias=False)
         self.out_norm = nn.RMSNorm(cfg.value_dim, eps=cfg.norm_eps)
+        if cfg.conv_width:
+            self.conv = nn.Parameter(torch.zeros(2 * keys + values, cfg.conv_width))
 
     @torch.no_grad()
     def init_weights(self, std: float = 0.02) -> None:
@@ -68,23 +75,32 @@ class DeltaLayer(nn.Module):
         self.decay.bias.copy_(rate.expm1().log())
         nn.init.zeros_(self.beta.bias)
         nn.init.zeros_(self.gate.bias)
+        if self.cfg.conv_width:
+            nn.init.uniform_(self.conv, -self.cfg.conv_width ** -0.5, self.cfg.conv_width ** -0.5)
 
-    def op_inputs(self, x: torch.Tensor):
+    def op_inputs(self, x: torch.Tensor, qkv: torch.Tensor | None = None):
         """(q, k, v, g, beta) in the operator's (B, T, H, ...) layout."""
         B, T, _ = x.shape
         c = self.cfg
         keys = c.key_heads * c.key_dim
-        q, k, v = self.qkv(x).split((keys, keys, c.heads * c.value_dim), dim=-1)
+        q, k, v = (self.qkv(x) if qkv is None else qkv).split((keys, keys, c.heads * c.value_dim), dim=-1)
         q = F.normalize(q.view(B, T, c.key_heads, c.key_dim), dim=-1)
         k = F.normalize(k.view(B, T, c.key_heads, c.key_dim), dim=-1)
         # (the decay in 32 bits: over long prompts its sum is what counts)
         return q, k, v.view(B, T, c.heads, c.value_dim), -F.softplus(self.decay(x).float()), torch.sigmoid(self.beta(x))
 
     def forward(self, x, state, lengths=None, inplace: bool = False, keep=None):
-        inputs = self.op_inputs(x)
+        qkv = tail = raw = None
+        if self.cfg.conv_width:
+            state, tail = state
+            raw = self.qkv(x)
+            qkv, tail = causal_conv(raw, self.conv, activation="silu", init_state=tail, lengths=lengths, inplace=inplace)
+        inputs = self.op_inputs(x, qkv)
         if keep is not None:
-            keep.append(inputs)
+            keep.append(inputs if raw is None else (inputs, raw, self.conv))
         y, state = gated_delta_rule(*inputs, init_state=state, lengths=lengths, inplace=inplace)
+        if tail is not None:
+            state = (state, tail)
         return self.out(torch.sigmoid(self.gate(x)) * self.out_norm(y).flatten(-2)), state
 
 
@@ -121,8 +137,13 @@ class DeltaLM(nn.Module):
             nn.init.normal_(blk.mlp.down.weight, 0.0, std)
 
     def fresh_state(self, batch: int, device) -> list:
+        """Zeros of each layer: the operator's matrices, with a convolution in a pair with its last inputs."""
         cfg = self.cfg
-        return [torch.zeros(batch, cfg.heads, cfg.key_dim, cfg.value_dim, device=device) for _ in range(cfg.layers)]
+        states = [torch.zeros(batch, cfg.heads, cfg.key_dim, cfg.value_dim, device=device) for _ in range(cfg.layers)]
+        if not cfg.conv_width:
+            return states
+        return [(s, blk.delta.conv.new_zeros(batch, cfg.conv_width - 1, blk.delta.conv.shape[0], device=device))
+                for s, blk in zip(states, self.blocks)]
 
     def forward(self, tokens: torch.Tensor, states: list, lengths=None, inplace: bool = False, keep=None):
         """Logits (B, T, vocab) and the states. `lengths` (B): the tokens of
@@ -140,6 +161,10 @@ class DeltaLM(nn.Module):
 def advance(kept: list, states: list, lengths: torch.Tensor) -> None:
     """Move the states, in place, over the first `lengths` tokens of a scoring call."""
     for inputs, state in zip(kept, states):
+        if isinstance(state, tuple):
+            inputs, raw, taps = inputs
+            state, tail = state
+            causal_conv(raw, taps, init_state=tail, lengths=lengths, inplace=True)
         gated_delta_rule(*inputs, init_state=state, lengths=lengths, inplace=True)
 
 
@@ -149,9 +174,11 @@ def _probabilities(logits: torch.Tensor, temperature: float) -> torch.Tensor:
 
 @torch.no_grad()
 def speculative_generate(model: DeltaLM, drafter: DeltaLM, prompt: torch.Tensor, new_tokens: int, drafts: int = 4,
-                         temperature: float = 1.0, generator: torch.Generator | None = None):
+                         temperature: float = 1.0, generator: torch.Generator | None = None, top_k: int | None = None,
+                         top_p: float | None = None, min_p: float | None = None):
     """Sample `new_tokens` tokens after ``prompt`` (B, T), with up to `drafts`
-    of them a step proposed by `drafter`; they are distributed as `model`'s own.
+    of them a step proposed by `drafter`; they are distributed as `model`'s own,
+    with what `top_k`, `top_p` and `min_p` leave of it.
 
     Rows advance by different counts: a row that is done has no drafts and its
     states stay. Returns the tokens (B, new_tokens), the model's states
@@ -159,9 +186,24 @@ def speculative_generate(model: DeltaLM, drafter: DeltaLM, prompt: torch.Tensor,
     if drafts < 1:
         raise ValueError(f"drafts must be at least 1, got {drafts}")
     B, dev = prompt.shape[0], prompt.device
+    settings = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+    filtered = any(v is not None for v in (top_k, top_p, min_p))
+
+    def probabilities(logits):
+        return token_probabilities(logits, **settings) if filtered else _probabilities(logits, temperature)
+
+    def draw(logits):
+        """(token (B, 1), probabilities (B, vocab))."""
+        if filtered:
+            token, chances = sample_tokens(logits, torch.rand(B, device=dev, generator=generator), **settings,
+                                           probabilities=True)
+            return token.unsqueeze(1), chances
+        chances = _probabilities(logits, temperature)
+        return torch.multinomial(chances, 1, generator=generator), chances
+
     logits, states = model(prompt, model.fresh_state(B, dev))
     _, drafter_states = drafter(prompt, drafter.fresh_state(B, dev))
-    last = torch.multinomial(_probabilities(logits[:, -1], temperature), 1, generator=generator)
+    last, _ = draw(logits[:, -1])
     # one column more, for what a row does not write
     out = torch.empty(B, new_tokens + 1, dtype=torch.long, device=dev)
     out[:, :1] = last
@@ -174,14 +216,15 @@ def speculative_generate(model: DeltaLM, drafter: DeltaLM, prompt: torch.Tensor,
         tokens, chances, tried = [last], [], drafter_states
         for _ in range(drafts):
             logits, tried = drafter(tokens[-1], tried)
-            chances.append(_probabilities(logits[:, -1], temperature))
-            tokens.append(torch.multinomial(chances[-1], 1, generator=generator))
+            token, chance = draw(logits[:, -1])
+            tokens.append(token)
+            chances.append(chance)
         block = torch.cat(tokens, dim=1)
         # all of them scored in one call, from states that stay
         kept = []
         logits, _ = model(block, states, keep=kept)
         drawn, taken = verify_drafts(
-            block[:, 1:], _probabilities(logits, temperature), torch.stack(chances, dim=1),
+            block[:, 1:], probabilities(logits), torch.stack(chances, dim=1),
             torch.rand(B, drafts, device=dev, generator=generator), torch.rand(B, device=dev, generator=generator),
             draft_lens=(left - 1).clamp(0, drafts).view(B).int())
         taken = taken.view(B, 1)
