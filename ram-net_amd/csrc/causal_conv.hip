@@ -9,6 +9,8 @@
 #include "ramnet_kernels.hpp"
 #include "vector16.hpp"
 
+#include <type_traits>
+
 namespace ramnet {
 
 namespace {
@@ -146,10 +148,10 @@ __global__ __launch_bounds__(kThreads) void conv_kernel(const ConvJob job, int64
         store_vec<Scalar, VEC>(y + (row + piece.t0 + piece.len + i) * D, Vec<Scalar, VEC>{});
 }
 
-// Sums of dweight and dbias over a block's pieces: kThreads threads of W + 1 rows of VEC, those
-// of the same channels `per_row` threads apart.
+// Gradients of a piece's inputs, and its sums of dweight and dbias. The inputs' convolution is made again; a gradient
+// is whole W - 1 tokens later, also where these lie in the next piece.
 template<typename Scalar, int W, int VEC>
-__global__ __launch_bounds__(kThreads) void conv_backward_kernel(const ConvJob job, const ConvGrads grads,
+__global__ __launch_bounds__(kThreads, W <= 4 && sizeof(Scalar) == 2 ? 4 : 2) void conv_backward_kernel(const ConvJob job, const ConvGrads grads,
                                                                  int64_t pieces) {
     ConvPlace<VEC> at;
     TimePiece piece;
@@ -204,45 +206,51 @@ __global__ __launch_bounds__(kThreads) void conv_backward_kernel(const ConvJob j
             const Scalar *x = static_cast<const Scalar *>(job.x) + piece.row * job.x_at[0] + piece.lo * job.x_at[1] + c0;
             const Scalar *dy = static_cast<const Scalar *>(grads.dy) + piece.row * grads.dy_at[0] +
                                piece.lo * grads.dy_at[1] + c0;
+            auto token = [&](int t, const Vec<Scalar, VEC> &xt, const Vec<Scalar, VEC> &dt, auto own) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+#pragma unroll
+                    for (int j = 0; j + 1 < W; ++j)
+                        win[j][e] = win[j + 1][e], pend[j][e] = pend[j + 1][e];
+                    win[W - 1][e] = xt[e], pend[W - 1][e] = 0.f;
+                    float d = dt[e];
+                    if (job.silu) {
+                        float s = taps.bias[e];
+#pragma unroll
+                        for (int j = 0; j < W; ++j)
+                            s = fmaf(taps.weight[j][e], win[j][e], s);
+                        const float g = sigmoid(s);
+                        d *= g * (1.f + s * (1.f - g));
+                    }
+#pragma unroll
+                    for (int j = 0; j < W; ++j) {
+                        pend[j][e] = fmaf(taps.weight[j][e], d, pend[j][e]);
+                        if constexpr (decltype(own)::value)
+                            dtap[j][e] = fmaf(d, win[j][e], dtap[j][e]);
+                    }
+                    if constexpr (decltype(own)::value)
+                        dbias[e] += d;
+                }
+                emit(t - (W - 1), pend[0]);
+            };
             constexpr int kDeep = 4;
-            for (int t0 = begin; t0 < stop; t0 += kDeep) {
+            for (int t0 = begin; t0 < end; t0 += kDeep) {
                 Vec<Scalar, VEC> xs[kDeep], ds[kDeep];
 #pragma unroll
                 for (int i = 0; i < kDeep; ++i) {
-                    xs[i] = t0 + i < stop ? load_vec<Scalar, VEC>(x + (t0 + i) * job.x_at[1]) : Vec<Scalar, VEC>{};
-                    ds[i] = t0 + i < stop ? load_vec<Scalar, VEC>(dy + (t0 + i) * grads.dy_at[1]) : Vec<Scalar, VEC>{};
+                    xs[i] = t0 + i < end ? load_vec<Scalar, VEC>(x + (t0 + i) * job.x_at[1]) : Vec<Scalar, VEC>{};
+                    ds[i] = t0 + i < end ? load_vec<Scalar, VEC>(dy + (t0 + i) * grads.dy_at[1]) : Vec<Scalar, VEC>{};
                 }
 #pragma unroll
                 for (int i = 0; i < kDeep; ++i) {
-                    const int t = t0 + i;
-                    if (t >= stop)
+                    if (t0 + i >= end)
                         break;
-                    const bool own = t < end;  // (tokens behind the piece count for its inputs alone)
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-#pragma unroll
-                        for (int j = 0; j + 1 < W; ++j)
-                            win[j][e] = win[j + 1][e], pend[j][e] = pend[j + 1][e];
-                        win[W - 1][e] = xs[i][e], pend[W - 1][e] = 0.f;
-                        float d = ds[i][e];
-                        if (job.silu) {
-                            float s = taps.bias[e];
-#pragma unroll
-                            for (int j = 0; j < W; ++j)
-                                s = fmaf(taps.weight[j][e], win[j][e], s);
-                            const float g = sigmoid(s);
-                            d *= g * (1.f + s * (1.f - g));
-                        }
-#pragma unroll
-                        for (int j = 0; j < W; ++j) {
-                            pend[j][e] = fmaf(taps.weight[j][e], d, pend[j][e]);
-                            dtap[j][e] = own ? fmaf(d, win[j][e], dtap[j][e]) : dtap[j][e];
-                        }
-                        dbias[e] += own ? d : 0.f;
-                    }
-                    emit(t - (W - 1), pend[0]);
+                    token(t0 + i, xs[i], ds[i], std::true_type{});
                 }
             }
+            for (int t = end; t < stop; ++t)  // (tokens behind the piece count for its inputs alone)
+                token(t, load_vec<Scalar, VEC>(x + t * job.x_at[1]), load_vec<Scalar, VEC>(dy + t * grads.dy_at[1]),
+                      std::false_type{});
             // (behind a sequence's last token: what is still pending)
 #pragma unroll
             for (int j = 1; j < W; ++j)
@@ -271,9 +279,11 @@ __global__ __launch_bounds__(1024) void conv_sum_kernel(const ConvJob job, const
     const int lane = static_cast<int>(threadIdx.x) % kWave, wave = static_cast<int>(threadIdx.x) / kWave;
     const int64_t columns = static_cast<int64_t>(job.W + 1) * job.D, column = static_cast<int64_t>(blockIdx.x) * kWave + lane;
     float sum = 0.f;
-    if (column < columns)
+    if (column < columns) {
+#pragma unroll 8
         for (int p = wave; p < pieces; p += 16)
             sum += grads.partial[p * columns + column];
+    }
     sums[wave][lane] = sum;
     __syncthreads();
     if (wave > 0 || column >= columns)
@@ -291,16 +301,24 @@ template<typename Scalar, int W, int VEC>
 hipError_t launch_of(const ConvJob &job, const ConvGrads *grads, int64_t pieces, hipStream_t stream) {
     const int64_t threads = pieces * ((job.D + VEC - 1) / VEC);
     const dim3 grid(static_cast<unsigned>((threads + kThreads - 1) / kThreads)), block(kThreads);
-    if (grads)
-        hipLaunchKernelGGL((conv_backward_kernel<Scalar, W, VEC>), grid, block, 0, stream, job, *grads, pieces);
-    else
-        hipLaunchKernelGGL((conv_kernel<Scalar, W, VEC>), grid, block, 0, stream, job, pieces);
+    if constexpr (VEC <= 4) {
+        if (grads) {
+            hipLaunchKernelGGL((conv_backward_kernel<Scalar, W, VEC>), grid, block, 0, stream, job, *grads, pieces);
+            return hipGetLastError();
+        }
+    }
+    hipLaunchKernelGGL((conv_kernel<Scalar, W, VEC>), grid, block, 0, stream, job, pieces);
     return hipGetLastError();
 }
 
 template<typename Scalar, int W>
 hipError_t launch_width(const ConvJob &job, const ConvGrads *grads, int64_t pieces, hipStream_t stream) {
-    constexpr int kWide = 16 / sizeof(Scalar);
+    // (the backward holds four rows of W a channel: with 16 bytes of 16-bit channels they leave two waves a SIMD, 53 us
+    // of 4 x 2048 x 2048 for 36)
+    constexpr int kWide = 16 / sizeof(Scalar), kNarrow = 4;
+    if (grads)
+        return job.D >= kNarrow ? launch_of<Scalar, W, kNarrow>(job, grads, pieces, stream)
+                                : launch_of<Scalar, W, 1>(job, grads, pieces, stream);
     return job.D >= kWide ? launch_of<Scalar, W, kWide>(job, grads, pieces, stream)
                           : launch_of<Scalar, W, 1>(job, grads, pieces, stream);
 }
@@ -336,13 +354,12 @@ hipError_t launch_any(const ConvJob &job, const ConvGrads *grads, hipStream_t st
 
 }  // namespace
 
-// Pieces of 16 tokens re-read W - 1 of theirs from the cache. The backward, which leaves W + 1
-// rows of sums a piece, takes longer ones where there are still enough of them.
+// Pieces of 16 tokens re-read W - 1 of theirs from the cache. The backward leaves W + 1 rows of sums a piece: a quarter
+// of what it reads with 16 bits and W 4, an eighth with pieces of 32, which it takes where there are enough of them
+// (4 x 2048 x 2048 channels, with the sums: pieces of 16 and of 32 43 us, of 64 56; 16000 x 4096 with 16 138, with 32 136).
 int conv_step(const ConvJob &job, bool backward) {
-    if (!backward)
-        return 16;
-    const int64_t rows = static_cast<int64_t>(job.seq.B) * job.seq.T * ((job.D + 7) / 8);
-    return rows >= (1 << 23) ? 64 : rows >= (1 << 21) ? 32 : 16;
+    const int64_t rows = static_cast<int64_t>(job.seq.B) * job.seq.T * ((job.D + 3) / 4);
+    return backward && rows >= (1 << 21) ? 32 : 16;
 }
 
 int64_t conv_layout(ConvJob &job, bool backward, char *base, ConvGrads *grads) {
