@@ -527,7 +527,9 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleJob job) {
     const uint64_t first = by_count ? static_cast<uint64_t>(k) : static_cast<uint64_t>(V);
     me.least = least > 0.0 ? (least < 1.0 ? least : 1.0) : 0.0;
     me.unit = job.unit, me.last_logit = -INFINITY, me.last_index = -1;
-    const double u = token ? static_cast<double>(job.random[r]) : 0.0;
+    // (below 0 draws as 0 does; from 1 on, or no number, the last kept token)
+    const float random = token ? job.random[r] : 0.f;
+    const double u = random < 0.f ? 0.0 : static_cast<double>(random);
     if (by_count ? k <= kListCount : !by_sum && me.least > 0.0) {
         float limit = me.top;
         if (by_count && k > 1) {

@@ -235,3 +235,13 @@ def test_graph_replays():
         torch.cuda.synchronize()
         want = f()
         assert torch.equal(tokens, want[0]) and torch.equal(probs, want[1])
+
+
+@pytest.mark.parametrize("V,kw", [(37, {}), (5000, dict(top_k=40)), (5000, dict(top_p=0.9)), (5000, dict(min_p=0.05)), (70001, {})])
+def test_random_numbers_out_of_range_draw_a_kept_token(V, kw):
+    from ramnet_ops import sample_tokens
+    logits = _logits(1, V, seed=7)[0].to(DEV).expand(6, V)
+    random = torch.tensor([0.0, -0.5, -math.inf, math.nan, 1.0, math.inf], device=DEV)
+    token, probs = sample_tokens(logits, random, probabilities=True, **kw)
+    kept = (probs[0] > 0).nonzero().flatten()
+    assert token.tolist() == [kept[0]] * 3 + [kept[-1]] * 3
