@@ -9,6 +9,8 @@
 #include "ramnet_kernels.hpp"
 #include "selective_scan.hpp"
 
+#include <algorithm>
+
 namespace ramnet {
 
 namespace {
@@ -200,9 +202,9 @@ __global__ __launch_bounds__(kThreads, 2) void scan_backward_kernel(const ScanJo
         const int64_t token = piece.t0, xr = piece.row * job.x_at[0], dr = piece.row * job.dt_at[0],
                       gr = piece.row * job.gate_at[0], yr = piece.row * grads.dy_at[0],
                       Br = piece.row * job.B_at[0] + at.group * job.B_at[2], Cr = piece.row * job.C_at[0] + at.group * job.C_at[2];
-        // (lanes without a channel read an x and a dy of 0, and so add nothing to the sums over channels)
-        const ScanRows<Scalar> x_rows(at, job.x_at[1], at.valid), dt_rows(at, job.dt_at[1], true), gate_rows(at, job.gate_at[1], true),
-            dy_rows(at, grads.dy_at[1], at.valid), d_rows(at, D, at.valid);
+        // (lanes without a channel read zeros, and so add nothing to the sums over channels)
+        const ScanRows<Scalar> x_rows(at, job.x_at[1], at.valid), dt_rows(at, job.dt_at[1], at.valid),
+            gate_rows(at, job.gate_at[1], at.valid), dy_rows(at, grads.dy_at[1], at.valid), d_rows(at, D, at.valid);
         const Groups B_rows(lane, job.B_at[1], job.S), C_rows(lane, job.C_at[1], job.S);
         uint32_t xs[kQuads], dts[kQuads], gates[kQuads], dys[kQuads], Bs[Groups::kLoads], Cs[Groups::kLoads];
         auto load = [&](int t) {
@@ -422,16 +424,16 @@ __global__ __launch_bounds__(kThreads, 2) void scan_backward_kernel(const ScanJo
 template<typename Scalar>
 __global__ __launch_bounds__(kThreads) void scan_groups_kernel(const ScanJob job, const ScanGrads grads, int blocks, int row) {
     const int64_t rows = static_cast<int64_t>(job.seq.B) * job.seq.T * job.G;
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-    if (i >= rows * row)
-        return;
-    float sum = 0.f;
-    for (int b = 0; b < blocks; ++b)
-        sum += grads.groups[b * rows * row + i];
-    const int64_t at = i / row;
-    const int e = static_cast<int>(i - at * row), which = e / (row / 2), n = e % (row / 2);
-    if (n < job.S)
-        store_f32(static_cast<Scalar *>(which ? grads.dC : grads.dB) + at * job.S + n, sum);
+    const int64_t threads = static_cast<int64_t>(gridDim.x) * kThreads;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < rows * row; i += threads) {
+        float sum = 0.f;
+        for (int b = 0; b < blocks; ++b)
+            sum += grads.groups[b * rows * row + i];
+        const int64_t at = i / row;
+        const int e = static_cast<int>(i - at * row), which = e / (row / 2), n = e % (row / 2);
+        if (n < job.S)
+            store_f32(static_cast<Scalar *>(which ? grads.dC : grads.dB) + at * job.S + n, sum);
+    }
 }
 
 // dA, dskip and dbias: likewise over the pieces (fewer where packed sequences have fewer).
@@ -439,7 +441,6 @@ __global__ __launch_bounds__(1024) void scan_sums_kernel(const ScanJob job, cons
     __shared__ float sums[16][kWave];
     const int lane = static_cast<int>(threadIdx.x) % kWave, wave = static_cast<int>(threadIdx.x) / kWave;
     const int64_t columns = static_cast<int64_t>(job.D) * row, column = static_cast<int64_t>(blockIdx.x) * kWave + lane;
-    TimePiece piece;
     float sum = 0.f;
     if (column < columns)
         for (int64_t p = wave; p < pieces; p += 16)
@@ -473,8 +474,9 @@ hipError_t launch_states(const ScanJob &job, const ScanGrads &grads, hipStream_t
     else
         hipLaunchKernelGGL((scan_backward_kernel<Scalar, NR, false>), grid, block, 0, stream, job, grads);
     const int64_t values = static_cast<int64_t>(job.seq.B) * job.seq.T * job.G * 8 * NR;
-    hipLaunchKernelGGL(scan_groups_kernel<Scalar>, dim3(static_cast<unsigned>((values + kThreads - 1) / kThreads)), block, 0,
-                       stream, job, grads, blocks, 8 * NR);
+    const int64_t value_blocks = std::min<int64_t>((values + kThreads - 1) / kThreads, 1 << 22);
+    hipLaunchKernelGGL(scan_groups_kernel<Scalar>, dim3(static_cast<unsigned>(value_blocks)), block, 0, stream, job, grads,
+                       blocks, 8 * NR);
     const int row = 4 * NR + 2;
     const int64_t columns = static_cast<int64_t>(job.D) * row;
     hipLaunchKernelGGL(scan_sums_kernel, dim3(static_cast<unsigned>((columns + kWave - 1) / kWave)), dim3(1024), 0, stream,

@@ -511,3 +511,18 @@ def test_gradients_graph_replays(T):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, grads(new)))
+
+
+def test_gradients_beside_an_infinite_gate():
+    """B and C are shared: an infinite gradient of one channel stays infinite over a block that has lanes to spare."""
+    case = [t.to(DEV) for t in _case(T=1, D=20)]
+    case[6][..., -1] = math.inf
+    B, C = case[3].requires_grad_(), case[4].requires_grad_()
+    y, _ = _run(case)
+    dB, dC = torch.autograd.grad(y, (B, C), torch.ones_like(y))
+    assert dB.isinf().all() and dC.isinf().all()
+
+
+@pytest.mark.parametrize("G,S,T", [(64, 64, 5), (300, 3, 70)])
+def test_gradients_many_groups(G, S, T):
+    _check_grads(_case(B=2, T=T, D=G, G=G, S=S))
