@@ -556,7 +556,7 @@ int ramnet_verify_drafts(const int64_t *tokens, const void *target, const void *
  * Short causal convolution of each channel over its last W tokens. No
  * counterpart in the reference.
  *     s[t, d] = bias[d] + sum_j weight[d, j] x[t - (W - 1) + j, d];   y = s, or silu(s)
- * `call` holds, all in `dtype`:
+ * `call` holds, all in `dtype`, D below 2^22:
  *   x              (B, T, D), last dimension dense, strides (elements): batch row, token
  *   weight, bias   (D, W), (D) or NULL; W from 1 to 8
  *   init_state     (N, W - 1, D) inputs before the first token, or NULL: zeros
@@ -612,7 +612,9 @@ int64_t ramnet_causal_conv_workspace_bytes(int64_t B, int64_t T, int64_t N, int6
  *   cu_seqlens, lengths  as above
  *   kept           NULL, or ramnet_selective_scan_kept_bytes for the backward
  *   workspace      ramnet_selective_scan_workspace_bytes
- *   strides        12: of x, dt, gate batch row and token, of Bm, Cm batch row, token and group
+ *   strides        12: of x, dt, gate batch row and token, of Bm, Cm batch row, token and group;
+ *                  tokens (dy's too) less than 2^22 elements apart
+ * D and G S are below 2^22, for very many rows or states less: the size queries tell.
  */
 typedef struct ramnet_selective_scan_call {
     const void *x, *dt, *gate, *Bm, *Cm;
@@ -653,8 +655,9 @@ int64_t ramnet_selective_scan_kept_bytes(int64_t B, int64_t T, int64_t N, int64_
  * the first top_k; of these, tokens with less than top_p times their sum before
  * them (at least one); tokens of w >= min_p. The token is the lowest index of a kept one
  * whose running sum, by index, passes random * sum.
- *   logits         (R, V) `dtype`, rows row_stride elements apart
- *   random         (R) fp32 uniform in [0, 1), or NULL where tokens is
+ *   logits         (R, V) `dtype`, rows row_stride elements apart; R below 2^22, V below 2^30
+ *   random         (R) fp32 uniform in [0, 1), or NULL where tokens is; below 0 it
+ *                  counts as 0, from 1 on (or a NaN) it draws the last kept token
  *   temperature, top_p, min_p  (R) fp32, or NULL: the value of all rows beside it;
  *                  temperature 0 (or below) takes the greatest logit, top_p of 1 and
  *                  min_p of 0 keep all

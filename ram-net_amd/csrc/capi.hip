@@ -1317,18 +1317,25 @@ static int check_sequences(ramnet::SequenceJob &seq, const char *what, int64_t B
     RAMNET_REQUIRE(B >= 0 && T >= 0 && N >= 0, std::string(what) + " shape must have B, T, N >= 0");
     RAMNET_REQUIRE(packed ? B == 1 : N == B,
                    std::string(what) + ": packed sequences lie in a batch of one, others one to a row");
-    RAMNET_REQUIRE(fits_int({B, T, N, B * T, T + N + 64}), std::string(what) + ": index overflow");
+    RAMNET_REQUIRE(fits_int({B, T, N, B * T, T + N + 4096}), std::string(what) + ": index overflow");
     seq.B = static_cast<int>(B), seq.T = static_cast<int>(T), seq.N = static_cast<int>(N);
     return RAMNET_OK;
 }
+
+// Pieces of up to `step` tokens that a call has at most. A launch has less than 2^32 threads.
+static int64_t pieces_at_most(const ramnet::SequenceJob &seq, bool packed, int step) {
+    return packed ? seq.T / step + seq.N + 2LL : static_cast<int64_t>(seq.B) * ramnet::pieces_of(seq.T, step);
+}
+constexpr int64_t kMaxThreads = (1LL << 32) - 1024;
 
 static int check_conv(ramnet::ConvJob &job, int64_t B, int64_t T, int64_t N, int64_t D, int64_t W, bool packed) {
     if (int rc = check_sequences(job.seq, "causal_conv", B, T, N, packed))
         return rc;
     RAMNET_REQUIRE(D > 0 && W > 0 && W <= ramnet::kConvMaxWidth, "causal_conv: D must be above 0 and W from 1 to 8");
     RAMNET_REQUIRE(D < (1LL << 22), "causal_conv: index overflow");
-    // (threads of a launch: a piece of 16 tokens and 16 bytes of channels each)
-    RAMNET_REQUIRE((B * (T / 16 + 1) + N + 2) * ((D + 3) / 4) < (1LL << 36), "causal_conv: index overflow");
+    // (a thread takes four channels at least of a piece of 16 tokens, or one where there are few)
+    RAMNET_REQUIRE(pieces_at_most(job.seq, packed, 16) <= kMaxThreads / (D < 8 ? D : (D + 3) / 4),
+                   "causal_conv: index overflow");
     job.D = static_cast<int>(D), job.W = static_cast<int>(W);
     return RAMNET_OK;
 }
@@ -1397,8 +1404,11 @@ static int check_scan(ramnet::ScanJob &job, int64_t B, int64_t T, int64_t N, int
     RAMNET_REQUIRE(S > 0 && S <= ramnet::kScanMaxStates, "selective_scan: S must be from 1 to 64");
     RAMNET_REQUIRE(D < ramnet::kScanStride && G * S < ramnet::kScanStride, "selective_scan: index overflow");
     job.D = static_cast<int>(D), job.S = static_cast<int>(S), job.G = static_cast<int>(G);
-    // blocks of a launch (64 channels of a piece of 64 tokens or more, or of a row) are counted in 32 bits
-    RAMNET_REQUIRE((B * (T / 64 + 1) + N + 2) * G * ((D / G + 63) / 64) < kIntMax, "selective_scan: index overflow");
+    // (a block takes 64 channels of a group and of a piece of 64 tokens or more)
+    RAMNET_REQUIRE(pieces_at_most(job.seq, packed, 64) <= kMaxThreads / 256 / (G * ((D / G + 63) / 64)),
+                   "selective_scan: index overflow");
+    // (the backward's sums over pieces: a block 64 of them)
+    RAMNET_REQUIRE(D * (4LL * ramnet::scan_lane_states(job.S) + 2) <= kMaxThreads / 16 - 64, "selective_scan: index overflow");
     return RAMNET_OK;
 }
 
@@ -1490,7 +1500,7 @@ int ramnet_sample_tokens(const ramnet_sample_tokens_call *call, void *stream) {
     RAMNET_REQUIRE(call, "null call");
     const ramnet_sample_tokens_call &c = *call;
     RAMNET_REQUIRE(c.R >= 0 && c.V > 0, "sample_tokens shape must have R >= 0 and V > 0");
-    RAMNET_REQUIRE(c.R < kIntMax && c.V < (1LL << 30), "sample_tokens: index overflow");
+    RAMNET_REQUIRE(c.R < (1LL << 22) && c.V < (1LL << 30), "sample_tokens: index overflow");
     RAMNET_REQUIRE(valid_dtype(static_cast<int>(c.dtype)), "sample_tokens dtype must be float32, float16 or bfloat16");
     if (c.R == 0)
         return RAMNET_OK;

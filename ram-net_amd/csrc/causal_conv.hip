@@ -151,8 +151,8 @@ __global__ __launch_bounds__(kThreads) void conv_kernel(const ConvJob job, int64
 // Gradients of a piece's inputs, and its sums of dweight and dbias. The inputs' convolution is made again; a gradient
 // is whole W - 1 tokens later, also where these lie in the next piece.
 template<typename Scalar, int W, int VEC>
-__global__ __launch_bounds__(kThreads, W <= 4 && sizeof(Scalar) == 2 ? 4 : 2) void conv_backward_kernel(const ConvJob job, const ConvGrads grads,
-                                                                 int64_t pieces) {
+__global__ __launch_bounds__(kThreads, W <= 4 && sizeof(Scalar) == 2 ? 4 : 2) void conv_backward_kernel(
+    const ConvJob job, const ConvGrads grads, int64_t pieces) {
     ConvPlace<VEC> at;
     TimePiece piece;
     if (!at.find(job, pieces))

@@ -249,3 +249,34 @@ def test_workspace_queries():
     assert lib.ramnet_selective_scan_kept_bytes(2, 8, 3, 16, 4, 1, 0) == -1
     for kind in range(3):
         assert lib.ramnet_selective_scan_workspace_bytes(0, 500, 0, 16, 4, 1, 0, kind) >= 0
+
+
+def test_sizes_past_a_launch():
+    """A launch has less than 2^32 threads: rows, sequences or channels past it are refused before any launch."""
+    lib, mega = _native().lib(), 2 ** 20
+    conv, scan = lib.ramnet_causal_conv_workspace_bytes, lib.ramnet_selective_scan_workspace_bytes
+    # a thread takes 4 channels of a row, or one of up to 7
+    assert conv(3 * mega, 1, 3 * mega, 4096, 4, 2, 0, 0) == 0
+    assert conv(4 * mega, 1, 4 * mega, 4096, 4, 2, 0, 0) == -1
+    assert conv(1024 * mega - 1, 1, 1024 * mega - 1, 3, 4, 2, 0, 0) == 0
+    assert conv(1024 * mega - 1, 1, 1024 * mega - 1, 4, 4, 2, 0, 0) == -1
+    assert conv(1, 16, 4 * mega, 4096, 4, 2, 1, 0) == -1
+    # 256 threads take 64 channels
+    assert scan(200000, 1, 200000, 4096, 16, 1, 0, 0) == 0
+    assert scan(270000, 1, 270000, 4096, 16, 1, 0, 0) == -1
+    assert scan(5000, 1, 5000, 4096, 16, 4096, 0, 0) == -1
+    assert scan(1, 1, 270000, 4096, 16, 1, 1, 0) == -1
+    # 1024 threads add up 64 sums over pieces
+    assert scan(1, 1, 1, 4 * mega - 1, 32, 1, 0, 2) > 0
+    assert scan(1, 1, 1, 4 * mega - 1, 64, 1, 0, 2) == -1
+    _einval("ramnet_sample_tokens", (_sample_call(R=4 * mega), None), "index overflow")
+
+
+def test_scan_tokens_far_apart():
+    strides = [80 * 16, 16, 0, 0, 0, 0] + [0] * 6
+    for i in (1, 3, 5, 7, 10):
+        far = list(strides)
+        far[i] = 2 ** 22
+        call = struct.pack("=15Q2q20q", FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 0, 0, 0, FAKE, FAKE, 0, 0, 0, FAKE, 0, 1 << 30,
+                           1, 80, 1, 16, 4, 1, *far, 0, 0)
+        _einval("ramnet_selective_scan_forward", (call, None), "2\\*\\*22 elements apart")
