@@ -430,7 +430,9 @@ struct Sampler {
 
     // The order of the k-th token, or of the last one with less than `target` before it, in the bin that find_bin
     // has found: as long as it holds more tokens than the list, it is cut into 2048 parts again, now by the order.
-    __device__ __forceinline__ uint64_t find_border(uint64_t k, double target) {
+    // `through`: with a target the weights up to that one, it among them (0: not known).
+    __device__ __forceinline__ uint64_t find_border(uint64_t k, double target, uint64_t &through) {
+        through = 0;
         const int level = lds().bin;
         const bool by_sum = target > 0.0;
         uint64_t base = by_sum ? lds().before : 0, lo = 0, hi = ~0ull;
@@ -480,9 +482,10 @@ struct Sampler {
         if (tid < members) {
             const double from = static_cast<double>(before), to = static_cast<double>(before + part);
             if (by_sum ? from < target && (to >= target || tid == members - 1) : static_cast<uint64_t>(count + tid + 1) == k)
-                lds().order = own;
+                lds().order = own, lds().before = before + part;
         }
         __syncthreads();
+        through = by_sum ? lds().before : 0;
         return lds().order;
     }
 };
@@ -546,6 +549,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleJob job) {
             return;
         }
     }
+    uint64_t kept_sum = 0;  // of the kept weights, where the search for the last one gives it
     if (by_count) {
         const float range = me.top - me.block_reduce(low, Least{});
         me.scale = range > 0.f && range < INFINITY ? static_cast<float>(kBins - 1) / range : 0.f;
@@ -559,7 +563,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleJob job) {
             me.finish(members, first, by_sum, p, 0, u, token, probs);
             return;
         }
-        me.end_with(me.find_border(first, 0.0));
+        me.end_with(me.find_border(first, 0.0, kept_sum));
     }
     if (by_sum) {
         me.scale = static_cast<float>(me.rate) * kBinsAHalving;
@@ -600,7 +604,9 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleJob job) {
                     return;
                 }
             }
-            me.end_with(me.find_border(0, target));
+            me.end_with(me.find_border(0, target, kept_sum));
+            if (me.weight(me.last_logit) < me.least)  // (min_p keeps fewer)
+                kept_sum = 0;
         }
     }
     // The kept weights by stretches of the vocabulary, a wave each, in order of the index: whole pieces of 16 bytes,
@@ -612,8 +618,16 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleJob job) {
         double w;
         return me.kept(l, i, w) ? me.whole(w) : 0;
     };
+    auto value = [&](double w, double inv) { return static_cast<float>(w * inv); };
+    auto put = [&](int at, const float (&out)[N]) {
+#pragma unroll
+        for (int e = 0; e < N; e += 4) {
+            const float four[4] = {out[e], out[e + 1], out[e + 2], out[e + 3]};
+            store_vec<float, 4>(probs + at + e, round_vec<float, 4>(four));
+        }
+    };
     uint64_t sum = wave == kWaves - 1 && full + lane < V ? share(load_f32(me.row + full + lane), full + lane) : 0;
-    auto stretch = [&](auto of) {
+    auto stretch = [&](auto of, auto then) {
         Vec<Scalar, N> next{};
         if (lo + lane * N < hi)
             next = load_vec<Scalar, N>(me.row + lo + lane * N);
@@ -621,15 +635,32 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleJob job) {
             const Vec<Scalar, N> x = next;
             if (at + kWave * N < hi)
                 next = load_vec<Scalar, N>(me.row + at + kWave * N);
+            float out[N];
 #pragma unroll
             for (int e = 0; e < N; ++e)
-                sum += of(x[e], at + e);
+                sum += of(x[e], at + e, out[e]);
+            then(at, out);
         }
     };
-    if (!by_count && !by_sum && me.least == 0.0)
-        stretch([&](float l, int) { return me.whole(me.weight(l)); });
-    else
-        stretch(share);
+    // Where their sum is known the probabilities go out in the same pass (a row of 128257, top_p of 0.9: 121 us for 149).
+    const auto nothing = [](int, const float(&)[N]) {};
+    if (probs && kept_sum) {
+        const double inv = me.unit / static_cast<double>(kept_sum);
+        stretch(
+            [&](float l, int i, float &out) -> uint64_t {
+                double w;
+                out = 0.f;
+                if (!me.kept(l, i, w))
+                    return 0;
+                out = value(w, inv);
+                return me.whole(w);
+            },
+            put);
+    } else if (!by_count && !by_sum && me.least == 0.0) {
+        stretch([&](float l, int, float &) { return me.whole(me.weight(l)); }, nothing);
+    } else {
+        stretch([&](float l, int i, float &) { return share(l, i); }, nothing);
+    }
     sum = wave_reduce(sum, Sum{});
     __syncthreads();
     if (lane == 0)
@@ -673,21 +704,20 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleJob job) {
     }
     if (probs) {
         const double inv = me.unit / total;
-        auto value = [&](float l, int i) {
+        auto of = [&](float l, int i) {
             double w;
-            return me.kept(l, i, w) ? static_cast<float>(w * inv) : 0.f;
+            return me.kept(l, i, w) ? value(w, inv) : 0.f;
         };
-        for (int at = tid * N; at < full; at += kThreads * N) {
+        for (int at = tid * N; at < full && !kept_sum; at += kThreads * N) {
             const Vec<Scalar, N> x = load_vec<Scalar, N>(me.row + at);
+            float out[N];
 #pragma unroll
-            for (int e = 0; e < N; e += 4) {
-                const float out[4] = {value(x[e], at + e), value(x[e + 1], at + e + 1), value(x[e + 2], at + e + 2),
-                                      value(x[e + 3], at + e + 3)};
-                store_vec<float, 4>(probs + at + e, round_vec<float, 4>(out));
-            }
+            for (int e = 0; e < N; ++e)
+                out[e] = of(x[e], at + e);
+            put(at, out);
         }
         if (full + tid < V)
-            probs[full + tid] = value(load_f32(me.row + full + tid), full + tid);
+            probs[full + tid] = of(load_f32(me.row + full + tid), full + tid);
     }
 }
 
