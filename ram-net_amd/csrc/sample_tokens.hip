@@ -205,7 +205,7 @@ struct Sampler {
 
     // (what is no number, as a difference of -inf or nothing times 0, is held to where no part of the sum is left)
     __device__ __forceinline__ double weight(float l) const {
-        const double x = (static_cast<double>(l) - static_cast<double>(top)) * rate;
+        const double x = fma(static_cast<double>(l), rate, -static_cast<double>(top) * rate);
         return power_of_2(l == top ? 0.0 : __builtin_fmax(x, -1000.0));
     }
     // A weight in whole parts of 1 / unit, below 2^52: they are the last bits of its sum with 2^52.
@@ -221,7 +221,8 @@ struct Sampler {
         return l > last_logit || (l == last_logit && index <= last_index);
     }
     __device__ __forceinline__ void end_with(uint64_t order) { last_logit = logit_of(order), last_index = index_of(order); }
-    // Whether a token is drawn from.
+    // Whether a token is drawn from. (A branch around the weight: without it rows that keep few took up to 15 us
+    // more, those that keep most no less.)
     __device__ __forceinline__ bool kept(float l, int index, double &w) const {
         if (!within(l, index))
             return false;
@@ -437,7 +438,12 @@ struct Sampler {
         const bool by_sum = target > 0.0;
         uint64_t base = by_sum ? lds().before : 0, lo = 0, hi = ~0ull;
         int count = by_sum ? 0 : lds().count_before;
-        int members = gather([&](float l, int i) { return bin(l) == level && within(l, i); });
+        // (two comparisons tell most tokens from those of the bin, which lie between these by more than the roundings)
+        const float slack = fabsf(top) * 1e-6f + static_cast<float>(level + 1) / scale * 1e-6f;
+        const bool narrow = scale > 0.f && slack < INFINITY;
+        const float high = narrow ? top - static_cast<float>(level) / scale + slack : INFINITY;
+        const float low = narrow && level < kBins - 1 ? top - static_cast<float>(level + 1) / scale - slack : -INFINITY;
+        int members = gather([&](float l, int i) { return l >= low && l <= high && bin(l) == level && within(l, i); });
         if (members > kList) {
             uint64_t least_o = ~0ull, most_o = 0;
             sweep([&](float l, int i) {
@@ -533,11 +539,13 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleJob job) {
     // (below 0 draws as 0 does; from 1 on, or no number, the last kept token)
     const float random = token ? job.random[r] : 0.f;
     const double u = random < 0.f ? 0.0 : static_cast<double>(random);
-    if (by_count ? k <= kListCount : !by_sum && me.least > 0.0) {
+    // A list of those that top_k or min_p may keep
+    const bool few = by_count && k <= kListCount;
+    if (few || (me.least > 0.0 && !by_sum)) {
         float limit = me.top;
-        if (by_count && k > 1) {
+        if (few && k > 1) {
             limit = me.limit_of(mine, static_cast<int>(k));
-        } else if (!by_count) {
+        } else if (!few) {
             // below the logit of weight min_p by more than the roundings on the way
             const double cut = static_cast<double>(me.top) + log2(me.least) / me.rate;
             limit = static_cast<float>(cut - (fabs(cut) + fabs(static_cast<double>(me.top))) * 1e-6 - 1e-37);
@@ -591,22 +599,38 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleJob job) {
         __syncthreads();
         const double target = p * static_cast<double>(all);
         if (me.find_bin(0, target, 0, 0)) {
-            const int level = lds().bin;
+            // min_p ends in bin `cut` or one beside it, by the roundings of a token's bin
+            const int cut = me.least > 0.0 ? static_cast<int>(__builtin_fmin(-log2(me.least) * kBinsAHalving, kBins)) : kBins;
+            const bool by_least = cut + 1 < lds().bin;  // before top_p does
+            const int level = by_least ? cut + 1 : lds().bin;
             // No weight is above its bin's first: a sum takes so many tokens at least. Where these fit the list, so
             // may all of them.
             double tokens = 0.0;
-            for (int i = tid; i <= level; i += kThreads)
+            uint64_t over = 0;  // of those that min_p keeps for sure
+            for (int i = tid; i <= level; i += kThreads) {
                 tokens += static_cast<double>(lds().sums[i]) * exp2(i / static_cast<double>(kBinsAHalving));
-            if (me.block_reduce(tokens, Sum{}) < kList * me.unit) {
+                over += i < cut - 1 ? lds().sums[i] : 0;
+            }
+            me.block_reduce(tokens, Sum{}, over, Sum{});
+            if (tokens < kList * me.unit) {
                 const int members = me.gather([&](float l, int i) { return me.bin(l) <= level && me.within(l, i); });
                 if (members <= kList) {
                     me.finish(members, static_cast<uint64_t>(V), true, p, all, u, token, probs);
                     return;
                 }
             }
-            me.end_with(me.find_border(0, target, kept_sum));
-            if (me.weight(me.last_logit) < me.least)  // (min_p keeps fewer)
-                kept_sum = 0;
+            if (!by_least)
+                me.end_with(me.find_border(0, target, kept_sum));
+            if (by_least || me.weight(me.last_logit) < me.least) {
+                uint64_t more = 0;
+                me.sweep([&](float l, int i) {
+                    const int b = me.bin(l);
+                    double w;
+                    if (b >= cut - 1 && b <= cut + 1 && me.kept(l, i, w))
+                        more += me.whole(w);
+                });
+                kept_sum = over + me.block_reduce(more, Sum{});
+            }
         }
     }
     // The kept weights by stretches of the vocabulary, a wave each, in order of the index: whole pieces of 16 bytes,
@@ -618,7 +642,10 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleJob job) {
         double w;
         return me.kept(l, i, w) ? me.whole(w) : 0;
     };
-    auto value = [&](double w, double inv) { return static_cast<float>(w * inv); };
+    auto value = [&](float l, int i, double inv) {
+        double w;
+        return me.kept(l, i, w) ? static_cast<float>(w * inv) : 0.f;
+    };
     auto put = [&](int at, const float (&out)[N]) {
 #pragma unroll
         for (int e = 0; e < N; e += 4) {
@@ -642,7 +669,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleJob job) {
             then(at, out);
         }
     };
-    // Where their sum is known the probabilities go out in the same pass (a row of 128257, top_p of 0.9: 121 us for 149).
+    // Where their sum is known the probabilities go out in the same pass (rows of 128257, top_p of 0.9: 115 us for 149).
     const auto nothing = [](int, const float(&)[N]) {};
     if (probs && kept_sum) {
         const double inv = me.unit / static_cast<double>(kept_sum);
@@ -652,7 +679,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleJob job) {
                 out = 0.f;
                 if (!me.kept(l, i, w))
                     return 0;
-                out = value(w, inv);
+                out = static_cast<float>(w * inv);
                 return me.whole(w);
             },
             put);
@@ -684,40 +711,50 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleJob job) {
             seen = next;
         }
         const int from = min(at * part, full), to = at == kWaves - 1 ? V : min(from + part, full);
-        const int each = (to - from + kThreads - 1) / kThreads, begin = min(from + tid * each, to), end = min(begin + each, to);
-        uint64_t own = 0;
-        for (int i = begin; i < end; ++i)
-            own += share(load_f32(me.row + i), i);
-        uint64_t run = before + me.block_scan(own, 1);
+        // The stretch in turns of N tokens a thread, until the sum passes; where it never does, its last with a weight
         int found = V, last = -1;
-        for (int i = begin; i < end && found == V; ++i) {
-            const uint64_t x = share(load_f32(me.row + i), i);
-            run += x;
-            if (x > 0) {
-                last = i;
-                found = static_cast<double>(run) > threshold ? i : V;
+        for (int base = from; base < to && found == V; base += kThreads * N) {
+            const int begin = base + tid * N;
+            Vec<Scalar, N> x{};
+            if (begin + N <= V)
+                x = load_vec<Scalar, N>(me.row + begin);
+            uint64_t parts_of[N], own = 0;
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const int i = begin + e;
+                const float l = begin + N <= V ? x[e] : i < V ? load_f32(me.row + i) : 0.f;
+                parts_of[e] = share(l, i);
+                parts_of[e] = i < to ? parts_of[e] : 0;
+                own += parts_of[e];
             }
+            uint64_t run = before + me.block_scan(own, 1);
+            int here = V, latest = -1;
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                run += parts_of[e];
+                const bool on = parts_of[e] > 0;
+                latest = on ? begin + e : latest;
+                here = on && here == V && static_cast<double>(run) > threshold ? begin + e : here;
+            }
+            before += me.block_reduce(own, Sum{});
+            me.block_reduce(here, Least{}, latest, Most{});
+            found = here, last = max(last, latest);
         }
-        me.block_reduce(found, Least{}, last, Most{});
         if (tid == 0)
             *token = found < V ? found : last;
     }
     if (probs) {
         const double inv = me.unit / total;
-        auto of = [&](float l, int i) {
-            double w;
-            return me.kept(l, i, w) ? value(w, inv) : 0.f;
-        };
         for (int at = tid * N; at < full && !kept_sum; at += kThreads * N) {
             const Vec<Scalar, N> x = load_vec<Scalar, N>(me.row + at);
             float out[N];
 #pragma unroll
             for (int e = 0; e < N; ++e)
-                out[e] = of(x[e], at + e);
+                out[e] = value(x[e], at + e, inv);
             put(at, out);
         }
         if (full + tid < V)
-            probs[full + tid] = of(load_f32(me.row + full + tid), full + tid);
+            probs[full + tid] = value(load_f32(me.row + full + tid), full + tid, inv);
     }
 }
 

@@ -237,6 +237,22 @@ def test_graph_replays():
         assert torch.equal(tokens, want[0]) and torch.equal(probs, want[1])
 
 
+@pytest.mark.parametrize("kw", [dict(min_p=0.02, top_p=0.9, temperature=1.5), dict(min_p=1e-4, top_p=0.97, temperature=1.5),
+                                dict(min_p=1e-3, top_p=0.999), dict(top_k=30000, min_p=1e-3, top_p=0.99),
+                                dict(min_p=0.5, top_p=0.01), dict(min_p=1e-9, top_p=0.5, temperature=3.0)], ids=str)
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("spread", [0.5, 2.0])
+def test_min_p_beside_top_p(kw, dtype, spread):
+    """Either one ends first, in a list or far past one."""
+    _check(*_logits(3, 50021, dtype, seed=9, spread=spread), **kw)
+
+
+@pytest.mark.parametrize("V", [8192 * 16, 8192 * 16 + 1, 8192 * 40 + 13])
+def test_drawn_tokens_of_long_rows(V):
+    logits, _ = _logits(5, V, "bf16", seed=3)
+    _check(logits, torch.tensor([0.0, 0.13, 0.5, 0.77, 1 - 2.0 ** -24]))
+
+
 @pytest.mark.parametrize("V,kw", [(37, {}), (5000, dict(top_k=40)), (5000, dict(top_p=0.9)), (5000, dict(min_p=0.05)), (70001, {})])
 def test_random_numbers_out_of_range_draw_a_kept_token(V, kw):
     from ramnet_ops import sample_tokens
