@@ -158,8 +158,13 @@ __device__ __forceinline__ void reread() {
 template<int NR>
 constexpr int scan_part() { return NR <= 2 ? kTile : NR <= 4 ? kTile / 2 : kTile / 4; }
 
+// Waves a SIMD, and by that registers: 256 a lane spill from 24 states on (4 x 2048 x 2048 channels; 24 states 744 us
+// with two waves, 779 with one; 32 states 979 and 784; 48 states 3004 and 1310; of 64 the LDS holds one block anyway).
+template<int NR>
+constexpr int scan_waves() { return NR >= 8 ? 1 : 2; }
+
 template<typename Scalar, int NR, bool kGate>
-__global__ __launch_bounds__(kThreads, 2) void scan_backward_kernel(const ScanJob job, const ScanGrads grads) {
+__global__ __launch_bounds__(kThreads, scan_waves<NR>()) void scan_backward_kernel(const ScanJob job, const ScanGrads grads) {
     using Groups = ScanGroups<Scalar, NR>;
     constexpr int kPart = scan_part<NR>(), kParts = kTile / kPart, kRow = Groups::kRow, kFloats = Groups::kFloats;
     constexpr int kSpread = 2 * kRow;  // dB and dC of a token
