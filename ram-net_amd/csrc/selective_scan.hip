@@ -184,62 +184,112 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(const ScanJob job) {
             store_vec<Scalar, 1>(y + static_cast<int64_t>(piece.len + i) * job.D, {{0u}});
 }
 
-// Decode steps of up to kScanStepTokens tokens, bound by reading and writing the states: no staging, one wave
-// 16 channels of one sequence.
+// NR values of a token's B or C, those past S zero.
 template<typename Scalar, int NR>
-__global__ __launch_bounds__(kThreads) void scan_step_kernel(const ScanJob job) {
-    const ScanPlace at(job);
-    const int b = at.piece, sub = at.sub, channel = at.channel, n0 = sub * NR, count = job.S - n0;
-    const int T = job.seq.T, len = job.seq.lengths ? clamped(job.seq.lengths[b], 0, T) : T;
-    float h[NR], A2[NR];
-    const int64_t where = (static_cast<int64_t>(b) * job.D + channel) * job.S + n0;
-    if (job.init) {
-        load_states<NR>(h, job.init + where, count);
-    } else {
+__device__ __forceinline__ void load_group(float (&to)[NR], const Scalar *p, int count) {
+    if constexpr (NR * sizeof(Scalar) % 4 == 0) {
+        if (count >= NR) {
+            const Vec<Scalar, NR> v = load_vec<Scalar, NR>(p);
 #pragma unroll
-        for (int j = 0; j < NR; ++j)
-            h[j] = 0.f;
+            for (int j = 0; j < NR; ++j)
+                to[j] = v[j];
+            return;
+        }
     }
+#pragma unroll
+    for (int j = 0; j < NR; ++j)
+        to[j] = j < count ? load_f32(p + j) : 0.f;
+}
+
+// Decode steps of up to kScanStepTokens tokens, bound by reading and writing the states: no staging, one wave
+// 16 channels of a sequence, and of others where the grid has fewer rows than the batch (its rates are read once).
+// kOne: of one token, which all lanes of a channel prepare alike; otherwise each prepares one of four.
+template<typename Scalar, int NR, bool kOne>
+__global__ __launch_bounds__(kThreads) void scan_step_kernel(const ScanJob job, int rows) {
+    const ScanPlace at(job);
+    const int sub = at.sub, channel = at.channel, n0 = sub * NR, count = job.S - n0, T = kOne ? 1 : job.seq.T;
+    float A2[NR];
     load_states<NR>(A2, job.A + static_cast<int64_t>(channel) * job.S + n0, count);
 #pragma unroll
     for (int j = 0; j < NR; ++j)
         A2[j] *= kLog2e;
     const float bias = job.bias ? job.bias[channel] : 0.f, skip = job.skip ? job.skip[channel] : 0.f;
-    const Scalar *x = static_cast<const Scalar *>(job.x) + b * job.x_at[0] + channel;
-    const Scalar *dt = static_cast<const Scalar *>(job.dt) + b * job.dt_at[0] + channel;
-    const Scalar *gate = job.gate ? static_cast<const Scalar *>(job.gate) + b * job.gate_at[0] + channel : nullptr;
-    const Scalar *B = static_cast<const Scalar *>(job.B) + b * job.B_at[0] + at.group * job.B_at[2];
-    const Scalar *C = static_cast<const Scalar *>(job.C) + b * job.C_at[0] + at.group * job.C_at[2];
-    Scalar *y = static_cast<Scalar *>(job.y) + static_cast<int64_t>(b) * T * job.D + channel;
-    for (int t = 0; t < T; ++t) {
-        float out = 0.f;
-        if (t < len) {
-            const float xv = load_f32(x + t * job.x_at[1]);
-            float d = load_f32(dt + t * job.dt_at[1]) + bias, e, s = 0.f;
-            d = job.softplus ? softplus(d, e) : d;
-            const float u = d * xv;
+    for (int b = at.piece; b < job.seq.B; b += rows) {
+        const int len = job.seq.lengths ? clamped(job.seq.lengths[b], 0, T) : T, last = max(len - 1, 0);
+        float h[NR];
+        const int64_t where = (static_cast<int64_t>(b) * job.D + channel) * job.S + n0;
+        if (job.init) {
+            load_states<NR>(h, job.init + where, count);
+        } else {
 #pragma unroll
-            for (int j = 0; j < NR; ++j) {
-                const bool on = j < count;
-                const float bv = on ? load_f32(B + t * job.B_at[1] + n0 + j) : 0.f;
-                const float cv = on ? load_f32(C + t * job.C_at[1] + n0 + j) : 0.f;
-                h[j] = fmaf(__builtin_amdgcn_exp2f(d * A2[j]), h[j], u * bv);
-                s = fmaf(cv, h[j], s);
-            }
-            s += quad_swap<1>(s);
-            s += quad_swap<2>(s);
-            out = fmaf(skip, xv, s);
-            if (gate) {
-                const float g = load_f32(gate + t * job.gate_at[1]);
-                out *= g * sigmoid(g);
-            }
+            for (int j = 0; j < NR; ++j)
+                h[j] = 0.f;
         }
-        if (sub == 0 && at.valid)
-            store_vec<Scalar, 1>(y + static_cast<int64_t>(t) * job.D, {{round_bits<Scalar>(out)}});
+        const Scalar *x = static_cast<const Scalar *>(job.x) + b * job.x_at[0] + channel;
+        const Scalar *dt = static_cast<const Scalar *>(job.dt) + b * job.dt_at[0] + channel;
+        const Scalar *gate = static_cast<const Scalar *>(job.gate) + b * job.gate_at[0] + channel;
+        const Scalar *B = static_cast<const Scalar *>(job.B) + b * job.B_at[0] + at.group * job.B_at[2] + n0;
+        const Scalar *C = static_cast<const Scalar *>(job.C) + b * job.C_at[0] + at.group * job.C_at[2] + n0;
+        Scalar *y = static_cast<Scalar *>(job.y) + static_cast<int64_t>(b) * T * job.D + channel;
+        constexpr int kTokens = kOne ? 1 : 4, kDeep = kOne ? 1 : NR <= 4 ? 4 : NR <= 8 ? 2 : 1;
+        for (int t0 = 0; t0 < T; t0 += kTokens) {
+            const int t = kOne ? 0 : t0 + sub, from = min(t, last);  // (what is read of no token that counts goes nowhere)
+            const float xv = load_f32(x + from * job.x_at[1]);
+            const float raw = load_f32(dt + from * job.dt_at[1]) + bias;
+            const float gv = job.gate ? load_f32(gate + from * job.gate_at[1]) : 0.f;
+            float sums[4] = {}, d = raw, e, b_of[kDeep][NR], c_of[kDeep][NR];
+            auto fetch = [&](int k0) {
+#pragma unroll
+                for (int k = 0; k < kDeep; ++k) {
+                    const int at_token = min(t0 + k0 + k, last);
+                    load_group<Scalar, NR>(b_of[k], B + at_token * job.B_at[1], count);
+                    load_group<Scalar, NR>(c_of[k], C + at_token * job.C_at[1], count);
+                }
+            };
+            fetch(0);
+            if (job.softplus)
+                d = softplus(raw, e);
+            const float u = d * xv;
+            auto token = [&](auto k_) {
+                constexpr int k = decltype(k_)::value;
+                if constexpr (k > 0 && k % kDeep == 0)
+                    fetch(k);
+                if (t0 + k >= len)
+                    return;
+                const float dk = kOne ? d : quad_lane<k>(d), uk = kOne ? u : quad_lane<k>(u);
+#pragma unroll
+                for (int j = 0; j < NR; ++j) {
+                    h[j] = fmaf(__builtin_amdgcn_exp2f(dk * A2[j]), h[j], uk * b_of[k % kDeep][j]);
+                    sums[k] = fmaf(c_of[k % kDeep][j], h[j], sums[k]);
+                }
+            };
+            token(std::integral_constant<int, 0>{});
+            if constexpr (!kOne) {
+                token(std::integral_constant<int, 1>{});
+                token(std::integral_constant<int, 2>{});
+                token(std::integral_constant<int, 3>{});
+            }
+            float s = sums[0];
+            if constexpr (kOne) {
+                s += quad_swap<1>(s);
+                s += quad_swap<2>(s);
+            } else {
+                s = quad_sums(sums, sub);
+            }
+            float out = fmaf(skip, xv, s);
+            if (job.gate)
+                out *= gv * sigmoid(gv);
+            if (at.valid && t < T && (!kOne || sub == 0))
+                store_vec<Scalar, 1>(y + static_cast<int64_t>(t) * job.D, {{round_bits<Scalar>(t < len ? out : 0.f)}});
+        }
+        if (at.valid)
+            store_states<NR>(job.state + where, h, count);
     }
-    if (at.valid)
-        store_states<NR>(job.state + where, h, count);
 }
+
+// Blocks of a decode step, past which they take several rows (2048 channels of 16 states, one token: 256 rows 18.6 us,
+// a row a block 22.3; 2048 rows 126 for 155; blocks of 8192 22.4 and 128).
+constexpr unsigned kStepBlocks = 4096;
 
 // Blocks of a launch over `pieces` pieces.
 unsigned blocks_of(const ScanJob &job, int64_t pieces) {
@@ -250,7 +300,12 @@ template<typename Scalar, int NR>
 hipError_t launch_states(const ScanJob &job, hipStream_t stream) {
     const dim3 block(kThreads);
     if (scan_is_step(job)) {
-        hipLaunchKernelGGL((scan_step_kernel<Scalar, NR>), dim3(blocks_of(job, job.seq.B)), block, 0, stream, job);
+        const unsigned per_row = blocks_of(job, 1);
+        const int rows = std::min(job.seq.B, static_cast<int>((kStepBlocks + per_row - 1) / per_row));
+        if (job.seq.T == 1)
+            hipLaunchKernelGGL((scan_step_kernel<Scalar, NR, true>), dim3(rows * per_row), block, 0, stream, job, rows);
+        else
+            hipLaunchKernelGGL((scan_step_kernel<Scalar, NR, false>), dim3(rows * per_row), block, 0, stream, job, rows);
         return hipGetLastError();
     }
     const dim3 grid(blocks_of(job, most_pieces(job.seq, job.step)));

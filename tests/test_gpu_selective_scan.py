@@ -526,3 +526,29 @@ def test_gradients_beside_an_infinite_gate():
 @pytest.mark.parametrize("G,S,T", [(64, 64, 5), (300, 3, 70)])
 def test_gradients_many_groups(G, S, T):
     _check_grads(_case(B=2, T=T, D=G, G=G, S=S))
+
+
+@pytest.mark.parametrize("T", [1, 3, 4, 5, 8])
+@pytest.mark.parametrize("D,S,G", [(40, 16, 1), (36, 10, 3), (20, 64, 2), (7, 3, 1), (130, 48, 1), (24, 24, 2)])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_steps_of_all_sizes(T, D, S, G, dtype):
+    case = _case(B=3, T=T, D=D, S=S, G=G, dtype=dtype, seed=T)
+    _check(case, _call(case))
+    lens = [0, T, (T + 1) // 2]
+    case[1][2, lens[2]:], case[4][2, lens[2]:], case[0][0] = math.nan, math.inf, math.nan  # none of them counts
+    _check(case, _call(case, lengths=torch.tensor(lens, device=DEV)), lens=lens)
+
+
+@pytest.mark.parametrize("B,T", [(4500, 1), (4200, 2)])
+def test_steps_of_more_rows_than_blocks(B, T):
+    """Blocks take several rows: each as one alone, also in place."""
+    case = [t.to(DEV) for t in _case(B=B, T=T, D=8, S=16, seed=1)]
+    lens = torch.arange(B, device=DEV) % (T + 1)
+    y, state = _run(case, lengths=lens)
+    for lo, hi in ((0, 3000), (3000, B)):
+        part = [t[lo:hi] if i in (0, 1, 3, 4, 6, 8) else t for i, t in enumerate(case)]
+        y_part, state_part = _run(part, lengths=lens[lo:hi])
+        assert torch.equal(y[lo:hi], y_part) and torch.equal(state[lo:hi], state_part)
+    own = case[8].clone()
+    y_own, _ = _run(case[:8] + [own], lengths=lens, inplace=True)
+    assert torch.equal(y_own, y) and torch.equal(own, state)
