@@ -12,6 +12,11 @@
 // are gathered in LDS and compared with each other: with some more, by a limit that each wave's greatest logits
 // give, or with the bin where the prefix ends, which counts (by top_k) or sums of the weights (by top_p) in 2048
 // bins tell. Otherwise the end is found within that bin, and a pass adds up what is kept by stretches of the index.
+//
+// 192 rows of 128257 bf16, a block on three of four compute units: greedy 27 us, top_k of 50 30 (49 MB read, 2 TB/s), no
+// filter 46, top_p of 0.9 at temperature 1.5 110, of which two passes of weights take 25 each, bound by their
+// instructions (some 35 a token, 12 of 64 bits), and the search 22. One row of 32000, fp32: 12 to 17 us, the latency of
+// its passes and barriers.
 #include "ramnet_kernels.hpp"
 #include "vector16.hpp"
 

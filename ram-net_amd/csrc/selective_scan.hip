@@ -1,4 +1,14 @@
 // Selective scan, forward: whole and packed prompts, decode steps, and what a training call keeps.
+//
+// Bound by vector instructions: every channel and state has a decay of its own, so no matrix product stands in for the
+// recurrence. A token of 16 channels with 16 states is 20 of a wave for its states (two products, an exponential, which
+// takes two's time, and two fused products each) and 13 around them. Pieces of a row are joined by linearity: with h_k
+// the state after piece k from zeros and D_k the sum of its dt, the state before piece k + 1 is
+// h_k + e^(A D_k) (the one before piece k). D_k is in 64 bits, as A D_k may be large where a decay ends.
+// B and C of 16 tokens are in LDS for the wave that reads them (no barriers), the next 16 tokens' rows on their way.
+//
+// 8 x 4096 x 2048, 16 states, gated, bf16: 391 us (287 by its instructions, 109 by its bytes), one wave a SIMD, 71% of the
+// time issuing. 1 x 32768 x 1024: 118 and 151, 92 to 96%. Decode, 64 rows x 2048: 8.0 us, 2048 rows: 126, 4.3 TB/s.
 #include "ramnet_kernels.hpp"
 #include "selective_scan.hpp"
 

@@ -4,8 +4,12 @@
 //     dC_t = ds_t h_t,   dB_t = dt_t x_t G_t          (both summed over a group's channels)
 //     d(dt x)_t = B_t . G_t,   d(dt_t) = x_t d(dt x)_t + sum_n A G_t a_t h_{t-1},   dA = sum_t dt_t G_t a_t h_{t-1}
 //
-// The states are walked again from those kept every 16 tokens; a_t and a_t h_{t-1} of a tile stay in
-// registers for the way back.
+// The states are walked again from those kept every 16 tokens; a_t and a_t h_{t-1} of a part of the tile stay in
+// registers for the way back. Pieces are joined as in the forward, from the last to the first.
+//
+// Bound by vector instructions, 114 a token and wave with 16 states, 20 of them for the sums of dB and dC over a wave's
+// channels: 4 x 2048 x 2048, gated, bf16: 282 us, 88% of the time issuing (bytes: 48 us), the pieces' ends 79, the sums 20.
+// Sums over channels and tokens go through memory in one order: results do not change from call to call.
 #include "ramnet_kernels.hpp"
 #include "selective_scan.hpp"
 
