@@ -51,10 +51,11 @@ def sample_tokens(
     The token is the lowest index whose running sum of kept weights passes ``random`` times their sum. Sums are in
     64 bits. A NaN logit counts as -inf; a row of nothing else gives token 0 and probabilities of 0.
 
-    Settings are numbers, or tensors that broadcast to the rows; a tensor's values are not checked.
+    Settings are numbers, or tensors that broadcast to the rows; a tensor's values are not checked. No gradients.
 
     :param logits: (..., V), a float type of 32 bits or fewer.
-    :param random: Uniform numbers in [0, 1) (...), any float type; used in 32 bits.
+    :param random: Uniform numbers in [0, 1) (...), any float type; used in 32 bits. Below 0 counts as 0, from 1 on
+        draws the last kept token.
     :param temperature: 0 takes the greatest logit (of equal ones the first).
     :param top_k: 0 or None keeps all.
     :param top_p: 1 or None keeps all.
