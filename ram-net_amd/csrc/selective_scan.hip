@@ -74,22 +74,26 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(const ScanJob job) {
         const float bias = job.bias ? job.bias[channel] : 0.f, skip = job.skip ? job.skip[channel] : 0.f;
         double span = 0.0;
         // Windows over the 16 tokens of a tile: tokens that are not there read 0 and are not written
-        const int64_t token = piece.t0, xr = piece.row * job.x_at[0], dr = piece.row * job.dt_at[0],
-                      gr = piece.row * job.gate_at[0], Br = piece.row * job.B_at[0] + at.group * job.B_at[2],
-                      Cr = piece.row * job.C_at[0] + at.group * job.C_at[2];
+        const int64_t token = piece.t0, first_row = piece.row;
+        ScanCursor<Scalar> x_at(job.x, first_row * job.x_at[0] + token * job.x_at[1], job.x_at[1], job.D),
+            dt_at(job.dt, first_row * job.dt_at[0] + token * job.dt_at[1], job.dt_at[1], job.D),
+            gate_at(job.gate, first_row * job.gate_at[0] + token * job.gate_at[1], job.gate_at[1], job.D),
+            B_at(job.B, first_row * job.B_at[0] + at.group * job.B_at[2] + token * job.B_at[1], job.B_at[1], job.S),
+            C_at(job.C, first_row * job.C_at[0] + at.group * job.C_at[2] + token * job.C_at[1], job.C_at[1], job.S),
+            y_at(job.y, row * job.D, job.D, job.D);
         const ScanRows<Scalar> x_rows(at, job.x_at[1], true), dt_rows(at, job.dt_at[1], true), gate_rows(at, job.gate_at[1], true),
             y_rows(at, job.D, at.valid);
         const Groups B_rows(lane, job.B_at[1], job.S), C_rows(lane, job.C_at[1], job.S);
         uint32_t xs[kQuads], ds[kQuads], gs[kQuads], Bs[Groups::kLoads], Cs[Groups::kLoads];
         auto load = [&](int t) {
             const int left = piece.len - t;
-            dt_rows.load(ds, dt_rows.over(job.dt, dr + (token + t) * job.dt_at[1], job.dt_at[1], job.D, left));
-            x_rows.load(xs, x_rows.over(job.x, xr + (token + t) * job.x_at[1], job.x_at[1], job.D, left));
-            B_rows.load(Bs, dt_rows.over(job.B, Br + (token + t) * job.B_at[1], job.B_at[1], job.S, left));
+            dt_rows.load(ds, dt_at.next(left));
+            x_rows.load(xs, x_at.next(left));
+            B_rows.load(Bs, B_at.next(left));
             if constexpr (kMode == kWhole) {
-                C_rows.load(Cs, dt_rows.over(job.C, Cr + (token + t) * job.C_at[1], job.C_at[1], job.S, left));
+                C_rows.load(Cs, C_at.next(left));
                 if constexpr (kGate)
-                    gate_rows.load(gs, gate_rows.over(job.gate, gr + (token + t) * job.gate_at[1], job.gate_at[1], job.D, left));
+                    gate_rows.load(gs, gate_at.next(left));
             }
         };
         auto walk = [&](int t, const float *bc, auto whole) {
@@ -106,9 +110,8 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(const ScanJob job) {
                 for (int g = 0; g < kQuads; ++g)
                     dv[g] = softplus(dv[g], e);
             }
-            if (t + kTile < piece.len)
-                load(t + kTile);
-            const __amdgpu_buffer_rsrc_t out = y_rows.over(job.y, (row + t) * job.D, job.D, job.D, piece.len - t);
+            load(t + kTile);  // (past the piece windows are empty: a branch would cost copies of all it may leave as it was)
+            const __amdgpu_buffer_rsrc_t out = y_at.next(piece.len - t);
             // B and C of four tokens at a time, read from LDS while the four before are walked
             float b[2][4][NR], c[2][4][NR];
             auto fetch = [&](int g) {

@@ -90,16 +90,14 @@ __device__ __forceinline__ float quad_sums(const float (&v)[4], int lane) {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-// log(1 + e^x) = max(x, 0) + log(1 + e), e = e^-|x| in (0, 1], the latter as 2 atanh(e / (2 + e)): the
-// series of atanh on (0, 1/3], to 2e-9 of its value. `e` comes out for the derivative.
+// log(1 + e^x) = max(x, 0) + log(1 + e), e = e^-|x| in (0, 1], the latter as 2 atanh(s), s = e / (2 + e): atanh(s) / s on
+// (0, 1/3] by the polynomial in s^2 whose greatest relative error is least, 8e-9. `e` comes out for the derivative.
 __device__ __forceinline__ float softplus(float x, float &e) {
     e = __builtin_amdgcn_exp2f(-fabsf(x) * kLog2e);
     const float s = e * __builtin_amdgcn_rcpf(2.f + e), q = s * s;
-    float sum = 1.f / 17.f;
-#pragma unroll
-    for (int k = 15; k >= 1; k -= 2)
-        sum = fmaf(sum, q, 1.f / static_cast<float>(k));
-    return fmaxf(x, 0.f) + 2.f * s * sum;
+    const float sum = fmaf(fmaf(fmaf(fmaf(0.140891677f, q, 0.139803015f), q, 0.200124551f), q, 0.333331573f), q, 1.f);
+    const float above = __int_as_float(max(__float_as_int(x), 0));  // (max(x, 0): of floats it is two instructions)
+    return fmaf(2.f * s, sum, above);
 }
 
 // Writes of some lanes of a wave to LDS before reads of others.
@@ -130,23 +128,38 @@ struct ScanPlace {
     }
 };
 
+// x as a value that the compiler cannot make from others again: offsets are made once, or (in load) for each load.
 __device__ __forceinline__ int anew(int x) {
     asm volatile("" : "+v"(x));
     return x;
 }
 
-// One value of a lane's channel for each four tokens of a tile, through a window over the tile's tokens that
-// are there.
+// The windows over a tensor's rows, one tile after the other: a tile's tokens that are there (none: it is empty). Steps
+// from tile to tile are kept, as addresses made anew are some 25 scalar instructions a tensor and tile.
+template<typename Scalar, int kSign = 1>
+struct ScanCursor {
+    const char *p;
+    int step, rest;  // bytes from token to token; of the last token's row less a step
+
+    __device__ __forceinline__ ScanCursor(const void *base, int64_t from, int64_t stride, int width)
+        : p(reinterpret_cast<const char *>(static_cast<const Scalar *>(base) + from)),
+          step(static_cast<int>(stride) * static_cast<int>(sizeof(Scalar))), rest(width * static_cast<int>(sizeof(Scalar)) - step) {}
+    // `left`: tokens from this tile's first to the last.
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t next(int left) {
+        const char *at = p;
+        p += kSign * kScanKept * static_cast<int64_t>(step);
+        return window(at, left > 0 ? min(left, kScanKept) * step + rest : 0);
+    }
+};
+
+// One value of a lane's channel for each four tokens of a tile, through a window over it.
 template<typename Scalar>
 struct ScanRows {
     int at, step;  // bytes: the lane's place in the first four tokens; four tokens on
 
     __device__ __forceinline__ ScanRows(const ScanPlace &place, int64_t stride, bool on) {
         step = 4 * static_cast<int>(stride) * static_cast<int>(sizeof(Scalar));
-        at = on ? (place.sub * static_cast<int>(stride) + place.channel) * static_cast<int>(sizeof(Scalar)) : kNowhere;
-    }
-    __device__ static __forceinline__ __amdgpu_buffer_rsrc_t over(const void *p, int64_t from, int64_t stride, int D, int tokens) {
-        return window(static_cast<const Scalar *>(p) + from, ((min(tokens, kScanKept) - 1) * stride + D) * static_cast<int>(sizeof(Scalar)));
+        at = anew(on ? (place.sub * static_cast<int>(stride) + place.channel) * static_cast<int>(sizeof(Scalar)) : kNowhere);
     }
     // (kAnew: offsets are made for each load; kept over a loop they fill registers)
     template<bool kAnew = false>
@@ -170,7 +183,8 @@ struct ScanGroups {
     __device__ __forceinline__ ScanGroups(int lane, int64_t stride, int S) {
         const bool on = lane / kRow < kSpan;
         step = kSpan * static_cast<int>(stride) * static_cast<int>(sizeof(Scalar));
-        at = on && lane % kRow < S ? (lane / kRow * static_cast<int>(stride) + lane % kRow) * static_cast<int>(sizeof(Scalar)) : kNowhere;
+        at = anew(on && lane % kRow < S ? (lane / kRow * static_cast<int>(stride) + lane % kRow) * static_cast<int>(sizeof(Scalar))
+                                        : kNowhere);
         to = on ? lane : -1;
     }
     template<bool kAnew = false>

@@ -79,20 +79,23 @@ __global__ __launch_bounds__(kThreads) void scan_backs_kernel(const ScanJob job,
         carry[j] = 0.f;
     const float bias = job.bias ? job.bias[at.channel] : 0.f;
     double span = 0.0;
-    const int64_t token = piece.t0, dr = piece.row * job.dt_at[0], gr = piece.row * job.gate_at[0],
-                  yr = piece.row * grads.dy_at[0], Cr = piece.row * job.C_at[0] + at.group * job.C_at[2];
+    int t = (piece.len - 1) / kTile * kTile;
+    const int64_t token = piece.t0 + t, first_row = piece.row;
+    ScanCursor<Scalar, -1> dt_at(job.dt, first_row * job.dt_at[0] + token * job.dt_at[1], job.dt_at[1], job.D),
+        gate_at(job.gate, first_row * job.gate_at[0] + token * job.gate_at[1], job.gate_at[1], job.D),
+        dy_at(grads.dy, first_row * grads.dy_at[0] + token * grads.dy_at[1], grads.dy_at[1], job.D),
+        C_at(job.C, first_row * job.C_at[0] + at.group * job.C_at[2] + token * job.C_at[1], job.C_at[1], job.S);
     const ScanRows<Scalar> dt_rows(at, job.dt_at[1], true), gate_rows(at, job.gate_at[1], true), dy_rows(at, grads.dy_at[1], true);
     const Groups C_rows(lane, job.C_at[1], job.S);
     uint32_t dts[kQuads], gates[kQuads], dys[kQuads], Cs[Groups::kLoads];
     auto load = [&](int t) {
         const int left = piece.len - t;
-        dt_rows.load(dts, dt_rows.over(job.dt, dr + (token + t) * job.dt_at[1], job.dt_at[1], job.D, left));
-        dy_rows.load(dys, dy_rows.over(grads.dy, yr + (token + t) * grads.dy_at[1], grads.dy_at[1], job.D, left));
+        dt_rows.load(dts, dt_at.next(left));
+        dy_rows.load(dys, dy_at.next(left));
         if (job.gate)
-            gate_rows.load(gates, gate_rows.over(job.gate, gr + (token + t) * job.gate_at[1], job.gate_at[1], job.D, left));
-        C_rows.load(Cs, dt_rows.over(job.C, Cr + (token + t) * job.C_at[1], job.C_at[1], job.S, left));
+            gate_rows.load(gates, gate_at.next(left));
+        C_rows.load(Cs, C_at.next(left));
     };
-    int t = (piece.len - 1) / kTile * kTile;
     load(t);
     for (int turn = 0; t >= 0; t -= kTile, turn ^= 1) {
         float dv[kQuads], sv[kQuads];
@@ -208,6 +211,11 @@ __global__ __launch_bounds__(kThreads, scan_waves<NR>()) void scan_backward_kern
         }
         const float bias = job.bias ? job.bias[channel] : 0.f, skip = job.skip ? job.skip[channel] : 0.f;
         const float *kept = job.kept + (scan_slot(job.seq, piece.seq, piece.lo) + (piece.t0 - piece.lo) / kScanKept) * wide + mine;
+        // (windows are made from the job for each tile: kept from one to the next they spill scalar registers, for the same time)
+        auto rows_at = [&](const void *p, int64_t from, int64_t stride, int width, int left) {
+            return window(static_cast<const Scalar *>(p) + from,
+                          ((min(left, kTile) - 1) * stride + width) * static_cast<int>(sizeof(Scalar)));
+        };
         const int64_t token = piece.t0, xr = piece.row * job.x_at[0], dr = piece.row * job.dt_at[0],
                       gr = piece.row * job.gate_at[0], yr = piece.row * grads.dy_at[0],
                       Br = piece.row * job.B_at[0] + at.group * job.B_at[2], Cr = piece.row * job.C_at[0] + at.group * job.C_at[2];
@@ -218,13 +226,13 @@ __global__ __launch_bounds__(kThreads, scan_waves<NR>()) void scan_backward_kern
         uint32_t xs[kQuads], dts[kQuads], gates[kQuads], dys[kQuads], Bs[Groups::kLoads], Cs[Groups::kLoads];
         auto load = [&](int t) {
             const int left = piece.len - t;
-            dt_rows.template load<true>(dts, dt_rows.over(job.dt, dr + (token + t) * job.dt_at[1], job.dt_at[1], D, left));
-            x_rows.template load<true>(xs, x_rows.over(job.x, xr + (token + t) * job.x_at[1], job.x_at[1], D, left));
-            dy_rows.template load<true>(dys, dy_rows.over(grads.dy, yr + (token + t) * grads.dy_at[1], grads.dy_at[1], D, left));
+            dt_rows.template load<true>(dts, rows_at(job.dt, dr + (token + t) * job.dt_at[1], job.dt_at[1], D, left));
+            x_rows.template load<true>(xs, rows_at(job.x, xr + (token + t) * job.x_at[1], job.x_at[1], D, left));
+            dy_rows.template load<true>(dys, rows_at(grads.dy, yr + (token + t) * grads.dy_at[1], grads.dy_at[1], D, left));
             if constexpr (kGate)
-                gate_rows.template load<true>(gates, gate_rows.over(job.gate, gr + (token + t) * job.gate_at[1], job.gate_at[1], D, left));
-            B_rows.template load<true>(Bs, dt_rows.over(job.B, Br + (token + t) * job.B_at[1], job.B_at[1], job.S, left));
-            C_rows.template load<true>(Cs, dt_rows.over(job.C, Cr + (token + t) * job.C_at[1], job.C_at[1], job.S, left));
+                gate_rows.template load<true>(gates, rows_at(job.gate, gr + (token + t) * job.gate_at[1], job.gate_at[1], D, left));
+            B_rows.template load<true>(Bs, rows_at(job.B, Br + (token + t) * job.B_at[1], job.B_at[1], job.S, left));
+            C_rows.template load<true>(Cs, rows_at(job.C, Cr + (token + t) * job.C_at[1], job.C_at[1], job.S, left));
             load_states<NR>(h_next, kept + t / kTile * wide, NR);
         };
         int t = (piece.len - 1) / kTile * kTile;
@@ -256,8 +264,8 @@ __global__ __launch_bounds__(kThreads, scan_waves<NR>()) void scan_backward_kern
                 load(t - kTile);
             const int left = piece.len - t;
             const int64_t first = (row + t) * D;
-            const auto dx_rows = d_rows.over(grads.dx, first, D, D, left), ddt_rows = d_rows.over(grads.ddt, first, D, D, left);
-            const auto dgate_rows = d_rows.over(kGate ? grads.dgate : grads.dx, first, D, D, left);
+            const auto dx_rows = rows_at(grads.dx, first, D, D, left), ddt_rows = rows_at(grads.ddt, first, D, D, left);
+            const auto dgate_rows = rows_at(kGate ? grads.dgate : grads.dx, first, D, D, left);
             // the states before each part of the tile
             float from[kParts][NR];
 #pragma unroll
