@@ -2,13 +2,13 @@
 //
 // Bound by vector instructions: every channel and state has a decay of its own, so no matrix product stands in for the
 // recurrence. A token of 16 channels with 16 states is 20 of a wave for its states (two products, an exponential, which
-// takes two's time, and two fused products each) and 13 around them. Pieces of a row are joined by linearity: with h_k
+// takes two's time, and two fused products each) and 11 around them. Pieces of a row are joined by linearity: with h_k
 // the state after piece k from zeros and D_k the sum of its dt, the state before piece k + 1 is
 // h_k + e^(A D_k) (the one before piece k). D_k is in 64 bits, as A D_k may be large where a decay ends.
 // B and C of 16 tokens are in LDS for the wave that reads them (no barriers), the next 16 tokens' rows on their way.
 //
-// 8 x 4096 x 2048, 16 states, gated, bf16: 391 us (287 by its instructions, 109 by its bytes), one wave a SIMD, 71% of the
-// time issuing. 1 x 32768 x 1024: 118 and 151, 92 to 96%. Decode, 64 rows x 2048: 8.0 us, 2048 rows: 126, 4.3 TB/s.
+// 8 x 4096 x 2048, 16 states, gated, bf16: 372 us (257 by its instructions, 109 by its bytes), one wave a SIMD, 69% of the
+// time issuing. 1 x 32768 x 1024: 111 and 145, 90 to 95%. Decode, 64 rows x 2048: 8.0 us, 2048 rows: 126, 4.3 TB/s.
 #include "ramnet_kernels.hpp"
 #include "selective_scan.hpp"
 
@@ -351,7 +351,7 @@ bool scan_is_step(const ScanJob &job) { return !job.seq.cu && !job.kept && job.s
 
 // Rows are cut into pieces where their channels alone leave compute units idle. The state after each piece from zeros
 // is a pass of its own that costs two thirds of the other, so a row in many pieces takes as long as 1.35 in one do
-// where the waves of either fill the machine: 4096 tokens of 1024 waves take 395 us in one piece, 550 in two
+// where the waves of either fill the machine: 4096 tokens of 1024 waves took 395 us in one piece, 550 in two
 // (336 + 230) and 515 in four. From 768 waves on, three quarters of what runs at once, rows stay whole. Below that
 // 4096 waves (four a SIMD) hide each other's latencies: 32768 tokens of 64 waves take 277 us in 32 pieces, 266 in 64.
 // The backward has registers for two waves a SIMD, and keeps to 2048. A piece joins the ends of those before it one by

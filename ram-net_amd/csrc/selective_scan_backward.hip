@@ -7,8 +7,8 @@
 // The states are walked again from those kept every 16 tokens; a_t and a_t h_{t-1} of a part of the tile stay in
 // registers for the way back. Pieces are joined as in the forward, from the last to the first.
 //
-// Bound by vector instructions, 114 a token and wave with 16 states, 20 of them for the sums of dB and dC over a wave's
-// channels: 4 x 2048 x 2048, gated, bf16: 282 us, 88% of the time issuing (bytes: 48 us), the pieces' ends 79, the sums 20.
+// Bound by vector instructions, 113 a token and wave with 16 states, 20 of them for the sums of dB and dC over a wave's
+// channels: 4 x 2048 x 2048, gated, bf16: 280 us, 87% of the time issuing (bytes: 48 us), the pieces' ends 75, the sums 20.
 // Sums over channels and tokens go through memory in one order: results do not change from call to call.
 #include "ramnet_kernels.hpp"
 #include "selective_scan.hpp"
