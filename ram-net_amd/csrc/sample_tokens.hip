@@ -16,7 +16,7 @@
 // 192 rows of 128257 bf16, a block on three of four compute units: greedy 27 us, top_k of 50 30 (49 MB read, 2 TB/s), no
 // filter 46, top_p of 0.9 at temperature 1.5 110, of which two passes of weights take 25 each, bound by their
 // instructions (some 35 a token, 12 of 64 bits), and the search 22. One row of 32000, fp32: 12 to 17 us, the latency of
-// its passes and barriers.
+// its passes and barriers. Masked rows take no longer: with 20 tokens left and a top_k of 50 28 us and 12.6.
 #include "ramnet_kernels.hpp"
 #include "vector16.hpp"
 
@@ -30,6 +30,8 @@ constexpr int kThreads = 1024, kWaves = kThreads / kWave, kBins = 2 * kThreads, 
 constexpr int kListCount = 256;
 // Bins of a sum for each halving of the weight: what lies past 2^-32 is in the last bin.
 constexpr float kBinsAHalving = 64.f;
+// The least logit of a token that can be drawn: one of -inf is in no list and no count.
+constexpr float kLeastLogit = -__FLT_MAX__;
 
 // A token's place in the order as one number, greater for earlier ones; its upper half goes by the logit alone.
 __device__ __forceinline__ uint32_t key_of(float l) {
@@ -221,7 +223,7 @@ struct Sampler {
         const float at = l == top ? 0.f : (top - l) * scale;  // (descending with l, whatever it rounds to; a NaN last)
         return static_cast<int>(__builtin_fminf(at, static_cast<float>(kBins - 1)));
     }
-    // Whether a token is in the prefix kept (a NaN is not).
+    // Whether a token is in the prefix kept. A NaN is not, nor is -inf, also where the prefix has no end yet.
     __device__ __forceinline__ bool within(float l, int index) const {
         return l > last_logit || (l == last_logit && index <= last_index);
     }
@@ -291,18 +293,19 @@ struct Sampler {
     }
 
     // A limit that at least `count` logits reach, from the greatest one of each lane: the waves whose lanes have
-    // logits all give their share of it, each to the 16 upper bits.
+    // logits all give their share of it, each to the 16 upper bits. Where that would be -inf (many tokens are masked)
+    // the least finite number, which all tokens reach that can be drawn.
     __device__ __forceinline__ float limit_of(float mine, int count) {
         const int waves = min(V / static_cast<int>(16 / sizeof(Scalar)) / kWave, kWaves), each = (count + waves - 1) / max(waves, 1);
         if (waves == 0 || each > kWave)
-            return -INFINITY;
+            return kLeastLogit;
         const uint32_t key = key_of(mine);
         uint32_t reached = 0;
 #pragma unroll
         for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1)
             reached |= __popcll(__ballot(key >= (reached | bit))) >= each ? bit : 0;
         reached = block_reduce(wave < waves ? reached : ~0u, Least{});
-        return reached > key_of(-INFINITY) ? logit_of_key(reached) : -INFINITY;
+        return reached > key_of(-INFINITY) ? logit_of_key(reached) : kLeastLogit;
     }
 
     // The tokens of which `wanted` is true in the list, in any order. How many they are: where
@@ -435,11 +438,14 @@ struct Sampler {
     }
 
     // The order of the k-th token, or of the last one with less than `target` before it, in the bin that find_bin
-    // has found: as long as it holds more tokens than the list, it is cut into 2048 parts again, now by the order.
+    // has found (of tokens that `within` holds, as all searches count them): as long as it holds more tokens than the
+    // list, it is cut into 2048 parts again, now by the order. Where no token is met, an end that keeps all.
     // `through`: with a target the weights up to that one, it among them (0: not known).
     __device__ __forceinline__ uint64_t find_border(uint64_t k, double target, uint64_t &through) {
         through = 0;
         const int level = lds().bin;
+        if (tid == 0)  // (behind barriers before a thread that meets its token writes)
+            lds().order = order_of(-INFINITY, -1);
         const bool by_sum = target > 0.0;
         uint64_t base = by_sum ? lds().before : 0, lo = 0, hi = ~0ull;
         int count = by_sum ? 0 : lds().count_before;
@@ -496,8 +502,9 @@ struct Sampler {
                 lds().order = own, lds().before = before + part;
         }
         __syncthreads();
-        through = by_sum ? lds().before : 0;
-        return lds().order;
+        const uint64_t order = lds().order;
+        through = by_sum && index_of(order) >= 0 ? lds().before : 0;
+        return order;
     }
 };
 
@@ -554,7 +561,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleJob job) {
             // below the logit of weight min_p by more than the roundings on the way
             const double cut = static_cast<double>(me.top) + log2(me.least) / me.rate;
             limit = static_cast<float>(cut - (fabs(cut) + fabs(static_cast<double>(me.top))) * 1e-6 - 1e-37);
-            limit = limit < me.top ? limit : -INFINITY;
+            limit = limit < me.top && limit > kLeastLogit ? limit : kLeastLogit;
         }
         const int members = me.gather([&](float l, int) { return l >= limit; });
         if (members <= kList) {
@@ -567,16 +574,23 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleJob job) {
         const float range = me.top - me.block_reduce(low, Least{});
         me.scale = range > 0.f && range < INFINITY ? static_cast<float>(kBins - 1) / range : 0.f;
         me.clear_bins();
-        me.sweep([&](float l, int) { atomicAdd(&lds().counts[me.bin(l)], 1u); });
+        me.sweep([&](float l, int i) {
+            if (me.within(l, i))
+                atomicAdd(&lds().counts[me.bin(l)], 1u);
+        });
         __syncthreads();
-        me.find_bin(first, 0.0, 0, 0);
-        const int level = lds().bin;
-        if (lds().count_through <= kList) {
-            const int members = me.gather([&](float l, int) { return me.bin(l) <= level; });
-            me.finish(members, first, by_sum, p, 0, u, token, probs);
-            return;
+        // (not found: fewer tokens than top_k can be drawn, and it keeps them all)
+        const bool found = me.find_bin(first, 0.0, 0, 0);
+        const int level = found ? lds().bin : kBins - 1;
+        if (!found || lds().count_through <= kList) {
+            const int members = me.gather([&](float l, int i) { return me.bin(l) <= level && me.within(l, i); });
+            if (members <= kList) {
+                me.finish(members, first, by_sum, p, 0, u, token, probs);
+                return;
+            }
         }
-        me.end_with(me.find_border(first, 0.0, kept_sum));
+        if (found)
+            me.end_with(me.find_border(first, 0.0, kept_sum));
     }
     if (by_sum) {
         me.scale = static_cast<float>(me.rate) * kBinsAHalving;
