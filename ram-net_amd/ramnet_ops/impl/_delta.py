@@ -110,6 +110,8 @@ def _rows(t: Tensor) -> Tensor:
 def _whole(t: Tensor | None) -> Tensor | None:
     if t is None or (t.dtype == torch.int32 and t.is_contiguous()):
         return t
+    if t.dtype == torch.int64:  # (a count past int32 is as good as the most it holds; cut off it would be another one)
+        t = t.clamp(0, 2 ** 31 - 1)
     return t.to(torch.int32).contiguous()
 
 
