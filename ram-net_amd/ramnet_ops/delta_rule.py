@@ -51,7 +51,8 @@ def gated_delta_rule(
     :param q: Queries (B, T, Hk, Dk), Dk up to 256; their last dimension dense, any other strides.
     :param k: Keys (B, T, Hk, Dk), as a rule of norm 1.
     :param v: Values (B, T, Hv, Dv); value head h reads key head ``h // (Hv // Hk)``.
-    :param g: Logarithm of the decay (B, T, Hv), any float type; -inf clears the state.
+    :param g: Logarithm of the decay (B, T, Hv), a float type of 32 bits or fewer, as for beta; -inf clears
+        the state.
     :param beta: Write strength (B, T, Hv).
     :param scale: Factor of o; default ``Dk ** -0.5``.
     :param init_state: State before the first token (N, Hv, Dk, Dv), a float type of 32 bits or fewer; default zeros.

@@ -51,7 +51,8 @@ def sample_tokens(
     The token is the lowest index whose running sum of kept weights passes ``random`` times their sum. Sums are in
     64 bits. A NaN logit counts as -inf; a row of nothing else gives token 0 and probabilities of 0.
 
-    Settings are numbers, or tensors that broadcast to the rows; a tensor's values are not checked. No gradients.
+    Settings are numbers, used in 64 bits, or tensors that broadcast to the rows (any float type, used in 32 bits; top_k
+    int32 or int64); a tensor's values are not checked. No gradients.
 
     :param logits: (..., V), a float type of 32 bits or fewer.
     :param random: Uniform numbers in [0, 1) (...), any float type; used in 32 bits. Below 0 counts as 0, from 1 on

@@ -93,12 +93,13 @@ def selective_scan(
 
     :param x: Inputs (batch, T, D); last dimension dense, any other strides, as for dt, B, C and gate.
     :param dt: Step of each token and channel (batch, T, D), before dt_bias and the softplus.
-    :param A: Rates (D, S), below 0 for decays; S up to 64; any float type, used in 32 bits.
+    :param A: Rates (D, S), below 0 for decays; S up to 64; a float type of 32 bits or fewer, used in
+        32, as for skip and dt_bias.
     :param B: What the state takes up (batch, T, G, S); channel d reads group ``d // (D // G)``.
     :param C: What is read of it (batch, T, G, S).
-    :param skip: Share of x in y (D), any float type.
+    :param skip: Share of x in y (D).
     :param gate: (batch, T, D).
-    :param dt_bias: (D), any float type.
+    :param dt_bias: (D).
     :param softplus: Whether dt goes through a softplus.
     :param init_state: State before the first token (N, D, S), a float type of 32 bits or fewer; default zeros.
     :param cu_seqlens: (N + 1) bounds of N sequences packed one after the other in a batch of one.
