@@ -164,10 +164,12 @@ struct Sampler {
 
     __device__ __forceinline__ float clean(float l) const { return l != l ? -INFINITY : l + 0.f; }
 
-    // f(logit, index) for all tokens, 16 bytes a thread, all threads of the block side by side.
-    template<int kDeep = 4, typename F>
+    // f(logit, index) for all tokens, 16 bytes a thread, all threads of the block side by side. (kRaw: of logits as
+    // they are stored, for an f that passes over a NaN by itself.)
+    template<bool kRaw = false, typename F>
     __device__ __forceinline__ void sweep(F f) const {
-        constexpr int N = 16 / sizeof(Scalar);
+        constexpr int N = 16 / sizeof(Scalar), kDeep = 4;
+        auto value = [&](float l) { return kRaw ? l : clean(l); };
         const int full = V / N * N;
         for (int at = tid * N; at < full; at += kDeep * kThreads * N) {
             Vec<Scalar, N> x[kDeep];
@@ -182,12 +184,12 @@ struct Sampler {
                 if (from < full) {
 #pragma unroll
                     for (int e = 0; e < N; ++e)
-                        f(clean(x[i][e]), from + e);
+                        f(value(x[i][e]), from + e);
                 }
             }
         }
         if (full + tid < V)
-            f(clean(load_f32(row + full + tid)), full + tid);
+            f(value(load_f32(row + full + tid)), full + tid);
     }
 
     // The same with one piece ahead, for an f that takes longer than the read.
@@ -310,17 +312,17 @@ struct Sampler {
 
     // The tokens of which `wanted` is true in the list, in any order. How many they are: where
     // more than kList the list has some of them.
-    template<typename F>
+    template<bool kRaw = false, typename F>
     __device__ __forceinline__ int gather(F wanted) {
         __syncthreads();
         if (tid == 0)
             lds().listed = 0;
         __syncthreads();
-        sweep([&](float l, int i) {
+        sweep<kRaw>([&](float l, int i) {
             if (wanted(l, i)) {
                 const int at = atomicAdd(&lds().listed, 1);
                 if (at < kList)
-                    lds().list[at] = order_of(l, i);
+                    lds().list[at] = order_of(kRaw ? clean(l) : l, i);
             }
         });
         __syncthreads();
@@ -574,8 +576,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleJob job) {
         const float range = me.top - me.block_reduce(low, Least{});
         me.scale = range > 0.f && range < INFINITY ? static_cast<float>(kBins - 1) / range : 0.f;
         me.clear_bins();
-        me.sweep([&](float l, int i) {
-            if (me.within(l, i))
+        me.template sweep<true>([&](float l, int) {
+            if (l > -INFINITY)
                 atomicAdd(&lds().counts[me.bin(l)], 1u);
         });
         __syncthreads();
@@ -583,7 +585,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleJob job) {
         const bool found = me.find_bin(first, 0.0, 0, 0);
         const int level = found ? lds().bin : kBins - 1;
         if (!found || lds().count_through <= kList) {
-            const int members = me.gather([&](float l, int i) { return me.bin(l) <= level && me.within(l, i); });
+            const int members = me.template gather<true>([&](float l, int) { return l > -INFINITY && me.bin(l) <= level; });
             if (members <= kList) {
                 me.finish(members, first, by_sum, p, 0, u, token, probs);
                 return;
