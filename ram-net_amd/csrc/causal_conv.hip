@@ -1,14 +1,16 @@
 // Short causal convolution of each channel over its last W <= 8 tokens, and its gradients.
 //
-// Bound by memory: x is read once and y written once (backward: x and dy read, dx written), 2 W
-// operations an element. A thread takes 16 bytes of adjacent channels and walks a piece of time
-// with the last W - 1 inputs in registers; what a piece reads of its forerunner comes from the L2.
+// The forward is bound by memory: x is read once and y written once, 2 W operations an element. A
+// thread takes 16 bytes of adjacent channels and walks a piece of time with the last W - 1 inputs in
+// registers; what a piece reads of its forerunner comes from the L2. So is the backward in fp32 (x and dy
+// read, dx written; 4.7 TB/s). In 16 bits it is not: its instructions a channel are the same for half the bytes, and at
+// two waves a SIMD loads of four tokens and the work on them take turns (vector units 67% busy, 3.3 TB/s).
 // Rows are read and written at any alignment: the last channels of a row whose length is no
 // multiple of 16 bytes are taken with some of those before them, which two threads then compute alike.
 //
 // 8 x 4096 x 2048, W 4, bf16: 54.6 us, 4.9 TB/s, what a large copy reaches (fp32 112 us, 4.8 TB/s). 64 rows of one token x
-// 4096: 6 us. The backward of 4 x 2048 x 2048, bf16: 36 us and 7 for the sums; 8003 packed tokens x 1001, W 3, fp32:
-// 25 and 5, the forward 16.
+// 4096: 6 us. The backward of 4 x 2048 x 2048, bf16: 38.6 us and 4 for the sums, the forward 17.9; 8003 packed tokens x
+// 1001, W 3, fp32: 25 and 5, the forward 16.
 #include "causal_conv.hpp"
 #include "ramnet_kernels.hpp"
 #include "vector16.hpp"

@@ -28,11 +28,11 @@ struct ConvGrads {
     const void *dstate;  // (N, W - 1, D), or null: zeros
     void *dx, *dinit;    // dinit may be null
     void *dweight, *dbias;  // dbias may be null
-    float *partial;      // [groups of pieces][W + 1][D] sums of dweight and dbias
+    float *partial;      // [piece][W + 1][D] sums of dweight and dbias
     int64_t dy_at[2];
 };
 
-// Tokens of a piece, and bytes of the workspace of a call (kind 0: forward, 1: backward).
+// Tokens of a piece, and bytes of the workspace of a call.
 int conv_step(const ConvJob &job, bool backward);
 int64_t conv_layout(ConvJob &job, bool backward, char *base, ConvGrads *grads);
 hipError_t launch_conv(const ConvJob &job, hipStream_t stream, const char **why);
